@@ -186,6 +186,64 @@ int minitp_attention(void* stream, int dtype, const void* q, const void* k_cache
                      int64_t Hkv, int64_t D, int64_t S, int64_t cache_len, void* workspace,
                      int64_t workspace_bytes);
 
+/* Attention of a batch whose rows share prefixes (the beams of one prompt,
+ * requests under one system prompt); no counterpart in the reference, whose
+ * attention (attention.py:77-105) reads every row's keys from that row's
+ * cache. The B rows form G groups of B / G consecutive rows. Group g's prefix
+ * is rows 0 .. P_g - 1 of k_prefix / v_prefix [G, Hkv, S_prefix, D]; row b's
+ * caches [B, Hkv, S, D] hold c_b rows and then its T new ones. Query t of row
+ * b attends the whole prefix of its group and own rows 0 .. c_b + t. q [B, T,
+ * Hq, D], out [B, T, Hq * D], scale 1/sqrt(D), head h on KV head h / (Hq/Hkv),
+ * D 16, 32, 64 or 128. prefix_lens [G] and cache_lens [B] are device arrays of
+ * P_g and c_b, taken as at most prefix_len and cache_len; NULL: prefix_len and
+ * cache_len everywhere. A negative cache_lens[b] marks an idle row: its output
+ * is zeros and its caches are not read. Rows past P_g and c_b + T are never
+ * read. prefix_len 0 serves rows without a prefix (the prefix pointers may be
+ * NULL). Workspace from the query below (bf16 and fp32 ask for different
+ * sizes); no initial value, nothing kept in it after the call's kernels. */
+int64_t minitp_shared_prefix_attention_workspace_bytes(int dtype, int64_t B, int64_t G, int64_t T, int64_t Hq,
+                                                       int64_t Hkv, int64_t D, int64_t prefix_len,
+                                                       int64_t cache_len);
+int minitp_shared_prefix_attention(void* stream, int dtype, const void* q, const void* k_prefix,
+                                   const void* v_prefix, const void* k_cache, const void* v_cache, void* out,
+                                   int64_t B, int64_t G, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
+                                   int64_t S_prefix, int64_t prefix_len, const int64_t* prefix_lens, int64_t S,
+                                   int64_t cache_len, const int64_t* cache_lens, void* workspace,
+                                   int64_t workspace_bytes);
+
+/* ---- beam search --------------------------------------------------------- */
+/* One step of beam search for G groups of W beams (1 <= W <= 32); the
+ * reference decodes greedily only (generation.py:54-67). logits of beam w of
+ * group g: V elements at logits + g * ld_group + w * ld_beam (ld_beam 0: one
+ * row for all beams). scores [G, W] are the cumulative log-probabilities
+ * (minus infinity: no beam in this slot; its logits are not read), finished
+ * [G, W] bytes (NULL: none is), lengths [G, W] tokens so far (NULL: 0).
+ * Token v continues beam w with score s + x_v - logsumexp(x); a finished beam
+ * continues with eos_token at its own score and length. Of a group's
+ * continuations above minus infinity the W of the largest score / length ^
+ * length_penalty win (length: with the new token, at least 1), equal ones by
+ * the lower beam, then the lower token. A NaN score wins over every number.
+ * The first winner of a parent stays in the parent's slot, the others fill the
+ * free slots in rank order; a slot left over is its own parent with a score of
+ * minus infinity, marked finished. Outputs, all [G, W], which may be the
+ * inputs of the same kind: tokens, parents (rows of the batch, g * W + w),
+ * scores, finished (parent's, or the token is eos_token), lengths. eos_token
+ * -1: none (finished must be NULL). */
+int64_t minitp_beam_select_workspace_bytes(int64_t G, int64_t W, int64_t V);
+int minitp_beam_select(void* stream, int dtype, const void* logits, int64_t ld_group, int64_t ld_beam, int64_t G,
+                       int64_t W, int64_t V, const float* scores, const uint8_t* finished, const int64_t* lengths,
+                       int64_t eos_token, double length_penalty, int64_t* tokens, int64_t* parents,
+                       float* scores_out, uint8_t* finished_out, int64_t* lengths_out, void* workspace,
+                       int64_t workspace_bytes);
+/* The K/V caches follow the beams: rows 0 .. rows - 1 of every layer and KV
+ * head of batch row b become those of row parents[b], in place, for buffers
+ * [L, G * W, Hkv, S, D] (1 <= W <= 32) and parents [G, W] on the device, batch
+ * rows of the same group in any combination. A row whose parent is itself, or
+ * no row of its group, keeps what it holds. Rows of D elements must be whole
+ * 16-byte pieces. */
+int minitp_kv_reorder(void* stream, int dtype, void* k_cache, void* v_cache, int64_t L, int64_t G, int64_t W,
+                      int64_t Hkv, int64_t S, int64_t D, int64_t rows, const int64_t* parents);
+
 /* ---- greedy selection --------------------------------------------------- */
 /* distributed_argmax tp=1 fast path (embedding.py:146-147; generation.py:59):
  * out[b * out_stride] = argmax over logits[b * ld + 0 .. V), torch.argmax

@@ -2,6 +2,7 @@
 // launch. Nothing here allocates, synchronises or throws.
 #include <hip/hip_runtime.h>
 
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <mutex>
@@ -354,6 +355,97 @@ int minitp_attention(void* stream, int dtype, const void* q, const void* k_cache
     return launch_decode_attention(S(stream), dtype, q, k_cache, v_cache, out, a, cache_len, nullptr, 0, workspace,
                                    workspace_bytes);
   return launch_prefill_attention(S(stream), dtype, q, k_cache, v_cache, out, a, cache_len);
+}
+
+namespace {
+
+bool shared_prefix_shape_ok(int64_t B, int64_t G, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t P, int64_t C) {
+  return B >= 0 && G > 0 && B % G == 0 && T >= 0 && Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && D > 0 && P >= 0 && C >= 0;
+}
+
+}  // namespace
+
+int64_t minitp_shared_prefix_attention_workspace_bytes(int dtype, int64_t B, int64_t G, int64_t T, int64_t Hq,
+                                                       int64_t Hkv, int64_t D, int64_t prefix_len,
+                                                       int64_t cache_len) {
+  if (!dtype_ok(dtype) || !shared_prefix_shape_ok(B, G, T, Hq, Hkv, D, prefix_len, cache_len)) return -1;
+  return shared_prefix_workspace_bytes(dtype, B, G, T, Hq, Hkv, D, prefix_len, cache_len);
+}
+
+int minitp_shared_prefix_attention(void* stream, int dtype, const void* q, const void* k_prefix, const void* v_prefix,
+                                   const void* k_cache, const void* v_cache, void* out, int64_t B, int64_t G,
+                                   int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t S_prefix,
+                                   int64_t prefix_len, const int64_t* prefix_lens, int64_t S_, int64_t cache_len,
+                                   const int64_t* cache_lens, void* workspace, int64_t workspace_bytes) {
+  CHECK_DTYPE(dtype);
+  MINITP_CHECK_ARG(B >= 0 && T >= 0 && Hq > 0 && Hkv > 0 && D > 0 && prefix_len >= 0 && cache_len >= 0,
+                   "shared_prefix_attention: bad shape");
+  MINITP_CHECK_ARG(G > 0, "shared_prefix_attention: %lld groups", (long long)G);
+  if (Hq % Hkv != 0 || B % G != 0) {
+    set_error(Hq % Hkv != 0 ? "local q heads %lld not divisible by local kv heads %lld"
+                            : "shared_prefix_attention: batch rows %lld not divisible by groups %lld",
+              (long long)(Hq % Hkv != 0 ? Hq : B), (long long)(Hq % Hkv != 0 ? Hkv : G));
+    return MINITP_ERR_DIVISIBLE;
+  }
+  if (cache_len + T > S_ || prefix_len > S_prefix) {
+    if (prefix_len > S_prefix)
+      set_error("KV cache overflow: prefix %lld > prefix rows %lld", (long long)prefix_len, (long long)S_prefix);
+    else
+      set_error("KV cache overflow: seq %lld+%lld > max_seq_len=%lld", (long long)cache_len, (long long)T,
+                (long long)S_);
+    return MINITP_ERR_OVERFLOW;
+  }
+  if (B * T == 0) return MINITP_OK;
+  MINITP_CHECK_ARG(q && k_cache && v_cache && out && (prefix_len == 0 || (k_prefix && v_prefix)),
+                   "shared_prefix_attention: NULL pointer");
+  MINITP_CHECK_ARG(D % vec_elems(dtype) == 0 && aligned16(q) && aligned16(out) && aligned16(k_cache) &&
+                       aligned16(v_cache) && (prefix_len == 0 || (aligned16(k_prefix) && aligned16(v_prefix))),
+                   "shared_prefix_attention: head_dim rows must be 16-byte aligned");
+  const SharedPrefixShape s{B, G, T, Hq, Hkv, D, S_prefix, S_, prefix_len, cache_len};
+  return launch_shared_prefix_attention(S(stream), dtype, s, q, k_prefix, v_prefix, k_cache, v_cache, out, prefix_lens,
+                                        cache_lens, workspace, workspace_bytes);
+}
+
+int64_t minitp_beam_select_workspace_bytes(int64_t G, int64_t W, int64_t V) {
+  if (G < 0 || W < 1 || W > BEAM_MAX || V <= 0) return -1;
+  return beam_select_workspace_bytes(G, W, V);
+}
+
+int minitp_beam_select(void* stream, int dtype, const void* logits, int64_t ld_group, int64_t ld_beam, int64_t G,
+                       int64_t W, int64_t V, const float* scores, const uint8_t* finished, const int64_t* lengths,
+                       int64_t eos_token, double length_penalty, int64_t* tokens, int64_t* parents, float* scores_out,
+                       uint8_t* finished_out, int64_t* lengths_out, void* workspace, int64_t workspace_bytes) {
+  CHECK_DTYPE(dtype);
+  MINITP_CHECK_ARG(G >= 0 && V > 0 && V < (1LL << 31) && ld_group >= 0 && ld_beam >= 0,
+                   "beam_select: G=%lld V=%lld ld=%lld/%lld", (long long)G, (long long)V, (long long)ld_group,
+                   (long long)ld_beam);
+  MINITP_CHECK_ARG(W >= 1 && W <= BEAM_MAX, "beam_select: %lld beams a group (1 to %d)", (long long)W, BEAM_MAX);
+  MINITP_CHECK_ARG(eos_token >= -1 && eos_token < V, "beam_select: eos_token %lld of %lld tokens",
+                   (long long)eos_token, (long long)V);
+  MINITP_CHECK_ARG(finished == nullptr || eos_token >= 0, "beam_select: finished beams need an eos_token");
+  MINITP_CHECK_ARG(std::isfinite(length_penalty), "beam_select: length_penalty %f", length_penalty);
+  if (G == 0) return MINITP_OK;
+  MINITP_CHECK_ARG(logits && scores && tokens && parents && scores_out && finished_out && lengths_out,
+                   "beam_select: NULL pointer");
+  const BeamSelect b{logits,         ld_group, ld_beam, G,          W,            V,          scores, finished, lengths, eos_token,
+                     length_penalty, tokens,   parents, scores_out, finished_out, lengths_out};
+  return launch_beam_select(S(stream), dtype, b, workspace, workspace_bytes);
+}
+
+int minitp_kv_reorder(void* stream, int dtype, void* k_cache, void* v_cache, int64_t L, int64_t G, int64_t W,
+                      int64_t Hkv, int64_t S_, int64_t D, int64_t rows, const int64_t* parents) {
+  CHECK_DTYPE(dtype);
+  MINITP_CHECK_ARG(L >= 0 && G >= 0 && Hkv >= 0 && D > 0 && S_ >= 0 && rows >= 0, "kv_reorder: bad shape");
+  MINITP_CHECK_ARG(W >= 1 && W <= BEAM_MAX, "kv_reorder: %lld beams a group (1 to %d)", (long long)W, BEAM_MAX);
+  if (rows > S_) {
+    set_error("KV cache overflow: %lld rows > max_seq_len=%lld", (long long)rows, (long long)S_);
+    return MINITP_ERR_OVERFLOW;
+  }
+  if (L * G * Hkv * rows == 0) return MINITP_OK;
+  MINITP_CHECK_ARG(k_cache && v_cache && parents, "kv_reorder: NULL pointer");
+  MINITP_CHECK_ARG(D % vec_elems(dtype) == 0 && aligned16(k_cache) && aligned16(v_cache),
+                   "kv_reorder: head_dim rows must be 16-byte aligned");
+  return launch_kv_reorder(S(stream), dtype, k_cache, v_cache, L, G, W, Hkv, S_, D, rows, parents);
 }
 
 int64_t minitp_argmax_workspace_bytes(int64_t B, int64_t V) {

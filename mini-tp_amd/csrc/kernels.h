@@ -280,6 +280,41 @@ int launch_argmax(hipStream_t st, int dtype, const void* logits, int64_t ld, int
                   int64_t out_stride, void* workspace, int64_t workspace_bytes, const StepState* state = nullptr,
                   int64_t row_offset = 0);
 
+// shared_prefix.hip: attention of G groups of B / G rows, each group over the P
+// rows of its prefix and each row over C + T rows of its own (layouts and
+// optional per-group / per-row lengths: minitp_shared_prefix_attention).
+struct SharedPrefixShape {
+  int64_t B, G, T, Hq, Hkv, D;
+  int64_t Sp, S;  // rows per (group, KV head) of the prefix buffers, per (row, KV head) of the caches
+  int64_t P, C;   // prefix rows, cached own rows
+};
+int64_t shared_prefix_workspace_bytes(int dtype, int64_t B, int64_t G, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
+                                      int64_t P, int64_t C);
+int launch_shared_prefix_attention(hipStream_t st, int dtype, const SharedPrefixShape& s, const void* q,
+                                   const void* k_prefix, const void* v_prefix, const void* k_cache,
+                                   const void* v_cache, void* out, const int64_t* prefix_lens,
+                                   const int64_t* cache_lens, void* workspace, int64_t workspace_bytes);
+
+// beam.hip
+constexpr int BEAM_MAX = 32;  // beams of a group
+struct BeamSelect {
+  const void* logits;
+  int64_t ld_group, ld_beam, G, W, V;
+  const float* scores;
+  const uint8_t* finished;
+  const int64_t* lengths;
+  int64_t eos;
+  double alpha;
+  int64_t *tokens, *parents;
+  float* scores_out;
+  uint8_t* finished_out;
+  int64_t* lengths_out;
+};
+int64_t beam_select_workspace_bytes(int64_t G, int64_t W, int64_t V);
+int launch_beam_select(hipStream_t st, int dtype, const BeamSelect& b, void* workspace, int64_t workspace_bytes);
+int launch_kv_reorder(hipStream_t st, int dtype, void* k, void* v, int64_t L, int64_t G, int64_t W, int64_t Hkv,
+                      int64_t S, int64_t D, int64_t rows, const int64_t* parents);
+
 // Raise the dynamic-LDS limit of a kernel once (needed above 64 KiB).
 int ensure_lds_limit(const void* kernel, int bytes);
 

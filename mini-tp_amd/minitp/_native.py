@@ -58,6 +58,13 @@ SIGNATURES = {
     "minitp_attention_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64]),
     "minitp_attention": (_int, [_vp, _int, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp,
                                 _i64]),
+    "minitp_shared_prefix_attention_workspace_bytes": (_i64, [_int, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64]),
+    "minitp_shared_prefix_attention": (_int, [_vp, _int, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64,
+                                              _i64, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64]),
+    "minitp_beam_select_workspace_bytes": (_i64, [_i64, _i64, _i64]),
+    "minitp_beam_select": (_int, [_vp, _int, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _f64, _vp, _vp,
+                                  _vp, _vp, _vp, _vp, _i64]),
+    "minitp_kv_reorder": (_int, [_vp, _int, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp]),
     "minitp_argmax_workspace_bytes": (_i64, [_i64, _i64]),
     "minitp_argmax": (_int, [_vp, _int, _vp, _i64, _i64, _i64, _vp, _i64, _vp, _i64]),
     "minitp_argmax_static_max_bytes": (_i64, []),

@@ -7,6 +7,7 @@ caller passes them. Launches go to torch's current stream.
 from __future__ import annotations
 
 import functools
+from typing import NamedTuple
 
 import torch
 
@@ -311,6 +312,178 @@ def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, cac
                                     v_cache.data_ptr(), out.data_ptr(), b, t, hq, hkv, d, s, cache_len, ws.data_ptr(),
                                     ws.numel()), "attention")
     return out
+
+
+def _one_device(what: str, *tensors: torch.Tensor | None) -> torch.device:
+    """The device that all of a call's tensors live on."""
+    N.require_gpu(*tensors, what=what)
+    dev = tensors[0].device
+    for t in tensors:
+        if t is not None and t.device != dev:
+            raise ValueError(f"{what}: tensors on {dev} and {t.device}")
+    return dev
+
+
+def _elsewhere(dev: torch.device) -> bool:
+    return dev.index != torch._C._cuda_getDevice()
+
+
+def _cache_view(what: str, k: torch.Tensor, v: torch.Tensor, batch: int, hkv: int, d: int, dtype: torch.dtype) -> int:
+    """Row stride of a [batch, hkv, S, d] cache pair (cache_rows), its sizes checked."""
+    for c in (k, v):
+        if c.dim() != 4 or c.shape[0] != batch or c.shape[1] != hkv or c.shape[3] != d:
+            raise ValueError(f"{what}: K/V rows {tuple(c.shape)}, expected [{batch}, {hkv}, S, {d}]")
+        if c.dtype != dtype:
+            raise TypeError(f"{what}: dtype mismatch {c.dtype} and {dtype}")
+    if k.shape != v.shape:
+        raise ValueError(f"{what}: K {tuple(k.shape)} and V {tuple(v.shape)} differ")
+    return cache_rows(k, v)
+
+
+def _lens(what: str, lens: torch.Tensor | None, count: int) -> torch.Tensor | None:
+    if lens is None:
+        return None
+    if lens.shape != (count,) or lens.is_floating_point() or lens.dtype == torch.bool:
+        raise ValueError(f"{what}: lengths {tuple(lens.shape)} {lens.dtype}, expected {count} whole numbers")
+    return lens.to(torch.long).contiguous()
+
+
+def shared_prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Tensor, k_cache: torch.Tensor,
+                            v_cache: torch.Tensor, prefix_len: int, cache_len: int,
+                            prefix_lens: torch.Tensor | None = None,
+                            cache_lens: torch.Tensor | None = None) -> torch.Tensor:
+    """``attention`` for a batch whose rows share prefixes: q [B, T, Hq, D] ->
+    [B, T, Hq * D].
+
+    The B rows form G groups of consecutive rows. ``k_prefix`` / ``v_prefix``
+    [G, Hkv, >= prefix_len, D] hold each group's common rows once; the caches
+    [B, Hkv, S, D] hold ``cache_len`` rows of each row's own and then its T new
+    ones. Query t of a row attends its group's whole prefix and its own rows up
+    to its new row t. ``prefix_lens`` [G] and ``cache_lens`` [B] (whole
+    numbers on the device) shorten single prefixes and rows: row b's new
+    tokens are then its rows cache_lens[b] .. + T - 1. A negative
+    ``cache_lens[b]`` marks an idle row, which gets zeros. Rows past these
+    lengths are never read."""
+    what = "shared_prefix_attention"
+    dev = _one_device(what, q, k_prefix, v_prefix, k_cache, v_cache, prefix_lens, cache_lens)
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return shared_prefix_attention(q, k_prefix, v_prefix, k_cache, v_cache, prefix_len, cache_len, prefix_lens,
+                                           cache_lens)
+    if q.dim() != 4 or k_cache.dim() != 4 or k_prefix.dim() != 4:
+        raise ValueError(f"{what}: q {tuple(q.shape)}, prefix {tuple(k_prefix.shape)}, cache {tuple(k_cache.shape)}")
+    b, t, hq, d = q.shape
+    hkv, groups = k_cache.shape[1], k_prefix.shape[0]
+    s = _cache_view(what, k_cache, v_cache, b, hkv, d, q.dtype)
+    sp = _cache_view(what, k_prefix, v_prefix, groups, hkv, d, q.dtype)
+    if cache_len + t > k_cache.shape[2]:
+        raise ValueError(f"KV cache overflow: seq {cache_len}+{t} > max_seq_len={k_cache.shape[2]}")
+    if prefix_len > k_prefix.shape[2]:
+        raise ValueError(f"KV cache overflow: prefix {prefix_len} > prefix rows {k_prefix.shape[2]}")
+    plens, clens = _lens(what, prefix_lens, groups), _lens(what, cache_lens, b)
+    q = q.contiguous()
+    out = torch.empty(b, t, hq * d, dtype=q.dtype, device=dev)
+    dt = N.dtype_code(q.dtype)
+    nbytes = _shared_prefix_bytes(dev, dt, b, groups, t, hq, hkv, d, prefix_len, cache_len)
+    # from the caching allocator on the current stream: calls on other streams
+    # and captured graphs have scratch of their own
+    ws = torch.empty(max(nbytes, 0), dtype=torch.uint8, device=dev)
+    N.check(_lib().minitp_shared_prefix_attention(
+        N.stream(), dt, q.data_ptr(), k_prefix.data_ptr(), v_prefix.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+        out.data_ptr(), b, groups, t, hq, hkv, d, sp, prefix_len, N.ptr(plens), s, cache_len, N.ptr(clens),
+        ws.data_ptr(), ws.numel()), what)
+    return out
+
+
+@functools.lru_cache(maxsize=4096)
+def _shared_prefix_bytes(device: torch.device, *sizes: int) -> int:
+    return _lib().minitp_shared_prefix_attention_workspace_bytes(*sizes)
+
+
+class BeamStep(NamedTuple):
+    """The beams after one step of ``beam_select``, all [G, W]."""
+
+    tokens: torch.Tensor    # long: the token that each beam appends
+    parents: torch.Tensor   # long: the batch row (g * W + w) that each beam continues
+    scores: torch.Tensor    # float32 cumulative log-probabilities
+    finished: torch.Tensor  # bool
+    lengths: torch.Tensor   # long: tokens so far, the end token among them
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: torch.Tensor | None = None,
+                lengths: torch.Tensor | None = None, *, eos_token_id: int | None = None,
+                length_penalty: float = 0.0) -> BeamStep:
+    """One step of beam search for G groups of W beams (at most 32).
+
+    logits [G, W, V] or [G * W, V] (rows of any strides, expanded ones too) of
+    the beams whose cumulative log-probabilities are ``scores`` [G, W] float32
+    (-inf: no beam in this slot). Of the continuations score + log_softmax(x)
+    of a group, a finished beam's only one being ``eos_token_id`` at its own
+    score, the W of the largest score / length ** length_penalty win, equal
+    ones by the lower (beam, token). The first winner of a parent stays in its
+    slot, the others fill the free slots in rank order; a slot left over holds
+    no beam (-inf, finished)."""
+    what = "beam_select"
+    dev = _one_device(what, logits, scores, finished, lengths)
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return beam_select(logits, scores, finished, lengths, eos_token_id=eos_token_id,
+                               length_penalty=length_penalty)
+    if scores.dim() != 2 or scores.dtype != torch.float32:
+        raise ValueError(f"{what}: scores {tuple(scores.shape)} {scores.dtype}, expected [G, W] float32")
+    groups, beams = scores.shape
+    if logits.dim() == 2 and logits.shape[0] == groups * beams:
+        logits = logits.unflatten(0, (groups, beams))
+    if logits.dim() != 3 or logits.shape[:2] != scores.shape:
+        raise ValueError(f"{what}: logits {tuple(logits.shape)} for scores {tuple(scores.shape)}")
+    for name, t, dtype in (("finished", finished, torch.bool), ("lengths", lengths, torch.long)):
+        if t is not None and (t.shape != scores.shape or t.dtype != dtype):
+            raise ValueError(f"{what}: {name} {tuple(t.shape)} {t.dtype}, expected {tuple(scores.shape)} {dtype}")
+    vocab = logits.shape[2]
+    if logits.stride(2) != 1 and vocab > 1:
+        logits = logits.contiguous()
+    scores = scores.contiguous()
+    finished = finished.contiguous() if finished is not None else None
+    lengths = lengths.contiguous() if lengths is not None else None
+    whole = torch.empty(3, groups, beams, dtype=torch.long, device=dev)
+    tokens, parents, new_lengths = whole.unbind(0)
+    new_scores = torch.empty_like(scores)
+    new_finished = torch.empty(groups, beams, dtype=torch.bool, device=dev)
+    ws = torch.empty(max(_beam_select_bytes(dev, groups, beams, vocab), 0), dtype=torch.uint8, device=dev)
+    N.check(_lib().minitp_beam_select(
+        N.stream(), N.dtype_code(logits.dtype), logits.data_ptr(), logits.stride(0), logits.stride(1), groups, beams,
+        vocab, scores.data_ptr(), N.ptr(finished), N.ptr(lengths), -1 if eos_token_id is None else eos_token_id,
+        float(length_penalty), tokens.data_ptr(), parents.data_ptr(), new_scores.data_ptr(), new_finished.data_ptr(),
+        new_lengths.data_ptr(), ws.data_ptr(), ws.numel()), what)
+    return BeamStep(tokens, parents, new_scores, new_finished, new_lengths)
+
+
+@functools.lru_cache(maxsize=4096)
+def _beam_select_bytes(device: torch.device, *sizes: int) -> int:
+    return _lib().minitp_beam_select_workspace_bytes(*sizes)
+
+
+def kv_reorder(k_buf: torch.Tensor, v_buf: torch.Tensor, parents: torch.Tensor, rows: int) -> None:
+    """The K/V caches follow the beams, in place: rows [0, rows) of every layer
+    and KV head of batch row b of the buffers [L, B, Hkv, S, D] become those of
+    row parents[b]. ``parents`` [G, W], G * W == B, W at most 32, holds batch
+    rows; one outside the row's own group leaves the row as it is."""
+    what = "kv_reorder"
+    dev = _one_device(what, k_buf, v_buf, parents)
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return kv_reorder(k_buf, v_buf, parents, rows)
+    if k_buf.dim() != 5 or k_buf.shape != v_buf.shape or k_buf.dtype != v_buf.dtype:
+        raise ValueError(f"{what}: buffers {tuple(k_buf.shape)} {k_buf.dtype} and {tuple(v_buf.shape)} {v_buf.dtype}")
+    if not (k_buf.is_contiguous() and v_buf.is_contiguous()):
+        raise ValueError(f"{what}: the cache buffers must be contiguous [L, B, Hkv, S, D]")
+    if parents.dim() != 2 or parents.numel() != k_buf.shape[1] or parents.dtype != torch.long:
+        raise ValueError(f"{what}: parents {tuple(parents.shape)} {parents.dtype}, expected [G, W] int64 for "
+                         f"{k_buf.shape[1]} batch rows")
+    layers, _, hkv, s, d = k_buf.shape
+    parents = parents.contiguous()
+    N.check(_lib().minitp_kv_reorder(N.stream(), N.dtype_code(k_buf.dtype), k_buf.data_ptr(), v_buf.data_ptr(), layers,
+                                     parents.shape[0], parents.shape[1], hkv, s, d, rows, parents.data_ptr()), what)
 
 
 def argmax(logits: torch.Tensor) -> torch.Tensor:

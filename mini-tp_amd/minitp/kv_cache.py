@@ -43,6 +43,7 @@ class KVCache:
         self.v_buf = torch.empty(shape, dtype=dtype, device=device)
         if init == "zeros":
             self._fill(0.0)
+        self.prefix: KVCache | None = None  # rows that groups of this cache's batch rows share (share_prefix)
         self.k = [t[:, :, :max_seq_len] for t in self.k_buf.unbind(0)]
         self.v = [t[:, :, :max_seq_len] for t in self.v_buf.unbind(0)]
 
@@ -65,6 +66,28 @@ class KVCache:
     def check_room(self, t: int) -> None:
         if self.seq_len + t > self.max_seq_len:
             raise ValueError(f"KV cache overflow: seq {self.seq_len}+{t} > max_seq_len={self.max_seq_len}")
+
+    def share_prefix(self, prefix: "KVCache") -> None:
+        """Put ``prefix`` in front of this cache: every run of batch / (prefix
+        batch) consecutive rows here continues one row of ``prefix``, whose
+        rows [0, prefix.seq_len) are kept once and attended by all of them (no
+        counterpart in the reference, whose caches hold a prompt per row)."""
+        mine, shared = self.k_buf.shape, prefix.k_buf.shape
+        if prefix.prefix is not None or prefix is self:
+            raise ValueError("a shared prefix cannot have a prefix of its own")
+        if mine[0] != shared[0] or mine[2] != shared[2] or mine[4] != shared[4] or \
+                prefix.k_buf.dtype != self.k_buf.dtype or prefix.k_buf.device != self.k_buf.device:
+            raise ValueError(f"prefix cache {tuple(shared)} {prefix.k_buf.dtype} on {prefix.k_buf.device} does not fit "
+                             f"{tuple(mine)} {self.k_buf.dtype} on {self.k_buf.device}")
+        if shared[1] == 0 or mine[1] % shared[1] != 0:
+            raise ValueError(f"batch {mine[1]} not divisible by the prefix cache's batch {shared[1]}")
+        self.prefix = prefix
+
+    def reorder(self, parents: torch.Tensor) -> None:
+        """The written rows follow their beams, in place: batch row b of every
+        layer takes the rows of batch row parents[b] (``kernels.kv_reorder``;
+        parents [G, W] int64, beams of a group). A shared prefix stays."""
+        K.kv_reorder(self.k_buf, self.v_buf, parents, self.seq_len)
 
     def advance(self, tokens: int) -> None:
         self.seq_len += tokens

@@ -1,0 +1,110 @@
+"""Refusals of the beam-search and shared-prefix entry points: every invalid
+call is turned down on the host, before any pointer is used (no GPU)."""
+
+import math
+
+import pytest
+import torch
+
+from minitp import _native as N
+from minitp import kernels as K
+
+P = 4096  # a 16-byte aligned address that no refused call looks at
+
+
+def attention(dtype=N.BF16, q=P, kp=P, vp=P, kc=P, vc=P, out=P, b=4, g=2, t=1, hq=4, hkv=2, d=64, sp=32, p=32, plens=None,
+              s=16, c=10, clens=None, ws=P, nbytes=1 << 30):
+    return N.lib().minitp_shared_prefix_attention(None, dtype, q, kp, vp, kc, vc, out, b, g, t, hq, hkv, d, sp, p, plens,
+                                                  s, c, clens, ws, nbytes)
+
+
+@pytest.mark.parametrize("status,change", [
+    (N.ERR_ARG, dict(dtype=2)), (N.ERR_ARG, dict(q=None)), (N.ERR_ARG, dict(kp=None)), (N.ERR_ARG, dict(vc=None)),
+    (N.ERR_ARG, dict(out=None)), (N.ERR_ARG, dict(g=0)), (N.ERR_ARG, dict(g=-2)), (N.ERR_ARG, dict(b=-4)),
+    (N.ERR_ARG, dict(t=-1)), (N.ERR_ARG, dict(p=-1)), (N.ERR_ARG, dict(c=-1)), (N.ERR_ARG, dict(hkv=0)),
+    (N.ERR_ARG, dict(d=12)), (N.ERR_ARG, dict(d=0)), (N.ERR_ARG, dict(q=P + 8)), (N.ERR_ARG, dict(kc=P + 2)),
+    (N.ERR_ARG, dict(vp=P + 4)), (N.ERR_ARG, dict(ws=None)), (N.ERR_ARG, dict(nbytes=64)), (N.ERR_ARG, dict(ws=P + 4)),
+    (N.ERR_DIVISIBLE, dict(hq=5)), (N.ERR_DIVISIBLE, dict(b=5)), (N.ERR_OVERFLOW, dict(c=16)),
+    (N.ERR_OVERFLOW, dict(t=7)), (N.ERR_OVERFLOW, dict(p=33)), (N.ERR_UNSUPPORTED, dict(d=256)),
+    (N.ERR_UNSUPPORTED, dict(d=40)),
+])
+def test_shared_prefix_attention_refuses(status, change):
+    assert attention(**change) == status and N.last_error()
+
+
+def test_shared_prefix_attention_of_nothing():
+    assert attention(b=0) == N.OK and attention(t=0) == N.OK
+    size = N.lib().minitp_shared_prefix_attention_workspace_bytes
+    assert size(N.F32, 0, 1, 1, 4, 2, 64, 10, 10) == 0
+    assert size(N.F32, 4, 2, 1, 4, 2, 64, 0, 0) > 0
+    for bad in ((5, 4, 2, 1, 4, 2, 64, 1, 1), (0, 4, 3, 1, 4, 2, 64, 1, 1), (0, 4, 2, 1, 3, 2, 64, 1, 1),
+                (0, 4, 0, 1, 4, 2, 64, 1, 1), (0, 4, 2, 1, 4, 2, 64, -1, 1)):
+        assert size(*bad) == -1
+
+
+def select(dtype=N.F32, logits=P, ldg=800, ldb=100, g=2, w=8, v=100, scores=P, finished=None, lengths=None, eos=-1,
+           alpha=0.0, outs=(P,) * 5, ws=P, nbytes=1 << 30):
+    return N.lib().minitp_beam_select(None, dtype, logits, ldg, ldb, g, w, v, scores, finished, lengths, eos, alpha, *outs,
+                                      ws, nbytes)
+
+
+@pytest.mark.parametrize("change", [
+    dict(dtype=7), dict(logits=None), dict(scores=None), dict(outs=(P, P, None, P, P)), dict(w=0), dict(w=33), dict(g=-1),
+    dict(v=0), dict(v=1 << 31), dict(ldg=-1), dict(ldb=-5), dict(eos=-2), dict(eos=100), dict(finished=P),
+    dict(alpha=math.nan), dict(alpha=math.inf), dict(ws=None), dict(nbytes=100), dict(ws=P + 8),
+])
+def test_beam_select_refuses(change):
+    assert select(**change) == N.ERR_ARG and N.last_error()
+
+
+def test_beam_select_of_nothing():
+    assert select(g=0) == N.OK
+    size = N.lib().minitp_beam_select_workspace_bytes
+    assert size(1, 33, 10) == size(1, 0, 10) == size(-1, 4, 10) == size(1, 4, 0) == -1 and size(1, 4, 10) > 0
+
+
+def reorder(dtype=N.BF16, k=P, v=P, layers=2, g=2, w=4, hkv=2, s=32, d=64, rows=10, parents=P):
+    return N.lib().minitp_kv_reorder(None, dtype, k, v, layers, g, w, hkv, s, d, rows, parents)
+
+
+@pytest.mark.parametrize("status,change", [
+    (N.ERR_ARG, dict(dtype=-1)), (N.ERR_ARG, dict(k=None)), (N.ERR_ARG, dict(parents=None)), (N.ERR_ARG, dict(w=0)),
+    (N.ERR_ARG, dict(w=33)), (N.ERR_ARG, dict(rows=-1)), (N.ERR_ARG, dict(layers=-1)), (N.ERR_ARG, dict(d=12)),
+    (N.ERR_ARG, dict(v=P + 8)), (N.ERR_OVERFLOW, dict(rows=33)), (N.ERR_UNSUPPORTED, dict(layers=1 << 16)),
+    (N.ERR_UNSUPPORTED, dict(g=1 << 16)), (N.ERR_UNSUPPORTED, dict(s=1 << 30, rows=1 << 29)),
+])
+def test_kv_reorder_refuses(status, change):
+    assert reorder(**change) == status and N.last_error()
+
+
+def test_kv_reorder_of_nothing():
+    assert reorder(rows=0, k=None, v=None, parents=None) == N.OK
+    assert reorder(layers=0) == N.OK and reorder(g=0) == N.OK
+
+
+def test_wrappers_have_no_cpu_path():
+    x = torch.zeros(2, 1, 4, 16)
+    with pytest.raises(RuntimeError, match="ROCm GPU"):
+        K.shared_prefix_attention(x, x, x, x, x, 1, 0)
+    with pytest.raises(RuntimeError, match="ROCm GPU"):
+        K.beam_select(torch.zeros(1, 2, 8), torch.zeros(1, 2))
+    with pytest.raises(RuntimeError, match="ROCm GPU"):
+        K.kv_reorder(torch.zeros(1, 2, 1, 4, 16), torch.zeros(1, 2, 1, 4, 16), torch.zeros(1, 2, dtype=torch.long), 1)
+
+
+def test_share_prefix_checks_the_caches():
+    from minitp.kv_cache import KVCache
+
+    def cache(layers=2, batch=4, heads=2, d=16, dtype=torch.float32):
+        return KVCache(layers, batch, heads, d, 8, dtype, torch.device("cpu"))
+
+    kv = cache(batch=6)
+    assert kv.prefix is None
+    for bad in (cache(layers=1), cache(heads=1), cache(d=32), cache(dtype=torch.bfloat16), cache(batch=4), kv):
+        with pytest.raises(ValueError):
+            kv.share_prefix(bad)
+    good = cache(batch=3)
+    kv.share_prefix(good)
+    assert kv.prefix is good
+    with pytest.raises(ValueError):
+        cache(batch=12).share_prefix(kv)
