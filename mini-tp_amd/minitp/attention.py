@@ -2,7 +2,8 @@
 
 Module-level path: packed QKV projection, one kernel that splits q/k/v,
 applies RoPE and writes k/v into the cache, GQA attention reading KV head
-h // (Hq/Hkv) directly (no repeat_interleave copy), then o_proj.
+h // (Hq/Hkv) directly (no repeat_interleave copy), then o_proj. A cache with a
+shared prefix (KVCache.share_prefix) takes the shared-prefix attention instead.
 """
 
 from __future__ import annotations
@@ -60,5 +61,9 @@ class TPQwen2Attention(nn.Module):
             pos = torch.arange(t, device=x.device)
         q = torch.empty(b, t, hq, d, dtype=x.dtype, device=x.device)
         K.rope_kv_write(y, q, kc, vc, cos, sin, pos, hq, hkv, cache_len)
-        out = K.attention(q, kc, vc, cache_len)
+        if kv_cache is not None and kv_cache.prefix is not None:
+            pre = kv_cache.prefix
+            out = K.shared_prefix_attention(q, pre.k[layer_idx], pre.v[layer_idx], kc, vc, pre.seq_len, cache_len)
+        else:
+            out = K.attention(q, kc, vc, cache_len)
         return self.o_proj(out)

@@ -87,11 +87,12 @@ class GenerationState:
         device = input_ids.device
         self.out_ids = torch.empty(b, self.total, dtype=torch.long, device=device)
         self.out_ids[:, :t] = input_ids
-        self.positions_buf = torch.arange(self.total, device=device)  # the only arange
+        start = self.kv.prefix.seq_len if self.kv.prefix is not None else 0  # positions continue a shared prefix
+        self.positions_buf = torch.arange(start, start + self.total, device=device)  # the only arange
         self.cursor = t
         self.finished: torch.Tensor | None = None
         self.eos = -1
-        self._native = model.native_path() and device.type == "cuda"
+        self._native = model.native_path() and device.type == "cuda" and self.kv.prefix is None
         self._last_logits: torch.Tensor | None = None
         self._last_tok: torch.Tensor | None = None
         self._decode_logits: torch.Tensor | None = None
@@ -209,6 +210,72 @@ def generate_greedy(model: TPQwen2ForCausalLM, input_ids: torch.Tensor, max_new_
         if step + 1 < max_new_tokens:
             logits = state.decode_step(tok, pos)
     return state.out_ids[:, : state.cursor] if early_stop else state.out_ids
+
+
+EOS_BEAM_STEPS = 8  # steps between the host's looks at the finished flags of a beam search
+
+
+@torch.inference_mode()
+def generate_beam(model: TPQwen2ForCausalLM, input_ids: torch.Tensor, max_new_tokens: int, num_beams: int,
+                  eos_token_id: int | None = None, length_penalty: float = 0.0,
+                  early_stop: bool = True) -> tuple[torch.Tensor, torch.Tensor]:
+    """Beam search from prompts [B, T] (no counterpart in the reference, which
+    decodes greedily): (ids [B, num_beams, T + n], scores [B, num_beams]), best
+    first by score / length ** length_penalty, n = max_new_tokens, or with
+    ``early_stop`` the longest beam's tokens once every beam has finished.
+
+    A prompt's K/V rows are computed and kept once; its beams share them
+    (KVCache.share_prefix) and only their new rows follow the selection. A
+    beam that has produced ``eos_token_id`` stays a candidate with its score
+    and length and is padded with that token. scores are summed
+    log-probabilities; a beam that does not exist (fewer continuations than
+    beams) scores minus infinity."""
+    from minitp import kernels as K
+
+    b, t = input_ids.shape
+    if num_beams < 1 or max_new_tokens < 1:
+        raise ValueError(f"generate_beam: num_beams={num_beams}, max_new_tokens={max_new_tokens}")
+    limit = model.cfg.max_position_embeddings
+    if t + max_new_tokens - 1 > limit:  # the last token is selected, not forwarded
+        raise IndexError(f"position {t + max_new_tokens - 2} out of range for RoPE table of {limit} rows")
+    device, beams = input_ids.device, b * num_beams
+    prompt = make_kv_cache(model, b, t)
+    if model.native_path() and device.type == "cuda":
+        logits = model._native(input_ids, torch.arange(t, device=device), prompt, last_only=True)
+    else:
+        logits = model(input_ids, kv_cache=prompt)[:, -1:]
+    kv = make_kv_cache(model, beams, max_new_tokens)
+    kv.share_prefix(prompt)
+    logits = logits.expand(b, num_beams, -1)  # one beam a prompt so far
+    scores = torch.full((b, num_beams), float("-inf"), device=device)
+    scores[:, 0] = 0.0
+    lengths = torch.zeros(b, num_beams, dtype=torch.long, device=device)
+    finished = None if eos_token_id is None else torch.zeros(b, num_beams, dtype=torch.bool, device=device)
+    steps: list[K.BeamStep] = []
+    for step in range(max_new_tokens):
+        s = K.beam_select(logits, scores, finished, lengths, eos_token_id=eos_token_id, length_penalty=length_penalty)
+        steps.append(s)
+        scores, lengths = s.scores, s.lengths
+        if eos_token_id is not None:
+            finished = s.finished
+            if early_stop and (step + 1) % EOS_BEAM_STEPS == 0 and bool(finished.all()):
+                break
+        if step + 1 < max_new_tokens:
+            kv.reorder(s.parents)
+            logits = model(s.tokens.view(-1, 1), kv_cache=kv).view(b, num_beams, -1)
+    # the beams' tokens, from the last step back through the parents
+    out = torch.empty(beams, t + len(steps), dtype=torch.long, device=device)
+    row = torch.arange(beams, device=device)
+    for i in reversed(range(len(steps))):
+        out[:, t + i] = steps[i].tokens.view(-1)[row]
+        row = steps[i].parents.view(-1)[row]
+    out = out.view(b, num_beams, -1)
+    out[:, :, :t] = input_ids[:, None]
+    order = (scores.double() / lengths.clamp(min=1).double() ** length_penalty).sort(
+        dim=1, descending=True, stable=True).indices
+    if early_stop and eos_token_id is not None:
+        out = out[:, :, :t + int(lengths.max())]
+    return out.gather(1, order[:, :, None].expand_as(out)), scores.gather(1, order)
 
 
 def _generate_device_eos(state: GenerationState, eos: int, max_new_tokens: int) -> torch.Tensor:

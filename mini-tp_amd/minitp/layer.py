@@ -5,8 +5,8 @@
 toggles it runs the whole forward as one native program (libminitp's
 minitp_qwen2_forward: fused norm/QKV/RoPE/KV-write, attention, o_proj +
 residual, norm/gate-up/SwiGLU, down + residual per layer). When an ablation
-toggle is changed, or profiling labels are on, it walks the modules instead;
-that path runs the same kernels one op at a time.
+toggle is changed, profiling labels are on, or the cache has a shared prefix, it
+walks the modules instead; that path runs the same kernels one op at a time.
 """
 
 from __future__ import annotations
@@ -269,6 +269,8 @@ class TPQwen2ForCausalLM(nn.Module):
         limit = self.cfg.max_position_embeddings
         if positions is None:  # layer.py:99-101
             offset = kv_cache.seq_len if kv_cache is not None and t == 1 else 0
+            if kv_cache is not None and kv_cache.prefix is not None:  # (no counterpart in the reference)
+                offset = kv_cache.prefix.seq_len + kv_cache.seq_len
             if offset + t > limit:
                 raise IndexError(f"position {offset + t - 1} out of range for RoPE table of {limit} rows")
             positions = torch.arange(offset, offset + t, device=input_ids.device)
@@ -283,7 +285,7 @@ class TPQwen2ForCausalLM(nn.Module):
             positions = torch.where(positions < 0, positions + limit, positions)
         if kv_cache is not None:
             kv_cache.check_room(t)
-        if self.native_path():
+        if self.native_path() and (kv_cache is None or kv_cache.prefix is None):
             return self._native(input_ids, positions, kv_cache)
         x = self.model.embed_tokens(input_ids)
         rotary = self._ensure_rotary(x.device) if self.use_rotary_cache else None
