@@ -294,6 +294,398 @@ __global__ __launch_bounds__(256) void shared_attn_f32_kernel(SharedArgs a) {
       for (int j = 0; j < E; ++j) orow[64 * hf + E * (4 * lq + e) + j] = o[hf][j][e];
 }
 
+// ---------------------------------------------------------------------------
+// bf16, head dims 32, 64 and 128. A block takes 128 query rows of a unit over
+// the keys of its split, four waves of 32 rows (v_mfma_f32_32x32x16_bf16), or,
+// where the unit has at most 16 rows (one token of a row's own part), those
+// rows over 64 keys at a time, 16 keys a wave (16x16 MFMAs).
+//
+// A tile of 64 K and V rows goes to LDS as it lies in memory, by loads that
+// bypass the registers, while the tile before it is computed (two stages, one
+// barrier a tile). Products are transposed, S^T = K Q^T and O^T = V^T P^T, so
+// a lane's scores belong to one query: its maximum takes one lane exchange, its
+// sum none until the end, and its probabilities are the second product's
+// operand as they are, the k-index of both operands permuted alike. V^T comes
+// out of LDS transposed by ds_read_b64_tr_b16: in each group of 16 lanes, lane
+// i gives the address of four columns of row i / 4 and receives column i of
+// the four rows.
+//
+// The 16-byte chunks of a row are permuted by its row number, which the loads
+// do on the global side, so that every LDS read reaches all banks: a K read
+// takes one chunk column of 16 rows, a V read 64 bytes of four rows.
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+constexpr int H_QT = 128, H_KT = 64, H_SMALL = 16;
+
+template <int D>
+struct Half {
+  static constexpr int ROWB = D * 2, CH = D / 8;
+  static constexpr int OPER = H_KT * ROWB, STAGE = 2 * OPER, LDS = 2 * STAGE;
+  static constexpr int PIECE_ROWS = 64 / CH, PIECES = H_KT / PIECE_ROWS, PPW = PIECES / 4;  // 1 KiB loads
+  // chunk c of row r lies at chunk c ^ swz(r)
+  __device__ static int k_swz(int r) { return r * ROWB / 256 % CH; }
+  __device__ static int v_swz(int r) { return r * ROWB / 256 % 4 * 4 % CH; }
+};
+
+// 16 bytes a lane from the resource at voff to LDS at lds_addr + 16 lane
+// (m0, wave-uniform; zeros past the resource's end). asm, so that the compiler
+// does not wait for these loads at every LDS read: stage_wait does. The s_nop
+// is the wait state between the write of m0 and a load to LDS.
+__device__ __forceinline__ void row_dma16(u32x4 r, uint32_t voff, uint32_t lds_addr) {
+  asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(r), "{m0}"(lds_addr) : "memory");
+}
+__device__ __forceinline__ u32x4 rows_rsrc(const void* base, int64_t key, int64_t key_hi, int row_bytes) {
+  const uint64_t p = (uint64_t)base + key * row_bytes;
+  u32x4 r;
+  r.x = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)p);
+  r.y = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(p >> 32));
+  r.z = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)std::min<int64_t>(key_hi - key, H_KT) * row_bytes);
+  r.w = 0x00020000u;
+  return r;
+}
+// this wave's loads have landed and its LDS reads are done; then the block's
+__device__ __forceinline__ void stage_wait() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+__device__ __forceinline__ s16x4 read_tr(const char* p) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p));
+}
+__device__ __forceinline__ bf16x8 join8(s16x4 lo, s16x4 hi) {
+  return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+// maximum / sum over lanes l and l ^ 32 (and, for the 16-lane form, l ^ 16)
+__device__ __forceinline__ float halves_max(float v) {
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float halves_sum(float v) {
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+__device__ __forceinline__ float quads_max(float v) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return halves_max(fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1])));
+}
+__device__ __forceinline__ float quads_sum(float v) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return halves_sum(__uint_as_float(a[0]) + __uint_as_float(a[1]));
+}
+
+// Tiles of an item through the two stages; compute(k0, stage) for each.
+template <int D, typename F>
+__device__ __forceinline__ void over_tiles(const Item& it, char* lds, F&& compute) {
+  using H = Half<D>;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
+  // piece w + 4 j of a tile: rows 4 PIECE_ROWS j + row; the swizzles do not depend on j
+  const int row = H::PIECE_ROWS * w + lane / H::CH;
+  const uint32_t koff = row * H::ROWB + ((lane % H::CH) ^ H::k_swz(row)) * 16;
+  const uint32_t voff = row * H::ROWB + ((lane % H::CH) ^ H::v_swz(row)) * 16;
+  auto issue = [&](int64_t k0, int st) {
+    const u32x4 kr = rows_rsrc(it.k, k0, it.key_hi, H::ROWB), vr = rows_rsrc(it.v, k0, it.key_hi, H::ROWB);
+    const uint32_t to = lds0 + st * H::STAGE + w * 1024;
+#pragma unroll
+    for (int j = 0; j < H::PPW; ++j) row_dma16(kr, koff + j * 4096, to + j * 4096);
+#pragma unroll
+    for (int j = 0; j < H::PPW; ++j) row_dma16(vr, voff + j * 4096, to + H::OPER + j * 4096);
+  };
+  if (it.key_lo < it.key_hi) issue(it.key_lo, 0);
+  int st = 0;
+  for (int64_t k0 = it.key_lo; k0 < it.key_hi; k0 += H_KT, st ^= 1) {
+    stage_wait();
+    if (k0 + H_KT < it.key_hi) issue(k0 + H_KT, st ^ 1);  // (its readers passed the barrier)
+    compute(k0, lds + st * H::STAGE);
+  }
+}
+
+// The running maximum moves only when some lane's passes it by this much (base
+// 2): until then probabilities stay below 2^8 and nothing is rescaled.
+constexpr float SLACK = 8.f;
+
+template <int D>
+__device__ __forceinline__ void shared_rows128(const SharedArgs& a, const Item& it, char* lds) {
+  using H = Half<D>;
+  constexpr int KS = D / 16, DB = D / 32;
+  const int per = a.Hq / a.Hkv;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n32 = lane & 31, h = lane >> 5;
+  const int r0 = it.tile * H_QT + w * 32, r = r0 + n32;
+  const bool live = r < it.rows;
+  const int64_t n = it.n0 + (live ? r : 0) / per;
+  const int head = it.kv * per + (live ? r : 0) % per;
+  const int64_t seen = it.own ? it.seen + (n - it.n0) : INT64_MAX;  // the last key this query sees
+  const int64_t seen_first = it.own ? it.seen + r0 / per : INT64_MAX, seen_last = it.own ? it.seen + (r0 + 31) / per : INT64_MAX;
+
+  bf16x8 qb[KS];
+  {
+    const bf16* q = (const bf16*)a.q + (n * a.Hq + head) * D + 8 * h;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) qb[k] = __builtin_bit_cast(bf16x8, *(const uint4*)(q + 16 * k));
+  }
+  f32x16 o[DB];
+#pragma unroll
+  for (int d = 0; d < DB; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
+  float m = -__builtin_inff(), lsum = 0.f;
+  const float sl2 = a.scale * 1.4426950408889634f;
+
+  // LDS bytes of this lane's operands: K row n32, chunk 2 k + h; V rows
+  // 4 h + (lane % 16) / 4 (+ 8), dims 32 d + 16 ((lane / 16) % 2) + 4 (lane % 4)
+  const int kat = n32 * H::ROWB, kx = (h ^ H::k_swz(n32)) << 4;
+  const int vrow = 4 * h + (lane & 15) / 4;
+  const int vat = H::OPER + vrow * H::ROWB + 8 * (lane & 1);
+  const int vx = ((2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) ^ H::v_swz(vrow)) << 4;
+
+  over_tiles<D>(it, lds, [&](int64_t k0, const char* st) {
+    if (r0 >= it.rows || k0 > seen_last) return;
+    f32x16 s[2];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[kb][i] = 0.f;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        const bf16x8 kf = __builtin_bit_cast(bf16x8, *(const uint4*)(st + kat + kb * 32 * H::ROWB + ((32 * k) ^ kx)));
+        s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qb[k], s[kb], 0, 0, 0);
+      }
+    }
+    bool odd = false;
+    const int limit = (int)std::min<int64_t>(std::min<int64_t>(seen, it.key_hi - 1) - k0, H_KT);
+    if (k0 + H_KT - 1 > std::min<int64_t>(seen_first, it.key_hi - 1)) {
+      // some query does not see some key: lane (query, h) holds keys
+      // 32 kb + 8 (i / 4) + 4 h + i % 4
+      __asm__ volatile("");  // (a branch, not selects on every tile)
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (32 * kb + 8 * (i / 4) + i % 4 > limit - 4 * h) s[kb][i] = -__builtin_inff();
+      if (seen_first < it.key_hi - 1) {
+        // hidden keys that other queries see: are their values finite?
+        for (int c = lane; c < H_KT * H::CH; c += 64) {
+          const uint4 x = *(const uint4*)(st + H::OPER + c * 16);
+          const uint32_t wd[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            odd |= (wd[e] & 0x7f80u) == 0x7f80u || (wd[e] & 0x7f800000u) == 0x7f800000u;
+        }
+        odd = __builtin_amdgcn_ballot_w64(odd) != 0;
+      }
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kb][i]);
+    mx = halves_max(mx) * sl2;
+    if (__builtin_amdgcn_ballot_w64(mx > m + SLACK)) {
+      const float mn = fmaxf(m, mx), alpha = mn == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+      m = mn;
+      lsum *= alpha;
+#pragma unroll
+      for (int d = 0; d < DB; ++d) o[d] *= alpha;
+    }
+    const float mref = m == -__builtin_inff() ? 0.f : m;  // (nothing seen yet)
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[kb][i] = __builtin_amdgcn_exp2f(fmaf(s[kb][i], sl2, -mref));
+        lsum += s[kb][i];
+      }
+    if (odd) {
+      // a value that some query may not touch is not finite (0 times it is no
+      // zero): key by key, for the queries that see it
+#pragma unroll 1
+      for (int key = 0; key < H_KT; ++key) {
+        const int idx = (key >> 5) * 16 + ((key >> 3) & 3) * 4 + (key & 3);
+        float p = 0.f;
+#pragma unroll
+        for (int c = 0; c < 32; ++c) p = c == idx ? s[c / 16][c % 16] : p;
+        p = __shfl(p, n32 + 32 * ((key >> 2) & 1), 64);
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const uint2 x = *(const uint2*)(st + H::OPER + key * H::ROWB + (((4 * d + c) ^ H::v_swz(key)) << 4) + 8 * h);
+            const float v[4] = {__uint_as_float(x.x << 16), __uint_as_float(x.x & 0xffff0000u),
+                                __uint_as_float(x.y << 16), __uint_as_float(x.y & 0xffff0000u)};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[d][4 * c + e] = key <= limit ? fmaf(p, v[e], o[d][4 * c + e]) : o[d][4 * c + e];
+          }
+      }
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {  // keys 16 j .. 16 j + 15
+      const f32x16& p = s[j / 2];
+      const int b = 8 * (j % 2);
+      const bf16x8 pb = __builtin_bit_cast(bf16x8, make_uint4(pack_bf16x2(p[b], p[b + 1]), pack_bf16x2(p[b + 2], p[b + 3]),
+                                                              pack_bf16x2(p[b + 4], p[b + 5]), pack_bf16x2(p[b + 6], p[b + 7])));
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+        const char* vp = st + vat + 16 * j * H::ROWB + ((64 * d) ^ vx);
+        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(join8(read_tr(vp), read_tr(vp + 8 * H::ROWB)), pb, o[d], 0, 0, 0);
+      }
+    }
+  });
+  if (!live) return;
+  const float l = halves_sum(lsum);
+  const int64_t at = (int64_t)it.slot * a.B * a.T * a.Hq + n * a.Hq + head;
+  if (h == 0) *(float2*)(a.ml + at * 2) = make_float2(m, l);
+  float* orow = a.o + at * D + 4 * h;
+#pragma unroll
+  for (int d = 0; d < DB; ++d)
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      *(float4*)(orow + 32 * d + 8 * c) = make_float4(o[d][4 * c], o[d][4 * c + 1], o[d][4 * c + 2], o[d][4 * c + 3]);
+}
+
+template <int D>
+__device__ __forceinline__ void shared_rows16(const SharedArgs& a, const Item& it, char* lds) {
+  using H = Half<D>;
+  constexpr int KS = D / 32, DB = D / 16;
+  const int per = a.Hq / a.Hkv;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n16 = lane & 15, q4 = lane >> 4;
+  const int r = n16;  // (one tile)
+  const bool live = r < it.rows;
+  const int64_t n = it.n0 + (live ? r : 0) / per;
+  const int head = it.kv * per + (live ? r : 0) % per;
+  const int64_t seen = it.own ? it.seen + (n - it.n0) : INT64_MAX;
+
+  bf16x8 qb[KS];
+  {
+    const bf16* q = (const bf16*)a.q + (n * a.Hq + head) * D + 8 * q4;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) qb[k] = __builtin_bit_cast(bf16x8, *(const uint4*)(q + 32 * k));
+  }
+  f32x4 o[DB];
+#pragma unroll
+  for (int d = 0; d < DB; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m = -__builtin_inff(), lsum = 0.f;
+  const float sl2 = a.scale * 1.4426950408889634f;
+
+  // K row 16 w + n16, chunk 4 k + q4; V rows 16 w + 4 q4 + n16 / 4, dims 16 d + 4 (lane % 4)
+  const int krow = 16 * w + n16, kat = krow * H::ROWB, kx = (q4 ^ H::k_swz(krow)) << 4;
+  const int vrow = 16 * w + 4 * q4 + n16 / 4;
+  const int vat = H::OPER + vrow * H::ROWB + 8 * (lane & 1), vx = (((lane >> 1) & 1) ^ H::v_swz(vrow)) << 4;
+
+  over_tiles<D>(it, lds, [&](int64_t k0, const char* st) {
+    const int64_t kw = k0 + 16 * w;
+    if (kw >= it.key_hi) return;
+    f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      const bf16x8 kf = __builtin_bit_cast(bf16x8, *(const uint4*)(st + kat + ((64 * k) ^ kx)));
+      s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qb[k], s, 0, 0, 0);
+    }
+    const int limit = (int)std::min<int64_t>(std::min<int64_t>(seen, it.key_hi - 1) - kw, 16);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (4 * q4 + i > limit) s[i] = -__builtin_inff();
+    const float mx = quads_max(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]))) * sl2;
+    if (__builtin_amdgcn_ballot_w64(mx > m)) {
+      const float mn = fmaxf(m, mx), alpha = mn == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+      m = mn;
+      lsum *= alpha;
+#pragma unroll
+      for (int d = 0; d < DB; ++d) o[d] *= alpha;
+    }
+    const float mref = m == -__builtin_inff() ? 0.f : m;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], sl2, -mref));
+      lsum += s[i];
+    }
+    // (several tokens: a hidden key's value may not be finite)
+    if (__builtin_amdgcn_ballot_w64(limit < std::min<int64_t>(it.key_hi - 1 - kw, 15))) {
+      bool odd = false;
+      for (int c = lane; c < 16 * H::CH; c += 64) {
+        const uint4 x = *(const uint4*)(st + H::OPER + 16 * w * H::ROWB + c * 16);
+        const uint32_t wd[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) odd |= (wd[e] & 0x7f80u) == 0x7f80u || (wd[e] & 0x7f800000u) == 0x7f800000u;
+      }
+      if (__builtin_amdgcn_ballot_w64(odd)) {
+#pragma unroll 1
+        for (int key = 0; key < 16; ++key) {
+          const float pi = (key & 3) == 0 ? s[0] : (key & 3) == 1 ? s[1] : (key & 3) == 2 ? s[2] : s[3];
+          const float p = __shfl(pi, n16 + 16 * (key >> 2), 64);
+          const int row = 16 * w + key;
+#pragma unroll
+          for (int d = 0; d < DB; ++d) {
+            const uint2 x = *(const uint2*)(st + H::OPER + row * H::ROWB + (((2 * d + (q4 >> 1)) ^ H::v_swz(row)) << 4) +
+                                            8 * (q4 & 1));
+            const float v[4] = {__uint_as_float(x.x << 16), __uint_as_float(x.x & 0xffff0000u),
+                                __uint_as_float(x.y << 16), __uint_as_float(x.y & 0xffff0000u)};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[d][e] = key <= limit ? fmaf(p, v[e], o[d][e]) : o[d][e];
+          }
+        }
+        return;
+      }
+    }
+    const s16x4 pb = __builtin_bit_cast(s16x4, make_uint2(pack_bf16x2(s[0], s[1]), pack_bf16x2(s[2], s[3])));
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+      o[d] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(read_tr(st + vat + ((32 * d) ^ vx)), pb, o[d], 0, 0, 0);
+  });
+
+  // ---- the four waves' keys joined through LDS ------------------------------
+  const float l = quads_sum(lsum);
+  float* po = (float*)lds;             // [wave][16][D]
+  float* pml = po + 4 * H_SMALL * D;   // [wave][16][2]
+  __syncthreads();                     // (every stage is free)
+  if (live) {
+#pragma unroll
+    for (int d = 0; d < DB; ++d) *(f32x4*)(po + (w * H_SMALL + r) * D + 16 * d + 4 * q4) = o[d];
+    if (q4 == 0) *(float2*)(pml + (w * H_SMALL + r) * 2) = make_float2(m, l);
+  }
+  __syncthreads();
+  constexpr int LPR = D / 4;
+  for (int i = tid; i < it.rows * LPR; i += 256) {
+    const int row = i / LPR, d = i % LPR * 4;
+    float2 ml[4];
+    float mx = -__builtin_inff(), ls = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      ml[j] = *(const float2*)(pml + (j * H_SMALL + row) * 2);
+      mx = fmaxf(mx, ml[j].x);
+    }
+    f32x4 os = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float sc = ml[j].x == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(ml[j].x - mx);
+      ls = fmaf(sc, ml[j].y, ls);
+      const f32x4 oj = *(const f32x4*)(po + (j * H_SMALL + row) * D + d);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) os[e] = fmaf(sc, oj[e], os[e]);
+    }
+    const int64_t nn = it.n0 + row / per;
+    const int64_t at = (int64_t)it.slot * a.B * a.T * a.Hq + nn * a.Hq + it.kv * per + row % per;
+    *(f32x4*)(a.o + at * D + d) = os;
+    if (d == 0) *(float2*)(a.ml + at * 2) = make_float2(mx, ls);
+  }
+}
+
+template <int D>
+__global__ __launch_bounds__(256, 2) void shared_attn_bf16_kernel(SharedArgs a) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  static_assert(Half<D>::LDS >= 4 * H_SMALL * (D + 2) * 4, "the waves' join fits the stages");
+  const Item it = shared_item<H_QT, H_KT>(a, D * 2);
+  if (it.rows <= H_SMALL)
+    shared_rows16<D>(a, it, lds);
+  else
+    shared_rows128<D>(a, it, lds);
+}
+
 // The slots of each query row joined, in slot order (maxima in base 2). A
 // query that saw no key, in an idle row or one without any, gets zeros.
 template <typename T, int D>
@@ -307,15 +699,34 @@ __global__ __launch_bounds__(256) void shared_join_kernel(SharedArgs a) {
   const bool idle = own_len(a, i / a.Hq / a.T) < 0;
   float m = -__builtin_inff(), l = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < slots; ++s) {
-    const float2 ml = *(const float2*)(a.ml + (s * rows + i) * 2);
-    const f32x4 os = *(const f32x4*)(a.o + (s * rows + i) * D + d);
-    if (ml.x == -__builtin_inff()) continue;  // the split saw no key
-    const float mn = fmaxf(m, ml.x);
-    const float a0 = __builtin_amdgcn_exp2f(m - mn), a1 = __builtin_amdgcn_exp2f(ml.x - mn);
-    l = l * a0 + ml.y * a1;
+  constexpr int NB = 8;  // slots whose loads are in flight together
+  for (int s0 = 0; s0 < slots; s0 += NB) {
+    float2 ml[NB];
+    f32x4 os[NB];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = o[e] * a0 + os[e] * a1;
+    for (int u = 0; u < NB; ++u) {
+      const int64_t at = std::min(s0 + u, slots - 1) * rows + i;  // (past the last: read again, left out)
+      ml[u] = *(const float2*)(a.ml + at * 2);
+      os[u] = *(const f32x4*)(a.o + at * D + d);
+    }
+    float mn = m;
+#pragma unroll
+    for (int u = 0; u < NB; ++u) {
+      if (s0 + u >= slots) ml[u].x = -__builtin_inff();
+      mn = fmaxf(mn, ml[u].x);
+    }
+    if (mn == -__builtin_inff()) continue;  // no split so far saw a key
+    const float a0 = __builtin_amdgcn_exp2f(m - mn);
+    l *= a0;
+    o *= a0;
+#pragma unroll
+    for (int u = 0; u < NB; ++u) {
+      if (ml[u].x == -__builtin_inff()) continue;
+      const float a1 = __builtin_amdgcn_exp2f(ml[u].x - mn);
+      l = fmaf(ml[u].y, a1, l);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = fmaf(os[u][e], a1, o[e]);
+    }
     m = mn;
   }
   float r[4];
@@ -349,13 +760,23 @@ Plan shared_plan(int64_t B, int64_t G, int64_t T, int64_t Hq, int64_t Hkv, int64
   return p;
 }
 
+bool bf16_tiles(int dtype, int64_t D) { return dtype == MINITP_BF16 && D >= 32; }
+
 Plan plan_of(int dtype, int64_t D, int64_t B, int64_t G, int64_t T, int64_t Hq, int64_t Hkv, int64_t P, int64_t C) {
+  if (bf16_tiles(dtype, D)) return shared_plan(B, G, T, Hq, Hkv, P, C, H_QT, H_KT);
   return shared_plan(B, G, T, Hq, Hkv, P, C, F_QT, D >= 128 ? 32 : 64);
 }
 
 template <typename T, int D>
 int shared_launch(hipStream_t st, const SharedArgs& a, const Plan& p) {
-  hipLaunchKernelGGL((shared_attn_f32_kernel<T, D>), dim3((unsigned)(p.items_p + p.items_s)), dim3(256), 0, st, a);
+  const dim3 grid((unsigned)(p.items_p + p.items_s));
+  if constexpr (sizeof(T) == 2 && D >= 32) {
+    const int rc = ensure_lds_limit((const void*)shared_attn_bf16_kernel<D>, Half<D>::LDS);
+    if (rc) return rc;
+    hipLaunchKernelGGL(shared_attn_bf16_kernel<D>, grid, dim3(256), Half<D>::LDS, st, a);
+  } else {
+    hipLaunchKernelGGL((shared_attn_f32_kernel<T, D>), grid, dim3(256), 0, st, a);
+  }
   MINITP_LAUNCH_CHECK();
   const int64_t rows = (int64_t)a.B * a.T * a.Hq;
   hipLaunchKernelGGL((shared_join_kernel<T, D>), dim3((unsigned)cdiv(rows, 256 / (D / 4))), dim3(256), 0, st, a);
