@@ -13,6 +13,8 @@
 // once per batch row; the own part takes the T (Hq / Hkv) queries of one (row,
 // KV head). Work items are (part, unit, query tile, key split); each writes its
 // (m, l, o) and a second launch joins them in slot order.
+#include <type_traits>
+
 #include "common.h"
 #include "kernels.h"
 
@@ -32,20 +34,34 @@ struct SharedArgs {
   float scale;
   int qtiles_p, qtiles_s;             // query tiles of a unit, prefix and own part
   int splits_p, splits_s;             // key splits
-  int64_t items_p;                    // items of the prefix part, which come first
+  int items_p, items_s;               // items of the two parts
+  int run_p, run_s;                   // ... of one XCD
+  bool joined;                        // an item takes both parts and writes the output: no slots
   float* ml;                          // [slot][B * T * Hq][2]: maximum, sum
   float* o;                           // [slot][B * T * Hq][D]
 };
 
-// What one block computes.
+// Consecutive K/V rows: query r of an item sees them up to seen + r / (heads
+// of the KV group).
+struct Keys {
+  const void *k, *v;
+  int n;
+  int64_t seen;
+};
+
+// The last of the keys that query r sees (-1: none).
+__device__ __forceinline__ int last_seen(const Keys& k, int r, int per) {
+  return (int)std::max<int64_t>(std::min<int64_t>(k.seen + r / per, k.n - 1), -1);
+}
+
+// What one block computes: a tile of a unit's query rows over the keys of the
+// prefix (part 0), of the own rows (part 1) or of one after the other.
 struct Item {
-  const void *k, *v;  // the unit's first K / V row
-  int64_t n0;         // first token (b * T + t) of the unit
-  int rows;           // query rows of the unit: (token, head of the KV group)
+  Keys pre, own;
+  int first, last;  // parts: 0 the prefix, 1 the own rows
+  int64_t n0;       // first token (b * T + t) of the unit
+  int rows;         // query rows of the unit: (token, head of the KV group)
   int tile, kv, slot;
-  int64_t key_lo, key_hi;  // keys of this split
-  int64_t seen;            // own part: query t sees keys 0 .. seen + t; prefix: every key
-  bool own;
 };
 
 // Cached own rows of batch row b, -1 for an idle row (nothing attends).
@@ -54,105 +70,163 @@ __device__ __forceinline__ int64_t own_len(const SharedArgs& a, int64_t b) {
   return std::min<int64_t>(std::max<int64_t>(a.clens[b], -1), a.C);
 }
 
-template <int QT, int KT>
-__device__ __forceinline__ Item shared_item(const SharedArgs& a, int64_t D_bytes) {
-  const int per = a.Hq / a.Hkv;
-  Item it;
-  int64_t i = blockIdx.x, keys;
-  int split, splits;
-  it.own = i >= a.items_p;
-  if (!it.own) {
-    splits = a.splits_p;
-    split = (int)(i % splits);
-    i /= splits;
-    it.tile = (int)(i % a.qtiles_p);
-    i /= a.qtiles_p;
-    const int64_t g = i / a.Hkv;
-    it.kv = (int)(i % a.Hkv);
-    const int w = a.B / a.G;
-    it.n0 = g * w * a.T;
-    it.rows = w * a.T * per;
-    it.k = (const char*)a.kp + i * a.Sp * D_bytes;
-    it.v = (const char*)a.vp + i * a.Sp * D_bytes;
-    keys = a.plens == nullptr ? a.P : std::min<int64_t>(std::max<int64_t>(a.plens[g], 0), a.P);
-    it.seen = 0;
-    it.slot = split;
-  } else {
-    i -= a.items_p;
-    splits = a.splits_s;
-    split = (int)(i % splits);
-    i /= splits;
-    it.tile = (int)(i % a.qtiles_s);
-    i /= a.qtiles_s;
-    const int64_t b = i / a.Hkv;
-    it.kv = (int)(i % a.Hkv);
-    it.n0 = b * a.T;
-    it.rows = a.T * per;
-    it.k = (const char*)a.kc + i * a.S * D_bytes;
-    it.v = (const char*)a.vc + i * a.S * D_bytes;
-    it.seen = own_len(a, b);
-    // the tile's last query sees the most keys
-    const int last = std::min(it.tile * QT + QT, it.rows) - 1;
-    keys = it.seen < 0 ? 0 : it.seen + last / per + 1;
-    it.slot = a.splits_p + split;
-  }
+// Rows key_lo .. of a prefix or of a batch row's cache, those of one split.
+template <int KT>
+__device__ __forceinline__ void set_keys(Keys& k, const void* kb, const void* vb, int64_t row0, int64_t row_bytes,
+                                         int64_t keys, int64_t seen, int split, int splits) {
   const int64_t span = cdiv(cdiv(keys, (int64_t)KT), (int64_t)splits) * KT;
-  it.key_lo = std::min<int64_t>(split * span, keys);
-  it.key_hi = std::min<int64_t>(it.key_lo + span, keys);
-  return it;
+  const int64_t lo = std::min<int64_t>(split * span, keys);
+  k.k = (const char*)kb + (row0 + lo) * row_bytes;
+  k.v = (const char*)vb + (row0 + lo) * row_bytes;
+  k.n = (int)(std::min<int64_t>(lo + span, keys) - lo);
+  k.seen = seen - lo;
+}
+
+// Block -> item. Blocks go to the eight XCDs round robin, each with an L2 of
+// its own, so every XCD takes a run of each part's items, in which the query
+// tiles of one (unit, split) follow each other and share its K/V rows. The
+// prefix part, bound by the matrix cores where the groups are large, goes
+// first; blocks of the own part, bound by memory, take the places it leaves.
+// False: no item.
+template <int QT, int KT>
+__device__ __forceinline__ bool shared_item(const SharedArgs& a, int64_t row_bytes, Item& it) {
+  const int per = a.Hq / a.Hkv;
+  const int xcd = blockIdx.x % 8, seq = blockIdx.x / 8;
+  const bool own = seq >= a.run_p;
+  int i = own ? xcd * a.run_s + seq - a.run_p : xcd * a.run_p + seq;
+  if (i >= (own ? a.items_s : a.items_p)) return false;
+  const int qtiles = own ? a.qtiles_s : a.qtiles_p, splits = own ? a.splits_s : a.splits_p;
+  it.tile = i % qtiles;
+  i /= qtiles;
+  const int split = i % splits;
+  i /= splits;  // (group or batch row, KV head)
+  it.kv = i % a.Hkv;
+  const int w = a.B / a.G, b = own ? i / a.Hkv : i / a.Hkv * w, g = b / w;
+  it.n0 = (int64_t)b * a.T;
+  it.rows = (own ? 1 : w) * a.T * per;
+  it.slot = own ? a.splits_p + split : split;
+  it.first = own && (!a.joined || a.P == 0) ? 1 : 0;
+  it.last = own ? 1 : 0;
+  if (it.first == 0) {
+    const int64_t keys = a.plens == nullptr ? a.P : std::min<int64_t>(std::max<int64_t>(a.plens[g], 0), a.P);
+    set_keys<KT>(it.pre, a.kp, a.vp, ((int64_t)g * a.Hkv + it.kv) * a.Sp, row_bytes, keys, INT64_MAX / 2,
+                 own ? 0 : split, own ? 1 : splits);
+  }
+  if (own) {
+    const int64_t seen = own_len(a, b);
+    const int last = std::min(it.tile * QT + QT, it.rows) - 1;  // (the tile's last query sees the most keys)
+    set_keys<KT>(it.own, a.kc, a.vc, (int64_t)i * a.S, row_bytes, seen < 0 ? 0 : seen + last / per + 1, seen, split,
+                 splits);
+    if (seen < 0) it.own.n = it.pre.n = 0;  // an idle row
+  }
+  return true;
 }
 
 // One tile of keys through a resource of its own (a head's rows may span more
 // than the 4 GiB that one reaches); rows past the item's last read zeros.
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t key_rows(const void* base, int64_t key, int64_t key_hi, int tile,
-                                                           int row_bytes) {
-  const int64_t n = std::min<int64_t>(std::max<int64_t>(key_hi - key, 0), tile);
-  return span_rsrc((const char*)base + key * row_bytes, (uint32_t)(n * row_bytes));
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t key_rows(const void* base, int key, int keys, int tile, int row_bytes) {
+  const int n = std::min(keys - key, tile);
+  return span_rsrc((const char*)base + (int64_t)key * row_bytes, (uint32_t)(n * row_bytes));
 }
 __device__ __forceinline__ uint4 rows_load16(__amdgpu_buffer_rsrc_t r, uint32_t off) {
   const u32x4 v = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0));
   return make_uint4(v.x, v.y, v.z, v.w);
 }
 
+// maximum / sum over lanes l and l ^ 32 (and, for the 16-lane form, l ^ 16)
+__device__ __forceinline__ float halves_max(float v) {
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float halves_sum(float v) {
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+__device__ __forceinline__ float quads_max(float v) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return halves_max(fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1])));
+}
+__device__ __forceinline__ float quads_sum(float v) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return halves_sum(__uint_as_float(a[0]) + __uint_as_float(a[1]));
+}
+
+// Results of query rows [0, rows) from base row r0 of the item that KW waves
+// hold over keys of their own, in LDS: po [KW][cap][D], pml [KW][cap] (maximum,
+// sum; exp2 or expf by BASE2). Joined, they go to the output or to the slot.
+template <typename T, int D, int KW, bool BASE2>
+__device__ __forceinline__ void finish_rows(const SharedArgs& a, const Item& it, const float* po, const float2* pml,
+                                            int cap, int r0, int rows) {
+  constexpr int LPR = D / 4;
+  const int per = a.Hq / a.Hkv;
+  for (int i = threadIdx.x; i < rows * LPR; i += 256) {
+    const int row = i / LPR, d = i % LPR * 4;
+    float2 ml[KW];
+    float m = -__builtin_inff(), l = 0.f;
+#pragma unroll
+    for (int j = 0; j < KW; ++j) {
+      ml[j] = pml[j * cap + row];
+      m = fmaxf(m, ml[j].x);
+    }
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < KW; ++j) {
+      if (ml[j].x == -__builtin_inff()) continue;
+      const float sc = BASE2 ? __builtin_amdgcn_exp2f(ml[j].x - m) : expf(ml[j].x - m);
+      l = fmaf(sc, ml[j].y, l);
+      const f32x4 oj = *(const f32x4*)(po + (j * cap + row) * D + d);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = fmaf(sc, oj[e], o[e]);
+    }
+    const int r = r0 + row;
+    const int64_t n = (it.n0 + r / per) * a.Hq + it.kv * per + r % per;
+    if (a.joined) {
+      float v[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = m == -__builtin_inff() ? 0.f : o[e] / l;
+      store_vec<T, 4>((T*)a.out + n * D + d, v);
+    } else {
+      const int64_t at = (int64_t)it.slot * a.B * a.T * a.Hq + n;
+      *(f32x4*)(a.o + at * D + d) = o;
+      if (d == 0) *(float2*)(a.ml + at * 2) = make_float2(BASE2 ? m : m * 1.4426950408889634f, l);
+    }
+  }
+}
+
 // ---------------------------------------------------------------------------
 // fp32 (and bf16 head dims below 32, widened on their way into LDS) on
-// v_mfma_f32_16x16x4_f32. Four waves of 16 queries share each KT-key tile in
-// LDS; products transposed: S^T = K Q^T leaves lane (quad, r) with keys 4 quad
-// .. 4 quad + 3 of query r, which is the B operand of O^T = V^T P^T as it is.
-// Score MFMA i of a chunk takes dims 16 c + 4 quad + i from both operands (one
-// 16-byte LDS read a lane), output MFMA j dims E r + j; rows are padded by 16
-// bytes against bank conflicts. A score is summed in four chains.
-constexpr int F_QT = 64;
+// v_mfma_f32_16x16x4_f32. Four waves share each 64-key tile in LDS: 4 / KW
+// strips of 16 queries, KW waves a strip over 64 / KW keys each (a unit of few
+// rows is bound by the latency of one wave's keys); products transposed: S^T =
+// K Q^T leaves lane (quad, r) with keys 4 quad .. 4 quad + 3 of query r, which
+// is the B operand of O^T = V^T P^T as it is. Score MFMA i of a chunk takes
+// dims 16 c + 4 quad + i from both operands (one 16-byte LDS read a lane),
+// output MFMA j dims E r + j; rows are padded by 16 bytes against bank
+// conflicts. A score is summed in four chains.
+constexpr int F_QT = 64, F_KT = 64;
 template <int D>
-constexpr int F_KT = D >= 128 ? 32 : 64;
+constexpr int F_LDS = 2 * F_KT * (D + 4) * 4;
 
-template <typename T, int D>
-__global__ __launch_bounds__(256) void shared_attn_f32_kernel(SharedArgs a) {
-  constexpr int KT = F_KT<D>, KB = KT / 16, KC = D / 16;
+template <typename T, int D, int KW>
+__device__ __forceinline__ void shared_rows_f32(const SharedArgs& a, const Item& it, float* lds, int* odd) {
+  constexpr int KT = F_KT, KB = KT / 16 / KW, KC = D / 16, SW = 4 / KW;
   constexpr int E = D / 16 < 4 ? D / 16 : 4, HALVES = D / 16 / E;
   constexpr int ROW = D + 4;
   constexpr int VE = Vec<T>::N, PIECES = KT * D / VE, PER = (PIECES + 255) / 256;
-  __shared__ __attribute__((aligned(16))) float Ks[KT * ROW];
-  __shared__ __attribute__((aligned(16))) float Vs[KT * ROW];
-  __shared__ int odd;  // a hidden value row of this tile is not finite
-  const Item it = shared_item<F_QT, KT>(a, D * (int64_t)sizeof(T));
+  float *Ks = lds, *Vs = lds + KT * ROW;
   const int per = a.Hq / a.Hkv;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int lr = lane % 16, lq = lane / 16;
-  const int r0 = it.tile * F_QT + wave * 16, r = r0 + lr;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lr = lane % 16, lq = lane / 16, strip = wave % SW, key0 = wave / SW * KB * 16;
+  const int t0 = it.tile * F_QT, r = t0 + strip * 16 + lr;
   const bool live = r < it.rows;
   const int64_t n = it.n0 + (live ? r : 0) / per;
   const int h = it.kv * per + (live ? r : 0) % per;
-  const int64_t seen = it.own ? it.seen + (n - it.n0) : INT64_MAX;  // the last key this query sees
-  const int64_t seen_first = it.own ? it.seen + (it.tile * F_QT) / per : INT64_MAX;
 
   f32x4 qa[KC];
   {
     const T* qrow = (const T*)a.q + (n * a.Hq + h) * D;
 #pragma unroll
-    for (int c = 0; c < KC; ++c)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) qa[c][i] = load_f32<T>(qrow, 16 * c + 4 * lq + i);
+    for (int c = 0; c < KC; ++c) load_vec<T, 4>(qrow + 16 * c + 4 * lq, (float*)&qa[c]);
   }
   f32x4 o[HALVES][E];
 #pragma unroll
@@ -161,137 +235,165 @@ __global__ __launch_bounds__(256) void shared_attn_f32_kernel(SharedArgs a) {
     for (int j = 0; j < E; ++j) o[hf][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   float m = -__builtin_inff(), lsum = 0.f;
 
-  uint4 kr[PER], vr[PER];
-  auto load_tile = [&](int64_t key) {
-    const __amdgpu_buffer_rsrc_t krs = key_rows(it.k, key, it.key_hi, KT, D * (int)sizeof(T));
-    const __amdgpu_buffer_rsrc_t vrs = key_rows(it.v, key, it.key_hi, KT, D * (int)sizeof(T));
+  for (int part = it.first; part <= it.last; ++part) {
+    const Keys ks = part == 0 ? it.pre : it.own;
+    const int seen = last_seen(ks, live ? r : 0, per), all_see = last_seen(ks, t0, per);
+    uint4 kr[PER], vr[PER];
+    auto load_tile = [&](int key) {
+      const __amdgpu_buffer_rsrc_t krs = key_rows(ks.k, key, ks.n, KT, D * (int)sizeof(T));
+      const __amdgpu_buffer_rsrc_t vrs = key_rows(ks.v, key, ks.n, KT, D * (int)sizeof(T));
 #pragma unroll
-    for (int u = 0; u < PER; ++u) {
-      const uint32_t off = (uint32_t)(tid + 256 * u) * 16;  // (past the tile: not stored)
-      kr[u] = rows_load16(krs, off);
-      vr[u] = rows_load16(vrs, off);
-    }
-  };
-  if (it.key_lo < it.key_hi) load_tile(it.key_lo);
-  for (int64_t k0 = it.key_lo; k0 < it.key_hi; k0 += KT) {
-    __syncthreads();  // the previous tile is consumed
-    if (tid == 0) odd = 0;
-    __syncthreads();
-    bool found = false;
+      for (int u = 0; u < PER; ++u) {
+        const uint32_t off = (uint32_t)(tid + 256 * u) * 16;  // (past the tile: not stored)
+        kr[u] = rows_load16(krs, off);
+        vr[u] = rows_load16(vrs, off);
+      }
+    };
+    if (ks.n > 0) load_tile(0);
+    for (int k0 = 0; k0 < ks.n; k0 += KT) {
+      __syncthreads();  // the previous tile is consumed
+      if (tid == 0) *odd = 0;
+      __syncthreads();
+      bool found = false;
 #pragma unroll
-    for (int u = 0; u < PER; ++u) {
-      const int i = tid + 256 * u;
-      if (i < PIECES) {
-        const int row = i / (D / VE), at = row * ROW + i % (D / VE) * VE;
-        float f[VE];
-        unpack16(kr[u], f, (T*)nullptr);
+      for (int u = 0; u < PER; ++u) {
+        const int i = tid + 256 * u;
+        if (i < PIECES) {
+          const int row = i / (D / VE), at = row * ROW + i % (D / VE) * VE;
+          float f[VE];
+          unpack16(kr[u], f, (T*)nullptr);
 #pragma unroll
-        for (int e = 0; e < VE; ++e) Ks[at + e] = f[e];
-        unpack16(vr[u], f, (T*)nullptr);
+          for (int e = 0; e < VE; e += 4) *(f32x4*)(Ks + at + e) = *(const f32x4*)(f + e);
+          unpack16(vr[u], f, (T*)nullptr);
 #pragma unroll
-        for (int e = 0; e < VE; ++e) {
-          Vs[at + e] = f[e];
-          found |= k0 + row > seen_first && !__builtin_isfinite(f[e]);
+          for (int e = 0; e < VE; e += 4) *(f32x4*)(Vs + at + e) = *(const f32x4*)(f + e);
+          if (k0 + row > all_see) {
+            // a key that some query does not see: is its value finite?
+#pragma unroll
+            for (int e = 0; e < VE; ++e) found |= !__builtin_isfinite(f[e]);
+          }
         }
       }
-    }
-    if (found) odd = 1;
-    __syncthreads();
-    if (k0 + KT < it.key_hi) load_tile(k0 + KT);
-    const bool slow = odd != 0;
-    const int64_t limit = std::min<int64_t>(seen, it.key_hi - 1) - k0;  // last key of the tile this query sees
-    float p[KB][4];
-    float mx = -__builtin_inff();
+      if (found) *odd = 1;
+      __syncthreads();
+      if (k0 + KT < ks.n) load_tile(k0 + KT);
+      const bool slow = *odd != 0;
+      const int limit = seen - k0 - key0;  // last of the wave's keys that this query sees
+      float p[KB][4];
+      float mx = -__builtin_inff();
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) {
-      f32x4 part[4];
+      for (int kb = 0; kb < KB; ++kb) {
+        f32x4 chain[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) part[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < 4; ++i) chain[i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int c = 0; c < KC; ++c) {
-        const f32x4 k4 = *(const f32x4*)(Ks + (kb * 16 + lr) * ROW + 16 * c + 4 * lq);
+        for (int c = 0; c < KC; ++c) {
+          const f32x4 k4 = *(const f32x4*)(Ks + (key0 + kb * 16 + lr) * ROW + 16 * c + 4 * lq);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) part[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(k4[i], qa[c][i], part[i], 0, 0, 0);
+          for (int i = 0; i < 4; ++i) chain[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(k4[i], qa[c][i], chain[i], 0, 0, 0);
+        }
+        const f32x4 acc = (chain[0] + chain[1]) + (chain[2] + chain[3]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          p[kb][e] = kb * 16 + 4 * lq + e <= limit ? acc[e] * a.scale : -__builtin_inff();
+          mx = fmaxf(mx, p[kb][e]);
+        }
       }
-      const f32x4 acc = (part[0] + part[1]) + (part[2] + part[3]);
+      mx = quads_max(mx);
+      const float mn = fmaxf(m, mx);
+      const float alpha = mn == -__builtin_inff() ? 1.f : expf(m - mn);
+      m = mn;
+      lsum *= alpha;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        p[kb][e] = kb * 16 + 4 * lq + e <= limit ? acc[e] * a.scale : -__builtin_inff();
-        mx = fmaxf(mx, p[kb][e]);
-      }
-    }
-    mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-    const float mn = fmaxf(m, mx);
-    const float alpha = mn == -__builtin_inff() ? 1.f : expf(m - mn);
-    m = mn;
-    lsum *= alpha;
+      for (int hf = 0; hf < HALVES; ++hf)
 #pragma unroll
-    for (int hf = 0; hf < HALVES; ++hf)
-#pragma unroll
-      for (int j = 0; j < E; ++j) o[hf][j] *= alpha;
-#pragma unroll
-    for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        p[kb][e] = p[kb][e] == -__builtin_inff() ? 0.f : expf(p[kb][e] - mn);
-        lsum += p[kb][e];
-      }
-    if (slow) {
-      // a hidden key's value is not finite: 0 times it is no zero, so the keys
-      // that this lane's query does not see are left out one by one
+        for (int j = 0; j < E; ++j) o[hf][j] *= alpha;
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-#pragma unroll 1
-          for (int src = 0; src < 4; ++src) {
-            const float pk = __shfl(p[kb][e], lr + 16 * src, 64);
-            const int key = kb * 16 + 4 * src + e;
-            if (key > limit) continue;
-#pragma unroll
-            for (int hf = 0; hf < HALVES; ++hf)
-#pragma unroll
-              for (int j = 0; j < E; ++j)
-#pragma unroll
-                for (int x = 0; x < 4; ++x)
-                  o[hf][j][x] = fmaf(pk, Vs[key * ROW + 64 * hf + E * (4 * lq + x) + j], o[hf][j][x]);
-          }
-      continue;
-    }
-#pragma unroll
-    for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float* vrow = Vs + (kb * 16 + 4 * lq + e) * ROW + E * lr;
-#pragma unroll
-        for (int hf = 0; hf < HALVES; ++hf) {
-          float v[E];
-          if constexpr (E == 4) {
-            const f32x4 v4 = *(const f32x4*)(vrow + 64 * hf);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = v4[j];
-          } else {
-#pragma unroll
-            for (int j = 0; j < E; ++j) v[j] = vrow[j];
-          }
-#pragma unroll
-          for (int j = 0; j < E; ++j) o[hf][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[j], p[kb][e], o[hf][j], 0, 0, 0);
+        for (int e = 0; e < 4; ++e) {
+          p[kb][e] = p[kb][e] == -__builtin_inff() ? 0.f : expf(p[kb][e] - mn);
+          lsum += p[kb][e];
         }
+      if (slow) {
+        // a hidden key's value is not finite: 0 times it is no zero, so the keys
+        // that this lane's query does not see are left out one by one
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+#pragma unroll 1
+            for (int src = 0; src < 4; ++src) {
+              const float pk = __shfl(p[kb][e], lr + 16 * src, 64);
+              const int key = kb * 16 + 4 * src + e;
+              const float* vrow = Vs + (key0 + key) * ROW;
+#pragma unroll
+              for (int hf = 0; hf < HALVES; ++hf)
+#pragma unroll
+                for (int j = 0; j < E; ++j)
+#pragma unroll
+                  for (int x = 0; x < 4; ++x) {
+                    const float v = vrow[64 * hf + E * (4 * lq + x) + j];
+                    o[hf][j][x] = key <= limit ? fmaf(pk, v, o[hf][j][x]) : o[hf][j][x];
+                  }
+            }
+        continue;
       }
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float* vrow = Vs + (key0 + kb * 16 + 4 * lq + e) * ROW + E * lr;
+#pragma unroll
+          for (int hf = 0; hf < HALVES; ++hf) {
+            float v[E];
+            if constexpr (E == 4) {
+              const f32x4 v4 = *(const f32x4*)(vrow + 64 * hf);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) v[j] = v4[j];
+            } else {
+#pragma unroll
+              for (int j = 0; j < E; ++j) v[j] = vrow[j];
+            }
+#pragma unroll
+            for (int j = 0; j < E; ++j)
+              o[hf][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[j], p[kb][e], o[hf][j], 0, 0, 0);
+          }
+        }
+    }
   }
-  lsum += __shfl_xor(lsum, 16, 64);
-  lsum += __shfl_xor(lsum, 32, 64);
-  if (!live) return;
-  const int64_t at = (int64_t)it.slot * a.B * a.T * a.Hq + n * a.Hq + h;
-  if (lq == 0) *(float2*)(a.ml + at * 2) = make_float2(m * 1.4426950408889634f, lsum);
-  float* orow = a.o + at * D;
+  // o[hf][j][x]: dim 64 hf + E (4 lq + x) + j of the lane's query
+  lsum = quads_sum(lsum);
+  constexpr int CAP = SW * 16;
+  float* po = lds;                        // [KW][CAP][D]
+  float2* pml = (float2*)(po + 64 * D);   // [KW][CAP]
+  const int at = wave / SW * CAP + strip * 16 + lr;
+  __syncthreads();  // (the last tile is consumed)
 #pragma unroll
   for (int hf = 0; hf < HALVES; ++hf)
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
+    for (int x = 0; x < 4; ++x)
 #pragma unroll
-      for (int j = 0; j < E; ++j) orow[64 * hf + E * (4 * lq + e) + j] = o[hf][j][e];
+      for (int j = 0; j < E; ++j) po[at * D + 64 * hf + E * (4 * lq + x) + j] = o[hf][j][x];
+  if (lq == 0) pml[at] = make_float2(m, lsum);
+  __syncthreads();
+  finish_rows<T, D, KW, false>(a, it, po, pml, CAP, t0, std::min(CAP, it.rows - t0));
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(256) void shared_attn_f32_kernel(SharedArgs a) {
+  extern __shared__ __attribute__((aligned(16))) float lds_f[];
+  static_assert(F_LDS<D> >= 64 * (D + 2) * 4, "the waves' results fit the tiles");
+  __shared__ int odd;
+  Item it;
+  if (!shared_item<F_QT, F_KT>(a, D * (int64_t)sizeof(T), it)) return;
+  const int rows = it.rows - it.tile * F_QT;
+  if (rows <= 16)
+    shared_rows_f32<T, D, 4>(a, it, lds_f, &odd);
+  else if (rows <= 32)
+    shared_rows_f32<T, D, 2>(a, it, lds_f, &odd);
+  else
+    shared_rows_f32<T, D, 1>(a, it, lds_f, &odd);
 }
 
 // ---------------------------------------------------------------------------
@@ -331,18 +433,22 @@ struct Half {
 
 // 16 bytes a lane from the resource at voff to LDS at lds_addr + 16 lane
 // (m0, wave-uniform; zeros past the resource's end). asm, so that the compiler
-// does not wait for these loads at every LDS read: stage_wait does. The s_nop
-// is the wait state between the write of m0 and a load to LDS.
+// does not wait for these loads at every LDS read: stage_wait does. It also
+// keeps the compiler from adding the wait states that the hardware asks for:
+// one between the write of m0 and a load to LDS (the s_nop 0), and five between
+// a vector instruction's write of a scalar register (v_readfirstlane) and a
+// load that reads it, which rows_rsrc leaves.
 __device__ __forceinline__ void row_dma16(u32x4 r, uint32_t voff, uint32_t lds_addr) {
   asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(r), "{m0}"(lds_addr) : "memory");
 }
-__device__ __forceinline__ u32x4 rows_rsrc(const void* base, int64_t key, int64_t key_hi, int row_bytes) {
-  const uint64_t p = (uint64_t)base + key * row_bytes;
+__device__ __forceinline__ u32x4 rows_rsrc(const void* base, int bytes) {
+  const uint64_t p = (uint64_t)base;
   u32x4 r;
   r.x = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)p);
   r.y = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(p >> 32));
-  r.z = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)std::min<int64_t>(key_hi - key, H_KT) * row_bytes);
+  r.z = (uint32_t)__builtin_amdgcn_readfirstlane(bytes);
   r.w = 0x00020000u;
+  asm volatile("s_nop 4" : "+s"(r));
   return r;
 }
 // this wave's loads have landed and its LDS reads are done; then the block's
@@ -352,56 +458,79 @@ __device__ __forceinline__ void stage_wait() {
   asm volatile("" ::: "memory");
 }
 
+// The queries are waited for here. Without it the compiler would wait for them
+// at their first use in the tile loop, every time round, and so for the next
+// tile's loads, which are counted with them.
+template <int N>
+__device__ __forceinline__ void arrived(bf16x8 (&q)[N]) {
+  if constexpr (N >= 4) {
+#pragma unroll
+    for (int k = 0; k < N; k += 4) asm volatile("" : "+v"(q[k]), "+v"(q[k + 1]), "+v"(q[k + 2]), "+v"(q[k + 3]));
+  } else if constexpr (N == 2) {
+    asm volatile("" : "+v"(q[0]), "+v"(q[1]));
+  } else {
+    asm volatile("" : "+v"(q[0]));
+  }
+}
+
 __device__ __forceinline__ s16x4 read_tr(const char* p) {
   return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p));
 }
 __device__ __forceinline__ bf16x8 join8(s16x4 lo, s16x4 hi) {
   return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 }
-// maximum / sum over lanes l and l ^ 32 (and, for the 16-lane form, l ^ 16)
-__device__ __forceinline__ float halves_max(float v) {
-  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+// one of eight bf16 values is infinite or NaN
+__device__ __forceinline__ bool not_finite(const uint4& x) {
+  const uint32_t wd[4] = {x.x, x.y, x.z, x.w};
+  bool odd = false;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) odd |= (wd[e] & 0x7f80u) == 0x7f80u || (wd[e] & 0x7f800000u) == 0x7f800000u;
+  return odd;
 }
-__device__ __forceinline__ float halves_sum(float v) {
-  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
-}
-__device__ __forceinline__ float quads_max(float v) {
-  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return halves_max(fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1])));
-}
-__device__ __forceinline__ float quads_sum(float v) {
-  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return halves_sum(__uint_as_float(a[0]) + __uint_as_float(a[1]));
-}
-
-// Tiles of an item through the two stages; compute(k0, stage) for each.
-template <int D, typename F>
-__device__ __forceinline__ void over_tiles(const Item& it, char* lds, F&& compute) {
+// The tiles of consecutive rows through the two stages (tile t in stage t % 2).
+template <int D>
+struct Tiles {
   using H = Half<D>;
-  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
-  // piece w + 4 j of a tile: rows 4 PIECE_ROWS j + row; the swizzles do not depend on j
-  const int row = H::PIECE_ROWS * w + lane / H::CH;
-  const uint32_t koff = row * H::ROWB + ((lane % H::CH) ^ H::k_swz(row)) * 16;
-  const uint32_t voff = row * H::ROWB + ((lane % H::CH) ^ H::v_swz(row)) * 16;
-  auto issue = [&](int64_t k0, int st) {
-    const u32x4 kr = rows_rsrc(it.k, k0, it.key_hi, H::ROWB), vr = rows_rsrc(it.v, k0, it.key_hi, H::ROWB);
-    const uint32_t to = lds0 + st * H::STAGE + w * 1024;
-#pragma unroll
-    for (int j = 0; j < H::PPW; ++j) row_dma16(kr, koff + j * 4096, to + j * 4096);
-#pragma unroll
-    for (int j = 0; j < H::PPW; ++j) row_dma16(vr, voff + j * 4096, to + H::OPER + j * 4096);
-  };
-  if (it.key_lo < it.key_hi) issue(it.key_lo, 0);
-  int st = 0;
-  for (int64_t k0 = it.key_lo; k0 < it.key_hi; k0 += H_KT, st ^= 1) {
-    stage_wait();
-    if (k0 + H_KT < it.key_hi) issue(k0 + H_KT, st ^ 1);  // (its readers passed the barrier)
-    compute(k0, lds + st * H::STAGE);
+  const char *k, *v;
+  uint32_t to, koff, voff;
+  int keys, n;
+  __device__ __forceinline__ Tiles(const Keys& ks, char* lds)
+      : k((const char*)ks.k), v((const char*)ks.v), keys(ks.n), n((ks.n + H_KT - 1) / H_KT) {
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds + w * 1024;
+    // piece w + 4 j of a tile: rows 4 PIECE_ROWS j + row; the swizzles do not depend on j
+    const int row = H::PIECE_ROWS * w + lane / H::CH;
+    koff = row * H::ROWB + ((lane % H::CH) ^ H::k_swz(row)) * 16;
+    voff = row * H::ROWB + ((lane % H::CH) ^ H::v_swz(row)) * 16;
   }
-}
+  __device__ __forceinline__ void load(int t) const {
+    if (t >= n) return;
+    const int left = std::min(keys - t * H_KT, H_KT) * H::ROWB;
+    const u32x4 kr = rows_rsrc(k + (int64_t)t * H::OPER, left), vr = rows_rsrc(v + (int64_t)t * H::OPER, left);
+    uint32_t at = __builtin_amdgcn_readfirstlane(to + (t & 1) * H::STAGE);
+    asm volatile("s_nop 4" : "+s"(at));
+#pragma unroll
+    for (int j = 0; j < H::PPW; ++j) row_dma16(kr, koff + j * 4096, at + j * 4096);
+#pragma unroll
+    for (int j = 0; j < H::PPW; ++j) row_dma16(vr, voff + j * 4096, at + H::OPER + j * 4096);
+  }
+  // compute(t, stage, masked) for each tile, tile 0 being on its way; the tiles
+  // from `masked_from` on have keys that some query does not see
+  template <typename F>
+  __device__ __forceinline__ void each(const char* lds, int masked_from, F&& compute) const {
+    int t = 0;
+    for (; t < masked_from; ++t) {
+      stage_wait();
+      load(t + 1);  // (the stage's readers passed the barrier)
+      compute(t, lds + (t & 1) * H::STAGE, std::false_type{});
+    }
+    for (; t < n; ++t) {
+      stage_wait();
+      load(t + 1);
+      compute(t, lds + (t & 1) * H::STAGE, std::true_type{});
+    }
+  }
+};
 
 // The running maximum moves only when some lane's passes it by this much (base
 // 2): until then probabilities stay below 2^8 and nothing is rescaled.
@@ -418,14 +547,16 @@ __device__ __forceinline__ void shared_rows128(const SharedArgs& a, const Item& 
   const bool live = r < it.rows;
   const int64_t n = it.n0 + (live ? r : 0) / per;
   const int head = it.kv * per + (live ? r : 0) % per;
-  const int64_t seen = it.own ? it.seen + (n - it.n0) : INT64_MAX;  // the last key this query sees
-  const int64_t seen_first = it.own ? it.seen + r0 / per : INT64_MAX, seen_last = it.own ? it.seen + (r0 + 31) / per : INT64_MAX;
+  Keys ks = it.first == 0 ? it.pre : it.own;
+  Tiles<D> tiles(ks, lds);
+  tiles.load(0);
 
   bf16x8 qb[KS];
   {
     const bf16* q = (const bf16*)a.q + (n * a.Hq + head) * D + 8 * h;
 #pragma unroll
-    for (int k = 0; k < KS; ++k) qb[k] = __builtin_bit_cast(bf16x8, *(const uint4*)(q + 16 * k));
+    for (int k = 0; k < KS; ++k) qb[k] = __builtin_bit_cast(bf16x8, *(const u32x4*)(q + 16 * k));
+    arrived(qb);
   }
   f32x16 o[DB];
 #pragma unroll
@@ -442,8 +573,17 @@ __device__ __forceinline__ void shared_rows128(const SharedArgs& a, const Item& 
   const int vat = H::OPER + vrow * H::ROWB + 8 * (lane & 1);
   const int vx = ((2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) ^ H::v_swz(vrow)) << 4;
 
-  over_tiles<D>(it, lds, [&](int64_t k0, const char* st) {
-    if (r0 >= it.rows || k0 > seen_last) return;
+  for (int part = it.first; part <= it.last; ++part) {
+  if (part != it.first) {
+    ks = it.own;
+    tiles = Tiles<D>(ks, lds);
+    __syncthreads();  // (every stage is free)
+    tiles.load(0);
+  }
+  const int seen = last_seen(ks, live ? r : 0, per), seen_last = last_seen(ks, r0 + 31, per);
+  const int all_see = last_seen(ks, it.tile * H_QT, per);  // the last key that every query of the block sees
+  tiles.each(lds, (all_see + 1) / H_KT, [&](int t, const char* st, auto masked) {
+    if (r0 >= it.rows || (masked && t * H_KT > seen_last)) return;
     f32x16 s[2];
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
@@ -456,25 +596,17 @@ __device__ __forceinline__ void shared_rows128(const SharedArgs& a, const Item& 
       }
     }
     bool odd = false;
-    const int limit = (int)std::min<int64_t>(std::min<int64_t>(seen, it.key_hi - 1) - k0, H_KT);
-    if (k0 + H_KT - 1 > std::min<int64_t>(seen_first, it.key_hi - 1)) {
-      // some query does not see some key: lane (query, h) holds keys
-      // 32 kb + 8 (i / 4) + 4 h + i % 4
-      __asm__ volatile("");  // (a branch, not selects on every tile)
+    const int limit = seen - t * H_KT;
+    if constexpr (masked) {
+      // lane (query, h) holds keys 32 kb + 8 (i / 4) + 4 h + i % 4
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
         for (int i = 0; i < 16; ++i)
           if (32 * kb + 8 * (i / 4) + i % 4 > limit - 4 * h) s[kb][i] = -__builtin_inff();
-      if (seen_first < it.key_hi - 1) {
+      if (all_see < ks.n - 1) {
         // hidden keys that other queries see: are their values finite?
-        for (int c = lane; c < H_KT * H::CH; c += 64) {
-          const uint4 x = *(const uint4*)(st + H::OPER + c * 16);
-          const uint32_t wd[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            odd |= (wd[e] & 0x7f80u) == 0x7f80u || (wd[e] & 0x7f800000u) == 0x7f800000u;
-        }
+        for (int c = lane; c < H_KT * H::CH; c += 64) odd |= not_finite(*(const uint4*)(st + H::OPER + c * 16));
         odd = __builtin_amdgcn_ballot_w64(odd) != 0;
       }
     }
@@ -499,7 +631,7 @@ __device__ __forceinline__ void shared_rows128(const SharedArgs& a, const Item& 
         s[kb][i] = __builtin_amdgcn_exp2f(fmaf(s[kb][i], sl2, -mref));
         lsum += s[kb][i];
       }
-    if (odd) {
+    if (masked && odd) {
       // a value that some query may not touch is not finite (0 times it is no
       // zero): key by key, for the queries that see it
 #pragma unroll 1
@@ -535,8 +667,22 @@ __device__ __forceinline__ void shared_rows128(const SharedArgs& a, const Item& 
       }
     }
   });
+  }
   if (!live) return;
   const float l = halves_sum(lsum);
+  if (a.joined) {
+    bf16* orow = (bf16*)a.out + (n * a.Hq + head) * D + 4 * h;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = m == -__builtin_inff() ? 0.f : o[d][4 * c + e] / l;
+        store_vec<bf16, 4>(orow + 32 * d + 8 * c, v);
+      }
+    return;
+  }
   const int64_t at = (int64_t)it.slot * a.B * a.T * a.Hq + n * a.Hq + head;
   if (h == 0) *(float2*)(a.ml + at * 2) = make_float2(m, l);
   float* orow = a.o + at * D + 4 * h;
@@ -558,13 +704,16 @@ __device__ __forceinline__ void shared_rows16(const SharedArgs& a, const Item& i
   const bool live = r < it.rows;
   const int64_t n = it.n0 + (live ? r : 0) / per;
   const int head = it.kv * per + (live ? r : 0) % per;
-  const int64_t seen = it.own ? it.seen + (n - it.n0) : INT64_MAX;
+  Keys ks = it.first == 0 ? it.pre : it.own;
+  Tiles<D> tiles(ks, lds);
+  tiles.load(0);
 
   bf16x8 qb[KS];
   {
     const bf16* q = (const bf16*)a.q + (n * a.Hq + head) * D + 8 * q4;
 #pragma unroll
-    for (int k = 0; k < KS; ++k) qb[k] = __builtin_bit_cast(bf16x8, *(const uint4*)(q + 32 * k));
+    for (int k = 0; k < KS; ++k) qb[k] = __builtin_bit_cast(bf16x8, *(const u32x4*)(q + 32 * k));
+    arrived(qb);
   }
   f32x4 o[DB];
 #pragma unroll
@@ -577,19 +726,29 @@ __device__ __forceinline__ void shared_rows16(const SharedArgs& a, const Item& i
   const int vrow = 16 * w + 4 * q4 + n16 / 4;
   const int vat = H::OPER + vrow * H::ROWB + 8 * (lane & 1), vx = (((lane >> 1) & 1) ^ H::v_swz(vrow)) << 4;
 
-  over_tiles<D>(it, lds, [&](int64_t k0, const char* st) {
-    const int64_t kw = k0 + 16 * w;
-    if (kw >= it.key_hi) return;
+  for (int part = it.first; part <= it.last; ++part) {
+  if (part != it.first) {
+    ks = it.own;
+    tiles = Tiles<D>(ks, lds);
+    __syncthreads();  // (every stage is free)
+    tiles.load(0);
+  }
+  const int seen = last_seen(ks, live ? r : 0, per), all_see = last_seen(ks, 0, per);
+  tiles.each(lds, (all_see + 1) / H_KT, [&](int t, const char* st, auto masked) {
+    const int kw = t * H_KT + 16 * w;
+    if (masked && kw >= ks.n) return;
     f32x4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int k = 0; k < KS; ++k) {
       const bf16x8 kf = __builtin_bit_cast(bf16x8, *(const uint4*)(st + kat + ((64 * k) ^ kx)));
       s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qb[k], s, 0, 0, 0);
     }
-    const int limit = (int)std::min<int64_t>(std::min<int64_t>(seen, it.key_hi - 1) - kw, 16);
+    const int limit = seen - kw;
+    if constexpr (masked) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (4 * q4 + i > limit) s[i] = -__builtin_inff();
+      for (int i = 0; i < 4; ++i)
+        if (4 * q4 + i > limit) s[i] = -__builtin_inff();
+    }
     const float mx = quads_max(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]))) * sl2;
     if (__builtin_amdgcn_ballot_w64(mx > m)) {
       const float mn = fmaxf(m, mx), alpha = mn == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(m - mn);
@@ -605,14 +764,10 @@ __device__ __forceinline__ void shared_rows16(const SharedArgs& a, const Item& i
       lsum += s[i];
     }
     // (several tokens: a hidden key's value may not be finite)
-    if (__builtin_amdgcn_ballot_w64(limit < std::min<int64_t>(it.key_hi - 1 - kw, 15))) {
+    if (masked && all_see < ks.n - 1) {
       bool odd = false;
-      for (int c = lane; c < 16 * H::CH; c += 64) {
-        const uint4 x = *(const uint4*)(st + H::OPER + 16 * w * H::ROWB + c * 16);
-        const uint32_t wd[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) odd |= (wd[e] & 0x7f80u) == 0x7f80u || (wd[e] & 0x7f800000u) == 0x7f800000u;
-      }
+      for (int c = lane; c < 16 * H::CH; c += 64)
+        odd |= not_finite(*(const uint4*)(st + H::OPER + 16 * w * H::ROWB + c * 16));
       if (__builtin_amdgcn_ballot_w64(odd)) {
 #pragma unroll 1
         for (int key = 0; key < 16; ++key) {
@@ -637,149 +792,170 @@ __device__ __forceinline__ void shared_rows16(const SharedArgs& a, const Item& i
     for (int d = 0; d < DB; ++d)
       o[d] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(read_tr(st + vat + ((32 * d) ^ vx)), pb, o[d], 0, 0, 0);
   });
+  }
 
   // ---- the four waves' keys joined through LDS ------------------------------
   const float l = quads_sum(lsum);
-  float* po = (float*)lds;             // [wave][16][D]
-  float* pml = po + 4 * H_SMALL * D;   // [wave][16][2]
-  __syncthreads();                     // (every stage is free)
-  if (live) {
+  float* po = (float*)lds;                     // [wave][16][D]
+  float2* pml = (float2*)(po + 4 * H_SMALL * D);  // [wave][16]
+  __syncthreads();                             // (every stage is free)
 #pragma unroll
-    for (int d = 0; d < DB; ++d) *(f32x4*)(po + (w * H_SMALL + r) * D + 16 * d + 4 * q4) = o[d];
-    if (q4 == 0) *(float2*)(pml + (w * H_SMALL + r) * 2) = make_float2(m, l);
-  }
+  for (int d = 0; d < DB; ++d) *(f32x4*)(po + (w * H_SMALL + r) * D + 16 * d + 4 * q4) = o[d];
+  if (q4 == 0) pml[w * H_SMALL + r] = make_float2(m, l);
   __syncthreads();
-  constexpr int LPR = D / 4;
-  for (int i = tid; i < it.rows * LPR; i += 256) {
-    const int row = i / LPR, d = i % LPR * 4;
-    float2 ml[4];
-    float mx = -__builtin_inff(), ls = 0.f;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      ml[j] = *(const float2*)(pml + (j * H_SMALL + row) * 2);
-      mx = fmaxf(mx, ml[j].x);
-    }
-    f32x4 os = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float sc = ml[j].x == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(ml[j].x - mx);
-      ls = fmaf(sc, ml[j].y, ls);
-      const f32x4 oj = *(const f32x4*)(po + (j * H_SMALL + row) * D + d);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) os[e] = fmaf(sc, oj[e], os[e]);
-    }
-    const int64_t nn = it.n0 + row / per;
-    const int64_t at = (int64_t)it.slot * a.B * a.T * a.Hq + nn * a.Hq + it.kv * per + row % per;
-    *(f32x4*)(a.o + at * D + d) = os;
-    if (d == 0) *(float2*)(a.ml + at * 2) = make_float2(mx, ls);
-  }
+  finish_rows<bf16, D, 4, true>(a, it, po, pml, H_SMALL, 0, it.rows);
 }
 
 template <int D>
 __global__ __launch_bounds__(256, 2) void shared_attn_bf16_kernel(SharedArgs a) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   static_assert(Half<D>::LDS >= 4 * H_SMALL * (D + 2) * 4, "the waves' join fits the stages");
-  const Item it = shared_item<H_QT, H_KT>(a, D * 2);
+  Item it;
+  if (!shared_item<H_QT, H_KT>(a, D * 2, it)) return;
   if (it.rows <= H_SMALL)
     shared_rows16<D>(a, it, lds);
   else
     shared_rows128<D>(a, it, lds);
 }
 
-// The slots of each query row joined, in slot order (maxima in base 2). A
-// query that saw no key, in an idle row or one without any, gets zeros.
-template <typename T, int D>
+// The slots of each query row joined (maxima in base 2); every LPR = D / 4 lanes
+// take four dims each. SG sets of lanes share a row, set j the slots j, j + SG,
+// ...: one set a row where there are many rows or few slots. A query that saw
+// no key, in an idle row or one without any, gets zeros.
+template <typename T, int D, int SG>
 __global__ __launch_bounds__(256) void shared_join_kernel(SharedArgs a) {
-  constexpr int LPR = D / 4;  // lanes of a query row, four dims each
+  constexpr int LPR = D / 4, RB = 256 / (LPR * SG);
+  __shared__ __attribute__((aligned(16))) float po[SG > 1 ? 256 * 4 : 4];
+  __shared__ float2 pml[SG > 1 ? SG * RB : 1];
   const int64_t rows = (int64_t)a.B * a.T * a.Hq;
-  const int64_t i = (int64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
-  if (i >= rows) return;
-  const int d = threadIdx.x % LPR * 4;
+  const int lane = threadIdx.x % LPR, sg = threadIdx.x / LPR % SG, rb = threadIdx.x / (LPR * SG);
+  const int64_t i = (int64_t)blockIdx.x * RB + rb;
+  const int64_t row = std::min<int64_t>(i, rows - 1);
   const int slots = a.splits_p + a.splits_s;
-  const bool idle = own_len(a, i / a.Hq / a.T) < 0;
   float m = -__builtin_inff(), l = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  constexpr int NB = 8;  // slots whose loads are in flight together
-  for (int s0 = 0; s0 < slots; s0 += NB) {
+  auto add = [&](float ms, float ls, const f32x4& os, float mn) {
+    if (ms == -__builtin_inff()) return;  // the split saw no key
+    const float a1 = __builtin_amdgcn_exp2f(ms - mn);
+    l = fmaf(ls, a1, l);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = fmaf(os[e], a1, o[e]);
+  };
+  constexpr int NB = 4;  // slots whose loads are in flight together
+  for (int s0 = sg; s0 < slots; s0 += NB * SG) {
     float2 ml[NB];
     f32x4 os[NB];
 #pragma unroll
     for (int u = 0; u < NB; ++u) {
-      const int64_t at = std::min(s0 + u, slots - 1) * rows + i;  // (past the last: read again, left out)
+      const int64_t at = std::min(s0 + u * SG, slots - 1) * rows + row;  // (past the last: read again, left out)
       ml[u] = *(const float2*)(a.ml + at * 2);
-      os[u] = *(const f32x4*)(a.o + at * D + d);
+      os[u] = *(const f32x4*)(a.o + at * D + 4 * lane);
     }
     float mn = m;
 #pragma unroll
     for (int u = 0; u < NB; ++u) {
-      if (s0 + u >= slots) ml[u].x = -__builtin_inff();
+      if (s0 + u * SG >= slots) ml[u].x = -__builtin_inff();
       mn = fmaxf(mn, ml[u].x);
     }
-    if (mn == -__builtin_inff()) continue;  // no split so far saw a key
+    if (mn == -__builtin_inff()) continue;
     const float a0 = __builtin_amdgcn_exp2f(m - mn);
     l *= a0;
     o *= a0;
 #pragma unroll
-    for (int u = 0; u < NB; ++u) {
-      if (ml[u].x == -__builtin_inff()) continue;
-      const float a1 = __builtin_amdgcn_exp2f(ml[u].x - mn);
-      l = fmaf(ml[u].y, a1, l);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] = fmaf(os[u][e], a1, o[e]);
-    }
+    for (int u = 0; u < NB; ++u) add(ml[u].x, ml[u].y, os[u], mn);
     m = mn;
   }
+  if constexpr (SG > 1) {
+    *(f32x4*)(po + threadIdx.x * 4) = o;
+    if (lane == 0) pml[rb * SG + sg] = make_float2(m, l);
+    __syncthreads();
+    if (sg != 0) return;
+    const float2* ml = pml + rb * SG;
+    m = ml[0].x;
+    for (int j = 1; j < SG; ++j) m = fmaxf(m, ml[j].x);
+    l = 0.f;
+    o = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (m != -__builtin_inff())
+      for (int j = 0; j < SG; ++j) add(ml[j].x, ml[j].y, *(const f32x4*)(po + (threadIdx.x + j * LPR) * 4), m);
+  }
+  if (i >= rows) return;
+  const bool empty = m == -__builtin_inff() || own_len(a, i / a.Hq / a.T) < 0;
   float r[4];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) r[e] = idle || m == -__builtin_inff() ? 0.f : o[e] / l;
-  store_vec<T, 4>((T*)a.out + i * D + d, r);
+  for (int e = 0; e < 4; ++e) r[e] = empty ? 0.f : o[e] / l;
+  store_vec<T, 4>((T*)a.out + i * D + 4 * lane, r);
 }
 
-// Query tiles and key splits of a call: enough blocks to fill the CUs twice,
-// no split shorter than two key tiles.
+// Query tiles and key splits of a call.
 struct Plan {
   int qtiles_p, qtiles_s, splits_p, splits_s;
   int64_t items_p, items_s;
+  bool joined;
 };
 
-int64_t splits_for(int64_t blocks, int64_t keys, int kt) {
-  const int64_t want = cdiv((int64_t)2 * 256, std::max<int64_t>(blocks, 1));
-  return std::max<int64_t>(1, std::min<int64_t>(want, keys / (2 * kt)));
-}
+bool bf16_tiles(int dtype, int64_t D) { return dtype == MINITP_BF16 && D >= 32; }
 
-Plan shared_plan(int64_t B, int64_t G, int64_t T, int64_t Hq, int64_t Hkv, int64_t P, int64_t C, int qt, int kt) {
-  const int64_t per = Hq / Hkv;
+// Splits: the prefix part takes 256 blocks, each of at least two key tiles (one
+// on the fp32 path, whose tiles take three times as long), or, where that
+// leaves a block 16 tiles and more, 448 of the 512 places that there are; the
+// own part 256 blocks of at least four tiles. Measured (us a call): 32 rows of
+// the 7B heads on 8,191 and up to 400 keys, 8 units: 16 splits 24.0, 32 22.1,
+// 48 25.3, 64 30.2; 256 rows on 32,256 and 511, 56 units: 7 splits 159.7, 8
+// 161.8, 9 176.1, 12 170.7; 8 rows x 4 of the 0.5B heads on 2,048: 8 splits
+// 12.2, 16 11.6, 32 12.4; fp32, 5 rows x 3 on 777: 6 19.3, 13 12.6.
+//
+// Joined, one item a query tile over both parts and straight to the output:
+// without a prefix; for few keys, where a second launch costs more than the
+// prefix read once a row (4 to 32 rows, 0.5B / 7B heads: 128 + 64 keys 5.8 / 6.8
+// against 8.9 / 10.9, 512 + 64 8.2 / 10.2 against 9.6 / 12.0, 1,024 + 64 11.2 / 15
+// against 10.0 / 12.6); and where the rows' own queries fill their tiles to
+// three quarters and the tiles the CUs (16 rows of 100 tokens on 4,096 keys 123
+// against 133, and no scratch, which grows with the tokens).
+Plan shared_plan(int dtype, int64_t D, int64_t B, int64_t G, int64_t T, int64_t Hq, int64_t Hkv, int64_t P, int64_t C) {
+  const bool tiles16 = bf16_tiles(dtype, D);
+  const int64_t qt = tiles16 ? H_QT : F_QT, kt = tiles16 ? H_KT : F_KT, per = Hq / Hkv;
   Plan p;
   p.qtiles_p = (int)cdiv(B / G * T * per, qt);
   p.qtiles_s = (int)cdiv(T * per, qt);
-  const int64_t bp = P > 0 ? G * Hkv * p.qtiles_p : 0, bs = B * Hkv * p.qtiles_s;
-  p.splits_p = P > 0 ? (int)splits_for(bp + bs, P, kt) : 0;
-  p.splits_s = (int)splits_for(bp * p.splits_p + bs, C + T, kt);
+  const int64_t bp = G * Hkv * p.qtiles_p, bs = B * Hkv * p.qtiles_s;
+  const int64_t tiles_p = cdiv(P, kt), tiles_s = cdiv(C + T, kt);
+  auto within = [](int64_t v, int64_t most) { return (int)std::max<int64_t>(1, std::min(v, most)); };
+  p.splits_p = P > 0 ? within(std::min(448 / bp, std::max(256 / bp, tiles_p / 16)), tiles16 ? tiles_p / 2 : tiles_p) : 0;
+  p.splits_s = within(256 / bs, tiles_s / 4);
+  p.joined = (P == 0 && p.splits_s == 1) || (T * per <= H_SMALL && bs <= 256 && tiles_p + tiles_s <= 8) ||
+             (T * per >= qt && 4 * T * per >= 3 * qt * p.qtiles_s && bs >= 256);
+  if (p.joined) {
+    p.splits_p = 0;
+    p.splits_s = 1;
+  }
   p.items_p = bp * p.splits_p;
   p.items_s = bs * p.splits_s;
   return p;
 }
 
-bool bf16_tiles(int dtype, int64_t D) { return dtype == MINITP_BF16 && D >= 32; }
-
-Plan plan_of(int dtype, int64_t D, int64_t B, int64_t G, int64_t T, int64_t Hq, int64_t Hkv, int64_t P, int64_t C) {
-  if (bf16_tiles(dtype, D)) return shared_plan(B, G, T, Hq, Hkv, P, C, H_QT, H_KT);
-  return shared_plan(B, G, T, Hq, Hkv, P, C, F_QT, D >= 128 ? 32 : 64);
-}
-
 template <typename T, int D>
 int shared_launch(hipStream_t st, const SharedArgs& a, const Plan& p) {
-  const dim3 grid((unsigned)(p.items_p + p.items_s));
+  const dim3 grid((unsigned)(8 * (a.run_p + a.run_s)));
   if constexpr (sizeof(T) == 2 && D >= 32) {
     const int rc = ensure_lds_limit((const void*)shared_attn_bf16_kernel<D>, Half<D>::LDS);
     if (rc) return rc;
     hipLaunchKernelGGL(shared_attn_bf16_kernel<D>, grid, dim3(256), Half<D>::LDS, st, a);
   } else {
-    hipLaunchKernelGGL((shared_attn_f32_kernel<T, D>), grid, dim3(256), 0, st, a);
+    const int rc = ensure_lds_limit((const void*)shared_attn_f32_kernel<T, D>, F_LDS<D>);
+    if (rc) return rc;
+    hipLaunchKernelGGL((shared_attn_f32_kernel<T, D>), grid, dim3(256), F_LDS<D>, st, a);
   }
   MINITP_LAUNCH_CHECK();
+  if (p.joined) return MINITP_OK;
   const int64_t rows = (int64_t)a.B * a.T * a.Hq;
-  hipLaunchKernelGGL((shared_join_kernel<T, D>), dim3((unsigned)cdiv(rows, 256 / (D / 4))), dim3(256), 0, st, a);
+  constexpr int SG = 256 / (D / 4);
+  // (several sets of lanes a row while there are few rows: 7,168 rows of 9
+  // slots 8.3 us with one set, 18.3 with eight; 896 rows of 33 slots 5.7 us with
+  // eight)
+  if (p.splits_p + p.splits_s >= 4 && rows * (D / 4) < 131072)
+    hipLaunchKernelGGL((shared_join_kernel<T, D, SG>), dim3((unsigned)rows), dim3(256), 0, st, a);
+  else
+    hipLaunchKernelGGL((shared_join_kernel<T, D, 1>), dim3((unsigned)cdiv(rows, SG)), dim3(256), 0, st, a);
   MINITP_LAUNCH_CHECK();
   return MINITP_OK;
 }
@@ -805,23 +981,28 @@ int shared_by_d(hipStream_t st, const SharedArgs& a, const Plan& p, int64_t D) {
 int64_t shared_prefix_workspace_bytes(int dtype, int64_t B, int64_t G, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
                                       int64_t P, int64_t C) {
   if (B * T == 0) return 0;
-  const Plan p = plan_of(dtype, D, B, G, T, Hq, Hkv, P, C);
-  return (p.splits_p + p.splits_s) * B * T * Hq * (D + 2) * 4;
+  const Plan p = shared_plan(dtype, D, B, G, T, Hq, Hkv, P, C);
+  return p.joined ? 0 : (p.splits_p + p.splits_s) * B * T * Hq * (D + 2) * 4;
 }
 
 int launch_shared_prefix_attention(hipStream_t st, int dtype, const SharedPrefixShape& s, const void* q,
                                    const void* k_prefix, const void* v_prefix, const void* k_cache,
                                    const void* v_cache, void* out, const int64_t* prefix_lens,
                                    const int64_t* cache_lens, void* workspace, int64_t workspace_bytes) {
-  const Plan p = plan_of(dtype, s.D, s.B, s.G, s.T, s.Hq, s.Hkv, s.P, s.C);
+  const Plan p = shared_plan(dtype, s.D, s.B, s.G, s.T, s.Hq, s.Hkv, s.P, s.C);
   const int64_t need = shared_prefix_workspace_bytes(dtype, s.B, s.G, s.T, s.Hq, s.Hkv, s.D, s.P, s.C);
-  if (workspace_bytes < need || workspace == nullptr || !aligned16(workspace)) {
+  if (workspace_bytes < need || (workspace == nullptr && need > 0) || !aligned16(workspace)) {
     set_error("shared_prefix_attention: workspace %p of %lld B, %lld B needed (16-byte aligned)", workspace,
               (long long)workspace_bytes, (long long)need);
     return MINITP_ERR_ARG;
   }
   const int64_t rows = s.B * s.T * s.Hq;
-  if (p.items_p + p.items_s >= (1LL << 31) || rows >= (1LL << 31) || s.B / s.G * s.T * (s.Hq / s.Hkv) >= (1LL << 31)) {
+  if (s.P >= (1LL << 31) - 64 || s.C + s.T >= (1LL << 31) - 64) {
+    set_error("shared_prefix_attention: %lld prefix and %lld + %lld own rows are too many", (long long)s.P,
+              (long long)s.C, (long long)s.T);
+    return MINITP_ERR_UNSUPPORTED;
+  }
+  if (p.items_p + p.items_s >= (1LL << 31) - 16 || rows >= (1LL << 31) || s.B / s.G * s.T * (s.Hq / s.Hkv) >= (1LL << 31)) {
     set_error("shared_prefix_attention: %lld query rows are too many for one call", (long long)rows);
     return MINITP_ERR_UNSUPPORTED;
   }
@@ -848,7 +1029,11 @@ int launch_shared_prefix_attention(hipStream_t st, int dtype, const SharedPrefix
   a.qtiles_s = p.qtiles_s;
   a.splits_p = p.splits_p;
   a.splits_s = p.splits_s;
-  a.items_p = p.items_p;
+  a.items_p = (int)p.items_p;
+  a.items_s = (int)p.items_s;
+  a.run_p = (int)cdiv(p.items_p, 8);
+  a.run_s = (int)cdiv(p.items_s, 8);
+  a.joined = p.joined;
   a.o = (float*)workspace;
   a.ml = a.o + (p.splits_p + p.splits_s) * rows * s.D;
   return dtype == MINITP_F32 ? shared_by_d<float>(st, a, p, s.D) : shared_by_d<bf16>(st, a, p, s.D);

@@ -103,13 +103,14 @@ def test_several_tokens(t, p, c, hq, hkv, d, dtype):
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("t", [1, 5])
 @pytest.mark.parametrize("hq,hkv,d", [(14, 2, 64), (28, 4, 128), (4, 2, 16)])
-def test_unequal_empty_and_idle_rows(hq, hkv, d, t, dtype):
+@pytest.mark.parametrize("p", [300, 1500])  # both parts by one block, or by blocks of their own
+def test_unequal_empty_and_idle_rows(p, hq, hkv, d, t, dtype):
     """Prefixes of length 0 and 1, rows without cached tokens, idle rows."""
     from minitp import kernels as K
 
-    plens, clens = [300, 0, 1], [0, 90, -1, 17, 64, -1, 90, 1, 33]
-    x = make(9, 3, t, hq, hkv, d, 300, 90, dtype, plens, clens)
-    out = K.shared_prefix_attention(*x[:5], 300, 90, prefix_lens=torch.tensor(plens, device=DEV),
+    plens, clens = [p, 0, 1], [0, 90, -1, 17, 64, -1, 90, 1, 33]
+    x = make(9, 3, t, hq, hkv, d, p, 90, dtype, plens, clens)
+    out = K.shared_prefix_attention(*x[:5], p, 90, prefix_lens=torch.tensor(plens, device=DEV),
                                     cache_lens=torch.tensor(clens, device=DEV, dtype=torch.int32))
     check(out, *x)
     assert (out[2] == 0).all() and (out[5] == 0).all()
@@ -208,6 +209,33 @@ def test_cache_views_streams_and_graph():
         q.normal_()
         clens.copy_((clens + 7) % 50)
         plens.copy_((plens + 41) % 301)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("hq,hkv,d", [(8, 8, 64), (28, 4, 128)])
+def test_prompts_that_fill_the_chip(hq, hkv, d, dtype):
+    """Rows whose own queries fill whole query tiles (one block over both
+    parts), unequal, one idle."""
+    from minitp import kernels as K
+
+    b, t, p, c = 36, 130 * hkv // hq if hq > hkv else 130, 200, 70
+    plens, clens = [p, 131], [c - i % 9 * 7 for i in range(b)]
+    clens[5] = -1
+    q, kp, vp, kc, vc, _, _ = make(b, 2, t, hq, hkv, d, p, c, dtype, plens, clens)
+    out = K.shared_prefix_attention(q, kp, vp, kc, vc, p, c, torch.tensor(plens, device=DEV),
+                                    torch.tensor(clens, device=DEV)).view(b, t, hq, d).double()
+    assert (out[5] == 0).all()
+    for i in range(b):
+        if clens[i] < 0:
+            continue
+        g, per = i // (b // 2), hq // hkv
+        k, v = (torch.cat([x[g, :, :plens[g]], y[i, :, :clens[i] + t]], 1).double().repeat_interleave(per, 0)
+                for x, y in ((kp, kc), (vp, vc)))
+        s = q[i].double().transpose(0, 1) @ k.transpose(-1, -2).contiguous() / d ** 0.5
+        last = plens[g] + clens[i] + torch.arange(t, device=DEV)
+        pr = s.masked_fill(torch.arange(k.shape[1], device=DEV) > last[:, None], float("-inf")).softmax(-1)
+        ref, mag = (pr @ v).transpose(0, 1), (pr @ v.abs()).transpose(0, 1)
+        assert ((out[i] - ref).abs() <= bars(ref, mag, dtype, d) + 1e-9).all(), i
 
 
 def test_many_keys_and_rows():
