@@ -221,8 +221,8 @@ int minitp_shared_prefix_attention(void* stream, int dtype, const void* q, const
  * Token v continues beam w with score s + x_v - logsumexp(x); a finished beam
  * continues with eos_token at its own score and length. Of a group's
  * continuations above minus infinity the W of the largest score / length ^
- * length_penalty win (length: with the new token, at least 1), equal ones by
- * the lower beam, then the lower token. A NaN score wins over every number.
+ * length_penalty (-16 to 16) win (length: with the new token, at least 1),
+ * equal ones by the lower beam, then the lower token. A NaN score wins over every number.
  * The first winner of a parent stays in the parent's slot, the others fill the
  * free slots in rank order; a slot left over is its own parent with a score of
  * minus infinity, marked finished. Outputs, all [G, W], which may be the

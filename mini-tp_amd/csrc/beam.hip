@@ -11,9 +11,13 @@
 // caches move as few rows as the selection allows (and no moved row's source
 // is overwritten).
 //
-// Two launches, as the argmax has: slices of the logits rows to (maximum, sum
-// of exponentials, W best tokens), then one block a group. The order of a row's
-// tokens is that of its logits, so a slice needs no sum of the whole row.
+// Two launches, as the argmax has. The first streams the logits: per wave a
+// maximum and a sum of exponentials, per set of 64 consecutive logits their
+// maximum. The second, one block a group, ranks the sets by the key of their
+// maximum: whatever is among the W best tokens lies in the W best sets (W
+// tokens, the sets' maxima, stand before every token of any other set), so
+// only those sets' logits are read again. The order of a row's tokens is that
+// of its logits, so the first launch needs no sum of the whole row.
 #include <cmath>
 
 #include "common.h"
@@ -23,15 +27,20 @@ namespace minitp {
 
 namespace {
 
-constexpr int SEL_T = 256, SEL_E = 16, SEL_SLICE = SEL_T * SEL_E;  // a slice: 16 consecutive logits a thread
+constexpr int SEL_T = 256, SEL_NV = 4;  // threads of a slice, 16-byte loads a thread
+constexpr int SET = 64;                 // logits of a set
 constexpr int MERGE_T = 1024;
-constexpr int MERGE_CAP = 1024;  // contenders that a group's final ranking takes
+constexpr int MERGE_CAP = 1024;  // sets that a group's ranking takes at once
+
+template <typename T>
+constexpr int SLICE = SEL_T * SEL_NV * Vec<T>::N;
 
 struct SelectArgs {
   const void* logits;
   int64_t ld_group, ld_beam;  // elements between groups and between beams (0: one row for all)
   int64_t V;
   int G, W, slices;
+  int sets;                 // of a row, padded to whole float4
   const float* scores;      // [G, W]
   const uint8_t* finished;  // [G, W] or NULL
   const int64_t* lengths;   // [G, W] or NULL (zeros)
@@ -41,11 +50,9 @@ struct SelectArgs {
   float* scores_out;
   uint8_t* finished_out;
   int64_t* lengths_out;
-  // per (row, slice)
-  double* sum;
-  float* top;
-  float* cand_v;    // [W] a slice, best first
-  int32_t* cand_i;  // token, -1: none
+  double* sum;     // [row][slice][wave]: sum of exponentials above ...
+  float* top;      // ... this maximum
+  float* set_top;  // [row][sets]
 };
 
 template <typename T>
@@ -53,143 +60,92 @@ __device__ __forceinline__ const T* logits_row(const SelectArgs& a, int64_t row)
   return (const T*)a.logits + row / a.W * a.ld_group + row % a.W * a.ld_beam;
 }
 
-// A row that is read: alive (a finite cumulative score) and not finished.
+// A row that is read: alive (a cumulative score above minus infinity) and not finished.
 __device__ __forceinline__ bool beam_open(const SelectArgs& a, int64_t row) {
   return a.scores[row] != -__builtin_inff() && !(a.finished != nullptr && a.finished[row]);
 }
 
-// Contenders of a slice without sorting it: the W-th largest of the 64 maxima
-// of four threads each (64 logits) bounds the slice's W-th largest logit from
-// below. Fewer than W of those sets hold a logit above the bound, at most 64
-// each; of the logits equal to it the first W in order are enough.
-constexpr int SEL_CAP = 31 * 64 + 32;
+// exp(x) for x <= 0 by the hardware's 2^x, the product x log2(e) carried in two
+// parts: its rounding alone, up to 2^-24 of an exponent of some tens, would be
+// the sum's largest error.
+__device__ __forceinline__ float exp_below(float x) {
+  constexpr float L = 1.44269502f, L_LO = 1.92596299e-8f, LN2 = 0.693147182f;
+  const float hi = x * L, lo = fmaf(x, L_LO, fmaf(x, L, -hi));
+  const float e = __builtin_amdgcn_exp2f(hi);
+  return x == -__builtin_inff() ? 0.f : fmaf(e, lo * LN2, e);
+}
 
+// One slice of a row a block: lanes take 16 bytes each of consecutive logits, so
+// that a set is 8 (bf16) or 16 (fp32) lanes of one load. Nothing is exchanged
+// between the waves.
 template <typename T>
 __global__ __launch_bounds__(SEL_T) void beam_slice_kernel(SelectArgs a) {
-  __shared__ __attribute__((aligned(16))) float quad_top[64];
-  __shared__ float lv[SEL_CAP];
-  __shared__ int32_t li[SEL_CAP];
-  __shared__ int wave_cnt[4];
-  __shared__ float wave_m[4];
-  __shared__ double wave_s[4];
+  constexpr int VE = Vec<T>::N, LPS = SET / VE;
   const int64_t row = blockIdx.x / a.slices, slice = blockIdx.x % a.slices;
   if (!beam_open(a, row)) return;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, W = a.W;
-  const T* lr = logits_row<T>(a, row) + slice * SEL_SLICE;
-  const int n = (int)std::min<int64_t>(a.V - slice * SEL_SLICE, SEL_SLICE);  // logits of this slice
-  const int j0 = tid * SEL_E;
-
-  float x[SEL_E];
-  if ((((uint64_t)lr) & 15) == 0 && j0 + SEL_E <= n) {
-    constexpr int VE = Vec<T>::N;
-    uint4 raw[SEL_E / VE];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const T* lr = logits_row<T>(a, row) + slice * SLICE<T>;
+  const int n = (int)std::min<int64_t>(a.V - slice * SLICE<T>, SLICE<T>);  // logits of this slice
+  float x[SEL_NV][VE];
+  if ((((uint64_t)lr) & 15) == 0) {
+    const __amdgpu_buffer_rsrc_t r = span_rsrc(lr, (uint32_t)(n * (int)sizeof(T)));
+    u32x4 raw[SEL_NV];
 #pragma unroll
-    for (int u = 0; u < SEL_E / VE; ++u) raw[u] = *(const uint4*)(lr + j0 + u * VE);
+    for (int v = 0; v < SEL_NV; ++v) {
+      // (whole vectors only; the others read zeros here)
+      const int j = (v * SEL_T + tid) * VE;
+      raw[v] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                             r, j + VE <= n ? (uint32_t)(j * (int)sizeof(T)) : 0xffffffffu, 0, 0));
+    }
 #pragma unroll
-    for (int u = 0; u < SEL_E / VE; ++u) unpack16(raw[u], x + u * VE, (T*)nullptr);
+    for (int v = 0; v < SEL_NV; ++v) {
+      unpack16(make_uint4(raw[v].x, raw[v].y, raw[v].z, raw[v].w), x[v], (T*)nullptr);
+      const int j = (v * SEL_T + tid) * VE;
+      if (j + VE > n) {
+#pragma unroll
+        for (int e = 0; e < VE; ++e) x[v][e] = j + e < n ? load_f32<T>(lr, j + e) : -__builtin_inff();
+      }
+    }
   } else {
 #pragma unroll
-    for (int e = 0; e < SEL_E; ++e) x[e] = j0 + e < n ? load_f32<T>(lr, j0 + e) : -__builtin_inff();
+    for (int v = 0; v < SEL_NV; ++v)
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        const int j = (v * SEL_T + tid) * VE + e;
+        x[v][e] = j < n ? load_f32<T>(lr, j) : -__builtin_inff();
+      }
   }
 
-  // ---- maximum and sum of exponentials (a NaN shows in the sum) -----------
-  float t = x[0];
+  const float ninf = -__builtin_inff();
+  float t = ninf;
 #pragma unroll
-  for (int e = 1; e < SEL_E; ++e) t = fmaxf(t, x[e]);
-  t = t == t ? t : -__builtin_inff();
-  const float wm = wave_max(t), ref = wm == -__builtin_inff() ? 0.f : wm;
-  float s = 0.f;
+  for (int v = 0; v < SEL_NV; ++v) {
+    float m = ninf;  // (a NaN is no maximum; it shows in the sum)
 #pragma unroll
-  for (int e = 0; e < SEL_E; ++e) s += expf(x[e] - ref);
-  double ws = s;
+    for (int e = 0; e < VE; ++e) m = fmaxf(m, x[v][e]);
+    t = fmaxf(t, m);
+    m = fmaxf(m, dpp_f32<0xB1>(ninf, m));   // lanes of the set: quad_perm [1,0,3,2]
+    m = fmaxf(m, dpp_f32<0x4E>(ninf, m));   // quad_perm [2,3,0,1]
+    m = fmaxf(m, dpp_f32<0x141>(ninf, m));  // row_half_mirror
+    if constexpr (LPS == 16) m = fmaxf(m, dpp_f32<0x140>(ninf, m));  // row_mirror
+    const int64_t set = (slice * SLICE<T> + (v * SEL_T + tid) * VE) / SET;
+    if (lane % LPS == 0 && set < a.sets) a.set_top[row * a.sets + set] = m;
+  }
+  const float wm = wave_max(t), ref = wm == ninf ? 0.f : wm;
+  float s[SEL_NV];  // (a chain a load)
+#pragma unroll
+  for (int v = 0; v < SEL_NV; ++v) {
+    s[v] = 0.f;
+#pragma unroll
+    for (int e = 0; e < VE; ++e) s[v] += exp_below(x[v][e] - ref);
+  }
+  double ws = (double)((s[0] + s[1]) + (s[2] + s[3]));
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) ws += __shfl_xor(ws, o, 64);
   if (lane == 0) {
-    wave_m[wave] = wm;
-    wave_s[wave] = ws;
-  }
-
-  // ---- the bound ------------------------------------------------------------
-  float qt = fmaxf(t, dpp_f32<0xB1>(t, t));
-  qt = fmaxf(qt, dpp_f32<0x4E>(qt, qt));
-  if ((lane & 3) == 0) quad_top[wave * 16 + lane / 4] = qt;
-  __syncthreads();
-  float bound;
-  {
-    const float v = quad_top[lane];
-    int better = 0;
-#pragma unroll
-    for (int j = 0; j < 64; ++j) {
-      const float u = quad_top[j];
-      better += u > v || (u == v && j < lane);
-    }
-    const uint64_t at = __builtin_amdgcn_ballot_w64(better == W - 1);
-    bound = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), __builtin_ctzll(at)));
-  }
-
-  // ---- contenders: above the bound in the low half, equal to it in the high
-  const bool low = bound == -__builtin_inff();  // (equal: not a candidate)
-  int cnt = 0;
-#pragma unroll
-  for (int e = 0; e < SEL_E; ++e) cnt += (x[e] > bound ? 1 : 0) + (x[e] == bound && !low ? 1 << 16 : 0);
-  int before = cnt;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int u = __shfl_up(before, o, 64);
-    if (lane >= o) before += u;
-  }
-  if (lane == 63) wave_cnt[wave] = before;
-  before -= cnt;
-  __syncthreads();
-  int total = 0;
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    if (w == wave) before += total;
-    total += wave_cnt[w];
-  }
-  const int above = total & 0xffff, equal = std::min(total >> 16, W);
-  if (cnt != 0) {
-    int pa = before & 0xffff, pe = before >> 16;
-#pragma unroll
-    for (int e = 0; e < SEL_E; ++e) {
-      if (x[e] > bound) {
-        lv[pa] = x[e];
-        li[pa++] = j0 + e;
-      } else if (x[e] == bound && !low) {
-        if (pe < equal) {
-          lv[above + pe] = x[e];
-          li[above + pe] = j0 + e;
-        }
-        ++pe;
-      }
-    }
-  }
-  __syncthreads();
-
-  // ---- rank them; the W best, best first -----------------------------------
-  const int c = above + equal;
-  const int64_t at = row * a.slices + slice;
-  float* cv = a.cand_v + at * W;
-  int32_t* ci = a.cand_i + at * W;
-  for (int i = tid; i < c; i += SEL_T) {
-    const float v = lv[i];
-    const int vi = li[i];
-    int rank = 0;
-    for (int j = 0; j < c; ++j) rank += lv[j] > v || (lv[j] == v && li[j] < vi);
-    if (rank < W) {
-      cv[rank] = v;
-      ci[rank] = (int32_t)(slice * SEL_SLICE + vi);
-    }
-  }
-  for (int i = c + tid; i < W; i += SEL_T) ci[i] = -1;
-  if (tid == 0) {
-    float m = wave_m[0];
-    for (int w = 1; w < 4; ++w) m = fmaxf(m, wave_m[w]);
-    double sum = 0.0;
-    for (int w = 0; w < 4; ++w)
-      sum += wave_m[w] == -__builtin_inff() ? wave_s[w] : wave_s[w] * exp((double)wave_m[w] - (double)m);
-    a.top[at] = m;
-    a.sum[at] = sum;
+    const int64_t at = (row * a.slices + slice) * (SEL_T / 64) + wave;
+    a.top[at] = wm;
+    a.sum[at] = ws;
   }
 }
 
@@ -204,37 +160,91 @@ __device__ __forceinline__ uint64_t order_key(double k) {
 
 enum { ROW_NONE = 0, ROW_OPEN = 1, ROW_DONE = 2, ROW_NAN = 3 };
 
-template <typename T>
-__global__ __launch_bounds__(MERGE_T) void beam_merge_kernel(SelectArgs a) {
+// The rows of a group, MERGE_T / wp threads each (wp >= W, a power of two). A
+// thread keeps its sets' maxima, at most 4 NR (0: any number, read again).
+template <typename T, int NR>
+__global__ __launch_bounds__(MERGE_T) void beam_merge_kernel(SelectArgs a, int wp) {
   __shared__ int kind[32];
   __shared__ float score[32];
   __shared__ double lse[32], inv[32];
   __shared__ uint64_t group_top[64];
-  __shared__ uint64_t lk[MERGE_CAP], lf[MERGE_CAP];  // key; beam << 32 | token
+  __shared__ uint64_t lk[MERGE_CAP], lf[MERGE_CAP];        // sets: key of the maximum; beam << 32 | set
+  __shared__ float lx[MERGE_CAP];                          // maximum
+  __shared__ uint64_t ek[32 * SET], ef[32 * SET];          // tokens of the best sets: key; beam << 32 | token
   __shared__ uint64_t best_k[MERGE_T / 64], best_f[MERGE_T / 64];
-  __shared__ int count;
-  __shared__ uint64_t sel[32];
+  __shared__ int count, ecount;
+  __shared__ uint64_t limit;
+  __shared__ uint64_t set_k[32], set_f[32], sel[32];
+  __shared__ float ex[32 * SET], sel_x[32];                // their logits
+  __shared__ uint8_t ended[32];
+  __shared__ int64_t length[32];
+  __shared__ int first[32];                                // best rank of a parent
   const int W = a.W, g = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t row0 = (int64_t)g * W;
   const int eos32 = (int)a.eos;
 
-  // ---- each beam's log sum, kind and length factor -------------------------
-  for (int w = wave; w < W; w += MERGE_T / 64) {
+  // This thread's sets, four at a time: f(set, maximum). (A row that is not open
+  // has no maxima: what its words hold is left out below.)
+  const int tpr = MERGE_T / wp, mw = tid / tpr, mj = tid % tpr, quads = mw < W ? a.sets / 4 : 0;
+  const float4* set_top = (const float4*)(a.set_top + (row0 + mw) * a.sets);
+  auto four = [&](int i, const float4& x, auto f) {
+    f(4 * i, x.x);
+    f(4 * i + 1, x.y);
+    f(4 * i + 2, x.z);
+    f(4 * i + 3, x.w);
+  };
+  auto read_sets = [&](auto f) {
+#pragma unroll 4
+    for (int i = mj; i < quads; i += tpr) four(i, set_top[i], f);
+  };
+  float4 kept[NR > 0 ? NR : 1];
+  auto each_set = [&](auto f) {
+    if constexpr (NR > 0) {
+#pragma unroll
+      for (int u = 0; u < NR; ++u)
+        if (mj + u * tpr < quads) four(mj + u * tpr, kept[u], f);
+    } else {
+      read_sets(f);
+    }
+  };
+
+  // ---- each beam's log sum, kind and length factor, a wave a beam; the first
+  // ones' loads are in flight with those of the sets' maxima -----------------
+  const int parts = a.slices * (SEL_T / 64);
+  constexpr int PRE = 3;
+  float sc = 0.f, pt[PRE];
+  double ps[PRE];
+  bool done = false;
+  int64_t len = 0;
+  auto load_beam = [&](int w) {
     const int64_t row = row0 + w;
-    const float sc = a.scores[row];
-    const bool done = a.finished != nullptr && a.finished[row];
+    sc = a.scores[row];
+    done = a.finished != nullptr && a.finished[row];
+    len = a.lengths != nullptr ? a.lengths[row] : 0;
+#pragma unroll
+    for (int u = 0; u < PRE; ++u) {
+      const int i = std::min(lane + 64 * u, parts - 1);
+      pt[u] = a.top[row * parts + i];
+      ps[u] = a.sum[row * parts + i];
+    }
+  };
+  auto beam = [&](int w) {
+    const int64_t row = row0 + w;
     int k = sc == -__builtin_inff() ? ROW_NONE : done ? ROW_DONE : sc != sc ? ROW_NAN : ROW_OPEN;
-    double m = -__builtin_inf(), s = 0.0;
+    double m = 0.0, s = 1.0;
     if (k == ROW_OPEN) {
+      s = 0.0;
       float mf = -__builtin_inff();
-      for (int i = lane; i < a.slices; i += 64) mf = fmaxf(mf, a.top[row * a.slices + i]);
+#pragma unroll
+      for (int u = 0; u < PRE; ++u)
+        if (lane + 64 * u < parts) mf = fmaxf(mf, pt[u]);
+      for (int i = lane + 64 * PRE; i < parts; i += 64) mf = fmaxf(mf, a.top[row * parts + i]);
       mf = wave_max(mf);
-      m = mf;
-      for (int i = lane; i < a.slices; i += 64) {
-        const float t = a.top[row * a.slices + i];
-        const double si = a.sum[row * a.slices + i];
-        s += t == -__builtin_inff() ? si : si * exp((double)t - m);
-      }
+      auto add = [&](float t, double si) { s += t == -__builtin_inff() ? si : si * (double)exp_below(t - mf); };
+#pragma unroll
+      for (int u = 0; u < PRE; ++u)
+        if (lane + 64 * u < parts) add(pt[u], ps[u]);
+      for (int i = lane + 64 * PRE; i < parts; i += 64) add(a.top[row * parts + i], a.sum[row * parts + i]);
 #pragma unroll
       for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o, 64);
       // no logit above minus infinity: nothing continues this beam
@@ -242,96 +252,130 @@ __global__ __launch_bounds__(MERGE_T) void beam_merge_kernel(SelectArgs a) {
         k = ROW_NAN;
       else if (mf == -__builtin_inff())
         k = ROW_NONE;
+      m = mf;
     }
+    // one logarithm for both: of the sum (lane 0) and of the length (lane 1)
+    const double lg = log(lane == 1 ? (double)std::max<int64_t>(len + (done ? 0 : 1), 1) : s);
     if (lane == 0) {
-      const int64_t len = (a.lengths != nullptr ? a.lengths[row] : 0) + (done ? 0 : 1);
       kind[w] = k;
       score[w] = sc;
-      lse[w] = k == ROW_OPEN ? m + log(s) : 0.0;
-      inv[w] = a.alpha == 0.0 ? 1.0 : pow((double)std::max<int64_t>(len, 1), -a.alpha);
+      ended[w] = done;
+      length[w] = len;
+      first[w] = 64;
+      lse[w] = m + lg;
     }
-  }
-  if (tid == 0) count = 0;
-  __syncthreads();
-
-  // candidate e = (beam, slice, rank): its key (0: none) and token
-  const int per_row = a.slices * W, entries = per_row * W;
-  auto candidate = [&](int e, uint64_t& flat) -> uint64_t {
-    const int w = e / per_row, i = e - w * per_row;
-    const int k = kind[w];
-    int token;
-    uint64_t key = 0;
-    if (k == ROW_OPEN) {
-      token = a.cand_i[row0 * per_row + e];
-      if (token >= 0) {
-        const double lp = (double)a.cand_v[row0 * per_row + e] - lse[w];
-        key = order_key(((double)score[w] + lp) * inv[w]);
-      }
-    } else if (k == ROW_DONE) {
-      token = eos32;
-      if (i == 0) key = order_key((double)score[w] * inv[w]);
-    } else {
-      token = i;
-      if (k == ROW_NAN && i < W && i < a.V) key = ~0ull;
-    }
-    flat = (uint64_t)w << 32 | (uint32_t)token;
-    return key;
+    if (lane == 1) inv[w] = a.alpha == 0.0 ? 1.0 : exp(-a.alpha * lg);
   };
-  auto better = [](uint64_t ka, uint64_t fa, uint64_t kb, uint64_t fb) { return ka > kb || (ka == kb && fa < fb); };
-
-  // ---- contenders, as in the slices: the W-th largest of 64 maxima ----------
-  uint64_t top = 0, flat;
-  for (int e = tid; e < entries; e += MERGE_T) top = std::max(top, candidate(e, flat));
+  if (tid == 0) count = ecount = 0;
+  if (wave < W) load_beam(wave);
+  if constexpr (NR > 0) {
 #pragma unroll
-  for (int o = 8; o >= 1; o >>= 1) {
-    const uint64_t u = __shfl_xor(top, o, 64);
-    top = u > top ? u : top;
+    for (int u = 0; u < NR; ++u) kept[u] = set_top[std::min(mj + u * tpr, std::max(quads - 1, 0))];
   }
-  if (lane % 16 == 0) group_top[tid / 16] = top;
+  float most = -__builtin_inff();
+  each_set([&](int, float x) { most = fmaxf(most, x); });
+  if (wave < W) beam(wave);
+  if (wave + MERGE_T / 64 < W) {
+    load_beam(wave + MERGE_T / 64);
+    beam(wave + MERGE_T / 64);
+  }
   __syncthreads();
-  uint64_t bound;
-  {
-    const uint64_t v = group_top[lane];
-    int ahead = 0;
-    for (int j = 0; j < 64; ++j) {
-      const uint64_t u = group_top[j];
-      ahead += u > v || (u == v && j < lane);
+
+  auto key_of = [&](int w, float x) { return order_key(((double)score[w] + ((double)x - lse[w])) * inv[w]); };
+  auto better = [](uint64_t ka, uint64_t fa, uint64_t kb, uint64_t fb) { return ka > kb || (ka == kb && fa < fb); };
+  // ranks of n entries, 32 lanes an entry: f(rank, index)
+  auto rank_all = [&](const uint64_t* k, const uint64_t* f, int n, auto put) {
+    for (int i = tid / 32; i < n; i += MERGE_T / 32) {
+      int ahead = 0;
+      for (int j = tid % 32; j < n; j += 32) ahead += better(k[j], f[j], k[i], f[i]);
+#pragma unroll
+      for (int o = 16; o >= 1; o >>= 1) ahead += __shfl_xor(ahead, o, 64);
+      if (tid % 32 == 0 && ahead < W) put(ahead, i);
     }
-    bound = __shfl(v, __builtin_ctzll(__builtin_amdgcn_ballot_w64(ahead == W - 1)), 64);
+  };
+  // A finished beam and one that is no number have one set, the first, with a
+  // key of its own.
+  const int mkind = mw < W ? kind[mw] : ROW_NONE;
+  const uint64_t only = mj != 0 ? 0 : mkind == ROW_DONE ? order_key((double)score[mw] * inv[mw])
+                                    : mkind == ROW_NAN  ? ~0ull
+                                                        : 0;
+
+  // ---- a bound: the W-th largest of the 64 maxima of 16 threads each ---------
+  // (16 threads of one row: one DPP row)
+  float rmost = most;
+  rmost = fmaxf(rmost, dpp_f32<0xB1>(rmost, rmost));
+  rmost = fmaxf(rmost, dpp_f32<0x4E>(rmost, rmost));
+  rmost = fmaxf(rmost, dpp_f32<0x141>(rmost, rmost));
+  rmost = fmaxf(rmost, dpp_f32<0x140>(rmost, rmost));
+  // (the row's thread of the one set is its first)
+  if (lane % 16 == 0) group_top[tid / 16] = mkind == ROW_OPEN ? key_of(mw, rmost) : only;
+  __syncthreads();
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {  // a wave ranks four of them
+    const int i = wave * 4 + c;
+    const uint64_t u = group_top[lane], v = group_top[i];
+    const uint64_t ahead = __builtin_amdgcn_ballot_w64(u > v || (u == v && lane < i));
+    if (lane == 0 && __builtin_popcountll(ahead) == W - 1) limit = std::max<uint64_t>(v, 1);
   }
-  bound = std::max<uint64_t>(bound, 1);
-  for (int e = tid; e < entries; e += MERGE_T) {
-    const uint64_t k = candidate(e, flat);
-    if (k < bound) continue;
+  __syncthreads();
+  const uint64_t bound = limit;
+
+  // ---- the W best sets: first those whose maxima reach the bound, taken as a
+  // logit of their row and lowered past what its rounding can be -------------
+  auto take = [&](float x, int set) {
     const int at = atomicAdd(&count, 1);
     if (at < MERGE_CAP) {
-      lk[at] = k;
-      lf[at] = flat;
+      lx[at] = x;
+      lf[at] = (uint64_t)mw << 32 | (uint32_t)set;
     }
+  };
+  if (mkind == ROW_OPEN && bound != ~0ull) {
+    const double bk = __builtin_bit_cast(double, bound >> 63 ? bound ^ (1ull << 63) : ~bound);
+    const float bx = (float)((bk / inv[mw] - (double)score[mw]) + lse[mw]);
+    // (above minus infinity at least: those are no candidates)
+    const float low = bound == 1 ? -3.402823466e38f : fmaxf(bx - (fabsf(bx) + 1.f) * 1e-5f, -3.402823466e38f);
+    if (most >= low)
+      each_set([&](int set, float x) {
+        if (x >= low) take(x, set);
+      });
+  } else if (only != 0) {
+    take(0.f, 0);
   }
   __syncthreads();
   int n = count;
-  if (n <= MERGE_CAP) {
-    for (int i = tid; i < n; i += MERGE_T) {
-      const uint64_t k = lk[i], f = lf[i];
-      int rank = 0;
-      for (int j = 0; j < n; ++j) rank += better(lk[j], lf[j], k, f);
-      if (rank < W) sel[rank] = f;
+  uint64_t least = bound;
+  for (int i = tid; i < std::min(n, MERGE_CAP); i += MERGE_T) {
+    const int w = (int)(lf[i] >> 32);
+    lk[i] = kind[w] == ROW_OPEN ? key_of(w, lx[i]) : kind[w] == ROW_DONE ? order_key((double)score[w] * inv[w]) : ~0ull;
+  }
+  __syncthreads();
+  if (n <= 32) {  // few enough to take all
+    if (tid < n) {
+      set_k[tid] = lk[tid];
+      set_f[tid] = lf[tid];
     }
-    n = std::min(n, W);
+  } else if (n <= MERGE_CAP) {
+    rank_all(lk, lf, n, [&](int rank, int i) {
+      set_k[rank] = lk[i];
+      set_f[rank] = lf[i];
+    });
+    n = W;
   } else {
-    // more equals than the list holds: one winner at a time
-    uint64_t pk = ~0ull, pf = 0;
-    bool first = true;
+    // more equal sets than the list holds: one winner at a time
+    uint64_t pk = 0, pf = 0;
     for (n = 0; n < W; ++n) {
       uint64_t bk = 0, bf = ~0ull;
-      for (int e = tid; e < entries; e += MERGE_T) {
-        const uint64_t k = candidate(e, flat);
-        if (k != 0 && (first || better(pk, pf, k, flat)) && better(k, flat, bk, bf)) {
+      auto see = [&](uint64_t k, int set) {
+        const uint64_t f = (uint64_t)mw << 32 | (uint32_t)set;
+        if (k != 0 && (n == 0 || better(pk, pf, k, f)) && better(k, f, bk, bf)) {
           bk = k;
-          bf = flat;
+          bf = f;
         }
-      }
+      };
+      if (mkind == ROW_OPEN)
+        read_sets([&](int set, float x) { see(key_of(mw, x), set); });
+      else
+        see(only, 0);
 #pragma unroll
       for (int o = 32; o >= 1; o >>= 1) {
         const uint64_t ok = __shfl_xor(bk, o, 64), of = __shfl_xor(bf, o, 64);
@@ -352,55 +396,77 @@ __global__ __launch_bounds__(MERGE_T) void beam_merge_kernel(SelectArgs a) {
           bf = best_f[j];
         }
       if (bk == 0) break;
-      if (tid == 0) sel[n] = bf;
+      if (tid == 0) {
+        set_k[n] = bk;
+        set_f[n] = bf;
+      }
       pk = bk;
       pf = bf;
-      first = false;
     }
   }
+  __syncthreads();
+
+  // ---- their tokens: those not below the last set's maximum, ranked ----------
+  if (count > 32 && n == W) least = set_k[W - 1];
+  for (int i = tid; i < n * SET; i += MERGE_T) {
+    const int w = (int)(set_f[i / SET] >> 32), set = (int)(uint32_t)set_f[i / SET], e = i % SET;
+    int token = set * SET + e;
+    uint64_t k = 0;
+    float x = 0.f;
+    if (kind[w] == ROW_OPEN) {
+      if (token < a.V) {
+        x = load_f32<T>(logits_row<T>(a, row0 + w), token);
+        k = key_of(w, x);
+      }
+    } else if (kind[w] == ROW_DONE) {
+      if (e == 0) k = set_k[i / SET];
+      token = eos32;
+    } else if (e < W && e < a.V) {
+      k = ~0ull;  // (no number: its lowest tokens)
+    }
+    if (k < least) continue;
+    const int at = atomicAdd(&ecount, 1);
+    ek[at] = k;
+    ef[at] = (uint64_t)w << 32 | (uint32_t)token;
+    ex[at] = x;
+  }
+  __syncthreads();
+  n = ecount;
+  rank_all(ek, ef, n, [&](int rank, int i) {
+    sel[rank] = ef[i];
+    sel_x[rank] = ex[i];
+    atomicMin(&first[ef[i] >> 32], rank);
+  });
+  n = std::min(n, W);
   __syncthreads();
 
   // ---- places, outputs (lane = rank) ----------------------------------------
   if (wave != 0) return;
   const bool chosen = lane < n;
-  const int p = chosen ? (int)(sel[lane] >> 32) : 0;
-  const int token = chosen ? (int)(uint32_t)sel[lane] : 0;
-  bool stays = chosen;
-  for (int j = 0; j < n; ++j) {
-    const int pj = (int)(sel[j] >> 32);
-    if (j < lane && pj == p) stays = false;
-  }
-  uint32_t taken = 0;
+  const int p = chosen ? (int)(sel[lane] >> 32) : 0, token = chosen ? (int)(uint32_t)sel[lane] : 0;
+  const bool stays = chosen && first[p] == lane;  // a parent's best continuation
   const uint64_t stay_mask = __builtin_amdgcn_ballot_w64(stays);
-  for (int j = 0; j < n; ++j)
-    if (stay_mask >> j & 1) taken |= 1u << (int)(sel[j] >> 32);
+  uint32_t free = ~(uint32_t)__builtin_amdgcn_ballot_w64(lane < W && first[lane & 31] < 64);
   int slot = p;
   if (!stays) {
     // the k-th free slot, k = the ranks below this one that do not stay
     int k = __builtin_popcountll(~stay_mask & ((1ull << lane) - 1));
-    uint32_t free = ~taken;
     for (; k > 0; --k) free &= free - 1;
     slot = free ? __builtin_ctz(free) : W;
   }
   if (lane >= W) return;
-  float sc = -__builtin_inff();
-  bool done = true;
-  int64_t len = a.lengths != nullptr ? a.lengths[row0 + slot] : 0;
-  if (chosen) {
-    const bool was = a.finished != nullptr && a.finished[row0 + p];
-    sc = kind[p] == ROW_DONE  ? score[p]
-         : kind[p] == ROW_NAN ? __builtin_nanf("")
-                              : (float)((double)score[p] + ((double)load_f32<T>(logits_row<T>(a, row0 + p), token) - lse[p]));
-    done = was || token == eos32;
-    len = (a.lengths != nullptr ? a.lengths[row0 + p] : 0) + (was ? 0 : 1);
-  }
-  // every input of the group has been read: the outputs may be the inputs
-  __builtin_amdgcn_wave_barrier();
+  const int from = chosen ? p : slot;  // (a slot left over is its own parent)
+  const bool was = ended[from];
+  float out = -__builtin_inff();
+  if (chosen)
+    out = kind[p] == ROW_DONE  ? score[p]
+          : kind[p] == ROW_NAN ? __builtin_nanf("")
+                               : (float)((double)score[p] + ((double)sel_x[lane] - lse[p]));
   a.tokens[row0 + slot] = chosen ? token : std::max(eos32, 0);
-  a.parents[row0 + slot] = row0 + (chosen ? p : slot);
-  a.scores_out[row0 + slot] = sc;
-  a.finished_out[row0 + slot] = done;
-  a.lengths_out[row0 + slot] = len;
+  a.parents[row0 + slot] = row0 + from;
+  a.scores_out[row0 + slot] = out;
+  a.finished_out[row0 + slot] = !chosen || was || token == eos32;
+  a.lengths_out[row0 + slot] = length[from] + (chosen && !was ? 1 : 0);
 }
 
 // ---------------------------------------------------------------------------
@@ -445,12 +511,29 @@ __global__ __launch_bounds__(256) void kv_reorder_kernel(ReorderArgs a) {
   }
 }
 
-int64_t select_slices(int64_t V) { return cdiv(V, SEL_SLICE); }
+template <typename T>
+void beam_merge(hipStream_t st, const SelectArgs& a) {
+  int wp = 1;
+  while (wp < a.W) wp *= 2;
+  const int quads = (int)cdiv(a.sets / 4, MERGE_T / wp);  // of a thread
+  auto go = [&](auto kern) { kern<<<(unsigned)a.G, MERGE_T, 0, st>>>(a, wp); };
+  if (quads <= 5)
+    go(beam_merge_kernel<T, 5>);
+  else if (quads <= 10)
+    go(beam_merge_kernel<T, 10>);
+  else if (quads <= 20)
+    go(beam_merge_kernel<T, 20>);
+  else
+    go(beam_merge_kernel<T, 0>);
+}
+
+int64_t select_slices(int64_t V) { return cdiv(V, SLICE<float>); }  // at most: fp32 has the smaller slices
+int64_t select_sets(int64_t V) { return cdiv(V, 4 * SET) * 4; }
 
 }  // namespace
 
 int64_t beam_select_workspace_bytes(int64_t G, int64_t W, int64_t V) {
-  return G * W * select_slices(V) * (8 + 4 + W * 8);
+  return G * W * (select_slices(V) * (SEL_T / 64) * (8 + 4) + select_sets(V) * 4);
 }
 
 int launch_beam_select(hipStream_t st, int dtype, const BeamSelect& b, void* workspace, int64_t workspace_bytes) {
@@ -460,8 +543,9 @@ int launch_beam_select(hipStream_t st, int dtype, const BeamSelect& b, void* wor
               (long long)workspace_bytes, (long long)need);
     return MINITP_ERR_ARG;
   }
-  const int64_t rows = b.G * b.W, parts = rows * select_slices(b.V);
-  if (parts >= (1LL << 31) || b.W * b.W * select_slices(b.V) >= (1LL << 30)) {
+  const int64_t rows = b.G * b.W, slices = cdiv(b.V, dtype == MINITP_F32 ? SLICE<float> : SLICE<bf16>);
+  const int64_t parts = rows * slices * (SEL_T / 64);
+  if (rows * slices >= (1LL << 31)) {
     set_error("beam_select: %lld rows of %lld logits are too many for one call", (long long)rows, (long long)b.V);
     return MINITP_ERR_UNSUPPORTED;
   }
@@ -472,7 +556,8 @@ int launch_beam_select(hipStream_t st, int dtype, const BeamSelect& b, void* wor
   a.V = b.V;
   a.G = (int)b.G;
   a.W = (int)b.W;
-  a.slices = (int)select_slices(b.V);
+  a.slices = (int)slices;
+  a.sets = (int)select_sets(b.V);
   a.scores = b.scores;
   a.finished = b.finished;
   a.lengths = b.lengths;
@@ -483,18 +568,17 @@ int launch_beam_select(hipStream_t st, int dtype, const BeamSelect& b, void* wor
   a.scores_out = b.scores_out;
   a.finished_out = b.finished_out;
   a.lengths_out = b.lengths_out;
-  a.sum = (double*)workspace;
+  a.set_top = (float*)workspace;  // (rows of whole float4)
+  a.sum = (double*)(a.set_top + rows * a.sets);
   a.top = (float*)(a.sum + parts);
-  a.cand_v = a.top + parts;
-  a.cand_i = (int32_t*)(a.cand_v + parts * b.W);
   if (dtype == MINITP_F32) {
-    beam_slice_kernel<float><<<(unsigned)parts, SEL_T, 0, st>>>(a);
+    beam_slice_kernel<float><<<(unsigned)(rows * slices), SEL_T, 0, st>>>(a);
     MINITP_LAUNCH_CHECK();
-    beam_merge_kernel<float><<<(unsigned)b.G, MERGE_T, 0, st>>>(a);
+    beam_merge<float>(st, a);
   } else {
-    beam_slice_kernel<bf16><<<(unsigned)parts, SEL_T, 0, st>>>(a);
+    beam_slice_kernel<bf16><<<(unsigned)(rows * slices), SEL_T, 0, st>>>(a);
     MINITP_LAUNCH_CHECK();
-    beam_merge_kernel<bf16><<<(unsigned)b.G, MERGE_T, 0, st>>>(a);
+    beam_merge<bf16>(st, a);
   }
   MINITP_LAUNCH_CHECK();
   return MINITP_OK;

@@ -2,7 +2,6 @@
 // launch. Nothing here allocates, synchronises or throws.
 #include <hip/hip_runtime.h>
 
-#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <mutex>
@@ -423,7 +422,8 @@ int minitp_beam_select(void* stream, int dtype, const void* logits, int64_t ld_g
   MINITP_CHECK_ARG(eos_token >= -1 && eos_token < V, "beam_select: eos_token %lld of %lld tokens",
                    (long long)eos_token, (long long)V);
   MINITP_CHECK_ARG(finished == nullptr || eos_token >= 0, "beam_select: finished beams need an eos_token");
-  MINITP_CHECK_ARG(std::isfinite(length_penalty), "beam_select: length_penalty %f", length_penalty);
+  MINITP_CHECK_ARG(length_penalty >= -16.0 && length_penalty <= 16.0, "beam_select: length_penalty %g (-16 to 16)",
+                   length_penalty);
   if (G == 0) return MINITP_OK;
   MINITP_CHECK_ARG(logits && scores && tokens && parents && scores_out && finished_out && lengths_out,
                    "beam_select: NULL pointer");

@@ -314,30 +314,30 @@ def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, cac
     return out
 
 
-def _one_device(what: str, *tensors: torch.Tensor | None) -> torch.device:
-    """The device that all of a call's tensors live on."""
-    N.require_gpu(*tensors, what=what)
-    dev = tensors[0].device
+def _one_device(what: str, *tensors: torch.Tensor | None) -> int:
+    """Index of the device that all of a call's tensors live on."""
+    dev = tensors[0].get_device()
     for t in tensors:
-        if t is not None and t.device != dev:
-            raise ValueError(f"{what}: tensors on {dev} and {t.device}")
+        if t is not None and (t.get_device() != dev or dev < 0):
+            N.require_gpu(*tensors, what=what)
+            raise ValueError(f"{what}: tensors on {tensors[0].device} and {t.device}")
     return dev
 
 
-def _elsewhere(dev: torch.device) -> bool:
-    return dev.index != torch._C._cuda_getDevice()
+def _elsewhere(dev: int) -> bool:
+    return dev != torch._C._cuda_getDevice()
 
 
 def _cache_view(what: str, k: torch.Tensor, v: torch.Tensor, batch: int, hkv: int, d: int, dtype: torch.dtype) -> int:
     """Row stride of a [batch, hkv, S, d] cache pair (cache_rows), its sizes checked."""
-    for c in (k, v):
-        if c.dim() != 4 or c.shape[0] != batch or c.shape[1] != hkv or c.shape[3] != d:
-            raise ValueError(f"{what}: K/V rows {tuple(c.shape)}, expected [{batch}, {hkv}, S, {d}]")
-        if c.dtype != dtype:
-            raise TypeError(f"{what}: dtype mismatch {c.dtype} and {dtype}")
-    if k.shape != v.shape:
-        raise ValueError(f"{what}: K {tuple(k.shape)} and V {tuple(v.shape)} differ")
-    return cache_rows(k, v)
+    shape, st = k.shape, k.stride()
+    if len(shape) != 4 or shape[0] != batch or shape[1] != hkv or shape[3] != d or v.shape != shape:
+        raise ValueError(f"{what}: K/V rows {tuple(shape)} and {tuple(v.shape)}, expected [{batch}, {hkv}, S, {d}]")
+    if k.dtype != dtype or v.dtype != dtype:
+        raise TypeError(f"{what}: dtype mismatch {k.dtype} / {v.dtype} and {dtype}")
+    if v.stride() != st or st[3] != 1 or st[2] != d or st[0] != hkv * st[1] or st[1] % d:
+        return cache_rows(k, v)  # (raises, or a layout of single rows)
+    return st[1] // d
 
 
 def _lens(what: str, lens: torch.Tensor | None, count: int) -> torch.Tensor | None:
@@ -373,31 +373,31 @@ def shared_prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: t
     if q.dim() != 4 or k_cache.dim() != 4 or k_prefix.dim() != 4:
         raise ValueError(f"{what}: q {tuple(q.shape)}, prefix {tuple(k_prefix.shape)}, cache {tuple(k_cache.shape)}")
     b, t, hq, d = q.shape
-    hkv, groups = k_cache.shape[1], k_prefix.shape[0]
-    s = _cache_view(what, k_cache, v_cache, b, hkv, d, q.dtype)
-    sp = _cache_view(what, k_prefix, v_prefix, groups, hkv, d, q.dtype)
-    if cache_len + t > k_cache.shape[2]:
-        raise ValueError(f"KV cache overflow: seq {cache_len}+{t} > max_seq_len={k_cache.shape[2]}")
-    if prefix_len > k_prefix.shape[2]:
-        raise ValueError(f"KV cache overflow: prefix {prefix_len} > prefix rows {k_prefix.shape[2]}")
+    dtype, (_, hkv, rows, _), (groups, _, prefix_rows, _) = q.dtype, k_cache.shape, k_prefix.shape
+    s = _cache_view(what, k_cache, v_cache, b, hkv, d, dtype)
+    sp = _cache_view(what, k_prefix, v_prefix, groups, hkv, d, dtype)
+    if cache_len + t > rows:
+        raise ValueError(f"KV cache overflow: seq {cache_len}+{t} > max_seq_len={rows}")
+    if prefix_len > prefix_rows:
+        raise ValueError(f"KV cache overflow: prefix {prefix_len} > prefix rows {prefix_rows}")
     plens, clens = _lens(what, prefix_lens, groups), _lens(what, cache_lens, b)
     q = q.contiguous()
-    out = torch.empty(b, t, hq * d, dtype=q.dtype, device=dev)
-    dt = N.dtype_code(q.dtype)
-    nbytes = _shared_prefix_bytes(dev, dt, b, groups, t, hq, hkv, d, prefix_len, cache_len)
+    out = q.new_empty((b, t, hq * d))
+    dt = N.dtype_code(dtype)
+    nbytes = _shared_prefix_bytes(dt, b, groups, t, hq, hkv, d, prefix_len, cache_len)
     # from the caching allocator on the current stream: calls on other streams
     # and captured graphs have scratch of their own
-    ws = torch.empty(max(nbytes, 0), dtype=torch.uint8, device=dev)
+    ws = q.new_empty((nbytes,), dtype=torch.uint8) if nbytes > 0 else None
     N.check(_lib().minitp_shared_prefix_attention(
         N.stream(), dt, q.data_ptr(), k_prefix.data_ptr(), v_prefix.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-        out.data_ptr(), b, groups, t, hq, hkv, d, sp, prefix_len, N.ptr(plens), s, cache_len, N.ptr(clens),
-        ws.data_ptr(), ws.numel()), what)
+        out.data_ptr(), b, groups, t, hq, hkv, d, sp, prefix_len, N.ptr(plens), s, cache_len, N.ptr(clens), N.ptr(ws),
+        nbytes), what)
     return out
 
 
 @functools.lru_cache(maxsize=4096)
-def _shared_prefix_bytes(device: torch.device, *sizes: int) -> int:
-    return _lib().minitp_shared_prefix_attention_workspace_bytes(*sizes)
+def _shared_prefix_bytes(*sizes: int) -> int:
+    return max(_lib().minitp_shared_prefix_attention_workspace_bytes(*sizes), 0)
 
 
 class BeamStep(NamedTuple):
@@ -429,38 +429,46 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: torch.Tens
         with torch.cuda.device(dev):
             return beam_select(logits, scores, finished, lengths, eos_token_id=eos_token_id,
                                length_penalty=length_penalty)
-    if scores.dim() != 2 or scores.dtype != torch.float32:
-        raise ValueError(f"{what}: scores {tuple(scores.shape)} {scores.dtype}, expected [G, W] float32")
-    groups, beams = scores.shape
+    shape = scores.shape
+    if len(shape) != 2 or scores.dtype != torch.float32:
+        raise ValueError(f"{what}: scores {tuple(shape)} {scores.dtype}, expected [G, W] float32")
+    groups, beams = shape
     if logits.dim() == 2 and logits.shape[0] == groups * beams:
-        logits = logits.unflatten(0, (groups, beams))
-    if logits.dim() != 3 or logits.shape[:2] != scores.shape:
-        raise ValueError(f"{what}: logits {tuple(logits.shape)} for scores {tuple(scores.shape)}")
-    for name, t, dtype in (("finished", finished, torch.bool), ("lengths", lengths, torch.long)):
-        if t is not None and (t.shape != scores.shape or t.dtype != dtype):
-            raise ValueError(f"{what}: {name} {tuple(t.shape)} {t.dtype}, expected {tuple(scores.shape)} {dtype}")
-    vocab = logits.shape[2]
-    if logits.stride(2) != 1 and vocab > 1:
+        ld_beam = logits.stride(0)
+        ld_group = beams * ld_beam
+    elif logits.dim() == 3 and logits.shape[:2] == shape:
+        ld_group, ld_beam, _ = logits.stride()
+    else:
+        raise ValueError(f"{what}: logits {tuple(logits.shape)} for scores {tuple(shape)}")
+    vocab = logits.shape[-1]
+    if logits.stride(-1) != 1 and vocab > 1:
         logits = logits.contiguous()
+        ld_group, ld_beam = beams * vocab, vocab
+    if finished is not None:
+        if finished.shape != shape or finished.dtype != torch.bool:
+            raise ValueError(f"{what}: finished {tuple(finished.shape)} {finished.dtype}, expected {tuple(shape)} bool")
+        finished = finished.contiguous()
+    if lengths is not None:
+        if lengths.shape != shape or lengths.dtype != torch.long:
+            raise ValueError(f"{what}: lengths {tuple(lengths.shape)} {lengths.dtype}, expected {tuple(shape)} int64")
+        lengths = lengths.contiguous()
     scores = scores.contiguous()
-    finished = finished.contiguous() if finished is not None else None
-    lengths = lengths.contiguous() if lengths is not None else None
-    whole = torch.empty(3, groups, beams, dtype=torch.long, device=dev)
-    tokens, parents, new_lengths = whole.unbind(0)
     new_scores = torch.empty_like(scores)
-    new_finished = torch.empty(groups, beams, dtype=torch.bool, device=dev)
-    ws = torch.empty(max(_beam_select_bytes(dev, groups, beams, vocab), 0), dtype=torch.uint8, device=dev)
+    tokens, parents, new_lengths = (scores.new_empty(shape, dtype=torch.long) for _ in range(3))
+    new_finished = scores.new_empty(shape, dtype=torch.bool)
+    nbytes = _beam_select_bytes(groups, beams, vocab)
+    ws = scores.new_empty((nbytes,), dtype=torch.uint8)
     N.check(_lib().minitp_beam_select(
-        N.stream(), N.dtype_code(logits.dtype), logits.data_ptr(), logits.stride(0), logits.stride(1), groups, beams,
-        vocab, scores.data_ptr(), N.ptr(finished), N.ptr(lengths), -1 if eos_token_id is None else eos_token_id,
-        float(length_penalty), tokens.data_ptr(), parents.data_ptr(), new_scores.data_ptr(), new_finished.data_ptr(),
-        new_lengths.data_ptr(), ws.data_ptr(), ws.numel()), what)
+        N.stream(), N.dtype_code(logits.dtype), logits.data_ptr(), ld_group, ld_beam, groups, beams, vocab,
+        scores.data_ptr(), N.ptr(finished), N.ptr(lengths), -1 if eos_token_id is None else eos_token_id,
+        length_penalty, tokens.data_ptr(), parents.data_ptr(), new_scores.data_ptr(), new_finished.data_ptr(),
+        new_lengths.data_ptr(), ws.data_ptr(), nbytes), what)
     return BeamStep(tokens, parents, new_scores, new_finished, new_lengths)
 
 
 @functools.lru_cache(maxsize=4096)
-def _beam_select_bytes(device: torch.device, *sizes: int) -> int:
-    return _lib().minitp_beam_select_workspace_bytes(*sizes)
+def _beam_select_bytes(*sizes: int) -> int:
+    return max(_lib().minitp_beam_select_workspace_bytes(*sizes), 0)
 
 
 def kv_reorder(k_buf: torch.Tensor, v_buf: torch.Tensor, parents: torch.Tensor, rows: int) -> None:
@@ -473,17 +481,19 @@ def kv_reorder(k_buf: torch.Tensor, v_buf: torch.Tensor, parents: torch.Tensor, 
     if _elsewhere(dev):
         with torch.cuda.device(dev):
             return kv_reorder(k_buf, v_buf, parents, rows)
-    if k_buf.dim() != 5 or k_buf.shape != v_buf.shape or k_buf.dtype != v_buf.dtype:
+    shape = k_buf.shape
+    if len(shape) != 5 or v_buf.shape != shape or k_buf.dtype != v_buf.dtype:
         raise ValueError(f"{what}: buffers {tuple(k_buf.shape)} {k_buf.dtype} and {tuple(v_buf.shape)} {v_buf.dtype}")
     if not (k_buf.is_contiguous() and v_buf.is_contiguous()):
         raise ValueError(f"{what}: the cache buffers must be contiguous [L, B, Hkv, S, D]")
-    if parents.dim() != 2 or parents.numel() != k_buf.shape[1] or parents.dtype != torch.long:
+    layers, batch, hkv, s, d = shape
+    if parents.dim() != 2 or parents.numel() != batch or parents.dtype != torch.long:
         raise ValueError(f"{what}: parents {tuple(parents.shape)} {parents.dtype}, expected [G, W] int64 for "
-                         f"{k_buf.shape[1]} batch rows")
-    layers, _, hkv, s, d = k_buf.shape
+                         f"{batch} batch rows")
+    groups, beams = parents.shape
     parents = parents.contiguous()
     N.check(_lib().minitp_kv_reorder(N.stream(), N.dtype_code(k_buf.dtype), k_buf.data_ptr(), v_buf.data_ptr(), layers,
-                                     parents.shape[0], parents.shape[1], hkv, s, d, rows, parents.data_ptr()), what)
+                                     groups, beams, hkv, s, d, rows, parents.data_ptr()), what)
 
 
 def argmax(logits: torch.Tensor) -> torch.Tensor:

@@ -12,7 +12,7 @@ from minitp import kernels as K
 P = 4096  # a 16-byte aligned address that no refused call looks at
 
 
-def attention(dtype=N.BF16, q=P, kp=P, vp=P, kc=P, vc=P, out=P, b=4, g=2, t=1, hq=4, hkv=2, d=64, sp=32, p=32, plens=None,
+def attention(dtype=N.BF16, q=P, kp=P, vp=P, kc=P, vc=P, out=P, b=4, g=2, t=1, hq=4, hkv=2, d=64, sp=5000, p=5000, plens=None,
               s=16, c=10, clens=None, ws=P, nbytes=1 << 30):
     return N.lib().minitp_shared_prefix_attention(None, dtype, q, kp, vp, kc, vc, out, b, g, t, hq, hkv, d, sp, p, plens,
                                                   s, c, clens, ws, nbytes)
@@ -25,7 +25,7 @@ def attention(dtype=N.BF16, q=P, kp=P, vp=P, kc=P, vc=P, out=P, b=4, g=2, t=1, h
     (N.ERR_ARG, dict(d=12)), (N.ERR_ARG, dict(d=0)), (N.ERR_ARG, dict(q=P + 8)), (N.ERR_ARG, dict(kc=P + 2)),
     (N.ERR_ARG, dict(vp=P + 4)), (N.ERR_ARG, dict(ws=None)), (N.ERR_ARG, dict(nbytes=64)), (N.ERR_ARG, dict(ws=P + 4)),
     (N.ERR_DIVISIBLE, dict(hq=5)), (N.ERR_DIVISIBLE, dict(b=5)), (N.ERR_OVERFLOW, dict(c=16)),
-    (N.ERR_OVERFLOW, dict(t=7)), (N.ERR_OVERFLOW, dict(p=33)), (N.ERR_UNSUPPORTED, dict(d=256)),
+    (N.ERR_OVERFLOW, dict(t=7)), (N.ERR_OVERFLOW, dict(p=5001)), (N.ERR_UNSUPPORTED, dict(d=256)),
     (N.ERR_UNSUPPORTED, dict(d=40)),
 ])
 def test_shared_prefix_attention_refuses(status, change):
@@ -36,7 +36,8 @@ def test_shared_prefix_attention_of_nothing():
     assert attention(b=0) == N.OK and attention(t=0) == N.OK
     size = N.lib().minitp_shared_prefix_attention_workspace_bytes
     assert size(N.F32, 0, 1, 1, 4, 2, 64, 10, 10) == 0
-    assert size(N.F32, 4, 2, 1, 4, 2, 64, 0, 0) > 0
+    assert size(N.F32, 4, 2, 1, 4, 2, 64, 0, 0) == 0  # (one block a row: nothing to join)
+    assert size(N.F32, 4, 2, 1, 4, 2, 64, 5000, 0) > 0
     for bad in ((5, 4, 2, 1, 4, 2, 64, 1, 1), (0, 4, 3, 1, 4, 2, 64, 1, 1), (0, 4, 2, 1, 3, 2, 64, 1, 1),
                 (0, 4, 0, 1, 4, 2, 64, 1, 1), (0, 4, 2, 1, 4, 2, 64, -1, 1)):
         assert size(*bad) == -1
@@ -51,7 +52,7 @@ def select(dtype=N.F32, logits=P, ldg=800, ldb=100, g=2, w=8, v=100, scores=P, f
 @pytest.mark.parametrize("change", [
     dict(dtype=7), dict(logits=None), dict(scores=None), dict(outs=(P, P, None, P, P)), dict(w=0), dict(w=33), dict(g=-1),
     dict(v=0), dict(v=1 << 31), dict(ldg=-1), dict(ldb=-5), dict(eos=-2), dict(eos=100), dict(finished=P),
-    dict(alpha=math.nan), dict(alpha=math.inf), dict(ws=None), dict(nbytes=100), dict(ws=P + 8),
+    dict(alpha=math.nan), dict(alpha=math.inf), dict(alpha=17.0), dict(alpha=-16.5), dict(ws=None), dict(nbytes=100), dict(ws=P + 8),
 ])
 def test_beam_select_refuses(change):
     assert select(**change) == N.ERR_ARG and N.last_error()

@@ -1,9 +1,10 @@
 """Beam selection and cache reordering (csrc/beam.hip) against plain forms: the
 selection by a full stable sort in 64 bits, the reordering by indexing.
 
-Bar of a score: its sum over the vocabulary is off by at most 20 steps (16 terms
-added in fp32, an exponential within 2 steps, the rest in 64 bits), which the
-logarithm turns into as much of an absolute error; the result is rounded once.
+Bar of a score: its sum over the vocabulary is off by at most 20 steps (chains of
+8 terms and 2 more additions in fp32, two exponentials of 2 steps each, a
+wave's and its part's weight, the rest in 64 bits), which the logarithm turns
+into as much of an absolute error; the result is rounded once.
 Tokens, parents, flags and lengths have to be equal.
 """
 
@@ -91,7 +92,7 @@ def test_selection(vocab, beams, dtype):
     compare(K.beam_select(logits, scores), reference(logits, scores, None, None, -1, 0.0))
 
 
-@pytest.mark.parametrize("alpha", [0.0, 0.7, 1.0, -0.5])
+@pytest.mark.parametrize("alpha", [0.0, 0.7, 1.0, -0.5, 16.0])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_finished_beams_lengths_and_empty_slots(dtype, alpha):
     from minitp import kernels as K
