@@ -427,8 +427,23 @@ int minitp_beam_select(void* stream, int dtype, const void* logits, int64_t ld_g
   if (G == 0) return MINITP_OK;
   MINITP_CHECK_ARG(logits && scores && tokens && parents && scores_out && finished_out && lengths_out,
                    "beam_select: NULL pointer");
-  const BeamSelect b{logits,         ld_group, ld_beam, G,          W,            V,          scores, finished, lengths, eos_token,
-                     length_penalty, tokens,   parents, scores_out, finished_out, lengths_out};
+  BeamSelect b{};
+  b.logits = logits;
+  b.ld_group = ld_group;
+  b.ld_beam = ld_beam;
+  b.G = G;
+  b.W = W;
+  b.V = V;
+  b.scores = scores;
+  b.finished = finished;
+  b.lengths = lengths;
+  b.eos = eos_token;
+  b.alpha = length_penalty;
+  b.tokens = tokens;
+  b.parents = parents;
+  b.scores_out = scores_out;
+  b.finished_out = finished_out;
+  b.lengths_out = lengths_out;
   return launch_beam_select(S(stream), dtype, b, workspace, workspace_bytes);
 }
 

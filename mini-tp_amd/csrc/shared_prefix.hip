@@ -124,7 +124,8 @@ __device__ __forceinline__ bool shared_item(const SharedArgs& a, int64_t row_byt
 
 // One tile of keys through a resource of its own (a head's rows may span more
 // than the 4 GiB that one reaches); rows past the item's last read zeros.
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t key_rows(const void* base, int key, int keys, int tile, int row_bytes) {
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t key_rows(const void* base, int key, int keys, int tile,
+                                                           int row_bytes) {
   const int n = std::min(keys - key, tile);
   return span_rsrc((const char*)base + (int64_t)key * row_bytes, (uint32_t)(n * row_bytes));
 }
@@ -290,7 +291,8 @@ __device__ __forceinline__ void shared_rows_f32(const SharedArgs& a, const Item&
         for (int c = 0; c < KC; ++c) {
           const f32x4 k4 = *(const f32x4*)(Ks + (key0 + kb * 16 + lr) * ROW + 16 * c + 4 * lq);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) chain[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(k4[i], qa[c][i], chain[i], 0, 0, 0);
+          for (int i = 0; i < 4; ++i)
+            chain[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(k4[i], qa[c][i], chain[i], 0, 0, 0);
         }
         const f32x4 acc = (chain[0] + chain[1]) + (chain[2] + chain[3]);
 #pragma unroll
@@ -574,99 +576,108 @@ __device__ __forceinline__ void shared_rows128(const SharedArgs& a, const Item& 
   const int vx = ((2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) ^ H::v_swz(vrow)) << 4;
 
   for (int part = it.first; part <= it.last; ++part) {
-  if (part != it.first) {
-    ks = it.own;
-    tiles = Tiles<D>(ks, lds);
-    __syncthreads();  // (every stage is free)
-    tiles.load(0);
-  }
-  const int seen = last_seen(ks, live ? r : 0, per), seen_last = last_seen(ks, r0 + 31, per);
-  const int all_see = last_seen(ks, it.tile * H_QT, per);  // the last key that every query of the block sees
-  tiles.each(lds, (all_see + 1) / H_KT, [&](int t, const char* st, auto masked) {
-    if (r0 >= it.rows || (masked && t * H_KT > seen_last)) return;
-    f32x16 s[2];
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) s[kb][i] = 0.f;
-#pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        const bf16x8 kf = __builtin_bit_cast(bf16x8, *(const uint4*)(st + kat + kb * 32 * H::ROWB + ((32 * k) ^ kx)));
-        s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qb[k], s[kb], 0, 0, 0);
-      }
+    if (part != it.first) {
+      ks = it.own;
+      tiles = Tiles<D>(ks, lds);
+      __syncthreads();  // (every stage is free)
+      tiles.load(0);
     }
-    bool odd = false;
-    const int limit = seen - t * H_KT;
-    if constexpr (masked) {
-      // lane (query, h) holds keys 32 kb + 8 (i / 4) + 4 h + i % 4
+    const int seen = last_seen(ks, live ? r : 0, per), seen_last = last_seen(ks, r0 + 31, per);
+    const int all_see = last_seen(ks, it.tile * H_QT, per);  // the last key that every query of the block sees
+    tiles.each(lds, (all_see + 1) / H_KT, [&](int t, const char* st, auto masked) {
+      if (r0 >= it.rows || (masked && t * H_KT > seen_last)) return;
+      f32x16 s[2];
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[kb][i] = 0.f;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          const bf16x8 kf = __builtin_bit_cast(bf16x8, *(const uint4*)(st + kat + kb * 32 * H::ROWB + ((32 * k) ^ kx)));
+          s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qb[k], s[kb], 0, 0, 0);
+        }
+      }
+      bool odd = false;
+      const int limit = seen - t * H_KT;
+      if constexpr (masked) {
+        // lane (query, h) holds keys 32 kb + 8 (i / 4) + 4 h + i % 4
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (32 * kb + 8 * (i / 4) + i % 4 > limit - 4 * h) s[kb][i] = -__builtin_inff();
+        if (all_see < ks.n - 1) {
+          // hidden keys that other queries see: are their values finite?
+          for (int c = lane; c < H_KT * H::CH; c += 64) odd |= not_finite(*(const uint4*)(st + H::OPER + c * 16));
+          odd = __builtin_amdgcn_ballot_w64(odd) != 0;
+        }
+      }
+      float mx = s[0][0];
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (32 * kb + 8 * (i / 4) + i % 4 > limit - 4 * h) s[kb][i] = -__builtin_inff();
-      if (all_see < ks.n - 1) {
-        // hidden keys that other queries see: are their values finite?
-        for (int c = lane; c < H_KT * H::CH; c += 64) odd |= not_finite(*(const uint4*)(st + H::OPER + c * 16));
-        odd = __builtin_amdgcn_ballot_w64(odd) != 0;
+        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kb][i]);
+      mx = halves_max(mx) * sl2;
+      if (__builtin_amdgcn_ballot_w64(mx > m + SLACK)) {
+        const float mn = fmaxf(m, mx), alpha = mn == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+        m = mn;
+        lsum *= alpha;
+#pragma unroll
+        for (int d = 0; d < DB; ++d) o[d] *= alpha;
       }
-    }
-    float mx = s[0][0];
+      const float mref = m == -__builtin_inff() ? 0.f : m;  // (nothing seen yet)
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
+      for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kb][i]);
-    mx = halves_max(mx) * sl2;
-    if (__builtin_amdgcn_ballot_w64(mx > m + SLACK)) {
-      const float mn = fmaxf(m, mx), alpha = mn == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-      m = mn;
-      lsum *= alpha;
-#pragma unroll
-      for (int d = 0; d < DB; ++d) o[d] *= alpha;
-    }
-    const float mref = m == -__builtin_inff() ? 0.f : m;  // (nothing seen yet)
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        s[kb][i] = __builtin_amdgcn_exp2f(fmaf(s[kb][i], sl2, -mref));
-        lsum += s[kb][i];
-      }
-    if (masked && odd) {
-      // a value that some query may not touch is not finite (0 times it is no
-      // zero): key by key, for the queries that see it
+        for (int i = 0; i < 16; ++i) {
+          s[kb][i] = __builtin_amdgcn_exp2f(fmaf(s[kb][i], sl2, -mref));
+          lsum += s[kb][i];
+        }
+      if (masked && odd) {
+        // a value that some query may not touch is not finite (0 times it is no
+        // zero): key by key, for the queries that see it
 #pragma unroll 1
-      for (int key = 0; key < H_KT; ++key) {
-        const int idx = (key >> 5) * 16 + ((key >> 3) & 3) * 4 + (key & 3);
-        float p = 0.f;
+        for (int key = 0; key < H_KT; ++key) {
+          const int idx = (key >> 5) * 16 + ((key >> 3) & 3) * 4 + (key & 3);
+          float p = 0.f;
 #pragma unroll
-        for (int c = 0; c < 32; ++c) p = c == idx ? s[c / 16][c % 16] : p;
-        p = __shfl(p, n32 + 32 * ((key >> 2) & 1), 64);
+          for (int c = 0; c < 32; ++c) p = c == idx ? s[c / 16][c % 16] : p;
+          p = __shfl(p, n32 + 32 * ((key >> 2) & 1), 64);
 #pragma unroll
-        for (int d = 0; d < DB; ++d)
+          for (int d = 0; d < DB; ++d)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const uint2 x = *(const uint2*)(st + H::OPER + key * H::ROWB + (((4 * d + c) ^ H::v_swz(key)) << 4) + 8 * h);
-            const float v[4] = {__uint_as_float(x.x << 16), __uint_as_float(x.x & 0xffff0000u),
-                                __uint_as_float(x.y << 16), __uint_as_float(x.y & 0xffff0000u)};
+            for (int c = 0; c < 4; ++c) {
+              const char* vp = st + H::OPER + key * H::ROWB + (((4 * d + c) ^ H::v_swz(key)) << 4) + 8 * h;
+              const uint2 x = *(const uint2*)vp;
+              const float v[4] = {__uint_as_float(x.x << 16), __uint_as_float(x.x & 0xffff0000u),
+                                  __uint_as_float(x.y << 16), __uint_as_float(x.y & 0xffff0000u)};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[d][4 * c + e] = key <= limit ? fmaf(p, v[e], o[d][4 * c + e]) : o[d][4 * c + e];
-          }
+              for (int e = 0; e < 4; ++e) {
+                const float old = o[d][4 * c + e];
+                o[d][4 * c + e] = key <= limit ? fmaf(p, v[e], old) : old;
+              }
+            }
+        }
+        return;
       }
-      return;
-    }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {  // keys 16 j .. 16 j + 15
-      const f32x16& p = s[j / 2];
-      const int b = 8 * (j % 2);
-      const bf16x8 pb = __builtin_bit_cast(bf16x8, make_uint4(pack_bf16x2(p[b], p[b + 1]), pack_bf16x2(p[b + 2], p[b + 3]),
-                                                              pack_bf16x2(p[b + 4], p[b + 5]), pack_bf16x2(p[b + 6], p[b + 7])));
+      for (int j = 0; j < 4; ++j) {  // keys 16 j .. 16 j + 15
+        const f32x16& p = s[j / 2];
+        const int b = 8 * (j % 2);
+        uint4 pk;
+        pk.x = pack_bf16x2(p[b], p[b + 1]);
+        pk.y = pack_bf16x2(p[b + 2], p[b + 3]);
+        pk.z = pack_bf16x2(p[b + 4], p[b + 5]);
+        pk.w = pack_bf16x2(p[b + 6], p[b + 7]);
+        const bf16x8 pb = __builtin_bit_cast(bf16x8, pk);
 #pragma unroll
-      for (int d = 0; d < DB; ++d) {
-        const char* vp = st + vat + 16 * j * H::ROWB + ((64 * d) ^ vx);
-        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(join8(read_tr(vp), read_tr(vp + 8 * H::ROWB)), pb, o[d], 0, 0, 0);
+        for (int d = 0; d < DB; ++d) {
+          const char* vp = st + vat + 16 * j * H::ROWB + ((64 * d) ^ vx);
+          const bf16x8 vf = join8(read_tr(vp), read_tr(vp + 8 * H::ROWB));
+          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pb, o[d], 0, 0, 0);
+        }
       }
-    }
-  });
+    });
   }
   if (!live) return;
   const float l = halves_sum(lsum);
@@ -727,71 +738,72 @@ __device__ __forceinline__ void shared_rows16(const SharedArgs& a, const Item& i
   const int vat = H::OPER + vrow * H::ROWB + 8 * (lane & 1), vx = (((lane >> 1) & 1) ^ H::v_swz(vrow)) << 4;
 
   for (int part = it.first; part <= it.last; ++part) {
-  if (part != it.first) {
-    ks = it.own;
-    tiles = Tiles<D>(ks, lds);
-    __syncthreads();  // (every stage is free)
-    tiles.load(0);
-  }
-  const int seen = last_seen(ks, live ? r : 0, per), all_see = last_seen(ks, 0, per);
-  tiles.each(lds, (all_see + 1) / H_KT, [&](int t, const char* st, auto masked) {
-    const int kw = t * H_KT + 16 * w;
-    if (masked && kw >= ks.n) return;
-    f32x4 s = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int k = 0; k < KS; ++k) {
-      const bf16x8 kf = __builtin_bit_cast(bf16x8, *(const uint4*)(st + kat + ((64 * k) ^ kx)));
-      s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qb[k], s, 0, 0, 0);
+    if (part != it.first) {
+      ks = it.own;
+      tiles = Tiles<D>(ks, lds);
+      __syncthreads();  // (every stage is free)
+      tiles.load(0);
     }
-    const int limit = seen - kw;
-    if constexpr (masked) {
+    const int seen = last_seen(ks, live ? r : 0, per), all_see = last_seen(ks, 0, per);
+    tiles.each(lds, (all_see + 1) / H_KT, [&](int t, const char* st, auto masked) {
+      const int kw = t * H_KT + 16 * w;
+      if (masked && kw >= ks.n) return;
+      f32x4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (4 * q4 + i > limit) s[i] = -__builtin_inff();
-    }
-    const float mx = quads_max(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]))) * sl2;
-    if (__builtin_amdgcn_ballot_w64(mx > m)) {
-      const float mn = fmaxf(m, mx), alpha = mn == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-      m = mn;
-      lsum *= alpha;
-#pragma unroll
-      for (int d = 0; d < DB; ++d) o[d] *= alpha;
-    }
-    const float mref = m == -__builtin_inff() ? 0.f : m;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], sl2, -mref));
-      lsum += s[i];
-    }
-    // (several tokens: a hidden key's value may not be finite)
-    if (masked && all_see < ks.n - 1) {
-      bool odd = false;
-      for (int c = lane; c < 16 * H::CH; c += 64)
-        odd |= not_finite(*(const uint4*)(st + H::OPER + 16 * w * H::ROWB + c * 16));
-      if (__builtin_amdgcn_ballot_w64(odd)) {
-#pragma unroll 1
-        for (int key = 0; key < 16; ++key) {
-          const float pi = (key & 3) == 0 ? s[0] : (key & 3) == 1 ? s[1] : (key & 3) == 2 ? s[2] : s[3];
-          const float p = __shfl(pi, n16 + 16 * (key >> 2), 64);
-          const int row = 16 * w + key;
-#pragma unroll
-          for (int d = 0; d < DB; ++d) {
-            const uint2 x = *(const uint2*)(st + H::OPER + row * H::ROWB + (((2 * d + (q4 >> 1)) ^ H::v_swz(row)) << 4) +
-                                            8 * (q4 & 1));
-            const float v[4] = {__uint_as_float(x.x << 16), __uint_as_float(x.x & 0xffff0000u),
-                                __uint_as_float(x.y << 16), __uint_as_float(x.y & 0xffff0000u)};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[d][e] = key <= limit ? fmaf(p, v[e], o[d][e]) : o[d][e];
-          }
-        }
-        return;
+      for (int k = 0; k < KS; ++k) {
+        const bf16x8 kf = __builtin_bit_cast(bf16x8, *(const uint4*)(st + kat + ((64 * k) ^ kx)));
+        s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qb[k], s, 0, 0, 0);
       }
-    }
-    const s16x4 pb = __builtin_bit_cast(s16x4, make_uint2(pack_bf16x2(s[0], s[1]), pack_bf16x2(s[2], s[3])));
+      const int limit = seen - kw;
+      if constexpr (masked) {
 #pragma unroll
-    for (int d = 0; d < DB; ++d)
-      o[d] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(read_tr(st + vat + ((32 * d) ^ vx)), pb, o[d], 0, 0, 0);
-  });
+        for (int i = 0; i < 4; ++i)
+          if (4 * q4 + i > limit) s[i] = -__builtin_inff();
+      }
+      const float mx = quads_max(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]))) * sl2;
+      if (__builtin_amdgcn_ballot_w64(mx > m)) {
+        const float mn = fmaxf(m, mx), alpha = mn == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+        m = mn;
+        lsum *= alpha;
+#pragma unroll
+        for (int d = 0; d < DB; ++d) o[d] *= alpha;
+      }
+      const float mref = m == -__builtin_inff() ? 0.f : m;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], sl2, -mref));
+        lsum += s[i];
+      }
+      // (several tokens: a hidden key's value may not be finite)
+      if (masked && all_see < ks.n - 1) {
+        bool odd = false;
+        for (int c = lane; c < 16 * H::CH; c += 64)
+          odd |= not_finite(*(const uint4*)(st + H::OPER + 16 * w * H::ROWB + c * 16));
+        if (__builtin_amdgcn_ballot_w64(odd)) {
+#pragma unroll 1
+          for (int key = 0; key < 16; ++key) {
+            const float pi = (key & 3) == 0 ? s[0] : (key & 3) == 1 ? s[1] : (key & 3) == 2 ? s[2] : s[3];
+            const float p = __shfl(pi, n16 + 16 * (key >> 2), 64);
+            const int row = 16 * w + key;
+#pragma unroll
+            for (int d = 0; d < DB; ++d) {
+              const int chunk = (2 * d + (q4 >> 1)) ^ H::v_swz(row);
+              const char* vp = st + H::OPER + row * H::ROWB + (chunk << 4) + 8 * (q4 & 1);
+              const uint2 x = *(const uint2*)vp;
+              const float v[4] = {__uint_as_float(x.x << 16), __uint_as_float(x.x & 0xffff0000u),
+                                  __uint_as_float(x.y << 16), __uint_as_float(x.y & 0xffff0000u)};
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[d][e] = key <= limit ? fmaf(p, v[e], o[d][e]) : o[d][e];
+            }
+          }
+          return;
+        }
+      }
+      const s16x4 pb = __builtin_bit_cast(s16x4, make_uint2(pack_bf16x2(s[0], s[1]), pack_bf16x2(s[2], s[3])));
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+        o[d] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(read_tr(st + vat + ((32 * d) ^ vx)), pb, o[d], 0, 0, 0);
+    });
   }
 
   // ---- the four waves' keys joined through LDS ------------------------------
@@ -825,13 +837,15 @@ __global__ __launch_bounds__(256, 2) void shared_attn_bf16_kernel(SharedArgs a) 
 template <typename T, int D, int SG>
 __global__ __launch_bounds__(256) void shared_join_kernel(SharedArgs a) {
   constexpr int LPR = D / 4, RB = 256 / (LPR * SG);
-  __shared__ __attribute__((aligned(16))) float po[SG > 1 ? 256 * 4 : 4];
-  __shared__ float2 pml[SG > 1 ? SG * RB : 1];
+  static_assert(RB == 1 || SG == 1, "a block's sets share one row, or each has its own");
+  __shared__ f32x4 po[4][LPR];
+  __shared__ float2 pml[4];
   const int64_t rows = (int64_t)a.B * a.T * a.Hq;
   const int lane = threadIdx.x % LPR, sg = threadIdx.x / LPR % SG, rb = threadIdx.x / (LPR * SG);
   const int64_t i = (int64_t)blockIdx.x * RB + rb;
   const int64_t row = std::min<int64_t>(i, rows - 1);
   const int slots = a.splits_p + a.splits_s;
+  const bool idle = own_len(a, row / a.Hq / a.T) < 0;
   float m = -__builtin_inff(), l = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
   auto add = [&](float ms, float ls, const f32x4& os, float mn) {
@@ -866,20 +880,36 @@ __global__ __launch_bounds__(256) void shared_join_kernel(SharedArgs a) {
     m = mn;
   }
   if constexpr (SG > 1) {
-    *(f32x4*)(po + threadIdx.x * 4) = o;
-    if (lane == 0) pml[rb * SG + sg] = make_float2(m, l);
+    // the sets of a wave by lane exchange, then the four waves through LDS
+    auto fold = [&](float mo, float lo, const f32x4& oo) {
+      const float mn = fmaxf(m, mo);
+      const float a0 = m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+      const float a1 = mo == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(mo - mn);
+      l = l * a0 + lo * a1;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = o[e] * a0 + oo[e] * a1;
+      m = mn;
+    };
+#pragma unroll
+    for (int x = LPR; x < 64; x *= 2) {
+      f32x4 oo;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) oo[e] = __shfl_xor(o[e], x, 64);
+      const float mo = __shfl_xor(m, x, 64), lo = __shfl_xor(l, x, 64);
+      fold(mo, lo, oo);
+    }
+    const int wave = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) < LPR) {
+      po[wave][lane] = o;
+      if (lane == 0) pml[wave] = make_float2(m, l);
+    }
     __syncthreads();
-    if (sg != 0) return;
-    const float2* ml = pml + rb * SG;
-    m = ml[0].x;
-    for (int j = 1; j < SG; ++j) m = fmaxf(m, ml[j].x);
-    l = 0.f;
-    o = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (m != -__builtin_inff())
-      for (int j = 0; j < SG; ++j) add(ml[j].x, ml[j].y, *(const f32x4*)(po + (threadIdx.x + j * LPR) * 4), m);
+    if (threadIdx.x >= LPR) return;
+#pragma unroll
+    for (int j = 1; j < 4; ++j) fold(pml[j].x, pml[j].y, po[j][lane]);
   }
   if (i >= rows) return;
-  const bool empty = m == -__builtin_inff() || own_len(a, i / a.Hq / a.T) < 0;
+  const bool empty = idle || m == -__builtin_inff();
   float r[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) r[e] = empty ? 0.f : o[e] / l;
@@ -898,7 +928,7 @@ bool bf16_tiles(int dtype, int64_t D) { return dtype == MINITP_BF16 && D >= 32; 
 // Splits: the prefix part takes 256 blocks, each of at least two key tiles (one
 // on the fp32 path, whose tiles take three times as long), or, where that
 // leaves a block 16 tiles and more, 448 of the 512 places that there are; the
-// own part 256 blocks of at least four tiles. Measured (us a call): 32 rows of
+// own part 256 blocks of at least two tiles. Measured (us a call): 32 rows of
 // the 7B heads on 8,191 and up to 400 keys, 8 units: 16 splits 24.0, 32 22.1,
 // 48 25.3, 64 30.2; 256 rows on 32,256 and 511, 56 units: 7 splits 159.7, 8
 // 161.8, 9 176.1, 12 170.7; 8 rows x 4 of the 0.5B heads on 2,048: 8 splits
@@ -920,8 +950,9 @@ Plan shared_plan(int dtype, int64_t D, int64_t B, int64_t G, int64_t T, int64_t 
   const int64_t bp = G * Hkv * p.qtiles_p, bs = B * Hkv * p.qtiles_s;
   const int64_t tiles_p = cdiv(P, kt), tiles_s = cdiv(C + T, kt);
   auto within = [](int64_t v, int64_t most) { return (int)std::max<int64_t>(1, std::min(v, most)); };
-  p.splits_p = P > 0 ? within(std::min(448 / bp, std::max(256 / bp, tiles_p / 16)), tiles16 ? tiles_p / 2 : tiles_p) : 0;
-  p.splits_s = within(256 / bs, tiles_s / 4);
+  const int64_t most_p = tiles16 ? tiles_p / 2 : tiles_p;
+  p.splits_p = P > 0 ? within(std::min(448 / bp, std::max(256 / bp, tiles_p / 16)), most_p) : 0;
+  p.splits_s = within(256 / bs, tiles_s / 2);
   p.joined = (P == 0 && p.splits_s == 1) || (T * per <= H_SMALL && bs <= 256 && tiles_p + tiles_s <= 8) ||
              (T * per >= qt && 4 * T * per >= 3 * qt * p.qtiles_s && bs >= 256);
   if (p.joined) {
@@ -1002,7 +1033,7 @@ int launch_shared_prefix_attention(hipStream_t st, int dtype, const SharedPrefix
               (long long)s.C, (long long)s.T);
     return MINITP_ERR_UNSUPPORTED;
   }
-  if (p.items_p + p.items_s >= (1LL << 31) - 16 || rows >= (1LL << 31) || s.B / s.G * s.T * (s.Hq / s.Hkv) >= (1LL << 31)) {
+  if (p.items_p + p.items_s >= (1LL << 31) - 16 || rows >= (1LL << 31)) {
     set_error("shared_prefix_attention: %lld query rows are too many for one call", (long long)rows);
     return MINITP_ERR_UNSUPPORTED;
   }
