@@ -185,8 +185,8 @@ __global__ __launch_bounds__(MERGE_T) void beam_merge_kernel(SelectArgs a, int w
 
   // This thread's sets, four at a time: f(set, maximum). (A row that is not open
   // has no maxima: what its words hold is left out below.)
-  const int tpr = MERGE_T / wp, mw = tid / tpr, mj = tid % tpr, quads = mw < W ? a.sets / 4 : 0;
-  const float4* set_top = (const float4*)(a.set_top + (row0 + mw) * a.sets);
+  int tpr = MERGE_T / wp, mw = tid / tpr, mj = tid % tpr, quads = mw < W ? a.sets / 4 : 0;
+  const float4* set_top = (const float4*)(a.set_top + (row0 + std::min(mw, W - 1)) * a.sets);
   auto four = [&](int i, const float4& x, auto f) {
     f(4 * i, x.x);
     f(4 * i + 1, x.y);
@@ -198,14 +198,12 @@ __global__ __launch_bounds__(MERGE_T) void beam_merge_kernel(SelectArgs a, int w
     for (int i = mj; i < quads; i += tpr) four(i, set_top[i], f);
   };
   float4 kept[NR > 0 ? NR : 1];
+  bool keeps = NR > 0;
   auto each_set = [&](auto f) {
-    if constexpr (NR > 0) {
+    if (!keeps) return read_sets(f);
 #pragma unroll
-      for (int u = 0; u < NR; ++u)
-        if (mj + u * tpr < quads) four(mj + u * tpr, kept[u], f);
-    } else {
-      read_sets(f);
-    }
+    for (int u = 0; u < NR; ++u)
+      if (mj + u * tpr < quads) four(mj + u * tpr, kept[u], f);
   };
 
   // ---- each beam's log sum, kind and length factor, a wave a beam; the first
@@ -270,7 +268,7 @@ __global__ __launch_bounds__(MERGE_T) void beam_merge_kernel(SelectArgs a, int w
   if (wave < W) load_beam(wave);
   if constexpr (NR > 0) {
 #pragma unroll
-    for (int u = 0; u < NR; ++u) kept[u] = set_top[std::min(mj + u * tpr, std::max(quads - 1, 0))];
+    for (int u = 0; u < NR; ++u) kept[u] = set_top[std::min(mj + u * tpr, a.sets / 4 - 1)];
   }
   float most = -__builtin_inff();
   each_set([&](int, float x) { most = fmaxf(most, x); });
@@ -294,11 +292,28 @@ __global__ __launch_bounds__(MERGE_T) void beam_merge_kernel(SelectArgs a, int w
     }
   };
   // A finished beam and one that is no number have one set, the first, with a
-  // key of its own.
-  const int mkind = mw < W ? kind[mw] : ROW_NONE;
-  const uint64_t only = mj != 0 ? 0 : mkind == ROW_DONE ? order_key((double)score[mw] * inv[mw])
-                                    : mkind == ROW_NAN  ? ~0ull
-                                                        : 0;
+  // key of its own: thread w's.
+  const int tkind = tid < W ? kind[tid] : ROW_NONE;
+  const uint64_t only = tkind == ROW_DONE ? order_key((double)score[tid] * inv[tid]) : tkind == ROW_NAN ? ~0ull : 0;
+
+  // Few open rows (the first step has one a group): all threads on them, so that
+  // the bound below comes from at least 32 of the 64 sets of threads.
+  uint32_t open = (uint32_t)__builtin_amdgcn_ballot_w64(lane < W && kind[lane & 31] == ROW_OPEN);
+  const int nopen = __builtin_popcount(open);
+  if (2 * nopen <= wp) {
+    int wq = 1;
+    while (wq < nopen) wq *= 2;
+    tpr = MERGE_T / wq;
+    mj = tid % tpr;
+    for (int j = tid / tpr; j > 0; --j) open &= open - 1;
+    mw = open ? __builtin_ctz(open) : W;
+    quads = mw < W ? a.sets / 4 : 0;
+    set_top = (const float4*)(a.set_top + (row0 + std::min(mw, W - 1)) * a.sets);
+    keeps = false;
+    most = -__builtin_inff();
+    read_sets([&](int, float x) { most = fmaxf(most, x); });
+  }
+  const bool mopen = mw < W && kind[mw] == ROW_OPEN;
 
   // ---- a bound: the W-th largest of the 64 maxima of 16 threads each ---------
   // (16 threads of one row: one DPP row)
@@ -307,8 +322,7 @@ __global__ __launch_bounds__(MERGE_T) void beam_merge_kernel(SelectArgs a, int w
   rmost = fmaxf(rmost, dpp_f32<0x4E>(rmost, rmost));
   rmost = fmaxf(rmost, dpp_f32<0x141>(rmost, rmost));
   rmost = fmaxf(rmost, dpp_f32<0x140>(rmost, rmost));
-  // (the row's thread of the one set is its first)
-  if (lane % 16 == 0) group_top[tid / 16] = mkind == ROW_OPEN ? key_of(mw, rmost) : only;
+  if (lane % 16 == 0) group_top[tid / 16] = mopen ? key_of(mw, rmost) : 0;
   __syncthreads();
 #pragma unroll
   for (int c = 0; c < 4; ++c) {  // a wave ranks four of them
@@ -322,25 +336,24 @@ __global__ __launch_bounds__(MERGE_T) void beam_merge_kernel(SelectArgs a, int w
 
   // ---- the W best sets: first those whose maxima reach the bound, taken as a
   // logit of their row and lowered past what its rounding can be -------------
-  auto take = [&](float x, int set) {
+  auto take = [&](int w, int set, float x) {
     const int at = atomicAdd(&count, 1);
     if (at < MERGE_CAP) {
       lx[at] = x;
-      lf[at] = (uint64_t)mw << 32 | (uint32_t)set;
+      lf[at] = (uint64_t)w << 32 | (uint32_t)set;
     }
   };
-  if (mkind == ROW_OPEN && bound != ~0ull) {
+  if (mopen) {
     const double bk = __builtin_bit_cast(double, bound >> 63 ? bound ^ (1ull << 63) : ~bound);
     const float bx = (float)((bk / inv[mw] - (double)score[mw]) + lse[mw]);
     // (above minus infinity at least: those are no candidates)
     const float low = bound == 1 ? -3.402823466e38f : fmaxf(bx - (fabsf(bx) + 1.f) * 1e-5f, -3.402823466e38f);
     if (most >= low)
       each_set([&](int set, float x) {
-        if (x >= low) take(x, set);
+        if (x >= low) take(mw, set, x);
       });
-  } else if (only != 0) {
-    take(0.f, 0);
   }
+  if (only >= bound) take(tid, 0, 0.f);
   __syncthreads();
   int n = count;
   uint64_t least = bound;
@@ -365,17 +378,15 @@ __global__ __launch_bounds__(MERGE_T) void beam_merge_kernel(SelectArgs a, int w
     uint64_t pk = 0, pf = 0;
     for (n = 0; n < W; ++n) {
       uint64_t bk = 0, bf = ~0ull;
-      auto see = [&](uint64_t k, int set) {
-        const uint64_t f = (uint64_t)mw << 32 | (uint32_t)set;
+      auto see = [&](uint64_t k, int w, int set) {
+        const uint64_t f = (uint64_t)w << 32 | (uint32_t)set;
         if (k != 0 && (n == 0 || better(pk, pf, k, f)) && better(k, f, bk, bf)) {
           bk = k;
           bf = f;
         }
       };
-      if (mkind == ROW_OPEN)
-        read_sets([&](int set, float x) { see(key_of(mw, x), set); });
-      else
-        see(only, 0);
+      if (mopen) read_sets([&](int set, float x) { see(key_of(mw, x), mw, set); });
+      see(only, tid, 0);
 #pragma unroll
       for (int o = 32; o >= 1; o >>= 1) {
         const uint64_t ok = __shfl_xor(bk, o, 64), of = __shfl_xor(bf, o, 64);

@@ -176,6 +176,26 @@ def test_first_step_from_one_row_and_strided_rows():
             reference(turned, torch.zeros(2, 2), None, None, -1, 0.0))
 
 
+@pytest.mark.parametrize("beams", [2, 6, 16, 17, 32])
+@pytest.mark.parametrize("vocab", [500, 70001, 151936])
+def test_few_open_beams(vocab, beams):
+    """One open beam a group (a search's first step), a few, and one beside
+    finished ones, over short and long rows."""
+    from minitp import kernels as K
+
+    logits, scores, g = make(4, beams, vocab, torch.bfloat16)
+    finished = torch.zeros(4, beams, dtype=torch.bool, device=DEV)
+    scores[0, 1:] = -math.inf
+    scores[1, : beams - 1] = -math.inf
+    finished[2] = True
+    finished[2, beams // 2] = False
+    scores[2, beams // 2] += 4.0
+    scores[3, beams // 3 :] = -math.inf
+    lengths = torch.full((4, beams), 3, device=DEV)
+    step = K.beam_select(logits, scores, finished, lengths, eos_token_id=7, length_penalty=0.5)
+    compare(step, reference(logits, scores, finished, lengths, 7, 0.5))
+
+
 def test_large_vocabulary():
     from minitp import kernels as K
 
