@@ -364,6 +364,25 @@ int minitp_qwen2_forward(void* handle, void* stream, const minitp_qwen2_step* st
  * workspace), with per-step scalars and pointers patched into the graph's
  * first node. */
 int minitp_qwen2_decode(void* handle, void* stream, const minitp_qwen2_step* step);
+/* minitp_qwen2_forward for a batch whose rows share prefixes (the beams of a
+ * prompt, requests under one system prompt; no counterpart in the reference):
+ * `groups` runs of consecutive batch rows attend rows 0 .. len - 1 of their
+ * group's prefix K/V rows [L, groups, Hkv, max_seq, D] before their own, as
+ * minitp_shared_prefix_attention does; positions go on from the prefix's.
+ * Direct launches for any token count. The prefix's workspace: the size that
+ * minitp_shared_prefix_attention_workspace_bytes gives for the step's batch,
+ * tokens and cache_len. */
+typedef struct minitp_shared_prefix {
+  const void* k;
+  const void* v;
+  int64_t groups;
+  int64_t len;
+  int64_t max_seq;
+  void* workspace;
+  int64_t workspace_bytes;
+} minitp_shared_prefix;
+int minitp_qwen2_forward_shared(void* handle, void* stream, const minitp_qwen2_step* step,
+                                const minitp_shared_prefix* prefix);
 /* Out-of-range RoPE positions (rope.py:37-45, where the reference's gather
  * raises): a forward whose position lies outside the table computes with NaN
  * rotary rows and sets a sticky error word in its workspace, because a

@@ -220,13 +220,15 @@ struct Qwen2Program {
   }
 
   // The launch sequence of one forward (also what a decode graph records).
-  int run(hipStream_t st, const minitp_qwen2_step& s, const Ws& w) {
-    const int rc = run_model(st, s, w);
+  int run(hipStream_t st, const minitp_qwen2_step& s, const Ws& w, const minitp_shared_prefix* pre = nullptr) {
+    const int rc = run_model(st, s, w, pre);
     if (rc || s.eos_state == nullptr) return rc;
     return launch_eos_update(st, w.st, s.batch);
   }
 
-  int run_model(hipStream_t st, const minitp_qwen2_step& s, const Ws& w) {
+  // pre: rows in front of the caches that groups of batch rows share (direct
+  // launches only: its pointers and lengths are the call's own).
+  int run_model(hipStream_t st, const minitp_qwen2_step& s, const Ws& w, const minitp_shared_prefix* pre) {
     const int64_t B = s.batch, T = s.tokens, M = B * T;
     const int64_t H = c.hidden, I = c.intermediate, V = c.vocab;
     const int D = c.head_dim;
@@ -245,9 +247,28 @@ struct Qwen2Program {
     AttnShape as{(int)B, (int)T, c.heads, c.kv_heads, D, s.max_seq};
     // one-row decode: attention + o_proj in one kernel, its per-head partials
     // summed (with the residual) by the gate/up prologue
-    const bool fo = fz && T == 1 && fuse_oproj && attn_oproj_supported(c.dtype, as, H, OPROJ_SLICES) &&
+    const bool fo = fz && T == 1 && pre == nullptr && fuse_oproj && attn_oproj_supported(c.dtype, as, H, OPROJ_SLICES) &&
                     gemv_part_supported(c.dtype, H, c.heads);
     const int64_t layer_elems = B * c.kv_heads * s.max_seq * D;
+    auto shared_attention = [&](int l) {
+      const int64_t pre_bytes = (int64_t)l * pre->groups * c.kv_heads * pre->max_seq * D * es();
+      SharedPrefixShape sh{};
+      sh.B = B;
+      sh.G = pre->groups;
+      sh.T = T;
+      sh.Hq = c.heads;
+      sh.Hkv = c.kv_heads;
+      sh.D = D;
+      sh.Sp = pre->max_seq;
+      sh.S = s.max_seq;
+      sh.P = pre->len;
+      sh.C = s.cache_len;
+      return launch_shared_prefix_attention(st, c.dtype, sh, w.q, (const char*)pre->k + pre_bytes,
+                                            (const char*)pre->v + pre_bytes,
+                                            (const char*)s.k_cache + l * layer_elems * es(),
+                                            (const char*)s.v_cache + l * layer_elems * es(), w.attn, nullptr, nullptr,
+                                            pre->workspace, pre->workspace_bytes);
+    };
     // Rows past the GEMV forms: plain GEMMs (the 256 x 256 MFMA tile kernel
     // or the smaller tiles, by the measured costs), gate/up with SwiGLU in the
     // epilogue. The residual adds go with the next RMSNorm (one fused kernel,
@@ -297,7 +318,8 @@ struct Qwen2Program {
         if (rc) return rc;
         const char* kc = (const char*)s.k_cache + l * layer_elems * es();
         const char* vc = (const char*)s.v_cache + l * layer_elems * es();
-        rc = T == 1 ? launch_decode_attention(st, c.dtype, w.q, nullptr, nullptr, w.attn, as, s.cache_len, w.st, l,
+        rc = pre != nullptr ? shared_attention(l)
+             : T == 1 ? launch_decode_attention(st, c.dtype, w.q, nullptr, nullptr, w.attn, as, s.cache_len, w.st, l,
                                               w.attn_ws, w.attn_ws_bytes)
                     : launch_prefill_attention(st, c.dtype, w.q, kc, vc, w.attn, as, s.cache_len, w.st, l);
         if (rc) return rc;
@@ -354,6 +376,8 @@ struct Qwen2Program {
       if (fo) {
         const OprojArgs o{L(l, MINITP_W_O), H, attn_oproj_rows(c.dtype, as, H, OPROJ_SLICES), w.opart};
         if ((rc = launch_decode_attention_oproj(st, c.dtype, w.q, as, w.st, l, o))) return rc;
+      } else if (pre != nullptr) {
+        if ((rc = shared_attention(l))) return rc;
       } else if (T == 1) {
         if ((rc = launch_decode_attention(st, c.dtype, w.q, nullptr, nullptr, w.attn, as, s.cache_len, w.st, l,
                                           w.attn_ws, w.attn_ws_bytes)))
@@ -730,6 +754,38 @@ int minitp_qwen2_forward(void* handle, void* stream, const minitp_qwen2_step* st
   if (rc) return rc;
   if (p->prompt_graphable(*step)) return minitp::run_graphed(p, (hipStream_t)stream, *step, w);
   return p->run((hipStream_t)stream, *step, w);
+}
+
+int minitp_qwen2_forward_shared(void* handle, void* stream, const minitp_qwen2_step* step,
+                                const minitp_shared_prefix* prefix) {
+  MINITP_CHECK_ARG(handle != nullptr && prefix != nullptr, "NULL argument");
+  auto* p = (Qwen2Program*)handle;
+  minitp::Ws w;
+  const int rc = p->check_step(step, w);
+  if (rc) return rc;
+  MINITP_CHECK_ARG(prefix->groups > 0 && prefix->len >= 0, "shared prefix: %lld groups of %lld rows",
+                   (long long)prefix->groups, (long long)prefix->len);
+  if (step->batch % prefix->groups != 0) {
+    minitp::set_error("shared prefix: batch rows %lld not divisible by groups %lld", (long long)step->batch,
+                      (long long)prefix->groups);
+    return MINITP_ERR_DIVISIBLE;
+  }
+  if (prefix->len > prefix->max_seq) {
+    minitp::set_error("KV cache overflow: prefix %lld > prefix rows %lld", (long long)prefix->len,
+                      (long long)prefix->max_seq);
+    return MINITP_ERR_OVERFLOW;
+  }
+  MINITP_CHECK_ARG(prefix->len == 0 || (prefix->k != nullptr && prefix->v != nullptr && minitp::aligned16(prefix->k) &&
+                                        minitp::aligned16(prefix->v)),
+                   "shared prefix: K/V rows must be there and 16-byte aligned");
+  const int64_t need =
+      minitp::shared_prefix_workspace_bytes(p->c.dtype, step->batch, prefix->groups, step->tokens, p->c.heads,
+                                            p->c.kv_heads, p->c.head_dim, prefix->len, step->cache_len);
+  MINITP_CHECK_ARG(prefix->workspace_bytes >= need && (prefix->workspace != nullptr || need == 0) &&
+                       minitp::aligned16(prefix->workspace),
+                   "shared prefix: workspace %p of %lld B, %lld B needed (16-byte aligned)", prefix->workspace,
+                   (long long)prefix->workspace_bytes, (long long)need);
+  return p->run((hipStream_t)stream, *step, w, prefix);
 }
 
 int minitp_qwen2_decode(void* handle, void* stream, const minitp_qwen2_step* step_in) {

@@ -73,6 +73,7 @@ SIGNATURES = {
     "minitp_qwen2_destroy": (_int, [_vp]),
     "minitp_qwen2_workspace_bytes": (_i64, [_vp, _i64, _i64, _i64]),
     "minitp_qwen2_forward": (_int, [_vp, _vp, _vp]),
+    "minitp_qwen2_forward_shared": (_int, [_vp, _vp, _vp, _vp]),
     "minitp_qwen2_decode": (_int, [_vp, _vp, _vp]),
     "minitp_qwen2_decode_check": (_int, [_vp, _vp, _vp]),
 }
@@ -94,6 +95,11 @@ class Qwen2Step(ctypes.Structure):
                 ("logits_all", _i32), ("next_tok", _vp), ("next_tok_ld", _i64), ("workspace", _vp),
                 ("workspace_bytes", _i64), ("eos_state", _vp), ("eos_token", _i64), ("cursor", _i64),
                 ("eos_host", _vp)]
+
+
+class SharedPrefix(ctypes.Structure):
+    _fields_ = [("k", _vp), ("v", _vp), ("groups", _i64), ("len", _i64), ("max_seq", _i64), ("workspace", _vp),
+                ("workspace_bytes", _i64)]
 
 
 _lib = None

@@ -384,7 +384,7 @@ def shared_prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: t
     q = q.contiguous()
     out = q.new_empty((b, t, hq * d))
     dt = N.dtype_code(dtype)
-    nbytes = _shared_prefix_bytes(dt, b, groups, t, hq, hkv, d, prefix_len, cache_len)
+    nbytes = shared_prefix_bytes(dt, b, groups, t, hq, hkv, d, prefix_len, cache_len)
     # from the caching allocator on the current stream: calls on other streams
     # and captured graphs have scratch of their own
     ws = q.new_empty((nbytes,), dtype=torch.uint8) if nbytes > 0 else None
@@ -396,7 +396,8 @@ def shared_prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: t
 
 
 @functools.lru_cache(maxsize=4096)
-def _shared_prefix_bytes(*sizes: int) -> int:
+def shared_prefix_bytes(*sizes: int) -> int:
+    """Scratch of shared_prefix_attention: dtype code, B, G, T, Hq, Hkv, D, prefix_len, cache_len."""
     return max(_lib().minitp_shared_prefix_attention_workspace_bytes(*sizes), 0)
 
 

@@ -5,8 +5,8 @@
 toggles it runs the whole forward as one native program (libminitp's
 minitp_qwen2_forward: fused norm/QKV/RoPE/KV-write, attention, o_proj +
 residual, norm/gate-up/SwiGLU, down + residual per layer). When an ablation
-toggle is changed, profiling labels are on, or the cache has a shared prefix, it
-walks the modules instead; that path runs the same kernels one op at a time.
+toggle is changed, or profiling labels are on, it walks the modules instead;
+that path runs the same kernels one op at a time.
 """
 
 from __future__ import annotations
@@ -225,7 +225,20 @@ class TPQwen2ForCausalLM(nn.Module):
                            kv.v_buf.data_ptr(), kv.capacity, logits.data_ptr(), 1 if all_rows else 0,
                            N.ptr(next_tok), next_tok.stride(0) if next_tok is not None else 0, ws.data_ptr(),
                            ws.numel(), *(eos or (None, 0, 0, None)))
-        N.check(N.lib().minitp_qwen2_forward(prog.handle, N.stream(), ctypes.byref(step)), "qwen2_forward")
+        if kv.prefix is None:
+            N.check(N.lib().minitp_qwen2_forward(prog.handle, N.stream(), ctypes.byref(step)), "qwen2_forward")
+        else:
+            pre = kv.prefix
+            groups = pre.k_buf.shape[1]
+            prog.check_cache(pre, groups)
+            a = self.model.layers[0].self_attn
+            need = K.shared_prefix_bytes(N.dtype_code(prog.dtype), b, groups, t, a.q_heads_local, a.kv_heads_local,
+                                         self.cfg.head_dim, pre.seq_len, kv.seq_len)
+            scratch = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+            shared = N.SharedPrefix(pre.k_buf.data_ptr(), pre.v_buf.data_ptr(), groups, pre.seq_len, pre.capacity,
+                                    N.ptr(scratch), need)
+            N.check(N.lib().minitp_qwen2_forward_shared(prog.handle, N.stream(), ctypes.byref(step),
+                                                        ctypes.byref(shared)), "qwen2_forward_shared")
         if kv_cache is not None:
             kv_cache.advance(t)
         return logits
@@ -285,7 +298,7 @@ class TPQwen2ForCausalLM(nn.Module):
             positions = torch.where(positions < 0, positions + limit, positions)
         if kv_cache is not None:
             kv_cache.check_room(t)
-        if self.native_path() and (kv_cache is None or kv_cache.prefix is None):
+        if self.native_path():
             return self._native(input_ids, positions, kv_cache)
         x = self.model.embed_tokens(input_ids)
         rotary = self._ensure_rotary(x.device) if self.use_rotary_cache else None

@@ -1,6 +1,7 @@
 """Refusals of the beam-search and shared-prefix entry points: every invalid
 call is turned down on the host, before any pointer is used (no GPU)."""
 
+import ctypes
 import math
 
 import pytest
@@ -81,6 +82,35 @@ def test_kv_reorder_refuses(status, change):
 def test_kv_reorder_of_nothing():
     assert reorder(rows=0, k=None, v=None, parents=None) == N.OK
     assert reorder(layers=0) == N.OK and reorder(g=0) == N.OK
+
+
+def test_forward_shared_refuses():
+    lib = N.lib()
+    cfg = N.Qwen2Config(N.BF16, 2, 64, 4, 2, 16, 128, 1000, 9000, 1e-6)
+    fake = (ctypes.c_void_p * 14)(*([P] * 14))
+    w = N.Qwen2Weights(P, P, P, P, P, ctypes.cast(fake, ctypes.POINTER(ctypes.c_void_p)))
+    h = ctypes.c_void_p()
+    assert lib.minitp_qwen2_create(ctypes.byref(cfg), ctypes.byref(w), ctypes.byref(h)) == N.OK
+    try:
+        step = N.Qwen2Step()
+        step.batch, step.tokens, step.cache_len, step.max_seq, step.ids_ld = 6, 1, 20, 24, 1
+        step.ids = step.positions = step.k_cache = step.v_cache = step.logits = step.workspace = P
+        step.workspace_bytes = 1 << 40
+
+        def call(cache_len=20, **change):
+            step.cache_len = cache_len
+            pre = N.SharedPrefix(P, P, 2, 5000, 8192, P, 1 << 40)
+            for name, value in change.items():
+                setattr(pre, name, value)
+            return lib.minitp_qwen2_forward_shared(h, None, ctypes.byref(step), ctypes.byref(pre))
+
+        assert lib.minitp_qwen2_forward_shared(h, None, ctypes.byref(step), None) == N.ERR_ARG
+        assert call(groups=0) == call(len=-1) == call(k=None) == call(v=P + 4) == N.ERR_ARG
+        assert call(workspace=None) == call(workspace_bytes=100) == call(workspace=P + 8) == N.ERR_ARG
+        assert call(groups=4) == N.ERR_DIVISIBLE
+        assert call(len=8193) == call(cache_len=24) == N.ERR_OVERFLOW
+    finally:
+        lib.minitp_qwen2_destroy(h)
 
 
 def test_wrappers_have_no_cpu_path():

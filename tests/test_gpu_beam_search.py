@@ -130,12 +130,25 @@ def test_greedy_under_a_shared_prefix(dtype):
         kv.share_prefix(pre)
         return kv
 
+    # the program and the modules walked one by one (other roundings of bf16)
+    kv = caches()
+    native = model(asks, kv_cache=kv)
+    for layer in model.model.layers:
+        layer.self_attn.use_fused_qkv = False
+    walked = model(asks, kv_cache=caches())
+    for layer in model.model.layers:
+        layer.self_attn.use_fused_qkv = True
     whole = torch.cat([system.repeat_interleave(3, 0), asks], 1)
     logits, plain = model(asks, kv_cache=caches()), model(whole)[:, 70:]
     # two forms of the same forward: each within the path's own bar of the
     # oracle's logits (bf16 0.5, fp32 1e-3)
     bar = 0.5 if dtype == torch.bfloat16 else 1e-3
-    assert (logits.float() - plain.float()).abs().max() <= 2 * bar
+    for got in (logits, native, walked):
+        assert (got.float() - plain.float()).abs().max() <= 2 * bar
+    # one more token on the program
+    tok = native[:, -1].argmax(-1, keepdim=True)
+    step, plain = model(tok, kv_cache=kv), model(torch.cat([whole, tok], 1))[:, -1:]
+    assert kv.seq_len == 10 and (step.float() - plain.float()).abs().max() <= 2 * bar
     if dtype == torch.float32:
         out = generate_greedy(model, asks, 10, kv=caches())
         assert torch.equal(out, generate_greedy(model, whole, 10)[:, 70:])
