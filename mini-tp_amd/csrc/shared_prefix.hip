@@ -24,34 +24,47 @@ namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
+// Division by a number the host knows: n / d for 0 <= n < 2^31 as one product
+// (m = ceil(2^(31 + l) / d) with 2^l >= d: n (m d - 2^(31 + l)) < 2^(31 + l)). The
+// index arithmetic in front of a block's first load is all latency: 1.0 us of
+// a 10 us call with the compiler's divisions, most of them in 64 bits.
+struct Div {
+  uint32_t mul;
+  int shift;
+  __device__ __forceinline__ int operator()(int n) const { return (int)(((uint64_t)(uint32_t)n * mul) >> shift); }
+};
+
 struct SharedArgs {
   const void *q, *kp, *vp, *kc, *vc;  // q [B, T, Hq, D]; prefix [G, Hkv, Sp, D]; own [B, Hkv, S, D]
   void* out;                          // [B, T, Hq * D]
-  int B, G, T, Hq, Hkv;
+  int B, T, Hq, Hkv;
+  int w, per;                         // batch rows of a group, query heads of a KV head
   int64_t Sp, S;
-  int64_t P, C;                       // prefix rows, cached own rows (bounds of the lengths below)
+  int64_t query_rows;                 // B * T * Hq
+  int P, C;                           // prefix rows, cached own rows (bounds of the lengths below)
   const int64_t *plens, *clens;       // [G], [B], or NULL: P and C everywhere
   float scale;
   int qtiles_p, qtiles_s;             // query tiles of a unit, prefix and own part
   int splits_p, splits_s;             // key splits
   int items_p, items_s;               // items of the two parts
   int run_p, run_s;                   // ... of one XCD
+  Div by_qtiles_p, by_qtiles_s, by_splits_p, by_splits_s, by_hkv, by_w, by_per;
   bool joined;                        // an item takes both parts and writes the output: no slots
   float* ml;                          // [slot][B * T * Hq][2]: maximum, sum
   float* o;                           // [slot][B * T * Hq][D]
 };
 
-// Consecutive K/V rows: query r of an item sees them up to seen + r / (heads
-// of the KV group).
+// Consecutive K/V rows, n of them; the queries of a unit's token t see those up
+// to seen + t.
 struct Keys {
   const void *k, *v;
-  int n;
-  int64_t seen;
+  int n, seen;
+  bool own;
 };
 
-// The last of the keys that query r sees (-1: none).
-__device__ __forceinline__ int last_seen(const Keys& k, int r, int per) {
-  return (int)std::max<int64_t>(std::min<int64_t>(k.seen + r / per, k.n - 1), -1);
+// The last of the keys that token t sees (-1: none).
+__device__ __forceinline__ int last_seen(const Keys& k, int t) {
+  return k.own ? std::max(std::min(k.seen + t, k.n - 1), -1) : k.n - 1;
 }
 
 // What one block computes: a tile of a unit's query rows over the keys of the
@@ -59,27 +72,28 @@ __device__ __forceinline__ int last_seen(const Keys& k, int r, int per) {
 struct Item {
   Keys pre, own;
   int first, last;  // parts: 0 the prefix, 1 the own rows
-  int64_t n0;       // first token (b * T + t) of the unit
+  int n0;           // first token (b * T + t) of the unit
   int rows;         // query rows of the unit: (token, head of the KV group)
   int tile, kv, slot;
 };
 
 // Cached own rows of batch row b, -1 for an idle row (nothing attends).
-__device__ __forceinline__ int64_t own_len(const SharedArgs& a, int64_t b) {
+__device__ __forceinline__ int own_len(const SharedArgs& a, int b) {
   if (a.clens == nullptr) return a.C;
-  return std::min<int64_t>(std::max<int64_t>(a.clens[b], -1), a.C);
+  return (int)std::min<int64_t>(std::max<int64_t>(a.clens[b], -1), a.C);
 }
 
-// Rows key_lo .. of a prefix or of a batch row's cache, those of one split.
+// Rows of a prefix or of a batch row's cache, those of one split.
 template <int KT>
 __device__ __forceinline__ void set_keys(Keys& k, const void* kb, const void* vb, int64_t row0, int64_t row_bytes,
-                                         int64_t keys, int64_t seen, int split, int splits) {
-  const int64_t span = cdiv(cdiv(keys, (int64_t)KT), (int64_t)splits) * KT;
-  const int64_t lo = std::min<int64_t>(split * span, keys);
+                                         int keys, int split, int splits, const Div& by_splits) {
+  const uint32_t tiles = ((uint32_t)keys + KT - 1) / KT;
+  const uint32_t span = (uint32_t)by_splits((int)tiles + splits - 1) * KT;
+  const int lo = (int)std::min<uint32_t>(split * span, (uint32_t)keys);
   k.k = (const char*)kb + (row0 + lo) * row_bytes;
   k.v = (const char*)vb + (row0 + lo) * row_bytes;
-  k.n = (int)(std::min<int64_t>(lo + span, keys) - lo);
-  k.seen = seen - lo;
+  k.n = (int)std::min<uint32_t>(span, (uint32_t)(keys - lo));
+  k.seen = -lo;
 }
 
 // Block -> item. Blocks go to the eight XCDs round robin, each with an L2 of
@@ -90,36 +104,48 @@ __device__ __forceinline__ void set_keys(Keys& k, const void* kb, const void* vb
 // False: no item.
 template <int QT, int KT>
 __device__ __forceinline__ bool shared_item(const SharedArgs& a, int64_t row_bytes, Item& it) {
-  const int per = a.Hq / a.Hkv;
   const int xcd = blockIdx.x % 8, seq = blockIdx.x / 8;
   const bool own = seq >= a.run_p;
   int i = own ? xcd * a.run_s + seq - a.run_p : xcd * a.run_p + seq;
   if (i >= (own ? a.items_s : a.items_p)) return false;
-  const int qtiles = own ? a.qtiles_s : a.qtiles_p, splits = own ? a.splits_s : a.splits_p;
-  it.tile = i % qtiles;
-  i /= qtiles;
-  const int split = i % splits;
-  i /= splits;  // (group or batch row, KV head)
-  it.kv = i % a.Hkv;
-  const int w = a.B / a.G, b = own ? i / a.Hkv : i / a.Hkv * w, g = b / w;
-  it.n0 = (int64_t)b * a.T;
-  it.rows = (own ? 1 : w) * a.T * per;
+  const int splits = own ? a.splits_s : a.splits_p;
+  const Div by_qtiles = own ? a.by_qtiles_s : a.by_qtiles_p, by_splits = own ? a.by_splits_s : a.by_splits_p;
+  const int j = by_qtiles(i), unit = by_splits(j), head0 = a.by_hkv(unit);  // (unit: group or batch row, KV head)
+  it.tile = i - j * (own ? a.qtiles_s : a.qtiles_p);
+  const int split = j - unit * splits;
+  it.kv = unit - head0 * a.Hkv;
+  const int b = own ? head0 : head0 * a.w, g = own ? a.by_w(head0) : head0;
+  it.n0 = b * a.T;
+  it.rows = (own ? 1 : a.w) * a.T * a.per;
   it.slot = own ? a.splits_p + split : split;
   it.first = own && (!a.joined || a.P == 0) ? 1 : 0;
   it.last = own ? 1 : 0;
+  it.pre.own = false;
+  it.own.own = true;
   if (it.first == 0) {
-    const int64_t keys = a.plens == nullptr ? a.P : std::min<int64_t>(std::max<int64_t>(a.plens[g], 0), a.P);
-    set_keys<KT>(it.pre, a.kp, a.vp, ((int64_t)g * a.Hkv + it.kv) * a.Sp, row_bytes, keys, INT64_MAX / 2,
-                 own ? 0 : split, own ? 1 : splits);
+    const int keys = a.plens == nullptr ? a.P : (int)std::min<int64_t>(std::max<int64_t>(a.plens[g], 0), a.P);
+    set_keys<KT>(it.pre, a.kp, a.vp, ((int64_t)g * a.Hkv + it.kv) * a.Sp, row_bytes, keys, own ? 0 : split,
+                 own ? 1 : splits, own ? Div{1u << 31, 31} : by_splits);
   }
   if (own) {
-    const int64_t seen = own_len(a, b);
+    const int seen = own_len(a, b);
     const int last = std::min(it.tile * QT + QT, it.rows) - 1;  // (the tile's last query sees the most keys)
-    set_keys<KT>(it.own, a.kc, a.vc, (int64_t)i * a.S, row_bytes, seen < 0 ? 0 : seen + last / per + 1, seen, split,
-                 splits);
+    set_keys<KT>(it.own, a.kc, a.vc, (int64_t)unit * a.S, row_bytes, seen < 0 ? 0 : seen + a.by_per(last) + 1, split,
+                 splits, by_splits);
+    it.own.seen += seen;
     if (seen < 0) it.own.n = it.pre.n = 0;  // an idle row
   }
   return true;
+}
+
+// Query row r of an item: its token of the unit, and its row of q and out.
+struct Query {
+  int t;
+  int64_t row;
+};
+__device__ __forceinline__ Query query_of(const SharedArgs& a, const Item& it, int r) {
+  const int t = a.by_per(r);
+  return Query{t, (int64_t)(it.n0 + t) * a.Hq + it.kv * a.per + (r - t * a.per)};
 }
 
 // One tile of keys through a resource of its own (a head's rows may span more
@@ -159,7 +185,6 @@ template <typename T, int D, int KW, bool BASE2>
 __device__ __forceinline__ void finish_rows(const SharedArgs& a, const Item& it, const float* po, const float2* pml,
                                             int cap, int r0, int rows) {
   constexpr int LPR = D / 4;
-  const int per = a.Hq / a.Hkv;
   for (int i = threadIdx.x; i < rows * LPR; i += 256) {
     const int row = i / LPR, d = i % LPR * 4;
     float2 ml[KW];
@@ -179,15 +204,14 @@ __device__ __forceinline__ void finish_rows(const SharedArgs& a, const Item& it,
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[e] = fmaf(sc, oj[e], o[e]);
     }
-    const int r = r0 + row;
-    const int64_t n = (it.n0 + r / per) * a.Hq + it.kv * per + r % per;
+    const int64_t n = query_of(a, it, r0 + row).row;
     if (a.joined) {
       float v[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] = m == -__builtin_inff() ? 0.f : o[e] / l;
       store_vec<T, 4>((T*)a.out + n * D + d, v);
     } else {
-      const int64_t at = (int64_t)it.slot * a.B * a.T * a.Hq + n;
+      const int64_t at = it.slot * a.query_rows + n;
       *(f32x4*)(a.o + at * D + d) = o;
       if (d == 0) *(float2*)(a.ml + at * 2) = make_float2(BASE2 ? m : m * 1.4426950408889634f, l);
     }
@@ -215,17 +239,14 @@ __device__ __forceinline__ void shared_rows_f32(const SharedArgs& a, const Item&
   constexpr int ROW = D + 4;
   constexpr int VE = Vec<T>::N, PIECES = KT * D / VE, PER = (PIECES + 255) / 256;
   float *Ks = lds, *Vs = lds + KT * ROW;
-  const int per = a.Hq / a.Hkv;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lr = lane % 16, lq = lane / 16, strip = wave % SW, key0 = wave / SW * KB * 16;
   const int t0 = it.tile * F_QT, r = t0 + strip * 16 + lr;
-  const bool live = r < it.rows;
-  const int64_t n = it.n0 + (live ? r : 0) / per;
-  const int h = it.kv * per + (live ? r : 0) % per;
+  const Query me = query_of(a, it, r < it.rows ? r : 0);
 
   f32x4 qa[KC];
   {
-    const T* qrow = (const T*)a.q + (n * a.Hq + h) * D;
+    const T* qrow = (const T*)a.q + me.row * D;
 #pragma unroll
     for (int c = 0; c < KC; ++c) load_vec<T, 4>(qrow + 16 * c + 4 * lq, (float*)&qa[c]);
   }
@@ -238,7 +259,7 @@ __device__ __forceinline__ void shared_rows_f32(const SharedArgs& a, const Item&
 
   for (int part = it.first; part <= it.last; ++part) {
     const Keys ks = part == 0 ? it.pre : it.own;
-    const int seen = last_seen(ks, live ? r : 0, per), all_see = last_seen(ks, t0, per);
+    const int seen = last_seen(ks, me.t), all_see = last_seen(ks, a.by_per(t0));
     uint4 kr[PER], vr[PER];
     auto load_tile = [&](int key) {
       const __amdgpu_buffer_rsrc_t krs = key_rows(ks.k, key, ks.n, KT, D * (int)sizeof(T));
@@ -542,24 +563,21 @@ template <int D>
 __device__ __forceinline__ void shared_rows128(const SharedArgs& a, const Item& it, char* lds) {
   using H = Half<D>;
   constexpr int KS = D / 16, DB = D / 32;
-  const int per = a.Hq / a.Hkv;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n32 = lane & 31, h = lane >> 5;
-  const int r0 = it.tile * H_QT + w * 32, r = r0 + n32;
-  const bool live = r < it.rows;
-  const int64_t n = it.n0 + (live ? r : 0) / per;
-  const int head = it.kv * per + (live ? r : 0) % per;
   Keys ks = it.first == 0 ? it.pre : it.own;
   Tiles<D> tiles(ks, lds);
   tiles.load(0);
+  const int r0 = it.tile * H_QT + w * 32, r = r0 + n32;
+  const Query me = query_of(a, it, r < it.rows ? r : 0);
 
   bf16x8 qb[KS];
   {
-    const bf16* q = (const bf16*)a.q + (n * a.Hq + head) * D + 8 * h;
+    const bf16* q = (const bf16*)a.q + me.row * D + 8 * h;
 #pragma unroll
     for (int k = 0; k < KS; ++k) qb[k] = __builtin_bit_cast(bf16x8, *(const u32x4*)(q + 16 * k));
-    arrived(qb);
   }
+  const int t_first = a.by_per(it.tile * H_QT), t_last = a.by_per(r0 + 31);  // of the block, of the wave
   f32x16 o[DB];
 #pragma unroll
   for (int d = 0; d < DB; ++d)
@@ -574,6 +592,7 @@ __device__ __forceinline__ void shared_rows128(const SharedArgs& a, const Item& 
   const int vrow = 4 * h + (lane & 15) / 4;
   const int vat = H::OPER + vrow * H::ROWB + 8 * (lane & 1);
   const int vx = ((2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) ^ H::v_swz(vrow)) << 4;
+  arrived(qb);
 
   for (int part = it.first; part <= it.last; ++part) {
     if (part != it.first) {
@@ -582,17 +601,19 @@ __device__ __forceinline__ void shared_rows128(const SharedArgs& a, const Item& 
       __syncthreads();  // (every stage is free)
       tiles.load(0);
     }
-    const int seen = last_seen(ks, live ? r : 0, per), seen_last = last_seen(ks, r0 + 31, per);
-    const int all_see = last_seen(ks, it.tile * H_QT, per);  // the last key that every query of the block sees
+    const int seen = last_seen(ks, me.t), seen_last = last_seen(ks, t_last);
+    const int all_see = last_seen(ks, t_first);  // the last key that every query of the block sees
     tiles.each(lds, (all_see + 1) / H_KT, [&](int t, const char* st, auto masked) {
       if (r0 >= it.rows || (masked && t * H_KT > seen_last)) return;
       f32x16 s[2];
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {
+      for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[kb][i] = 0.f;
 #pragma unroll
-        for (int k = 0; k < KS; ++k) {
+      for (int k = 0; k < KS; ++k) {
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {  // (two chains in turn)
           const bf16x8 kf = __builtin_bit_cast(bf16x8, *(const uint4*)(st + kat + kb * 32 * H::ROWB + ((32 * k) ^ kx)));
           s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qb[k], s[kb], 0, 0, 0);
         }
@@ -679,52 +700,61 @@ __device__ __forceinline__ void shared_rows128(const SharedArgs& a, const Item& 
       }
     });
   }
-  if (!live) return;
+  // ---- results through LDS, so that a store covers whole rows ---------------
+  __syncthreads();  // (every stage is free)
+  if (r0 >= it.rows) return;
   const float l = halves_sum(lsum);
   if (a.joined) {
-    bf16* orow = (bf16*)a.out + (n * a.Hq + head) * D + 4 * h;
+    const float f = m == -__builtin_inff() ? 0.f : 1.f / l;
 #pragma unroll
-    for (int d = 0; d < DB; ++d)
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        float v[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = m == -__builtin_inff() ? 0.f : o[d][4 * c + e] / l;
-        store_vec<bf16, 4>(orow + 32 * d + 8 * c, v);
-      }
-    return;
+    for (int d = 0; d < DB; ++d) o[d] *= f;
+  } else if (h == 0 && r < it.rows) {
+    *(float2*)(a.ml + (it.slot * a.query_rows + me.row) * 2) = make_float2(m, l);
   }
-  const int64_t at = (int64_t)it.slot * a.B * a.T * a.Hq + n * a.Hq + head;
-  if (h == 0) *(float2*)(a.ml + at * 2) = make_float2(m, l);
-  float* orow = a.o + at * D + 4 * h;
+  constexpr int CPR = D / 4, RPI = 64 / CPR;  // 16-byte chunks of a row, rows of a store
+  float* po = (float*)lds + w * 32 * D;       // this wave's [32][D], chunk c of row i at c ^ i
 #pragma unroll
   for (int d = 0; d < DB; ++d)
 #pragma unroll
     for (int c = 0; c < 4; ++c)
-      *(float4*)(orow + 32 * d + 8 * c) = make_float4(o[d][4 * c], o[d][4 * c + 1], o[d][4 * c + 2], o[d][4 * c + 3]);
+      *(f32x4*)(po + n32 * D + ((8 * d + 2 * c + h) ^ (n32 % CPR)) * 4) =
+          f32x4{o[d][4 * c], o[d][4 * c + 1], o[d][4 * c + 2], o[d][4 * c + 3]};
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  const int ch = lane % CPR;
+#pragma unroll
+  for (int i = 0; i < 32 / RPI; ++i) {
+    const int row = i * RPI + lane / CPR;
+    const f32x4 x = *(const f32x4*)(po + row * D + (ch ^ (row % CPR)) * 4);
+    const int64_t at = __shfl(me.row, row, 64);
+    if (r0 + row >= it.rows) continue;
+    if (a.joined) {
+      const float v[4] = {x[0], x[1], x[2], x[3]};
+      store_vec<bf16, 4>((bf16*)a.out + at * D + 4 * ch, v);
+    } else {
+      *(f32x4*)(a.o + (it.slot * a.query_rows + at) * D + 4 * ch) = x;
+    }
+  }
 }
 
 template <int D>
 __device__ __forceinline__ void shared_rows16(const SharedArgs& a, const Item& it, char* lds) {
   using H = Half<D>;
   constexpr int KS = D / 32, DB = D / 16;
-  const int per = a.Hq / a.Hkv;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n16 = lane & 15, q4 = lane >> 4;
-  const int r = n16;  // (one tile)
-  const bool live = r < it.rows;
-  const int64_t n = it.n0 + (live ? r : 0) / per;
-  const int head = it.kv * per + (live ? r : 0) % per;
   Keys ks = it.first == 0 ? it.pre : it.own;
   Tiles<D> tiles(ks, lds);
   tiles.load(0);
+  const int r = n16;  // (one tile)
+  const Query me = query_of(a, it, r < it.rows ? r : 0);
 
   bf16x8 qb[KS];
   {
-    const bf16* q = (const bf16*)a.q + (n * a.Hq + head) * D + 8 * q4;
+    const bf16* q = (const bf16*)a.q + me.row * D + 8 * q4;
 #pragma unroll
     for (int k = 0; k < KS; ++k) qb[k] = __builtin_bit_cast(bf16x8, *(const u32x4*)(q + 32 * k));
-    arrived(qb);
   }
   f32x4 o[DB];
 #pragma unroll
@@ -736,6 +766,7 @@ __device__ __forceinline__ void shared_rows16(const SharedArgs& a, const Item& i
   const int krow = 16 * w + n16, kat = krow * H::ROWB, kx = (q4 ^ H::k_swz(krow)) << 4;
   const int vrow = 16 * w + 4 * q4 + n16 / 4;
   const int vat = H::OPER + vrow * H::ROWB + 8 * (lane & 1), vx = (((lane >> 1) & 1) ^ H::v_swz(vrow)) << 4;
+  arrived(qb);
 
   for (int part = it.first; part <= it.last; ++part) {
     if (part != it.first) {
@@ -744,7 +775,7 @@ __device__ __forceinline__ void shared_rows16(const SharedArgs& a, const Item& i
       __syncthreads();  // (every stage is free)
       tiles.load(0);
     }
-    const int seen = last_seen(ks, live ? r : 0, per), all_see = last_seen(ks, 0, per);
+    const int seen = last_seen(ks, me.t), all_see = last_seen(ks, 0);
     tiles.each(lds, (all_see + 1) / H_KT, [&](int t, const char* st, auto masked) {
       const int kw = t * H_KT + 16 * w;
       if (masked && kw >= ks.n) return;
@@ -840,12 +871,12 @@ __global__ __launch_bounds__(256) void shared_join_kernel(SharedArgs a) {
   static_assert(RB == 1 || SG == 1, "a block's sets share one row, or each has its own");
   __shared__ f32x4 po[4][LPR];
   __shared__ float2 pml[4];
-  const int64_t rows = (int64_t)a.B * a.T * a.Hq;
+  const int64_t rows = a.query_rows;
   const int lane = threadIdx.x % LPR, sg = threadIdx.x / LPR % SG, rb = threadIdx.x / (LPR * SG);
   const int64_t i = (int64_t)blockIdx.x * RB + rb;
   const int64_t row = std::min<int64_t>(i, rows - 1);
   const int slots = a.splits_p + a.splits_s;
-  const bool idle = own_len(a, row / a.Hq / a.T) < 0;
+  const bool idle = a.clens != nullptr && own_len(a, (int)((uint32_t)row / (uint32_t)(a.Hq * a.T))) < 0;
   float m = -__builtin_inff(), l = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
   auto add = [&](float ms, float ls, const f32x4& os, float mn) {
@@ -978,7 +1009,7 @@ int shared_launch(hipStream_t st, const SharedArgs& a, const Plan& p) {
   }
   MINITP_LAUNCH_CHECK();
   if (p.joined) return MINITP_OK;
-  const int64_t rows = (int64_t)a.B * a.T * a.Hq;
+  const int64_t rows = a.query_rows;
   constexpr int SG = 256 / (D / 4);
   // (several sets of lanes a row while there are few rows: 7,168 rows of 9
   // slots 8.3 us with one set, 18.3 with eight; 896 rows of 33 slots 5.7 us with
@@ -1044,15 +1075,22 @@ int launch_shared_prefix_attention(hipStream_t st, int dtype, const SharedPrefix
   a.kc = k_cache;
   a.vc = v_cache;
   a.out = out;
+  auto div = [](int64_t d) {
+    int l = 0;
+    while ((1LL << l) < d) ++l;
+    return Div{(uint32_t)(((1ull << (31 + l)) + (uint64_t)d - 1) / (uint64_t)d), 31 + l};
+  };
   a.B = (int)s.B;
-  a.G = (int)s.G;
+  a.w = (int)(s.B / s.G);
+  a.per = (int)(s.Hq / s.Hkv);
+  a.query_rows = rows;
   a.T = (int)s.T;
   a.Hq = (int)s.Hq;
   a.Hkv = (int)s.Hkv;
   a.Sp = s.Sp;
   a.S = s.S;
-  a.P = s.P;
-  a.C = s.C;
+  a.P = (int)s.P;
+  a.C = (int)s.C;
   a.plens = prefix_lens;
   a.clens = cache_lens;
   a.scale = 1.0f / sqrtf((float)s.D);
@@ -1064,6 +1102,13 @@ int launch_shared_prefix_attention(hipStream_t st, int dtype, const SharedPrefix
   a.items_s = (int)p.items_s;
   a.run_p = (int)cdiv(p.items_p, 8);
   a.run_s = (int)cdiv(p.items_s, 8);
+  a.by_qtiles_p = div(p.qtiles_p);
+  a.by_qtiles_s = div(p.qtiles_s);
+  a.by_splits_p = div(std::max(p.splits_p, 1));
+  a.by_splits_s = div(p.splits_s);
+  a.by_hkv = div(s.Hkv);
+  a.by_w = div(a.w);
+  a.by_per = div(a.per);
   a.joined = p.joined;
   a.o = (float*)workspace;
   a.ml = a.o + (p.splits_p + p.splits_s) * rows * s.D;
