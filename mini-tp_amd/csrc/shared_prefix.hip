@@ -700,42 +700,30 @@ __device__ __forceinline__ void shared_rows128(const SharedArgs& a, const Item& 
       }
     });
   }
-  // ---- results through LDS, so that a store covers whole rows ---------------
-  __syncthreads();  // (every stage is free)
-  if (r0 >= it.rows) return;
+  if (r >= it.rows) return;
   const float l = halves_sum(lsum);
   if (a.joined) {
     const float f = m == -__builtin_inff() ? 0.f : 1.f / l;
+    bf16* orow = (bf16*)a.out + me.row * D + 4 * h;
 #pragma unroll
-    for (int d = 0; d < DB; ++d) o[d] *= f;
-  } else if (h == 0 && r < it.rows) {
-    *(float2*)(a.ml + (it.slot * a.query_rows + me.row) * 2) = make_float2(m, l);
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = o[d][4 * c + e] * f;
+        store_vec<bf16, 4>(orow + 32 * d + 8 * c, v);
+      }
+    return;
   }
-  constexpr int CPR = D / 4, RPI = 64 / CPR;  // 16-byte chunks of a row, rows of a store
-  float* po = (float*)lds + w * 32 * D;       // this wave's [32][D], chunk c of row i at c ^ i
+  const int64_t at = it.slot * a.query_rows + me.row;
+  if (h == 0) *(float2*)(a.ml + at * 2) = make_float2(m, l);
+  float* orow = a.o + at * D + 4 * h;
 #pragma unroll
   for (int d = 0; d < DB; ++d)
 #pragma unroll
     for (int c = 0; c < 4; ++c)
-      *(f32x4*)(po + n32 * D + ((8 * d + 2 * c + h) ^ (n32 % CPR)) * 4) =
-          f32x4{o[d][4 * c], o[d][4 * c + 1], o[d][4 * c + 2], o[d][4 * c + 3]};
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-  const int ch = lane % CPR;
-#pragma unroll
-  for (int i = 0; i < 32 / RPI; ++i) {
-    const int row = i * RPI + lane / CPR;
-    const f32x4 x = *(const f32x4*)(po + row * D + (ch ^ (row % CPR)) * 4);
-    const int64_t at = __shfl(me.row, row, 64);
-    if (r0 + row >= it.rows) continue;
-    if (a.joined) {
-      const float v[4] = {x[0], x[1], x[2], x[3]};
-      store_vec<bf16, 4>((bf16*)a.out + at * D + 4 * ch, v);
-    } else {
-      *(f32x4*)(a.o + (it.slot * a.query_rows + at) * D + 4 * ch) = x;
-    }
-  }
+      *(f32x4*)(orow + 32 * d + 8 * c) = f32x4{o[d][4 * c], o[d][4 * c + 1], o[d][4 * c + 2], o[d][4 * c + 3]};
 }
 
 template <int D>
