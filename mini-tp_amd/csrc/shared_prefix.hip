@@ -219,8 +219,7 @@ __device__ __forceinline__ void finish_rows(const SharedArgs& a, const Item& it,
 }
 
 // ---------------------------------------------------------------------------
-// fp32 (and bf16 head dims below 32, widened on their way into LDS) on
-// v_mfma_f32_16x16x4_f32. Four waves share each 64-key tile in LDS: 4 / KW
+// fp32, on v_mfma_f32_16x16x4_f32. Four waves share each 64-key tile in LDS: 4 / KW
 // strips of 16 queries, KW waves a strip over 64 / KW keys each (a unit of few
 // rows is bound by the latency of one wave's keys); products transposed: S^T =
 // K Q^T leaves lane (quad, r) with keys 4 quad .. 4 quad + 3 of query r, which
@@ -232,12 +231,12 @@ constexpr int F_QT = 64, F_KT = 64;
 template <int D>
 constexpr int F_LDS = 2 * F_KT * (D + 4) * 4;
 
-template <typename T, int D, int KW>
+template <int D, int KW>
 __device__ __forceinline__ void shared_rows_f32(const SharedArgs& a, const Item& it, float* lds, int* odd) {
   constexpr int KT = F_KT, KB = KT / 16 / KW, KC = D / 16, SW = 4 / KW;
   constexpr int E = D / 16 < 4 ? D / 16 : 4, HALVES = D / 16 / E;
   constexpr int ROW = D + 4;
-  constexpr int VE = Vec<T>::N, PIECES = KT * D / VE, PER = (PIECES + 255) / 256;
+  constexpr int PIECES = KT * D / 4, PER = (PIECES + 255) / 256;
   float *Ks = lds, *Vs = lds + KT * ROW;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lr = lane % 16, lq = lane / 16, strip = wave % SW, key0 = wave / SW * KB * 16;
@@ -246,9 +245,9 @@ __device__ __forceinline__ void shared_rows_f32(const SharedArgs& a, const Item&
 
   f32x4 qa[KC];
   {
-    const T* qrow = (const T*)a.q + me.row * D;
+    const float* qrow = (const float*)a.q + me.row * D;
 #pragma unroll
-    for (int c = 0; c < KC; ++c) load_vec<T, 4>(qrow + 16 * c + 4 * lq, (float*)&qa[c]);
+    for (int c = 0; c < KC; ++c) qa[c] = *(const f32x4*)(qrow + 16 * c + 4 * lq);
   }
   f32x4 o[HALVES][E];
 #pragma unroll
@@ -262,8 +261,8 @@ __device__ __forceinline__ void shared_rows_f32(const SharedArgs& a, const Item&
     const int seen = last_seen(ks, me.t), all_see = last_seen(ks, a.by_per(t0));
     uint4 kr[PER], vr[PER];
     auto load_tile = [&](int key) {
-      const __amdgpu_buffer_rsrc_t krs = key_rows(ks.k, key, ks.n, KT, D * (int)sizeof(T));
-      const __amdgpu_buffer_rsrc_t vrs = key_rows(ks.v, key, ks.n, KT, D * (int)sizeof(T));
+      const __amdgpu_buffer_rsrc_t krs = key_rows(ks.k, key, ks.n, KT, D * 4);
+      const __amdgpu_buffer_rsrc_t vrs = key_rows(ks.v, key, ks.n, KT, D * 4);
 #pragma unroll
       for (int u = 0; u < PER; ++u) {
         const uint32_t off = (uint32_t)(tid + 256 * u) * 16;  // (past the tile: not stored)
@@ -281,18 +280,14 @@ __device__ __forceinline__ void shared_rows_f32(const SharedArgs& a, const Item&
       for (int u = 0; u < PER; ++u) {
         const int i = tid + 256 * u;
         if (i < PIECES) {
-          const int row = i / (D / VE), at = row * ROW + i % (D / VE) * VE;
-          float f[VE];
-          unpack16(kr[u], f, (T*)nullptr);
-#pragma unroll
-          for (int e = 0; e < VE; e += 4) *(f32x4*)(Ks + at + e) = *(const f32x4*)(f + e);
-          unpack16(vr[u], f, (T*)nullptr);
-#pragma unroll
-          for (int e = 0; e < VE; e += 4) *(f32x4*)(Vs + at + e) = *(const f32x4*)(f + e);
+          const int row = i / (D / 4), at = row * ROW + i % (D / 4) * 4;
+          *(uint4*)(Ks + at) = kr[u];
+          *(uint4*)(Vs + at) = vr[u];
           if (k0 + row > all_see) {
             // a key that some query does not see: is its value finite?
+            const f32x4 f = __builtin_bit_cast(f32x4, vr[u]);
 #pragma unroll
-            for (int e = 0; e < VE; ++e) found |= !__builtin_isfinite(f[e]);
+            for (int e = 0; e < 4; ++e) found |= !__builtin_isfinite(f[e]);
           }
         }
       }
@@ -300,6 +295,7 @@ __device__ __forceinline__ void shared_rows_f32(const SharedArgs& a, const Item&
       __syncthreads();
       if (k0 + KT < ks.n) load_tile(k0 + KT);
       const bool slow = *odd != 0;
+      if (k0 + key0 >= ks.n) continue;  // (none of this wave's keys)
       const int limit = seen - k0 - key0;  // last of the wave's keys that this query sees
       float p[KB][4];
       float mx = -__builtin_inff();
@@ -400,27 +396,27 @@ __device__ __forceinline__ void shared_rows_f32(const SharedArgs& a, const Item&
       for (int j = 0; j < E; ++j) po[at * D + 64 * hf + E * (4 * lq + x) + j] = o[hf][j][x];
   if (lq == 0) pml[at] = make_float2(m, lsum);
   __syncthreads();
-  finish_rows<T, D, KW, false>(a, it, po, pml, CAP, t0, std::min(CAP, it.rows - t0));
+  finish_rows<float, D, KW, false>(a, it, po, pml, CAP, t0, std::min(CAP, it.rows - t0));
 }
 
-template <typename T, int D>
+template <int D>
 __global__ __launch_bounds__(256) void shared_attn_f32_kernel(SharedArgs a) {
   extern __shared__ __attribute__((aligned(16))) float lds_f[];
   static_assert(F_LDS<D> >= 64 * (D + 2) * 4, "the waves' results fit the tiles");
   __shared__ int odd;
   Item it;
-  if (!shared_item<F_QT, F_KT>(a, D * (int64_t)sizeof(T), it)) return;
+  if (!shared_item<F_QT, F_KT>(a, D * 4, it)) return;
   const int rows = it.rows - it.tile * F_QT;
   if (rows <= 16)
-    shared_rows_f32<T, D, 4>(a, it, lds_f, &odd);
+    shared_rows_f32<D, 4>(a, it, lds_f, &odd);
   else if (rows <= 32)
-    shared_rows_f32<T, D, 2>(a, it, lds_f, &odd);
+    shared_rows_f32<D, 2>(a, it, lds_f, &odd);
   else
-    shared_rows_f32<T, D, 1>(a, it, lds_f, &odd);
+    shared_rows_f32<D, 1>(a, it, lds_f, &odd);
 }
 
 // ---------------------------------------------------------------------------
-// bf16, head dims 32, 64 and 128. A block takes 128 query rows of a unit over
+// bf16. A block takes 128 query rows of a unit over
 // the keys of its split, four waves of 32 rows (v_mfma_f32_32x32x16_bf16), or,
 // where the unit has at most 16 rows (one token of a row's own part), those
 // rows over 64 keys at a time, 16 keys a wave (16x16 MFMAs).
@@ -440,6 +436,7 @@ __global__ __launch_bounds__(256) void shared_attn_f32_kernel(SharedArgs a) {
 // takes one chunk column of 16 rows, a V read 64 bytes of four rows.
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int H_QT = 128, H_KT = 64, H_SMALL = 16;
@@ -448,7 +445,9 @@ template <int D>
 struct Half {
   static constexpr int ROWB = D * 2, CH = D / 8;
   static constexpr int OPER = H_KT * ROWB, STAGE = 2 * OPER, LDS = 2 * STAGE;
-  static constexpr int PIECE_ROWS = 64 / CH, PIECES = H_KT / PIECE_ROWS, PPW = PIECES / 4;  // 1 KiB loads
+  // 1 KiB loads of a tile: PPW of K and of V a wave (D = 16: one of either)
+  static constexpr int PIECE_ROWS = 64 / CH, PIECES = H_KT / PIECE_ROWS, PPW = PIECES / 4;
+  static_assert(PPW >= 1 || PIECES == 2, "each wave loads alike, or waves 0, 1 K and waves 2, 3 V");
   // chunk c of row r lies at chunk c ^ swz(r)
   __device__ static int k_swz(int r) { return r * ROWB / 256 % CH; }
   __device__ static int v_swz(int r) { return r * ROWB / 256 % 4 * 4 % CH; }
@@ -522,7 +521,7 @@ struct Tiles {
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds + w * 1024;
     // piece w + 4 j of a tile: rows 4 PIECE_ROWS j + row; the swizzles do not depend on j
-    const int row = H::PIECE_ROWS * w + lane / H::CH;
+    const int row = H::PIECE_ROWS * (H::PPW > 0 ? w : w & 1) + lane / H::CH;
     koff = row * H::ROWB + ((lane % H::CH) ^ H::k_swz(row)) * 16;
     voff = row * H::ROWB + ((lane % H::CH) ^ H::v_swz(row)) * 16;
   }
@@ -532,6 +531,12 @@ struct Tiles {
     const u32x4 kr = rows_rsrc(k + (int64_t)t * H::OPER, left), vr = rows_rsrc(v + (int64_t)t * H::OPER, left);
     uint32_t at = __builtin_amdgcn_readfirstlane(to + (t & 1) * H::STAGE);
     asm volatile("s_nop 4" : "+s"(at));
+    if constexpr (H::PPW == 0) {
+      if (__builtin_amdgcn_readfirstlane(threadIdx.x >> 7) == 0)
+        row_dma16(kr, koff, at);
+      else
+        row_dma16(vr, voff, at);
+    }
 #pragma unroll
     for (int j = 0; j < H::PPW; ++j) row_dma16(kr, koff + j * 4096, at + j * 4096);
 #pragma unroll
@@ -562,7 +567,8 @@ constexpr float SLACK = 8.f;
 template <int D>
 __device__ __forceinline__ void shared_rows128(const SharedArgs& a, const Item& it, char* lds) {
   using H = Half<D>;
-  constexpr int KS = D / 16, DB = D / 32;
+  // (D = 16: the output's 32-row operand holds the 16 dims twice)
+  constexpr int KS = D / 16, DB = D >= 32 ? D / 32 : 1, OC = D >= 32 ? 4 : 2;  // OC: 8-dim chunks of a block
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n32 = lane & 31, h = lane >> 5;
   Keys ks = it.first == 0 ? it.pre : it.own;
@@ -591,7 +597,7 @@ __device__ __forceinline__ void shared_rows128(const SharedArgs& a, const Item& 
   const int kat = n32 * H::ROWB, kx = (h ^ H::k_swz(n32)) << 4;
   const int vrow = 4 * h + (lane & 15) / 4;
   const int vat = H::OPER + vrow * H::ROWB + 8 * (lane & 1);
-  const int vx = ((2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) ^ H::v_swz(vrow)) << 4;
+  const int vx = (((D >= 32 ? 2 * ((lane >> 4) & 1) : 0) + ((lane >> 1) & 1)) ^ H::v_swz(vrow)) << 4;
   arrived(qb);
 
   for (int part = it.first; part <= it.last; ++part) {
@@ -667,7 +673,7 @@ __device__ __forceinline__ void shared_rows128(const SharedArgs& a, const Item& 
 #pragma unroll
           for (int d = 0; d < DB; ++d)
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
+            for (int c = 0; c < OC; ++c) {
               const char* vp = st + H::OPER + key * H::ROWB + (((4 * d + c) ^ H::v_swz(key)) << 4) + 8 * h;
               const uint2 x = *(const uint2*)vp;
               const float v[4] = {__uint_as_float(x.x << 16), __uint_as_float(x.x & 0xffff0000u),
@@ -708,7 +714,7 @@ __device__ __forceinline__ void shared_rows128(const SharedArgs& a, const Item& 
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
+      for (int c = 0; c < OC; ++c) {
         float v[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = o[d][4 * c + e] * f;
@@ -722,14 +728,14 @@ __device__ __forceinline__ void shared_rows128(const SharedArgs& a, const Item& 
 #pragma unroll
   for (int d = 0; d < DB; ++d)
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
+    for (int c = 0; c < OC; ++c)
       *(f32x4*)(orow + 32 * d + 8 * c) = f32x4{o[d][4 * c], o[d][4 * c + 1], o[d][4 * c + 2], o[d][4 * c + 3]};
 }
 
 template <int D>
 __device__ __forceinline__ void shared_rows16(const SharedArgs& a, const Item& it, char* lds) {
   using H = Half<D>;
-  constexpr int KS = D / 32, DB = D / 16;
+  constexpr int KS = D >= 32 ? D / 32 : 1, DB = D / 16;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n16 = lane & 15, q4 = lane >> 4;
   Keys ks = it.first == 0 ? it.pre : it.own;
@@ -738,11 +744,18 @@ __device__ __forceinline__ void shared_rows16(const SharedArgs& a, const Item& i
   const int r = n16;  // (one tile)
   const Query me = query_of(a, it, r < it.rows ? r : 0);
 
-  bf16x8 qb[KS];
+  bf16x8 qb[KS];  // (D = 16: four dims a lane, in the low half)
   {
-    const bf16* q = (const bf16*)a.q + me.row * D + 8 * q4;
+    const bf16* q = (const bf16*)a.q + me.row * D + (D >= 32 ? 8 : 4) * q4;
 #pragma unroll
-    for (int k = 0; k < KS; ++k) qb[k] = __builtin_bit_cast(bf16x8, *(const u32x4*)(q + 32 * k));
+    for (int k = 0; k < KS; ++k) {
+      if constexpr (D >= 32) {
+        qb[k] = __builtin_bit_cast(bf16x8, *(const u32x4*)(q + 32 * k));
+      } else {
+        const uint2 x = *(const uint2*)q;
+        qb[k] = __builtin_bit_cast(bf16x8, make_uint4(x.x, x.y, 0, 0));
+      }
+    }
   }
   f32x4 o[DB];
 #pragma unroll
@@ -751,7 +764,9 @@ __device__ __forceinline__ void shared_rows16(const SharedArgs& a, const Item& i
   const float sl2 = a.scale * 1.4426950408889634f;
 
   // K row 16 w + n16, chunk 4 k + q4; V rows 16 w + 4 q4 + n16 / 4, dims 16 d + 4 (lane % 4)
-  const int krow = 16 * w + n16, kat = krow * H::ROWB, kx = (q4 ^ H::k_swz(krow)) << 4;
+  // (D = 16: 8 bytes, half q4 % 2 of chunk q4 / 2)
+  const int krow = 16 * w + n16, kat = krow * H::ROWB + (D >= 32 ? 0 : 8 * (q4 & 1));
+  const int kx = ((D >= 32 ? q4 : q4 >> 1) ^ H::k_swz(krow)) << 4;
   const int vrow = 16 * w + 4 * q4 + n16 / 4;
   const int vat = H::OPER + vrow * H::ROWB + 8 * (lane & 1), vx = (((lane >> 1) & 1) ^ H::v_swz(vrow)) << 4;
   arrived(qb);
@@ -770,8 +785,14 @@ __device__ __forceinline__ void shared_rows16(const SharedArgs& a, const Item& i
       f32x4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
-        const bf16x8 kf = __builtin_bit_cast(bf16x8, *(const uint4*)(st + kat + ((64 * k) ^ kx)));
-        s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qb[k], s, 0, 0, 0);
+        if constexpr (D >= 32) {
+          const bf16x8 kf = __builtin_bit_cast(bf16x8, *(const uint4*)(st + kat + ((64 * k) ^ kx)));
+          s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qb[k], s, 0, 0, 0);
+        } else {
+          const s16x4 kf = *(const s16x4*)(st + kat + kx);
+          const auto q = __builtin_bit_cast(s16x8, qb[0]);
+          s = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(kf, s16x4{q[0], q[1], q[2], q[3]}, s, 0, 0, 0);
+        }
       }
       const int limit = seen - kw;
       if constexpr (masked) {
@@ -942,8 +963,6 @@ struct Plan {
   bool joined;
 };
 
-bool bf16_tiles(int dtype, int64_t D) { return dtype == MINITP_BF16 && D >= 32; }
-
 // Splits: the prefix part takes 256 blocks, each of at least two key tiles (one
 // on the fp32 path, whose tiles take three times as long), or, where that
 // leaves a block 16 tiles and more, 448 of the 512 places that there are; the
@@ -960,8 +979,8 @@ bool bf16_tiles(int dtype, int64_t D) { return dtype == MINITP_BF16 && D >= 32; 
 // against 10.0 / 12.6); and where the rows' own queries fill their tiles to
 // three quarters and the tiles the CUs (16 rows of 100 tokens on 4,096 keys 123
 // against 133, and no scratch, which grows with the tokens).
-Plan shared_plan(int dtype, int64_t D, int64_t B, int64_t G, int64_t T, int64_t Hq, int64_t Hkv, int64_t P, int64_t C) {
-  const bool tiles16 = bf16_tiles(dtype, D);
+Plan shared_plan(int dtype, int64_t B, int64_t G, int64_t T, int64_t Hq, int64_t Hkv, int64_t P, int64_t C) {
+  const bool tiles16 = dtype == MINITP_BF16;
   const int64_t qt = tiles16 ? H_QT : F_QT, kt = tiles16 ? H_KT : F_KT, per = Hq / Hkv;
   Plan p;
   p.qtiles_p = (int)cdiv(B / G * T * per, qt);
@@ -986,14 +1005,14 @@ Plan shared_plan(int dtype, int64_t D, int64_t B, int64_t G, int64_t T, int64_t 
 template <typename T, int D>
 int shared_launch(hipStream_t st, const SharedArgs& a, const Plan& p) {
   const dim3 grid((unsigned)(8 * (a.run_p + a.run_s)));
-  if constexpr (sizeof(T) == 2 && D >= 32) {
+  if constexpr (sizeof(T) == 2) {
     const int rc = ensure_lds_limit((const void*)shared_attn_bf16_kernel<D>, Half<D>::LDS);
     if (rc) return rc;
     hipLaunchKernelGGL(shared_attn_bf16_kernel<D>, grid, dim3(256), Half<D>::LDS, st, a);
   } else {
-    const int rc = ensure_lds_limit((const void*)shared_attn_f32_kernel<T, D>, F_LDS<D>);
+    const int rc = ensure_lds_limit((const void*)shared_attn_f32_kernel<D>, F_LDS<D>);
     if (rc) return rc;
-    hipLaunchKernelGGL((shared_attn_f32_kernel<T, D>), grid, dim3(256), F_LDS<D>, st, a);
+    hipLaunchKernelGGL((shared_attn_f32_kernel<D>), grid, dim3(256), F_LDS<D>, st, a);
   }
   MINITP_LAUNCH_CHECK();
   if (p.joined) return MINITP_OK;
@@ -1031,7 +1050,7 @@ int shared_by_d(hipStream_t st, const SharedArgs& a, const Plan& p, int64_t D) {
 int64_t shared_prefix_workspace_bytes(int dtype, int64_t B, int64_t G, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
                                       int64_t P, int64_t C) {
   if (B * T == 0) return 0;
-  const Plan p = shared_plan(dtype, D, B, G, T, Hq, Hkv, P, C);
+  const Plan p = shared_plan(dtype, B, G, T, Hq, Hkv, P, C);
   return p.joined ? 0 : (p.splits_p + p.splits_s) * B * T * Hq * (D + 2) * 4;
 }
 
@@ -1039,7 +1058,7 @@ int launch_shared_prefix_attention(hipStream_t st, int dtype, const SharedPrefix
                                    const void* k_prefix, const void* v_prefix, const void* k_cache,
                                    const void* v_cache, void* out, const int64_t* prefix_lens,
                                    const int64_t* cache_lens, void* workspace, int64_t workspace_bytes) {
-  const Plan p = shared_plan(dtype, s.D, s.B, s.G, s.T, s.Hq, s.Hkv, s.P, s.C);
+  const Plan p = shared_plan(dtype, s.B, s.G, s.T, s.Hq, s.Hkv, s.P, s.C);
   const int64_t need = shared_prefix_workspace_bytes(dtype, s.B, s.G, s.T, s.Hq, s.Hkv, s.D, s.P, s.C);
   if (workspace_bytes < need || (workspace == nullptr && need > 0) || !aligned16(workspace)) {
     set_error("shared_prefix_attention: workspace %p of %lld B, %lld B needed (16-byte aligned)", workspace,
