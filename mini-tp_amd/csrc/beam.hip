@@ -556,7 +556,7 @@ int launch_beam_select(hipStream_t st, int dtype, const BeamSelect& b, void* wor
   }
   const int64_t rows = b.G * b.W, slices = cdiv(b.V, dtype == MINITP_F32 ? SLICE<float> : SLICE<bf16>);
   const int64_t parts = rows * slices * (SEL_T / 64);
-  if (rows * slices >= (1LL << 31)) {
+  if (rows * slices >= (1LL << 24)) {  // (a launch's threads are counted in 32 bits)
     set_error("beam_select: %lld rows of %lld logits are too many for one call", (long long)rows, (long long)b.V);
     return MINITP_ERR_UNSUPPORTED;
   }
@@ -598,7 +598,7 @@ int launch_beam_select(hipStream_t st, int dtype, const BeamSelect& b, void* wor
 int launch_kv_reorder(hipStream_t st, int dtype, void* k, void* v, int64_t L, int64_t G, int64_t W, int64_t Hkv,
                       int64_t S, int64_t D, int64_t rows, const int64_t* parents) {
   const int64_t es = dtype == MINITP_F32 ? 4 : 2;
-  if (rows * D * es >= (1LL << 31) || L * Hkv > 65535 || G > 32767) {
+  if (D >= (1LL << 31) || rows >= (1LL << 31) / (D * es) || L > 65535 || Hkv > 65535 || L * Hkv > 65535 || G > 32767) {
     set_error("kv_reorder: %lld rows of %lld, %lld layers of %lld heads, %lld groups are too many for one call",
               (long long)rows, (long long)D, (long long)L, (long long)Hkv, (long long)G);
     return MINITP_ERR_UNSUPPORTED;

@@ -368,7 +368,7 @@ int64_t minitp_shared_prefix_attention_workspace_bytes(int dtype, int64_t B, int
                                                        int64_t Hkv, int64_t D, int64_t prefix_len,
                                                        int64_t cache_len) {
   if (!dtype_ok(dtype) || !shared_prefix_shape_ok(B, G, T, Hq, Hkv, D, prefix_len, cache_len)) return -1;
-  return shared_prefix_workspace_bytes(dtype, B, G, T, Hq, Hkv, D, prefix_len, cache_len);
+  return shared_prefix_workspace_bytes(dtype, SharedPrefixShape{B, G, T, Hq, Hkv, D, 0, 0, prefix_len, cache_len});
 }
 
 int minitp_shared_prefix_attention(void* stream, int dtype, const void* q, const void* k_prefix, const void* v_prefix,
@@ -386,7 +386,7 @@ int minitp_shared_prefix_attention(void* stream, int dtype, const void* q, const
               (long long)(Hq % Hkv != 0 ? Hq : B), (long long)(Hq % Hkv != 0 ? Hkv : G));
     return MINITP_ERR_DIVISIBLE;
   }
-  if (cache_len + T > S_ || prefix_len > S_prefix) {
+  if (cache_len > S_ - T || prefix_len > S_prefix) {
     if (prefix_len > S_prefix)
       set_error("KV cache overflow: prefix %lld > prefix rows %lld", (long long)prefix_len, (long long)S_prefix);
     else
@@ -394,7 +394,7 @@ int minitp_shared_prefix_attention(void* stream, int dtype, const void* q, const
                 (long long)S_);
     return MINITP_ERR_OVERFLOW;
   }
-  if (B * T == 0) return MINITP_OK;
+  if (B == 0 || T == 0) return MINITP_OK;
   MINITP_CHECK_ARG(q && k_cache && v_cache && out && (prefix_len == 0 || (k_prefix && v_prefix)),
                    "shared_prefix_attention: NULL pointer");
   MINITP_CHECK_ARG(D % vec_elems(dtype) == 0 && aligned16(q) && aligned16(out) && aligned16(k_cache) &&
@@ -406,7 +406,7 @@ int minitp_shared_prefix_attention(void* stream, int dtype, const void* q, const
 }
 
 int64_t minitp_beam_select_workspace_bytes(int64_t G, int64_t W, int64_t V) {
-  if (G < 0 || W < 1 || W > BEAM_MAX || V <= 0) return -1;
+  if (G < 0 || G >= (1LL << 31) || W < 1 || W > BEAM_MAX || V <= 0 || V >= (1LL << 31)) return -1;
   return beam_select_workspace_bytes(G, W, V);
 }
 
@@ -415,7 +415,7 @@ int minitp_beam_select(void* stream, int dtype, const void* logits, int64_t ld_g
                        int64_t eos_token, double length_penalty, int64_t* tokens, int64_t* parents, float* scores_out,
                        uint8_t* finished_out, int64_t* lengths_out, void* workspace, int64_t workspace_bytes) {
   CHECK_DTYPE(dtype);
-  MINITP_CHECK_ARG(G >= 0 && V > 0 && V < (1LL << 31) && ld_group >= 0 && ld_beam >= 0,
+  MINITP_CHECK_ARG(G >= 0 && G < (1LL << 31) && V > 0 && V < (1LL << 31) && ld_group >= 0 && ld_beam >= 0,
                    "beam_select: G=%lld V=%lld ld=%lld/%lld", (long long)G, (long long)V, (long long)ld_group,
                    (long long)ld_beam);
   MINITP_CHECK_ARG(W >= 1 && W <= BEAM_MAX, "beam_select: %lld beams a group (1 to %d)", (long long)W, BEAM_MAX);
@@ -456,7 +456,7 @@ int minitp_kv_reorder(void* stream, int dtype, void* k_cache, void* v_cache, int
     set_error("KV cache overflow: %lld rows > max_seq_len=%lld", (long long)rows, (long long)S_);
     return MINITP_ERR_OVERFLOW;
   }
-  if (L * G * Hkv * rows == 0) return MINITP_OK;
+  if (L == 0 || G == 0 || Hkv == 0 || rows == 0) return MINITP_OK;
   MINITP_CHECK_ARG(k_cache && v_cache && parents, "kv_reorder: NULL pointer");
   MINITP_CHECK_ARG(D % vec_elems(dtype) == 0 && aligned16(k_cache) && aligned16(v_cache),
                    "kv_reorder: head_dim rows must be 16-byte aligned");

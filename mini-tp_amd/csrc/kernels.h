@@ -288,8 +288,8 @@ struct SharedPrefixShape {
   int64_t Sp, S;  // rows per (group, KV head) of the prefix buffers, per (row, KV head) of the caches
   int64_t P, C;   // prefix rows, cached own rows
 };
-int64_t shared_prefix_workspace_bytes(int dtype, int64_t B, int64_t G, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
-                                      int64_t P, int64_t C);
+int shared_prefix_check(int dtype, const SharedPrefixShape& s);  // what one launch does not take is an error
+int64_t shared_prefix_workspace_bytes(int dtype, const SharedPrefixShape& s);
 int launch_shared_prefix_attention(hipStream_t st, int dtype, const SharedPrefixShape& s, const void* q,
                                    const void* k_prefix, const void* v_prefix, const void* k_cache,
                                    const void* v_cache, void* out, const int64_t* prefix_lens,

@@ -252,17 +252,7 @@ struct Qwen2Program {
     const int64_t layer_elems = B * c.kv_heads * s.max_seq * D;
     auto shared_attention = [&](int l) {
       const int64_t pre_bytes = (int64_t)l * pre->groups * c.kv_heads * pre->max_seq * D * es();
-      SharedPrefixShape sh{};
-      sh.B = B;
-      sh.G = pre->groups;
-      sh.T = T;
-      sh.Hq = c.heads;
-      sh.Hkv = c.kv_heads;
-      sh.D = D;
-      sh.Sp = pre->max_seq;
-      sh.S = s.max_seq;
-      sh.P = pre->len;
-      sh.C = s.cache_len;
+      const SharedPrefixShape sh{B, pre->groups, T, c.heads, c.kv_heads, D, pre->max_seq, s.max_seq, pre->len, s.cache_len};
       return launch_shared_prefix_attention(st, c.dtype, sh, w.q, (const char*)pre->k + pre_bytes,
                                             (const char*)pre->v + pre_bytes,
                                             (const char*)s.k_cache + l * layer_elems * es(),
@@ -778,9 +768,10 @@ int minitp_qwen2_forward_shared(void* handle, void* stream, const minitp_qwen2_s
   MINITP_CHECK_ARG(prefix->len == 0 || (prefix->k != nullptr && prefix->v != nullptr && minitp::aligned16(prefix->k) &&
                                         minitp::aligned16(prefix->v)),
                    "shared prefix: K/V rows must be there and 16-byte aligned");
-  const int64_t need =
-      minitp::shared_prefix_workspace_bytes(p->c.dtype, step->batch, prefix->groups, step->tokens, p->c.heads,
-                                            p->c.kv_heads, p->c.head_dim, prefix->len, step->cache_len);
+  const minitp::SharedPrefixShape sh{step->batch,      prefix->groups,  step->tokens, p->c.heads,  p->c.kv_heads,
+                                     p->c.head_dim,    prefix->max_seq, step->max_seq, prefix->len, step->cache_len};
+  if (const int unfit = minitp::shared_prefix_check(p->c.dtype, sh)) return unfit;
+  const int64_t need = minitp::shared_prefix_workspace_bytes(p->c.dtype, sh);
   MINITP_CHECK_ARG(prefix->workspace_bytes >= need && (prefix->workspace != nullptr || need == 0) &&
                        minitp::aligned16(prefix->workspace),
                    "shared prefix: workspace %p of %lld B, %lld B needed (16-byte aligned)", prefix->workspace,

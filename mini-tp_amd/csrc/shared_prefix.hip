@@ -1038,42 +1038,58 @@ int shared_by_d(hipStream_t st, const SharedArgs& a, const Plan& p, int64_t D) {
       return shared_launch<T, 32>(st, a, p);
     case 64:
       return shared_launch<T, 64>(st, a, p);
-    case 128:
+    default:
       return shared_launch<T, 128>(st, a, p);
   }
-  set_error("shared_prefix_attention: head_dim %lld not supported (16, 32, 64, 128)", (long long)D);
-  return MINITP_ERR_UNSUPPORTED;
 }
 
 }  // namespace
 
-int64_t shared_prefix_workspace_bytes(int dtype, int64_t B, int64_t G, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
-                                      int64_t P, int64_t C) {
-  if (B * T == 0) return 0;
-  const Plan p = shared_plan(dtype, B, G, T, Hq, Hkv, P, C);
-  return p.joined ? 0 : (p.splits_p + p.splits_s) * B * T * Hq * (D + 2) * 4;
+// Whether one launch takes the shape: 32-bit row, key and thread numbers.
+int shared_prefix_check(int dtype, const SharedPrefixShape& s) {
+  if (s.D != 16 && s.D != 32 && s.D != 64 && s.D != 128) {
+    set_error("shared_prefix_attention: head_dim %lld not supported (16, 32, 64, 128)", (long long)s.D);
+    return MINITP_ERR_UNSUPPORTED;
+  }
+  constexpr int64_t MOST = 1LL << 31;
+  if (s.P >= MOST - 64 || s.C >= MOST || s.T >= MOST || s.C + s.T >= MOST - 64) {
+    set_error("shared_prefix_attention: %lld prefix and %lld + %lld own rows are too many", (long long)s.P,
+              (long long)s.C, (long long)s.T);
+    return MINITP_ERR_UNSUPPORTED;
+  }
+  bool fits = s.B < MOST && s.Hq < MOST && s.B * s.T < MOST && s.B * s.T * s.Hq < MOST - 256;
+  if (fits && s.B * s.T > 0) {
+    const Plan p = shared_plan(dtype, s.B, s.G, s.T, s.Hq, s.Hkv, s.P, s.C);
+    fits = p.items_p + p.items_s < (1LL << 24) - 16;
+  }
+  if (!fits) {
+    set_error("shared_prefix_attention: %lld x %lld x %lld query rows are too many for one call", (long long)s.B,
+              (long long)s.T, (long long)s.Hq);
+    return MINITP_ERR_UNSUPPORTED;
+  }
+  return MINITP_OK;
+}
+
+int64_t shared_prefix_workspace_bytes(int dtype, const SharedPrefixShape& s) {
+  if (s.B == 0 || s.T == 0) return 0;
+  if (shared_prefix_check(dtype, s)) return -1;
+  const Plan p = shared_plan(dtype, s.B, s.G, s.T, s.Hq, s.Hkv, s.P, s.C);
+  return p.joined ? 0 : (p.splits_p + p.splits_s) * s.B * s.T * s.Hq * (s.D + 2) * 4;
 }
 
 int launch_shared_prefix_attention(hipStream_t st, int dtype, const SharedPrefixShape& s, const void* q,
                                    const void* k_prefix, const void* v_prefix, const void* k_cache,
                                    const void* v_cache, void* out, const int64_t* prefix_lens,
                                    const int64_t* cache_lens, void* workspace, int64_t workspace_bytes) {
+  const int rc = shared_prefix_check(dtype, s);
+  if (rc) return rc;
   const Plan p = shared_plan(dtype, s.B, s.G, s.T, s.Hq, s.Hkv, s.P, s.C);
-  const int64_t need = shared_prefix_workspace_bytes(dtype, s.B, s.G, s.T, s.Hq, s.Hkv, s.D, s.P, s.C);
+  const int64_t rows = s.B * s.T * s.Hq;
+  const int64_t need = p.joined ? 0 : (p.splits_p + p.splits_s) * rows * (s.D + 2) * 4;
   if (workspace_bytes < need || (workspace == nullptr && need > 0) || !aligned16(workspace)) {
     set_error("shared_prefix_attention: workspace %p of %lld B, %lld B needed (16-byte aligned)", workspace,
               (long long)workspace_bytes, (long long)need);
     return MINITP_ERR_ARG;
-  }
-  const int64_t rows = s.B * s.T * s.Hq;
-  if (s.P >= (1LL << 31) - 64 || s.C + s.T >= (1LL << 31) - 64) {
-    set_error("shared_prefix_attention: %lld prefix and %lld + %lld own rows are too many", (long long)s.P,
-              (long long)s.C, (long long)s.T);
-    return MINITP_ERR_UNSUPPORTED;
-  }
-  if (p.items_p + p.items_s >= (1LL << 31) - 16 || rows >= (1LL << 31)) {
-    set_error("shared_prefix_attention: %lld query rows are too many for one call", (long long)rows);
-    return MINITP_ERR_UNSUPPORTED;
   }
   SharedArgs a{};
   a.q = q;

@@ -84,6 +84,28 @@ def test_kv_reorder_of_nothing():
     assert reorder(layers=0) == N.OK and reorder(g=0) == N.OK
 
 
+@pytest.mark.parametrize("change", [
+    dict(t=1 << 40, s=1 << 41, c=0), dict(t=(1 << 31) - 70, s=1 << 32, c=0), dict(b=1 << 33), dict(b=1 << 62, t=4),
+    dict(b=1 << 30, hq=1 << 30), dict(hq=1 << 40, hkv=1 << 40), dict(b=1 << 26, hq=2), dict(c=1 << 31, s=1 << 32),
+    dict(p=(1 << 31) - 64, sp=1 << 31),
+])
+def test_shared_prefix_attention_too_large(change):
+    """Past 32-bit rows, keys and launches: refused before any size is computed from it."""
+    assert attention(**change) == N.ERR_UNSUPPORTED and "too many" in N.last_error()
+    x = dict(b=4, g=2, t=1, hq=4, hkv=2, d=64, p=5000, c=10) | {k: v for k, v in change.items() if k not in ("s", "sp")}
+    size = N.lib().minitp_shared_prefix_attention_workspace_bytes
+    assert size(N.BF16, *(x[k] for k in ("b", "g", "t", "hq", "hkv", "d", "p", "c"))) == -1
+
+
+def test_sizes_that_pass_64_bits_are_refused():
+    top = (1 << 63) - 1
+    assert attention(c=top) == attention(c=top - 3, t=4) == N.ERR_OVERFLOW
+    assert select(g=1 << 60) == select(g=1 << 31) == N.ERR_ARG
+    assert select(g=1 << 22) in (N.ERR_ARG, N.ERR_UNSUPPORTED) and select(g=1 << 22, nbytes=1 << 62) == N.ERR_UNSUPPORTED
+    assert N.lib().minitp_beam_select_workspace_bytes(1 << 31, 4, 10) == -1
+    assert reorder(d=1 << 62) == reorder(layers=1 << 62, hkv=4) == N.ERR_UNSUPPORTED
+
+
 def test_forward_shared_refuses():
     lib = N.lib()
     cfg = N.Qwen2Config(N.BF16, 2, 64, 4, 2, 16, 128, 1000, 9000, 1e-6)
@@ -109,6 +131,7 @@ def test_forward_shared_refuses():
         assert call(workspace=None) == call(workspace_bytes=100) == call(workspace=P + 8) == N.ERR_ARG
         assert call(groups=4) == N.ERR_DIVISIBLE
         assert call(len=8193) == call(cache_len=24) == N.ERR_OVERFLOW
+        assert call(len=(1 << 31) - 64, max_seq=1 << 31) == N.ERR_UNSUPPORTED
     finally:
         lib.minitp_qwen2_destroy(h)
 
