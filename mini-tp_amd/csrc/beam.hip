@@ -67,12 +67,13 @@ __device__ __forceinline__ bool beam_open(const SelectArgs& a, int64_t row) {
 
 // exp(x) for x <= 0 by the hardware's 2^x, the product x log2(e) carried in two
 // parts: its rounding alone, up to 2^-24 of an exponent of some tens, would be
-// the sum's largest error.
+// the sum's largest error. Below -104 the result is zero (a product of the type's
+// lowest values would overflow); a NaN stays one.
 __device__ __forceinline__ float exp_below(float x) {
   constexpr float L = 1.44269502f, L_LO = 1.92596299e-8f, LN2 = 0.693147182f;
   const float hi = x * L, lo = fmaf(x, L_LO, fmaf(x, L, -hi));
   const float e = __builtin_amdgcn_exp2f(hi);
-  return x == -__builtin_inff() ? 0.f : fmaf(e, lo * LN2, e);
+  return x < -104.f ? 0.f : fmaf(e, lo * LN2, e);
 }
 
 // One slice of a row a block: lanes take 16 bytes each of consecutive logits, so
@@ -166,7 +167,7 @@ template <typename T, int NR>
 __global__ __launch_bounds__(MERGE_T) void beam_merge_kernel(SelectArgs a, int wp) {
   __shared__ int kind[32];
   __shared__ float score[32];
-  __shared__ double lse[32], inv[32];
+  __shared__ double top[32], lse[32], inv[32];             // (log sum above the row's maximum: that may be -3e38)
   __shared__ uint64_t group_top[64];
   __shared__ uint64_t lk[MERGE_CAP], lf[MERGE_CAP];        // sets: key of the maximum; beam << 32 | set
   __shared__ float lx[MERGE_CAP];                          // maximum
@@ -260,7 +261,8 @@ __global__ __launch_bounds__(MERGE_T) void beam_merge_kernel(SelectArgs a, int w
       ended[w] = done;
       length[w] = len;
       first[w] = 64;
-      lse[w] = m + lg;
+      top[w] = m;
+      lse[w] = lg;
     }
     if (lane == 1) inv[w] = a.alpha == 0.0 ? 1.0 : exp(-a.alpha * lg);
   };
@@ -279,7 +281,7 @@ __global__ __launch_bounds__(MERGE_T) void beam_merge_kernel(SelectArgs a, int w
   }
   __syncthreads();
 
-  auto key_of = [&](int w, float x) { return order_key(((double)score[w] + ((double)x - lse[w])) * inv[w]); };
+  auto key_of = [&](int w, float x) { return order_key(((double)score[w] + (((double)x - top[w]) - lse[w])) * inv[w]); };
   auto better = [](uint64_t ka, uint64_t fa, uint64_t kb, uint64_t fb) { return ka > kb || (ka == kb && fa < fb); };
   // ranks of n entries, 32 lanes an entry: f(rank, index)
   auto rank_all = [&](const uint64_t* k, const uint64_t* f, int n, auto put) {
@@ -345,9 +347,11 @@ __global__ __launch_bounds__(MERGE_T) void beam_merge_kernel(SelectArgs a, int w
   };
   if (mopen) {
     const double bk = __builtin_bit_cast(double, bound >> 63 ? bound ^ (1ull << 63) : ~bound);
-    const float bx = (float)((bk / inv[mw] - (double)score[mw]) + lse[mw]);
+    const double need = bk / inv[mw];
+    const float bx = (float)(((need - (double)score[mw]) + lse[mw]) + top[mw]);
+    const float off = (fabsf(bx) + 1.f) * 1e-5f + (float)(fabs(need) + fabs((double)score[mw])) * 1e-14f;
     // (above minus infinity at least: those are no candidates)
-    const float low = bound == 1 ? -3.402823466e38f : fmaxf(bx - (fabsf(bx) + 1.f) * 1e-5f, -3.402823466e38f);
+    const float low = bound == 1 ? -3.402823466e38f : fmaxf(bx - off, -3.402823466e38f);
     if (most >= low)
       each_set([&](int set, float x) {
         if (x >= low) take(mw, set, x);
@@ -472,7 +476,7 @@ __global__ __launch_bounds__(MERGE_T) void beam_merge_kernel(SelectArgs a, int w
   if (chosen)
     out = kind[p] == ROW_DONE  ? score[p]
           : kind[p] == ROW_NAN ? __builtin_nanf("")
-                               : (float)((double)score[p] + ((double)sel_x[lane] - lse[p]));
+                               : (float)((double)score[p] + (((double)sel_x[lane] - top[p]) - lse[p]));
   a.tokens[row0 + slot] = chosen ? token : std::max(eos32, 0);
   a.parents[row0 + slot] = row0 + from;
   a.scores_out[row0 + slot] = out;

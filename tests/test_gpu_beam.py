@@ -157,6 +157,62 @@ def test_nan_and_infinite_logits():
     assert step.tokens[3:].tolist() == want[0] and (step.parents[3:] - 12).tolist() == want[1]
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_logits_masked_by_the_lowest_value(dtype):
+    """Masks of the type's lowest value and far below the rest; a row of
+    nothing else is an even choice, as its softmax is."""
+    from minitp import kernels as K
+
+    logits, scores, _ = make(3, 5, 6007, dtype, seed=11)
+    low = torch.finfo(dtype).min
+    logits[0, :, 1::2] = low
+    logits[1, 2] = low
+    logits[1, 3, 9:] = low
+    logits[2, :, 40:6000] = -1e30
+    compare(K.beam_select(logits, scores), reference(logits, scores, None, None, -1, 0.0))
+
+
+def test_scores_far_beyond_the_logits():
+    """Scores so large that neighbouring logits give equal keys in 64 bits:
+    the lower token of them wins."""
+    from minitp import kernels as K
+
+    logits, scores, _ = make(4, 6, 9001, torch.float32, seed=21)
+    scores[0] *= 1e12
+    scores[1] = -2.0 ** 50
+    scores[2, 1:] = -2.0 ** 45
+    scores[3] = 2.0 ** 40
+    step, want = K.beam_select(logits, scores), reference(logits, scores, None, None, -1, 0.0)
+    # a key of 2^50 has steps of 2^-3: the two forms' sums of three may round one step apart
+    for g in range(4):
+        key = logits[g].double().log_softmax(-1).cpu() + scores[g].double().cpu()[:, None]
+        picked = [key[p - 6 * g, t].item() for t, p in zip(step.tokens[g].tolist(), step.parents[g].tolist())]
+        best = [key[p - 6 * g, t].item() for t, p in zip(want[0][g], want[1][g])]
+        step_of = 2.0 ** -52 * max(abs(b) for b in best)
+        assert all(abs(a - b) <= 2 * step_of for a, b in zip(sorted(picked), sorted(best)))
+        assert len(set(zip(step.tokens[g].tolist(), step.parents[g].tolist()))) == 6
+
+
+def test_outputs_over_the_inputs():
+    """The C entry's outputs may be its inputs."""
+    from minitp import _native as N
+    from minitp import kernels as K
+
+    logits, scores, g = make(4, 7, 2000, torch.bfloat16, seed=3)
+    finished = torch.rand(4, 7, generator=g, device=DEV) < 0.3
+    lengths = torch.randint(0, 9, (4, 7), generator=g, device=DEV)
+    want = K.beam_select(logits, scores, finished, lengths, eos_token_id=3, length_penalty=1.0)
+    size = N.lib().minitp_beam_select_workspace_bytes(4, 7, 2000)
+    ws = torch.empty(size, dtype=torch.uint8, device=DEV)
+    tokens, parents = (torch.empty(4, 7, dtype=torch.long, device=DEV) for _ in range(2))
+    N.check(N.lib().minitp_beam_select(N.stream(), N.BF16, logits.data_ptr(), 7 * 2000, 2000, 4, 7, 2000, scores.data_ptr(),
+                                       finished.data_ptr(), lengths.data_ptr(), 3, 1.0, tokens.data_ptr(),
+                                       parents.data_ptr(), scores.data_ptr(), finished.data_ptr(), lengths.data_ptr(),
+                                       ws.data_ptr(), size), "beam_select")
+    for got, w in zip((tokens, parents, scores, finished, lengths), want):
+        assert torch.equal(got, w)
+
+
 def test_first_step_from_one_row_and_strided_rows():
     from minitp import kernels as K
 
