@@ -178,6 +178,10 @@ __device__ __forceinline__ float quads_sum(float v) {
   return halves_sum(__uint_as_float(a[0]) + __uint_as_float(a[1]));
 }
 
+// A maximum to join by. Scores that are no numbers are no maximum but show in
+// the sum; what has none above minus infinity and such a sum is no empty set.
+__device__ __forceinline__ float join_max(float m, float l) { return l != l ? 0.f : m; }
+
 // Results of query rows [0, rows) from base row r0 of the item that KW waves
 // hold over keys of their own, in LDS: po [KW][cap][D], pml [KW][cap] (maximum,
 // sum; exp2 or expf by BASE2). Joined, they go to the output or to the slot.
@@ -394,7 +398,7 @@ __device__ __forceinline__ void shared_rows_f32(const SharedArgs& a, const Item&
     for (int x = 0; x < 4; ++x)
 #pragma unroll
       for (int j = 0; j < E; ++j) po[at * D + 64 * hf + E * (4 * lq + x) + j] = o[hf][j][x];
-  if (lq == 0) pml[at] = make_float2(m, lsum);
+  if (lq == 0) pml[at] = make_float2(join_max(m, lsum), lsum);
   __syncthreads();
   finish_rows<float, D, KW, false>(a, it, po, pml, CAP, t0, std::min(CAP, it.rows - t0));
 }
@@ -708,6 +712,7 @@ __device__ __forceinline__ void shared_rows128(const SharedArgs& a, const Item& 
   }
   if (r >= it.rows) return;
   const float l = halves_sum(lsum);
+  m = join_max(m, l);
   if (a.joined) {
     const float f = m == -__builtin_inff() ? 0.f : 1.f / l;
     bf16* orow = (bf16*)a.out + me.row * D + 4 * h;
@@ -853,7 +858,7 @@ __device__ __forceinline__ void shared_rows16(const SharedArgs& a, const Item& i
   __syncthreads();                             // (every stage is free)
 #pragma unroll
   for (int d = 0; d < DB; ++d) *(f32x4*)(po + (w * H_SMALL + r) * D + 16 * d + 4 * q4) = o[d];
-  if (q4 == 0) pml[w * H_SMALL + r] = make_float2(m, l);
+  if (q4 == 0) pml[w * H_SMALL + r] = make_float2(join_max(m, l), l);
   __syncthreads();
   finish_rows<bf16, D, 4, true>(a, it, po, pml, H_SMALL, 0, it.rows);
 }

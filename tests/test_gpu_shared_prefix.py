@@ -150,6 +150,22 @@ def test_hidden_values_that_are_not_finite_stay_hidden(d, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("p", [100, 1500])
+@pytest.mark.parametrize("hq,hkv,d,t", [(14, 2, 64, 1), (28, 4, 128, 40), (4, 2, 16, 3)])
+def test_a_query_that_is_no_number_shows(hq, hkv, d, t, p, dtype):
+    """Its own output is NaN, as its softmax is; no other row changes."""
+    from minitp import kernels as K
+
+    x = make(6, 2, t, hq, hkv, d, p, 33, dtype)
+    clean = K.shared_prefix_attention(*x[:5], p, 33).view(6, t, hq, d)
+    x[0][1, t - 1, 2, 5] = float("nan")
+    out = K.shared_prefix_attention(*x[:5], p, 33).view(6, t, hq, d)
+    assert torch.isnan(out[1, t - 1, 2]).all()
+    out[1, t - 1, 2] = clean[1, t - 1, 2]
+    assert torch.equal(out, clean)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_a_prefix_equals_the_same_rows_in_every_cache(dtype):
     """The prefix's rows copied in front of each row's own: the plain
     attention of the framework gives the same within both forms' bars."""
