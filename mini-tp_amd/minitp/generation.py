@@ -87,8 +87,8 @@ class GenerationState:
         device = input_ids.device
         self.out_ids = torch.empty(b, self.total, dtype=torch.long, device=device)
         self.out_ids[:, :t] = input_ids
-        start = self.kv.prefix.seq_len if self.kv.prefix is not None else 0  # positions continue a shared prefix
-        self.positions_buf = torch.arange(start, start + self.total, device=device)  # the only arange
+        self._start = self._prefix_rows()  # positions continue a shared prefix
+        self.positions_buf = torch.arange(self._start, self._start + self.total, device=device)  # the only arange
         self.cursor = t
         self.finished: torch.Tensor | None = None
         self.eos = -1
@@ -99,6 +99,9 @@ class GenerationState:
         self._eos_dev: torch.Tensor | None = None  # [B + 2] finished flags, halted, stop column
         self._eos_host: torch.Tensor | None = None  # pinned stop column (0 = running)
         self._eos_host_dev: int | None = None
+
+    def _prefix_rows(self) -> int:
+        return self.kv.prefix.seq_len if self.kv.prefix is not None else 0
 
     def _enable_device_eos(self, eos: int) -> None:
         """Keep generate_greedy's finished mask and stop test on the device."""
@@ -129,6 +132,8 @@ class GenerationState:
 
     def prefill(self) -> torch.Tensor:
         """Prompt forward; positions come from the buffer (0..T-1)."""
+        if self._prefix_rows() != self._start:
+            raise ValueError(f"GenerationState: built for {self._start} prefix rows, the cache has {self._prefix_rows()}")
         positions = self.positions_buf[: self.prompt_len]
         ids = self.out_ids[:, : self.prompt_len]
         if not self._native:

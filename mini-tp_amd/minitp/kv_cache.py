@@ -44,6 +44,7 @@ class KVCache:
         if init == "zeros":
             self._fill(0.0)
         self.prefix: KVCache | None = None  # rows that groups of this cache's batch rows share (share_prefix)
+        self.is_prefix = False
         self.k = [t[:, :, :max_seq_len] for t in self.k_buf.unbind(0)]
         self.v = [t[:, :, :max_seq_len] for t in self.v_buf.unbind(0)]
 
@@ -71,10 +72,13 @@ class KVCache:
         """Put ``prefix`` in front of this cache: every run of batch / (prefix
         batch) consecutive rows here continues one row of ``prefix``, whose
         rows [0, prefix.seq_len) are kept once and attended by all of them (no
-        counterpart in the reference, whose caches hold a prompt per row)."""
+        counterpart in the reference, whose caches hold a prompt per row). This
+        cache must be empty: its rows' positions go on from the prefix's."""
         mine, shared = self.k_buf.shape, prefix.k_buf.shape
-        if prefix.prefix is not None or prefix is self:
+        if prefix.prefix is not None or prefix is self or self.is_prefix:
             raise ValueError("a shared prefix cannot have a prefix of its own")
+        if self.seq_len != 0:
+            raise ValueError(f"share_prefix: the cache holds {self.seq_len} rows already")
         if mine[0] != shared[0] or mine[2] != shared[2] or mine[4] != shared[4] or \
                 prefix.k_buf.dtype != self.k_buf.dtype or prefix.k_buf.device != self.k_buf.device:
             raise ValueError(f"prefix cache {tuple(shared)} {prefix.k_buf.dtype} on {prefix.k_buf.device} does not fit "
@@ -82,6 +86,7 @@ class KVCache:
         if shared[1] == 0 or mine[1] % shared[1] != 0:
             raise ValueError(f"batch {mine[1]} not divisible by the prefix cache's batch {shared[1]}")
         self.prefix = prefix
+        prefix.is_prefix = True
 
     def reorder(self, parents: torch.Tensor) -> None:
         """The written rows follow their beams, in place: batch row b of every

@@ -249,6 +249,8 @@ class TPQwen2ForCausalLM(nn.Module):
         tok [B] (any stride), pos 0-d long, logits [B, 1, V] written in place.
         eos: (state pointer, token, cursor, host word pointer) of the
         on-device early stop, or None."""
+        if kv_cache.prefix is not None:
+            raise ValueError("decode_native: the decode graph takes no shared prefix")
         prog = self._prog if self._prog is not None else self.program()
         b = tok.shape[0]
         N.require_gpu(tok, pos, next_tok, what="GenerationState.decode_step")

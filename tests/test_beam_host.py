@@ -162,3 +162,37 @@ def test_share_prefix_checks_the_caches():
     assert kv.prefix is good
     with pytest.raises(ValueError):
         cache(batch=12).share_prefix(kv)
+    with pytest.raises(ValueError):
+        good.share_prefix(cache(batch=1))  # (it serves as a prefix itself)
+    full = cache(batch=6)
+    full.advance(2)
+    with pytest.raises(ValueError, match="2 rows"):
+        full.share_prefix(good)
+
+
+def test_generation_state_keeps_to_its_prefix():
+    """A prefix put in front of the cache, or grown, after the positions were
+    laid out is refused, and so is the decode graph with one."""
+    from minitp.config import ModelConfig
+    from minitp.distributed.context import ParallelContext
+    from minitp.generation import GenerationState, make_kv_cache
+    from minitp.layer import TPQwen2ForCausalLM
+
+    cfg = ModelConfig(32, 48, 1, 2, 1, 16, 64, 1e-6, 1e6, 64)
+    model = TPQwen2ForCausalLM(cfg, ParallelContext(0, 0, 1, 0, 1, torch.device("cpu"), None), init_weights=False)
+    ids = torch.zeros(2, 3, dtype=torch.long)
+    pre = make_kv_cache(model, 1, 8)
+    pre.advance(5)
+    late = GenerationState(model, ids, 4)
+    late.kv.share_prefix(pre)
+    with pytest.raises(ValueError, match="prefix rows"):
+        late.prefill()
+    with pytest.raises(ValueError, match="shared prefix"):
+        model.decode_native(ids[:, 0], torch.tensor(0), late.kv, torch.zeros(2, 1, 64), None)
+    kv = make_kv_cache(model, 2, 8)
+    kv.share_prefix(pre)
+    state = GenerationState(model, ids, 4, kv=kv)
+    assert state.positions_buf.tolist() == list(range(5, 12))
+    pre.advance(1)
+    with pytest.raises(ValueError, match="prefix rows"):
+        state.prefill()
