@@ -353,3 +353,25 @@ def test_selection_and_reorder_in_a_graph_and_on_a_side_stream():
         assert torch.equal(k, want)
         eager = K.beam_select(logits, scores)
         assert all(torch.equal(a, b) for a, b in zip(eager, s))
+
+
+def test_offsets_past_32_bits():
+    """Rows of logits 2^31 elements apart, caches of more than 4 GiB a beam row."""
+    from minitp import kernels as K
+
+    far = (1 << 31) + 24
+    flat = torch.empty(far + 8000, dtype=torch.bfloat16, device=DEV)
+    logits = flat.as_strided((2, 4, 2000), (far, 2000, 1))
+    src, scores, g = make(2, 4, 2000, torch.bfloat16, seed=4)
+    logits.copy_(src)
+    compare(K.beam_select(logits, scores), reference(src, scores, None, None, -1, 0.0))
+    del flat, logits
+    k, v = (torch.empty(1, 3, 2, (1 << 23) + 16, 128, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    for x in (k, v):
+        x[:, :, :, :40] = torch.randn(1, 3, 2, 40, 128, generator=g, device=DEV)
+    parents = torch.tensor([[2, 0, 1]], device=DEV)
+    want = [x[:, [2, 0, 1], :, :33] for x in (k, v)]
+    rest = [x[:, :, :, 33:40].clone() for x in (k, v)]
+    K.kv_reorder(k, v, parents, 33)
+    for x, w, r in zip((k, v), want, rest):
+        assert torch.equal(x[:, :, :, :33], w) and torch.equal(x[:, :, :, 33:40], r)

@@ -269,3 +269,24 @@ def test_many_keys_and_rows():
         pr = s.softmax(-1)
         ref, mag = (pr @ v).view(b, 14, 64), (pr @ v.abs()).view(b, 14, 64)
         assert ((out - ref).abs() <= bars(ref, mag, dtype, 64) + 1e-9).all()
+
+
+@pytest.mark.parametrize("own", [False, True])
+def test_keys_past_four_gib_of_a_head(own):
+    """2^24 rows and some of 256 bytes, all zeros but for the last ones: one of
+    those takes nearly all of a query's weight."""
+    from minitp import kernels as K
+
+    d, n = 128, (1 << 24) + 200
+    long_k, long_v = (torch.zeros(1, 1, n + 8, d, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    short = torch.zeros(1, 1, 8, d, dtype=torch.bfloat16, device=DEV)
+    q = torch.zeros(1, 1, 2, d, dtype=torch.bfloat16, device=DEV)
+    for h, row in enumerate((n - 1, n - 150)):  # (256 n bytes are past 2^32)
+        q[0, 0, h, h], long_k[0, 0, row, h] = 16.0, 20.0
+        long_v[0, 0, row] = torch.arange(d, device=DEV) * (1 + h) / 64
+    args = (short, short, long_k, long_v, 3, n - 1) if own else (long_k, long_v, short, short, n, 2)
+    out = K.shared_prefix_attention(q, *args).view(2, d).double().cpu()
+    weight = torch.tensor(16.0 * 20.0 / d ** 0.5, dtype=torch.float64).exp()
+    ref = torch.stack([long_v[0, 0, r].double().cpu() for r in (n - 1, n - 150)]) * weight / (weight + n + 2)
+    # the product's and the output's rounding, 2^-8 each; sums of 600 tiles of 32 and less in a row
+    assert ((out - ref).abs() <= ref.abs() * (2 * 2 ** -8 + 2 * 600 * 32 * 2 ** -24)).all()
