@@ -977,14 +977,22 @@ struct Plan {
 // 161.8, 9 176.1, 12 170.7; 8 rows x 4 of the 0.5B heads on 2,048: 8 splits
 // 12.2, 16 11.6, 32 12.4; fp32, 5 rows x 3 on 777: 6 19.3, 13 12.6.
 //
-// Joined, one item a query tile over both parts and straight to the output:
-// without a prefix; for few keys, where a second launch costs more than the
-// prefix read once a row (4 to 32 rows, 0.5B / 7B heads: 128 + 64 keys 5.8 / 6.8
-// against 8.9 / 10.9, 512 + 64 8.2 / 10.2 against 9.6 / 12.0, 1,024 + 64 11.2 / 15
-// against 10.0 / 12.6); and where the rows' own queries fill their tiles to
-// three quarters and the tiles the CUs (16 rows of 100 tokens on 4,096 keys 123
-// against 133, and no scratch, which grows with the tokens).
-Plan shared_plan(int dtype, int64_t B, int64_t G, int64_t T, int64_t Hq, int64_t Hkv, int64_t P, int64_t C) {
+// Joined, one item a query tile over both parts and straight to the output, where
+// a second launch and the partial results cost more than the prefix computed
+// for half-empty tiles. Measured (us, joined against apart; own: tiles of all rows):
+//   own < 256: bf16, up to 10 key tiles in all, fp32, rows of at most 16 queries
+//     and up to 7 tiles, two of them the prefix's: own 128, 7B heads, 512 + 65 keys
+//     10.4 against 12.0, 1,024 + 1 14.2 against 12.9; fp32 128 + 257 25.3 against
+//     27.9, 256 + 1 17.6 against 16.2;
+//   rows of at most 16 queries, whose tiles are not shared: own x prefix tiles
+//     up to 8,192 (fp32 131,072 / D): own 512, 7B heads, 1,024 + 1 keys 18.4
+//     against 24.7, own 2,048 256 + 65 39.5 against 36.4; fp32 own 256 256 + 65
+//     20.9 against 23.4, own 512 256 + 65 42.7 against 37.8;
+//   longer rows: the empty part of their tiles, in queries x prefix keys a
+//     query, up to 1,200 (fp32 100): 63 queries of 128, own 512, 1,024 keys
+//     38.1 against 40.4, 4,096 110.6 against 103.0; 98: 4,096 139 against 145;
+//     700 of 768, 4,096 keys 123 against 133.
+Plan shared_plan(int dtype, int64_t D, int64_t B, int64_t G, int64_t T, int64_t Hq, int64_t Hkv, int64_t P, int64_t C) {
   const bool tiles16 = dtype == MINITP_BF16;
   const int64_t qt = tiles16 ? H_QT : F_QT, kt = tiles16 ? H_KT : F_KT, per = Hq / Hkv;
   Plan p;
@@ -996,8 +1004,15 @@ Plan shared_plan(int dtype, int64_t B, int64_t G, int64_t T, int64_t Hq, int64_t
   const int64_t most_p = tiles16 ? tiles_p / 2 : tiles_p;
   p.splits_p = P > 0 ? within(std::min(448 / bp, std::max(256 / bp, tiles_p / 16)), most_p) : 0;
   p.splits_s = within(256 / bs, tiles_s / 2);
-  p.joined = (P == 0 && p.splits_s == 1) || (T * per <= H_SMALL && bs <= 256 && tiles_p + tiles_s <= 8) ||
-             (T * per >= qt && 4 * T * per >= 3 * qt * p.qtiles_s && bs >= 256);
+  const bool few = T * per <= H_SMALL;
+  if (P == 0 && p.splits_s == 1)
+    p.joined = true;
+  else if (bs < 256)
+    p.joined = tiles16 ? tiles_p + tiles_s <= 10 : few && tiles_p <= 2 && tiles_p + tiles_s <= 7;
+  else if (few)
+    p.joined = tiles_p <= 16 && bs * tiles_p <= (tiles16 ? 8192 : 131072 / D) && (tiles_p <= 4 || tiles_p + tiles_s <= 20);
+  else
+    p.joined = (qt * p.qtiles_s - T * per) * P <= (tiles16 ? 1200 : 100) * T * per;
   if (p.joined) {
     p.splits_p = 0;
     p.splits_s = 1;
@@ -1064,7 +1079,7 @@ int shared_prefix_check(int dtype, const SharedPrefixShape& s) {
   }
   bool fits = s.B < MOST && s.Hq < MOST && s.B * s.T < MOST && s.B * s.T * s.Hq < MOST - 256;
   if (fits && s.B * s.T > 0) {
-    const Plan p = shared_plan(dtype, s.B, s.G, s.T, s.Hq, s.Hkv, s.P, s.C);
+    const Plan p = shared_plan(dtype, s.D, s.B, s.G, s.T, s.Hq, s.Hkv, s.P, s.C);
     fits = p.items_p + p.items_s < (1LL << 24) - 16;
   }
   if (!fits) {
@@ -1078,7 +1093,7 @@ int shared_prefix_check(int dtype, const SharedPrefixShape& s) {
 int64_t shared_prefix_workspace_bytes(int dtype, const SharedPrefixShape& s) {
   if (s.B == 0 || s.T == 0) return 0;
   if (shared_prefix_check(dtype, s)) return -1;
-  const Plan p = shared_plan(dtype, s.B, s.G, s.T, s.Hq, s.Hkv, s.P, s.C);
+  const Plan p = shared_plan(dtype, s.D, s.B, s.G, s.T, s.Hq, s.Hkv, s.P, s.C);
   return p.joined ? 0 : (p.splits_p + p.splits_s) * s.B * s.T * s.Hq * (s.D + 2) * 4;
 }
 
@@ -1088,7 +1103,7 @@ int launch_shared_prefix_attention(hipStream_t st, int dtype, const SharedPrefix
                                    const int64_t* cache_lens, void* workspace, int64_t workspace_bytes) {
   const int rc = shared_prefix_check(dtype, s);
   if (rc) return rc;
-  const Plan p = shared_plan(dtype, s.B, s.G, s.T, s.Hq, s.Hkv, s.P, s.C);
+  const Plan p = shared_plan(dtype, s.D, s.B, s.G, s.T, s.Hq, s.Hkv, s.P, s.C);
   const int64_t rows = s.B * s.T * s.Hq;
   const int64_t need = p.joined ? 0 : (p.splits_p + p.splits_s) * rows * (s.D + 2) * 4;
   if (workspace_bytes < need || (workspace == nullptr && need > 0) || !aligned16(workspace)) {
