@@ -583,7 +583,8 @@ struct Tiles {
 // 2): until then probabilities stay below 2^8 and nothing is rescaled.
 constexpr float SLACK = 8.f;
 
-template <int D>
+// AHEAD: a wave's second products go before other waves' work (below).
+template <int D, bool AHEAD>
 __device__ __forceinline__ void shared_rows128(const SharedArgs& a, const Item& it, char* lds) {
   using H = Half<D>;
   // (D = 16: the output's 32-row operand holds the 16 dims twice)
@@ -706,6 +707,7 @@ __device__ __forceinline__ void shared_rows128(const SharedArgs& a, const Item& 
         }
         return;
       }
+      if (AHEAD) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {  // keys 16 j .. 16 j + 15
         const f32x16& p = s[j / 2];
@@ -723,6 +725,7 @@ __device__ __forceinline__ void shared_rows128(const SharedArgs& a, const Item& 
           o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pb, o[d], 0, 0, 0);
         }
       }
+      if (AHEAD) __builtin_amdgcn_s_setprio(0);
     });
   }
   if (r >= it.rows) return;
@@ -878,16 +881,21 @@ __device__ __forceinline__ void shared_rows16(const SharedArgs& a, const Item& i
   finish_rows<bf16, D, 4, true>(a, it, po, pml, H_SMALL, 0, it.rows);
 }
 
-template <int D>
+// FEW: the own part's units have at most 16 rows. Where they have more, all blocks
+// are alike and the two on a CU fall into step best, one in its softmax while
+// the other multiplies, when a wave's second products go first: 16 rows of 100
+// tokens on 4,096 keys, 7B heads, 123 -> 115 us. Beside blocks of few rows it
+// costs them their turns (256 rows of one token on 32,256 keys 158 -> 164 us).
+template <int D, bool FEW>
 __global__ __launch_bounds__(256, 2) void shared_attn_bf16_kernel(SharedArgs a) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   static_assert(Half<D>::LDS >= 4 * H_SMALL * (D + 2) * 4, "the waves' join fits the stages");
   Item it;
   if (!shared_item<H_QT, H_KT>(a, D * 2, it)) return;
-  if (it.rows <= H_SMALL)
+  if (FEW && it.rows <= H_SMALL)
     shared_rows16<D>(a, it, lds);
   else
-    shared_rows128<D>(a, it, lds);
+    shared_rows128<D, !FEW>(a, it, lds);
 }
 
 // The slots of each query row joined (maxima in base 2); every LPR = D / 4 lanes
@@ -1041,9 +1049,10 @@ template <typename T, int D>
 int shared_launch(hipStream_t st, const SharedArgs& a, const Plan& p) {
   const dim3 grid((unsigned)(8 * (a.run_p + a.run_s)));
   if constexpr (sizeof(T) == 2) {
-    const int rc = ensure_lds_limit((const void*)shared_attn_bf16_kernel<D>, Half<D>::LDS);
+    const auto kern = a.T * a.per <= H_SMALL ? shared_attn_bf16_kernel<D, true> : shared_attn_bf16_kernel<D, false>;
+    const int rc = ensure_lds_limit((const void*)kern, Half<D>::LDS);
     if (rc) return rc;
-    hipLaunchKernelGGL(shared_attn_bf16_kernel<D>, grid, dim3(256), Half<D>::LDS, st, a);
+    hipLaunchKernelGGL(kern, grid, dim3(256), Half<D>::LDS, st, a);
   } else {
     const int rc = ensure_lds_limit((const void*)shared_attn_f32_kernel<D>, F_LDS<D>);
     if (rc) return rc;
