@@ -450,7 +450,7 @@ __global__ __launch_bounds__(256) void shared_attn_f32_kernel(SharedArgs a) {
 // takes one chunk column of 16 rows, a V read 64 bytes of four rows.
 //
 // Two blocks a CU (64 KiB of LDS each at D = 128) cover each other's softmax:
-// 512 even blocks run at 1.0 PFLOP/s. Not faster: a tile's scores computed
+// 512 even blocks run at 1.06 PFLOP/s. Not faster: a tile's scores computed
 // before the tile in front of it is used (946 against 961 TFLOP/s), the next
 // loads issued behind the scores (-7 %) or spread over the product.
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -1012,9 +1012,10 @@ struct Plan {
 //     against 24.7, own 2,048 256 + 65 39.5 against 36.4; fp32 own 256 256 + 65
 //     20.9 against 23.4, own 512 256 + 65 42.7 against 37.8;
 //   longer rows: the empty part of their tiles, in queries x prefix keys a
-//     query, up to 1,200 (fp32 100): 63 queries of 128, own 512, 1,024 keys
-//     38.1 against 40.4, 4,096 110.6 against 103.0; 98: 4,096 139 against 145;
-//     700 of 768, 4,096 keys 123 against 133.
+//     query, up to 1,200 (fp32 100): 7B heads, 63 queries of 128, own 512, 1,024
+//     keys 34.8 against 40.3, 4,096 101 against 102; 98: 4,096 132 against 136;
+//     700 of 768, 4,096 keys 114 against 120; fp32 98 of 128, own 512, 256 keys
+//     156 against 163, 1,024 486 against 465.
 Plan shared_plan(int dtype, int64_t D, int64_t B, int64_t G, int64_t T, int64_t Hq, int64_t Hkv, int64_t P, int64_t C) {
   const bool tiles16 = dtype == MINITP_BF16;
   const int64_t qt = tiles16 ? H_QT : F_QT, kt = tiles16 ? H_KT : F_KT, per = Hq / Hkv;

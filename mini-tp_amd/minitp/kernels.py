@@ -343,9 +343,10 @@ def _cache_view(what: str, k: torch.Tensor, v: torch.Tensor, batch: int, hkv: in
 def _lens(what: str, lens: torch.Tensor | None, count: int) -> torch.Tensor | None:
     if lens is None:
         return None
-    if lens.shape != (count,) or lens.is_floating_point() or lens.dtype == torch.bool:
-        raise ValueError(f"{what}: lengths {tuple(lens.shape)} {lens.dtype}, expected {count} whole numbers")
-    return lens.to(torch.long).contiguous()
+    dtype = lens.dtype
+    if lens.shape != (count,) or dtype.is_floating_point or dtype.is_complex or dtype is torch.bool:
+        raise ValueError(f"{what}: lengths {tuple(lens.shape)} {dtype}, expected {count} whole numbers")
+    return lens if dtype is torch.long and lens.is_contiguous() else lens.to(torch.long).contiguous()
 
 
 def shared_prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Tensor, k_cache: torch.Tensor,
