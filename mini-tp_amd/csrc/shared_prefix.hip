@@ -240,7 +240,8 @@ __device__ __forceinline__ void finish_rows(const SharedArgs& a, const Item& it,
 // output MFMA j dims E r + j; rows are padded by 16 bytes against bank
 // conflicts. A score is summed in four chains. Measured: 3 x 5 rows on 777 + 100
 // keys, 0.5B heads, 8 us and 4 us for the join (latency); 11 x 116 rows on 421 +
-// up to 206 keys, 7B heads, 10.4 GFLOP in 220 us (572 blocks on 512 places).
+// up to 206 keys, 7B heads, 10.4 GFLOP in 171 us (572 blocks on 512 places; 220
+// us before the bound of two blocks a CU, which kept D = 128 to one).
 constexpr int F_QT = 64, F_KT = 64;
 template <int D>
 constexpr int F_LDS = 2 * F_KT * (D + 4) * 4;
@@ -414,7 +415,7 @@ __device__ __forceinline__ void shared_rows_f32(const SharedArgs& a, const Item&
 }
 
 template <int D>
-__global__ __launch_bounds__(256) void shared_attn_f32_kernel(SharedArgs a) {
+__global__ __launch_bounds__(256, 2) void shared_attn_f32_kernel(SharedArgs a) {
   extern __shared__ __attribute__((aligned(16))) float lds_f[];
   static_assert(F_LDS<D> >= 64 * (D + 2) * 4, "the waves' results fit the tiles");
   __shared__ int odd;
