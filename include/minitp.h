@@ -200,7 +200,9 @@ int minitp_attention(void* stream, int dtype, const void* q, const void* k_cache
  * is zeros and its caches are not read. Rows past P_g and c_b + T are never
  * read. prefix_len 0 serves rows without a prefix (the prefix pointers may be
  * NULL). Workspace from the query below (bf16 and fp32 ask for different
- * sizes); no initial value, nothing kept in it after the call's kernels. */
+ * sizes; 0 where the call needs none, -1 for a call that is refused); no
+ * initial value, nothing kept in it after the call's kernels. 2^31 query rows
+ * or keys and more are MINITP_ERR_UNSUPPORTED. */
 int64_t minitp_shared_prefix_attention_workspace_bytes(int dtype, int64_t B, int64_t G, int64_t T, int64_t Hq,
                                                        int64_t Hkv, int64_t D, int64_t prefix_len,
                                                        int64_t cache_len);
@@ -222,10 +224,10 @@ int minitp_shared_prefix_attention(void* stream, int dtype, const void* q, const
  * continues with eos_token at its own score and length. Of a group's
  * continuations above minus infinity the W of the largest score / length ^
  * length_penalty (-16 to 16) win (length: with the new token, at least 1),
- * equal ones by the lower beam, then the lower token. A NaN score wins over every number.
- * The first winner of a parent stays in the parent's slot, the others fill the
- * free slots in rank order; a slot left over is its own parent with a score of
- * minus infinity, marked finished. Outputs, all [G, W], which may be the
+ * equal ones by the lower beam, then the lower token. A NaN score wins over
+ * every number. The first winner of a parent stays in the parent's slot, the
+ * others fill the free slots in rank order; a slot left over is its own parent
+ * with a score of minus infinity, marked finished. Outputs, all [G, W], which may be the
  * inputs of the same kind: tokens, parents (rows of the batch, g * W + w),
  * scores, finished (parent's, or the token is eos_token), lengths. eos_token
  * -1: none (finished must be NULL). */

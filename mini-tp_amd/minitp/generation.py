@@ -238,7 +238,7 @@ def generate_beam(model: TPQwen2ForCausalLM, input_ids: torch.Tensor, max_new_to
     from minitp import kernels as K
 
     b, t = input_ids.shape
-    if num_beams < 1 or max_new_tokens < 1:
+    if not 1 <= num_beams <= K.MAX_BEAMS or max_new_tokens < 1:
         raise ValueError(f"generate_beam: num_beams={num_beams}, max_new_tokens={max_new_tokens}")
     limit = model.cfg.max_position_embeddings
     if t + max_new_tokens - 1 > limit:  # the last token is selected, not forwarded

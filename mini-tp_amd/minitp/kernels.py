@@ -402,6 +402,9 @@ def shared_prefix_bytes(*sizes: int) -> int:
     return max(_lib().minitp_shared_prefix_attention_workspace_bytes(*sizes), 0)
 
 
+MAX_BEAMS = 32  # beams of a group
+
+
 class BeamStep(NamedTuple):
     """The beams after one step of ``beam_select``, all [G, W]."""
 
@@ -415,7 +418,7 @@ class BeamStep(NamedTuple):
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: torch.Tensor | None = None,
                 lengths: torch.Tensor | None = None, *, eos_token_id: int | None = None,
                 length_penalty: float = 0.0) -> BeamStep:
-    """One step of beam search for G groups of W beams (at most 32).
+    """One step of beam search for G groups of W beams (at most MAX_BEAMS).
 
     logits [G, W, V] or [G * W, V] (rows of any strides, expanded ones too) of
     the beams whose cumulative log-probabilities are ``scores`` [G, W] float32
@@ -476,8 +479,8 @@ def _beam_select_bytes(*sizes: int) -> int:
 def kv_reorder(k_buf: torch.Tensor, v_buf: torch.Tensor, parents: torch.Tensor, rows: int) -> None:
     """The K/V caches follow the beams, in place: rows [0, rows) of every layer
     and KV head of batch row b of the buffers [L, B, Hkv, S, D] become those of
-    row parents[b]. ``parents`` [G, W], G * W == B, W at most 32, holds batch
-    rows; one outside the row's own group leaves the row as it is."""
+    row parents[b]. ``parents`` [G, W], G * W == B, W at most MAX_BEAMS, holds
+    batch rows; one outside the row's own group leaves the row as it is."""
     what = "kv_reorder"
     dev = _one_device(what, k_buf, v_buf, parents)
     if _elsewhere(dev):

@@ -152,3 +152,68 @@ def test_greedy_under_a_shared_prefix(dtype):
     if dtype == torch.float32:
         out = generate_greedy(model, asks, 10, kv=caches())
         assert torch.equal(out, generate_greedy(model, whole, 10)[:, 70:])
+
+
+def test_an_end_token_under_a_shared_prefix():
+    """generate_greedy's early stop behind prefixes: the same ids, the same end."""
+    from minitp.generation import generate_greedy, make_kv_cache
+
+    model, _ = _pair("tiny")
+    g = torch.Generator().manual_seed(5)
+    system = torch.randint(0, 1000, (2, 33), generator=g).to(DEV)
+    asks = torch.randint(0, 1000, (4, 6), generator=g).to(DEV)
+    whole = torch.cat([system.repeat_interleave(2, 0), asks], 1)
+    free = generate_greedy(model, whole, 20)
+    for eos in {int(free[0, 42]), int(free[3, 50])}:
+        pre = make_kv_cache(model, 2, 33)
+        model(system, kv_cache=pre)
+        kv = make_kv_cache(model, 4, 26)
+        kv.share_prefix(pre)
+        out = generate_greedy(model, asks, 20, eos_token_id=eos, kv=kv)
+        assert torch.equal(out, generate_greedy(model, whole, 20, eos_token_id=eos)[:, 33:])
+
+
+def test_beam_search_module_by_module():
+    """The modules walked one by one give the program's beams."""
+    from minitp.generation import generate_beam
+
+    model, _ = _pair("tiny")
+    prompts = torch.randint(0, 1000, (3, 8), generator=torch.Generator().manual_seed(6)).to(DEV)
+    ids, scores = generate_beam(model, prompts.int(), 7, 4)
+    for layer in model.model.layers:
+        layer.self_attn.use_fused_qkv = False
+    walked, other = generate_beam(model, prompts, 7, 4)
+    assert torch.equal(ids, walked) and (scores - other).abs().max() <= 7e-5
+
+
+def test_a_step_behind_a_prefix_in_a_graph():
+    """One captured step of a beam search, replayed for other tokens between the
+    program's own eager work."""
+    from minitp.generation import make_kv_cache
+
+    model, _ = _pair("qwen2.5-0.5b", torch.bfloat16)
+    g = torch.Generator().manual_seed(9)
+    system = torch.randint(0, 151936, (2, 600), generator=g).to(DEV)
+    pre = make_kv_cache(model, 2, 256)
+    model(system[:, :200], kv_cache=pre)
+    toks = [torch.randint(0, 151936, (6, 1), generator=g).to(DEV) for _ in range(4)]
+
+    def behind():
+        kv = make_kv_cache(model, 6, 8)
+        kv.share_prefix(pre)
+        model(toks[3], kv_cache=kv)
+        return kv
+
+    with torch.inference_mode():
+        kv, tok = behind(), toks[0].clone()
+        model(tok, kv_cache=kv)  # (workspaces of this shape are there)
+        kv.seq_len = 1
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = model(tok, kv_cache=kv)
+        for t in toks[:3]:
+            want = model(t, kv_cache=behind())
+            tok.copy_(t)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want)
