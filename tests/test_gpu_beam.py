@@ -375,3 +375,23 @@ def test_offsets_past_32_bits():
     K.kv_reorder(k, v, parents, 33)
     for x, w, r in zip((k, v), want, rest):
         assert torch.equal(x[:, :, :, :33], w) and torch.equal(x[:, :, :, 33:40], r)
+
+
+def test_calls_on_two_streams_at_once():
+    """Selections and attention queued on two streams: scratch of their own."""
+    from minitp import kernels as K
+
+    logits, scores, g = make(6, 8, 20000, torch.float32)
+    q = torch.randn(12, 1, 8, 64, generator=g, device=DEV)
+    pre, own = torch.randn(2, 2, 900, 64, generator=g, device=DEV), torch.randn(12, 2, 60, 64, generator=g, device=DEV)
+    calls = (lambda: list(K.beam_select(logits, scores)), lambda: [K.shared_prefix_attention(q, pre, pre, own, own, 900, 59)])
+    want = [c() for c in calls]
+    streams = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    outs = []
+    for i in range(12):
+        with torch.cuda.stream(streams[i % 2]):
+            outs.append([c() for c in calls])
+    torch.cuda.synchronize()
+    for out in outs:
+        assert all(torch.equal(a, b) for got, ref in zip(out, want) for a, b in zip(got, ref))
