@@ -47,7 +47,7 @@ class TPQwen2Attention(nn.Module):
         y = self.qkv_proj.project(x, fused=self.use_fused_qkv)
         if kv_cache is not None:
             kv_cache.check_room(t)
-            cache_len = kv_cache.seq_len
+            cache_len, prefix_rows = kv_cache.seq_len, kv_cache.prefix_rows()
             kc, vc = kv_cache.k[layer_idx], kv_cache.v[layer_idx]
         else:
             cache_len = 0
@@ -63,7 +63,7 @@ class TPQwen2Attention(nn.Module):
         K.rope_kv_write(y, q, kc, vc, cos, sin, pos, hq, hkv, cache_len)
         if kv_cache is not None and kv_cache.prefix is not None:
             pre = kv_cache.prefix
-            out = K.shared_prefix_attention(q, pre.k[layer_idx], pre.v[layer_idx], kc, vc, pre.seq_len, cache_len)
+            out = K.shared_prefix_attention(q, pre.k[layer_idx], pre.v[layer_idx], kc, vc, prefix_rows, cache_len)
         else:
             out = K.attention(q, kc, vc, cache_len)
         return self.o_proj(out)

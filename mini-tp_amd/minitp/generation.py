@@ -87,7 +87,7 @@ class GenerationState:
         device = input_ids.device
         self.out_ids = torch.empty(b, self.total, dtype=torch.long, device=device)
         self.out_ids[:, :t] = input_ids
-        self._start = self._prefix_rows()  # positions continue a shared prefix
+        self._start = self.kv.prefix_rows()  # positions continue a shared prefix
         self.positions_buf = torch.arange(self._start, self._start + self.total, device=device)  # the only arange
         self.cursor = t
         self.finished: torch.Tensor | None = None
@@ -100,8 +100,11 @@ class GenerationState:
         self._eos_host: torch.Tensor | None = None  # pinned stop column (0 = running)
         self._eos_host_dev: int | None = None
 
-    def _prefix_rows(self) -> int:
-        return self.kv.prefix.seq_len if self.kv.prefix is not None else 0
+    def _check_prefix(self) -> None:
+        """The positions in the buffer go on from the prefix that the cache had."""
+        rows = self.kv.prefix_rows()
+        if rows != self._start:
+            raise ValueError(f"GenerationState: built for {self._start} prefix rows, the cache has {rows}")
 
     def _enable_device_eos(self, eos: int) -> None:
         """Keep generate_greedy's finished mask and stop test on the device."""
@@ -132,8 +135,7 @@ class GenerationState:
 
     def prefill(self) -> torch.Tensor:
         """Prompt forward; positions come from the buffer (0..T-1)."""
-        if self._prefix_rows() != self._start:
-            raise ValueError(f"GenerationState: built for {self._start} prefix rows, the cache has {self._prefix_rows()}")
+        self._check_prefix()
         positions = self.positions_buf[: self.prompt_len]
         ids = self.out_ids[:, : self.prompt_len]
         if not self._native:
@@ -161,6 +163,7 @@ class GenerationState:
 
     def decode_step(self, tok: torch.Tensor, pos: torch.Tensor) -> torch.Tensor:
         if not self._native:
+            self._check_prefix()
             return self.model(tok.unsqueeze(-1), positions=pos.unsqueeze(-1), kv_cache=self.kv)
         b = tok.shape[0]
         if pos.data_ptr() == self.positions_buf.data_ptr() + (self.cursor - 1) * 8:

@@ -36,17 +36,31 @@ class KVCache:
             raise ValueError(f"init must be 'empty' or 'zeros', got {init!r}")
         self.max_seq_len = max_seq_len
         self.capacity = cache_capacity(max_seq_len)
-        self.seq_len = 0
+        self.prefix: KVCache | None = None  # rows that groups of this cache's batch rows share (share_prefix)
+        self.is_prefix = False
+        self._rewrites = 0  # times that rows [0, seq_len) may have become others
+        self._behind: tuple[int, int] | None = None  # the prefix's rows and rewrites under the rows written here
+        self._seq_len = 0
         self.num_layers = num_layers
         shape = (num_layers, batch_size, kv_heads_local, self.capacity, head_dim)
         self.k_buf = torch.empty(shape, dtype=dtype, device=device)
         self.v_buf = torch.empty(shape, dtype=dtype, device=device)
         if init == "zeros":
             self._fill(0.0)
-        self.prefix: KVCache | None = None  # rows that groups of this cache's batch rows share (share_prefix)
-        self.is_prefix = False
         self.k = [t[:, :, :max_seq_len] for t in self.k_buf.unbind(0)]
         self.v = [t[:, :, :max_seq_len] for t in self.v_buf.unbind(0)]
+
+    @property
+    def seq_len(self) -> int:
+        return self._seq_len
+
+    @seq_len.setter
+    def seq_len(self, rows: int) -> None:
+        if rows < self._seq_len:
+            self._rewrites += 1
+        if self._seq_len == 0 and self.prefix is not None:
+            self._behind = self.prefix._seq_len, self.prefix._rewrites
+        self._seq_len = rows
 
     def _fill(self, value: float) -> None:
         for buf in (self.k_buf, self.v_buf):
@@ -73,7 +87,8 @@ class KVCache:
         batch) consecutive rows here continues one row of ``prefix``, whose
         rows [0, prefix.seq_len) are kept once and attended by all of them (no
         counterpart in the reference, whose caches hold a prompt per row). This
-        cache must be empty: its rows' positions go on from the prefix's."""
+        cache must be empty: its rows' positions go on from the prefix's, and
+        once there are some the prefix has to stay as it is (prefix_rows)."""
         mine, shared = self.k_buf.shape, prefix.k_buf.shape
         if prefix.prefix is not None or prefix is self or self.is_prefix:
             raise ValueError("a shared prefix cannot have a prefix of its own")
@@ -88,11 +103,25 @@ class KVCache:
         self.prefix = prefix
         prefix.is_prefix = True
 
+    def prefix_rows(self) -> int:
+        """Rows of the shared prefix in front of this cache, 0 without one. A
+        prefix that was continued, cut, filled anew or reordered since the first
+        row was written here is refused: this cache's rows have positions, and
+        hold keys and values, that go on from the rows that it had then."""
+        pre = self.prefix
+        if pre is None:
+            return 0
+        if self._seq_len > 0 and self._behind != (pre._seq_len, pre._rewrites):
+            raise ValueError(f"shared prefix: the cache's {self._seq_len} rows were written behind {self._behind[0]} prefix "
+                             f"rows, and the prefix, now of {pre._seq_len} rows, has changed since")
+        return pre._seq_len
+
     def reorder(self, parents: torch.Tensor) -> None:
         """The written rows follow their beams, in place: batch row b of every
         layer takes the rows of batch row parents[b] (``kernels.kv_reorder``;
         parents [G, W] int64, beams of a group). A shared prefix stays."""
         K.kv_reorder(self.k_buf, self.v_buf, parents, self.seq_len)
+        self._rewrites += 1
 
     def advance(self, tokens: int) -> None:
         self.seq_len += tokens

@@ -218,6 +218,7 @@ class TPQwen2ForCausalLM(nn.Module):
             a = self.model.layers[0].self_attn
             kv = KVCache(self.cfg.num_hidden_layers, b, a.kv_heads_local, self.cfg.head_dim, t, prog.dtype, dev)
         kv.check_room(t)
+        prefix_rows = kv.prefix_rows()
         all_rows = t > 1 and not last_only
         logits = torch.empty(b, t if all_rows else 1, self.cfg.vocab_size, dtype=prog.dtype, device=dev)
         ws = prog.forward_ws(b * t, b, kv.capacity)
@@ -233,9 +234,9 @@ class TPQwen2ForCausalLM(nn.Module):
             prog.check_cache(pre, groups)
             a = self.model.layers[0].self_attn
             need = K.shared_prefix_bytes(N.dtype_code(prog.dtype), b, groups, t, a.q_heads_local, a.kv_heads_local,
-                                         self.cfg.head_dim, pre.seq_len, kv.seq_len)
+                                         self.cfg.head_dim, prefix_rows, kv.seq_len)
             scratch = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-            shared = N.SharedPrefix(pre.k_buf.data_ptr(), pre.v_buf.data_ptr(), groups, pre.seq_len, pre.capacity,
+            shared = N.SharedPrefix(pre.k_buf.data_ptr(), pre.v_buf.data_ptr(), groups, prefix_rows, pre.capacity,
                                     N.ptr(scratch), need)
             N.check(N.lib().minitp_qwen2_forward_shared(prog.handle, N.stream(), ctypes.byref(step),
                                                         ctypes.byref(shared)), "qwen2_forward_shared")
@@ -285,7 +286,7 @@ class TPQwen2ForCausalLM(nn.Module):
         if positions is None:  # layer.py:99-101
             offset = kv_cache.seq_len if kv_cache is not None and t == 1 else 0
             if kv_cache is not None and kv_cache.prefix is not None:  # (no counterpart in the reference)
-                offset = kv_cache.prefix.seq_len + kv_cache.seq_len
+                offset = kv_cache.prefix_rows() + kv_cache.seq_len
             if offset + t > limit:
                 raise IndexError(f"position {offset + t - 1} out of range for RoPE table of {limit} rows")
             positions = torch.arange(offset, offset + t, device=input_ids.device)
@@ -300,6 +301,7 @@ class TPQwen2ForCausalLM(nn.Module):
             positions = torch.where(positions < 0, positions + limit, positions)
         if kv_cache is not None:
             kv_cache.check_room(t)
+            kv_cache.prefix_rows()
         if self.native_path():
             return self._native(input_ids, positions, kv_cache)
         x = self.model.embed_tokens(input_ids)

@@ -1,0 +1,121 @@
+"""Caches behind a shared prefix on the host (no GPU): what each forward takes
+as its prefix, and the calls that would attend other rows than those that the
+cache's own rows were written behind."""
+
+import pytest
+import torch
+
+from minitp.config import ModelConfig
+from minitp.distributed.context import ParallelContext
+from minitp.generation import GenerationState, make_kv_cache
+from minitp.layer import TPQwen2ForCausalLM
+
+
+def _model():
+    cfg = ModelConfig(32, 48, 1, 2, 1, 16, 64, 1e-6, 1e6, 64)
+    return TPQwen2ForCausalLM(cfg, ParallelContext(0, 0, 1, 0, 1, torch.device("cpu"), None), init_weights=False)
+
+
+def _behind(model, rows=5, batch=2, prefixes=1):
+    """(a cache behind a prefix of `rows` rows, the prefix)."""
+    pre, kv = make_kv_cache(model, prefixes, 16), make_kv_cache(model, batch, 16)
+    pre.advance(rows)
+    kv.share_prefix(pre)
+    return kv, pre
+
+
+def _grow(pre):
+    pre.advance(4)
+
+
+def _cut(pre):
+    pre.seq_len = 3
+
+
+def _refill(pre):
+    rows = pre.seq_len
+    pre.seq_len = 0
+    pre.advance(rows)
+
+
+def _permute(pre, monkeypatch):
+    from minitp import kernels as K
+
+    monkeypatch.setattr(K, "kv_reorder", lambda *a: None)
+    pre.reorder(torch.zeros(1, 1, dtype=torch.long))
+
+
+@pytest.mark.parametrize("change", ["grow", "cut", "refill", "permute"])
+def test_a_prefix_that_changes_under_written_rows_is_refused(change, monkeypatch):
+    """Rows behind a prefix hold positions that go on from it: once there are
+    some, a prefix of another length or with other rows is refused by every
+    way to a forward, and nothing is written."""
+    model = _model()
+    seen = []
+    monkeypatch.setattr("minitp._native.require_gpu", lambda *a, **k: None)
+    monkeypatch.setattr(model, "_native", lambda ids, pos, kv, **k: seen.append(pos.tolist()) or kv.advance(ids.shape[1]))
+    ids = torch.zeros(2, 3, dtype=torch.long)
+    kv, pre = _behind(model)
+    state = GenerationState(model, ids, 4, kv=kv)
+    state.prefill()
+    assert seen == [[5, 6, 7]] and kv.seq_len == 3
+    pos = state.append(ids[:, 0])
+    if change == "permute":
+        _permute(pre, monkeypatch)
+    else:
+        {"grow": _grow, "cut": _cut, "refill": _refill}[change](pre)
+    for call in (lambda: state.decode_step(ids[:, 0], pos), lambda: model(ids[:, :1], kv_cache=kv),
+                 lambda: model(ids[:, :1], positions=torch.tensor([8]), kv_cache=kv),
+                 lambda: GenerationState(model, ids, 4, kv=kv), kv.prefix_rows):
+        with pytest.raises(ValueError, match="prefix"):
+            call()
+    model.use_rotary_cache = False  # (the modules one by one)
+    with pytest.raises(ValueError, match="prefix"):
+        model(ids[:, :1], kv_cache=kv)
+    assert kv.seq_len == 3 and len(seen) == 1
+
+
+def test_attention_alone_refuses_a_changed_prefix(monkeypatch):
+    """The attention module is a way of its own to a prefix's rows."""
+    from minitp import kernels as K
+
+    model = _model()
+    attn = model.model.layers[0].self_attn
+    monkeypatch.setattr(attn.qkv_proj, "project", lambda x, fused: x)
+    monkeypatch.setattr(K, "rope_kv_write", lambda *a: None)
+    taken = []
+    monkeypatch.setattr(K, "shared_prefix_attention", lambda *a: taken.append(a[5:]) or torch.zeros(2, 1, 32))
+    monkeypatch.setattr(attn.o_proj, "forward", lambda x: x)
+    kv, pre = _behind(model)
+    x, pos = torch.zeros(2, 1, 32), torch.tensor([5])
+    attn(x, pos, kv, 0)
+    kv.advance(1)
+    attn(x, pos, kv, 0)
+    pre.advance(2)
+    with pytest.raises(ValueError, match="prefix"):
+        attn(x, pos, kv, 0)
+    assert taken == [(5, 0), (5, 1)]
+
+
+def test_an_empty_cache_takes_its_prefix_as_it_is():
+    """Until a row is written the prefix may be filled, and after the cache is
+    emptied it may be another one."""
+    model = _model()
+    pre, kv = make_kv_cache(model, 1, 16), make_kv_cache(model, 2, 16)
+    kv.share_prefix(pre)
+    assert kv.prefix_rows() == 0
+    pre.advance(6)
+    assert kv.prefix_rows() == 6
+    kv.advance(2)
+    assert kv.prefix_rows() == 6
+    pre.advance(1)
+    with pytest.raises(ValueError, match="6 prefix rows"):
+        kv.prefix_rows()
+    kv.seq_len = 0
+    assert kv.prefix_rows() == 7
+    kv.advance(1)
+    assert kv.prefix_rows() == 7
+    kv.seq_len = 2  # (more rows, or fewer, of its own: the prefix is the same)
+    kv.seq_len = 1
+    assert kv.prefix_rows() == 7
+    assert make_kv_cache(model, 2, 8).prefix_rows() == 0
