@@ -119,7 +119,12 @@ class KVCache:
     def reorder(self, parents: torch.Tensor) -> None:
         """The written rows follow their beams, in place: batch row b of every
         layer takes the rows of batch row parents[b] (``kernels.kv_reorder``;
-        parents [G, W] int64, beams of a group). A shared prefix stays."""
+        parents [G, W] int64, beams of a group). A shared prefix stays, so
+        the beams of a group have to share one."""
+        if self.prefix is not None and parents.dim() == 2 and parents.shape[1] > 0:
+            rows = self.k_buf.shape[1] // self.prefix.k_buf.shape[1]
+            if rows % parents.shape[1] != 0:
+                raise ValueError(f"reorder: groups of {parents.shape[1]} beams span several prefixes, of {rows} rows each")
         K.kv_reorder(self.k_buf, self.v_buf, parents, self.seq_len)
         self._rewrites += 1
 

@@ -119,3 +119,26 @@ def test_an_empty_cache_takes_its_prefix_as_it_is():
     kv.seq_len = 1
     assert kv.prefix_rows() == 7
     assert make_kv_cache(model, 2, 8).prefix_rows() == 0
+
+
+@pytest.mark.parametrize("prefixes,groups", [(2, 1), (2, 3), (3, 2), (3, 1), (6, 3)])
+def test_reordering_over_several_prefixes_is_refused(prefixes, groups, monkeypatch):
+    """Groups of beams that span rows of two prefixes: a row would go on behind
+    a prefix that it was not computed behind."""
+    from minitp import kernels as K
+
+    moved = []
+    monkeypatch.setattr(K, "kv_reorder", lambda *a: moved.append(a[2:]))
+    model = _model()
+    kv, _ = _behind(model, batch=6, prefixes=prefixes)
+    kv.advance(2)
+    with pytest.raises(ValueError, match="prefix"):
+        kv.reorder(torch.zeros(groups, 6 // groups, dtype=torch.long))
+    assert not moved
+    for fits in (prefixes, 6):
+        parents = torch.arange(6).view(fits, -1)
+        kv.reorder(parents)
+        assert moved.pop() == (parents, 2)
+    free = make_kv_cache(model, 6, 8)
+    free.reorder(torch.zeros(groups, 6 // groups, dtype=torch.long))  # (no prefix: any groups)
+    assert moved
