@@ -352,10 +352,13 @@ int minitp_qwen2_create(const minitp_qwen2_config* cfg, const minitp_qwen2_weigh
                         void** handle);
 int minitp_qwen2_destroy(void* handle);
 /* Workspace for forwards of up to max_tokens = B*T rows, batch B, cache S.
- * A workspace must be zero-filled once before its first use (its first
- * bytes hold the step state: the error word and the arrival words of the
- * split products, which every launch leaves at zero) and then only be used
- * with this handle. */
+ * The first MINITP_QWEN2_STATE_BYTES of a workspace must be zero-filled once
+ * before its first use (they hold the step state: the error word and the
+ * arrival words of the split products, which every launch leaves at zero);
+ * the rest needs no initial value. It may then only be used with this
+ * handle, and by one forward at a time: forwards on two streams, and graphs
+ * that a caller captures, need a workspace each. */
+#define MINITP_QWEN2_STATE_BYTES 16384
 int64_t minitp_qwen2_workspace_bytes(void* handle, int64_t max_tokens, int64_t batch,
                                      int64_t max_seq);
 /* GenerationState.prefill / TPQwen2ForCausalLM.forward (generation.py:112-117,

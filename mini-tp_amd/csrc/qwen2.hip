@@ -164,6 +164,8 @@ struct Qwen2Program {
   int q_rows() const { return c.heads * c.head_dim; }
   const void* L(int layer, int which) const { return lw[(size_t)layer * MINITP_W_PER_LAYER + which]; }
 
+  static_assert(sizeof(StepState) <= MINITP_QWEN2_STATE_BYTES, "what a workspace's user zero-fills");
+
   Ws layout(void* base, int64_t M, int64_t B, int64_t S) const {
     Ws w{};
     char* p = (char*)base;

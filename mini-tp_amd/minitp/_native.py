@@ -21,6 +21,7 @@ OK, ERR_ARG, ERR_HIP, ERR_OVERFLOW, ERR_RANGE, ERR_UNSUPPORTED, ERR_DIVISIBLE = 
 F32, BF16 = 0, 1
 EPI_NONE, EPI_RESID, EPI_SWIGLU = 0, 1, 2
 W_PER_LAYER = 7
+QWEN2_STATE_BYTES = 16384  # MINITP_QWEN2_STATE_BYTES
 
 _DTYPES = {torch.float32: F32, torch.bfloat16: BF16}
 

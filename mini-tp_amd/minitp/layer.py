@@ -93,7 +93,7 @@ class _Program:
         self.cfg = c
         self.device = head[0].device
         self.dtype = head[0].dtype
-        self.fwd_ws: torch.Tensor | None = None
+        self.fwd_ws: dict[int, torch.Tensor] = {}  # by stream
         self.decode_ws: dict[tuple[int, int], torch.Tensor] = {}
 
     def decode_path_name(self, batch: int = 1) -> str:
@@ -116,8 +116,10 @@ class _Program:
     def check_decode(self) -> None:
         """Synchronise and raise IndexError if a forward on any of this
         program's workspaces ran at a position outside the RoPE table (the
-        sticky error word of the step state; cleared by the check)."""
-        for ws in list(self.decode_ws.values()) + ([self.fwd_ws] if self.fwd_ws is not None else []):
+        sticky error word of the step state; cleared by the check). Captured
+        forwards have workspaces of their graphs and are not seen here."""
+        torch.cuda.synchronize(self.device)  # (the workspaces are used on several streams)
+        for ws in list(self.decode_ws.values()) + list(self.fwd_ws.values()):
             N.check(N.lib().minitp_qwen2_decode_check(self.handle, N.stream(), ws.data_ptr()), "qwen2_decode")
 
     def valid_for(self, model: "TPQwen2ForCausalLM") -> bool:
@@ -128,10 +130,20 @@ class _Program:
         return N.lib().minitp_qwen2_workspace_bytes(self.handle, tokens, batch, max_seq)
 
     def forward_ws(self, tokens: int, batch: int, max_seq: int) -> torch.Tensor:
+        """Scratch of one direct forward. A stream's forwards follow each other
+        and share a buffer that grows with them; those of two streams may run
+        at once. A captured forward is replayed whenever its graph is, so its
+        scratch is the graph's own memory."""
         need = self.workspace_bytes(tokens, batch, max_seq)
-        if self.fwd_ws is None or self.fwd_ws.numel() < need:
-            self.fwd_ws = torch.zeros(need, dtype=torch.uint8, device=self.device)
-        return self.fwd_ws
+        if torch.cuda.is_current_stream_capturing():
+            ws = torch.empty(need, dtype=torch.uint8, device=self.device)
+            ws[: N.QWEN2_STATE_BYTES].zero_()
+            return ws
+        stream = N.stream()
+        ws = self.fwd_ws.get(stream)
+        if ws is None or ws.numel() < need:
+            ws = self.fwd_ws[stream] = torch.zeros(need, dtype=torch.uint8, device=self.device)
+        return ws
 
     def decode_workspace(self, batch: int, max_seq: int) -> torch.Tensor:
         # One buffer per (batch, max_seq) for the life of the program: the

@@ -1,0 +1,119 @@
+"""Steps behind a shared prefix that run beside other work of the same model:
+on two streams at once, and captured, with larger forwards between replays."""
+
+import pytest
+import torch
+
+from tests.test_gpu_beam_search import _pair
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def _busy(streams):
+    """Work in front of what is queued next, so that the streams' queues fill
+    before either begins."""
+    a = torch.randn(8192, 8192, device=DEV, dtype=torch.bfloat16)
+    torch.cuda.synchronize()
+    for s in streams:
+        with torch.cuda.stream(s):
+            for _ in range(30):
+                a @ a
+    return a
+
+
+def _prefix(model, rows=200, seed=9):
+    from minitp.generation import make_kv_cache
+
+    ids = torch.randint(0, 151936, (2, rows), generator=torch.Generator().manual_seed(seed)).to(DEV)
+    pre = make_kv_cache(model, 2, 256)
+    model(ids, kv_cache=pre)
+    return pre
+
+
+def _behind(model, pre, first):
+    """A cache of six rows behind `pre` that holds one row of its own."""
+    from minitp.generation import make_kv_cache
+
+    kv = make_kv_cache(model, 6, 8)
+    kv.share_prefix(pre)
+    model(first, kv_cache=kv)
+    return kv
+
+
+def _tokens(count, seed):
+    g = torch.Generator().manual_seed(seed)
+    return [torch.randint(0, 151936, (6, 1), generator=g).to(DEV) for _ in range(count)]
+
+
+def test_two_beam_searches_at_once():
+    from minitp.generation import generate_beam
+
+    model, _ = _pair("qwen2.5-0.5b", torch.bfloat16)
+    g = torch.Generator().manual_seed(4)
+    prompts = [torch.randint(0, 151936, (2, t), generator=g).to(DEV) for t in (40, 57)]
+    want = [generate_beam(model, p, 8, 4) for p in prompts]
+    streams = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(2):
+        held = _busy(streams)
+        got = []
+        for s, p in zip(streams, prompts):
+            with torch.cuda.stream(s):
+                got.append(generate_beam(model, p, 8, 4))
+        torch.cuda.synchronize()
+        del held
+        for (ids, scores), (i, s) in zip(got, want):
+            assert torch.equal(ids, i) and torch.equal(scores, s)
+
+
+def test_a_captured_step_beside_larger_forwards():
+    """The forwards between the replays outgrow every workspace, and memory
+    that was given back is taken and filled."""
+    model, _ = _pair("qwen2.5-0.5b", torch.bfloat16)
+    pre, toks = _prefix(model), _tokens(4, 2)
+    with torch.inference_mode():
+        want = [model(t, kv_cache=_behind(model, pre, toks[3])) for t in toks[:3]]
+        kv, tok = _behind(model, pre, toks[3]), toks[0].clone()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = model(tok, kv_cache=kv)
+        for i in range(3):
+            long = torch.randint(0, 151936, (8, 100 + 70 * i), device=DEV)
+            model(long)
+            taken = [torch.full((1 << 22,), float("nan"), device=DEV) for _ in range(16)]
+            tok.copy_(toks[i])
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want[i])
+            assert all(torch.isnan(x).all() for x in taken)
+
+
+def test_two_captured_steps_at_once():
+    """Each graph has its scratch; replays on two streams and an eager step on
+    a third do not meet."""
+    model, _ = _pair("qwen2.5-0.5b", torch.bfloat16)
+    pre, toks = _prefix(model), _tokens(4, 6)
+    with torch.inference_mode():
+        want = [model(t, kv_cache=_behind(model, pre, toks[3])) for t in toks[:3]]
+        graphs, outs = [], []
+        caches = [_behind(model, pre, toks[3]) for _ in range(3)]
+        for i in range(2):
+            graphs.append(torch.cuda.CUDAGraph())
+            with torch.cuda.graph(graphs[i]):
+                outs.append(model(toks[i], kv_cache=caches[i]))
+        streams = [torch.cuda.Stream() for _ in range(3)]
+        for _ in range(3):
+            held = _busy(streams)
+            for i in range(2):
+                with torch.cuda.stream(streams[i]):
+                    for _ in range(4):
+                        graphs[i].replay()
+            with torch.cuda.stream(streams[2]):
+                eager = []
+                for _ in range(4):
+                    caches[2].seq_len = 1
+                    eager.append(model(toks[2], kv_cache=caches[2]))
+            torch.cuda.synchronize()
+            del held
+            assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
+            assert all(torch.equal(e, want[2]) for e in eager)

@@ -142,3 +142,47 @@ def test_reordering_over_several_prefixes_is_refused(prefixes, groups, monkeypat
     free = make_kv_cache(model, 6, 8)
     free.reorder(torch.zeros(groups, 6 // groups, dtype=torch.long))  # (no prefix: any groups)
     assert moved
+
+
+def test_forwards_have_a_workspace_a_stream_and_captured_ones_their_own(monkeypatch):
+    """Forwards of one program on two streams may run at once. A captured one is
+    replayed later, beside others: its workspace is memory of its graph (from
+    the allocator, within the capture), not the one that the next larger
+    forward replaces."""
+    from minitp import _native as N
+    from minitp.layer import _Program
+
+    now = {"stream": 11, "capturing": False}
+    monkeypatch.setattr(N, "stream", lambda: now["stream"])
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: now["capturing"])
+    prog = _Program.__new__(_Program)
+    prog.device, prog.fwd_ws, prog.decode_ws = torch.device("cpu"), {}, {}
+    prog.workspace_bytes = lambda tokens, batch, max_seq: 40000 + tokens
+    one = prog.forward_ws(4, 1, 8)
+    assert (one == 0).all() and prog.forward_ws(3, 1, 8) is one
+    now["stream"] = 22
+    two = prog.forward_ws(4, 1, 8)
+    assert two.data_ptr() != one.data_ptr() and prog.forward_ws(4, 1, 8) is two
+    now["stream"] = 11
+    more = prog.forward_ws(90, 1, 8)
+    assert more.numel() >= 40090 and (more == 0).all() and prog.forward_ws(4, 1, 8) is more
+    now["stream"] = 22
+    assert prog.forward_ws(4, 1, 8) is two
+    now["capturing"] = True
+    kept = [x.data_ptr() for x in prog.fwd_ws.values()]
+    first, second = prog.forward_ws(4, 1, 8), prog.forward_ws(4, 1, 8)
+    assert len({first.data_ptr(), second.data_ptr(), *kept}) == 4
+    assert (first[: N.QWEN2_STATE_BYTES] == 0).all() and first.numel() >= 40004
+    now["capturing"] = False
+    assert prog.forward_ws(4, 1, 8) is two and [x.data_ptr() for x in prog.fwd_ws.values()] == kept
+
+
+def test_the_step_state_size_is_the_headers():
+    import os
+    import re
+
+    from minitp import _native as N
+    from tests.conftest import ROOT
+
+    header = open(os.path.join(ROOT, "include", "minitp.h")).read()
+    assert N.QWEN2_STATE_BYTES == int(re.search(r"#define MINITP_QWEN2_STATE_BYTES (\d+)", header).group(1))
