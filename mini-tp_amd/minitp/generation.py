@@ -134,16 +134,22 @@ class GenerationState:
             raise IndexError(f"position {last} out of range for RoPE table of {limit} rows")
 
     def prefill(self) -> torch.Tensor:
-        """Prompt forward; positions come from the buffer (0..T-1)."""
+        """Prompt forward; positions come from the buffer (0..T-1, behind a
+        shared prefix the T after it)."""
         self._check_prefix()
         positions = self.positions_buf[: self.prompt_len]
         ids = self.out_ids[:, : self.prompt_len]
+        last_only = self.prefill_logits == "last"
         if not self._native:
-            return self.model(ids, positions=positions, kv_cache=self.kv)
+            if last_only and self.kv.prefix is not None and self.model.native_path() and ids.is_cuda:
+                self._check_position(self._start + self.prompt_len - 1)
+                return self.model._native(ids, positions, self.kv, last_only=True)
+            logits = self.model(ids, positions=positions, kv_cache=self.kv)
+            return logits[:, -1:] if last_only else logits
         self._check_position(self.prompt_len - 1)
         col = self._next_column()
         logits = self.model._native(ids, positions, self.kv, next_tok=col, eos=self._eos_args(),
-                                    last_only=self.prefill_logits == "last")
+                                    last_only=last_only)
         self._last_logits, self._last_tok = logits, col
         return logits
 

@@ -117,3 +117,54 @@ def test_two_captured_steps_at_once():
             del held
             assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
             assert all(torch.equal(e, want[2]) for e in eager)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("t", [1, 9, 40])
+def test_the_last_positions_logits_behind_a_prefix(t, dtype):
+    """prefill_logits="last" gives [B, 1, V], the last row of the whole form,
+    and never holds the others; greedy generation uses it."""
+    from minitp.generation import GenerationState, generate_greedy, make_kv_cache
+
+    model, _ = _pair("qwen2.5-0.5b", dtype)
+    pre = _prefix(model, 70)
+    asks = torch.randint(0, 151936, (6, t), generator=torch.Generator().manual_seed(t)).to(DEV)
+
+    def behind():
+        kv = make_kv_cache(model, 6, t + 4)
+        kv.share_prefix(pre)
+        return kv
+
+    got, last_kv, all_kv = {}, behind(), behind()
+    for form, kv in (("all", all_kv), ("last", last_kv)):
+        st = GenerationState(model, asks, 4, kv=kv, prefill_logits=form)
+        st.prefill()  # (workspaces are there)
+        kv.seq_len = 0
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        start = torch.cuda.memory_allocated()
+        got[form] = st.prefill()
+        peak = torch.cuda.max_memory_allocated() - start
+        assert got[form].shape == (6, t if form == "all" else 1, 151936) and kv.seq_len == t
+    if t >= 9:
+        assert peak < got["all"].numel() * got["all"].element_size() / 2
+    # two forms of one forward, each within the path's own bar of the oracle's
+    # logits (bf16 0.5, fp32 1e-3)
+    bar = 0.5 if dtype == torch.bfloat16 else 1e-3
+    assert (got["last"].float() - got["all"][:, -1:].float()).abs().max() <= 2 * bar
+    assert torch.equal(last_kv.k_buf[:, :, :, :t], all_kv.k_buf[:, :, :, :t])
+    ids = generate_greedy(model, asks, 4, kv=behind())
+    assert torch.equal(ids[:, t].cpu(), got["last"][:, 0].float().cpu().argmax(-1))
+
+
+def test_positions_past_the_table_behind_a_prefix():
+    from minitp.generation import GenerationState, make_kv_cache
+
+    model, _ = _pair("qwen2.5-0.5b", torch.bfloat16)
+    pre = _prefix(model, 250)  # (of 256 positions)
+    for form in ("all", "last"):
+        kv = make_kv_cache(model, 2, 16)
+        kv.share_prefix(pre)
+        with pytest.raises(IndexError, match="position 256"):
+            GenerationState(model, torch.zeros(2, 7, dtype=torch.long, device=DEV), 4, kv=kv, prefill_logits=form).prefill()
+        assert kv.seq_len == 0

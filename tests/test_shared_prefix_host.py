@@ -186,3 +186,15 @@ def test_the_step_state_size_is_the_headers():
 
     header = open(os.path.join(ROOT, "include", "minitp.h")).read()
     assert N.QWEN2_STATE_BYTES == int(re.search(r"#define MINITP_QWEN2_STATE_BYTES (\d+)", header).group(1))
+
+
+@pytest.mark.parametrize("prefixed", [False, True])
+def test_the_last_positions_logits_alone_on_every_path(prefixed, monkeypatch):
+    """prefill_logits="last" is [B, 1, V] whatever runs the forward."""
+    model = _model()
+    every = torch.arange(2 * 3 * 64, dtype=torch.float32).view(2, 3, 64)
+    monkeypatch.setattr(model, "forward", lambda ids, positions, kv_cache: every)
+    ids = torch.zeros(2, 3, dtype=torch.long)
+    for form, want in (("last", every[:, -1:]), ("all", every)):
+        kv = _behind(model)[0] if prefixed else make_kv_cache(model, 2, 8)
+        assert torch.equal(GenerationState(model, ids, 4, kv=kv, prefill_logits=form).prefill(), want)
