@@ -201,8 +201,11 @@ int minitp_attention(void* stream, int dtype, const void* q, const void* k_cache
  * read. prefix_len 0 serves rows without a prefix (the prefix pointers may be
  * NULL). Workspace from the query below (bf16 and fp32 ask for different
  * sizes; 0 where the call needs none, -1 for a call that is refused); no
- * initial value, nothing kept in it after the call's kernels. 2^31 query rows
- * or keys and more are MINITP_ERR_UNSUPPORTED. */
+ * initial value, nothing kept in it after the call's kernels. Calls
+ * past a launch's 32-bit numbers are MINITP_ERR_UNSUPPORTED before anything is
+ * queued: 2^31 query rows or keys, 2^24 tiles of up to 128 (fp32: 64) query
+ * rows of one batch row, or group, and KV head, and, where the call needs a
+ * workspace, 2^34 / D query rows (a second launch joins the parts). */
 int64_t minitp_shared_prefix_attention_workspace_bytes(int dtype, int64_t B, int64_t G, int64_t T, int64_t Hq,
                                                        int64_t Hkv, int64_t D, int64_t prefix_len,
                                                        int64_t cache_len);

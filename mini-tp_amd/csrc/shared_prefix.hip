@@ -1091,7 +1091,8 @@ int shared_by_d(hipStream_t st, const SharedArgs& a, const Plan& p, int64_t D) {
 
 }  // namespace
 
-// Whether one launch takes the shape: 32-bit row, key and thread numbers.
+// Whether the launches take the shape: 32-bit row, key and thread numbers, of
+// the join too (a thread for four elements of the output, where parts are joined).
 int shared_prefix_check(int dtype, const SharedPrefixShape& s) {
   if (s.D != 16 && s.D != 32 && s.D != 64 && s.D != 128) {
     set_error("shared_prefix_attention: head_dim %lld not supported (16, 32, 64, 128)", (long long)s.D);
@@ -1106,7 +1107,7 @@ int shared_prefix_check(int dtype, const SharedPrefixShape& s) {
   bool fits = s.B < MOST && s.Hq < MOST && s.B * s.T < MOST && s.B * s.T * s.Hq < MOST - 256;
   if (fits && s.B * s.T > 0) {
     const Plan p = shared_plan(dtype, s.D, s.B, s.G, s.T, s.Hq, s.Hkv, s.P, s.C);
-    fits = p.items_p + p.items_s < (1LL << 24) - 16;
+    fits = p.items_p + p.items_s < (1LL << 24) - 16 && (p.joined || cdiv(s.B * s.T * s.Hq, 1024 / s.D) < (1LL << 24));
   }
   if (!fits) {
     set_error("shared_prefix_attention: %lld x %lld x %lld query rows are too many for one call", (long long)s.B,
