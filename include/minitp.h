@@ -233,7 +233,8 @@ int minitp_shared_prefix_attention(void* stream, int dtype, const void* q, const
  * with a score of minus infinity, marked finished. Outputs, all [G, W], which may be the
  * inputs of the same kind: tokens, parents (rows of the batch, g * W + w),
  * scores, finished (parent's, or the token is eos_token), lengths. eos_token
- * -1: none (finished must be NULL). */
+ * -1: none (finished must be NULL). 2^22 groups, and 2^24 slices of 8,192 (fp32:
+ * 4,096) logits of a beam, and more are MINITP_ERR_UNSUPPORTED. */
 int64_t minitp_beam_select_workspace_bytes(int64_t G, int64_t W, int64_t V);
 int minitp_beam_select(void* stream, int dtype, const void* logits, int64_t ld_group, int64_t ld_beam, int64_t G,
                        int64_t W, int64_t V, const float* scores, const uint8_t* finished, const int64_t* lengths,

@@ -565,7 +565,8 @@ int launch_beam_select(hipStream_t st, int dtype, const BeamSelect& b, void* wor
   }
   const int64_t rows = b.G * b.W, slices = cdiv(b.V, dtype == MINITP_F32 ? SLICE<float> : SLICE<bf16>);
   const int64_t parts = rows * slices * (SEL_T / 64);
-  if (rows * slices >= (1LL << 24)) {  // (a launch's threads are counted in 32 bits)
+  // (a launch's threads are counted in 32 bits, the second's too: a block a group)
+  if (rows * slices >= (1LL << 32) / SEL_T || b.G >= (1LL << 32) / MERGE_T) {
     set_error("beam_select: %lld rows of %lld logits are too many for one call", (long long)rows, (long long)b.V);
     return MINITP_ERR_UNSUPPORTED;
   }

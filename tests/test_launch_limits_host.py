@@ -4,7 +4,7 @@ the host, before the first kernel is queued (no GPU)."""
 import pytest
 
 from minitp import _native as N
-from tests.test_beam_host import attention
+from tests.test_beam_host import attention, select
 
 
 def _most_rows(d):
@@ -41,3 +41,11 @@ def test_rows_that_one_launch_takes_are_not_refused():
     """Without a second launch the bound is that of the query rows."""
     size = N.lib().minitp_shared_prefix_attention_workspace_bytes
     assert size(N.BF16, 1 << 17, 1, 2048, 4, 4, 128, 0, 0) == 0  # 2^30 rows, no prefix
+
+
+@pytest.mark.parametrize("dtype", [N.BF16, N.F32])
+def test_selection_of_too_many_groups(dtype):
+    """A block of 1,024 threads a group."""
+    for g in (1 << 22, (1 << 24) - 1):
+        assert select(dtype, g=g, w=1, nbytes=1 << 62) == N.ERR_UNSUPPORTED and "too many" in N.last_error()
+    assert select(dtype, g=(1 << 22) - 1, w=1, nbytes=64) == N.ERR_ARG  # (refused for its scratch alone)
