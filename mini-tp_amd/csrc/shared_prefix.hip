@@ -225,7 +225,7 @@ __device__ __forceinline__ void finish_rows(const SharedArgs& a, const Item& it,
     } else {
       const int64_t at = it.slot * a.query_rows + n;
       *(f32x4*)(a.o + at * D + d) = o;
-      if (d == 0) *(float2*)(a.ml + at * 2) = make_float2(BASE2 ? m : m * 1.4426950408889634f, l);
+      if (d == 0) *(float2*)(a.ml + at * 2) = make_float2(m, l);
     }
   }
 }
@@ -899,8 +899,9 @@ __global__ __launch_bounds__(256, 2) void shared_attn_bf16_kernel(SharedArgs a) 
     shared_rows128<D, !FEW>(a, it, lds);
 }
 
-// The slots of each query row joined (maxima in base 2); every LPR = D / 4 lanes
-// take four dims each. SG sets of lanes share a row, set j the slots j, j + SG,
+// The slots of each query row joined, by powers of the base that their maxima are
+// in (fp32 e, bf16 2: changing it would round a maximum once more, and so weigh
+// the parts by as much as 2^-24 of it); every LPR = D / 4 lanes take four dims each. SG sets of lanes share a row, set j the slots j, j + SG,
 // ...: one set a row where there are many rows or few slots. A query that saw
 // no key, in an idle row or one without any, gets zeros.
 template <typename T, int D, int SG>
@@ -917,9 +918,10 @@ __global__ __launch_bounds__(256) void shared_join_kernel(SharedArgs a) {
   const bool idle = a.clens != nullptr && own_len(a, (int)((uint32_t)row / (uint32_t)(a.Hq * a.T))) < 0;
   float m = -__builtin_inff(), l = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  auto power = [](float x) { return sizeof(T) == 2 ? __builtin_amdgcn_exp2f(x) : expf(x); };
   auto add = [&](float ms, float ls, const f32x4& os, float mn) {
     if (ms == -__builtin_inff()) return;  // the split saw no key
-    const float a1 = __builtin_amdgcn_exp2f(ms - mn);
+    const float a1 = power(ms - mn);
     l = fmaf(ls, a1, l);
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] = fmaf(os[e], a1, o[e]);
@@ -941,7 +943,7 @@ __global__ __launch_bounds__(256) void shared_join_kernel(SharedArgs a) {
       mn = fmaxf(mn, ml[u].x);
     }
     if (mn == -__builtin_inff()) continue;
-    const float a0 = __builtin_amdgcn_exp2f(m - mn);
+    const float a0 = power(m - mn);
     l *= a0;
     o *= a0;
 #pragma unroll
@@ -952,8 +954,8 @@ __global__ __launch_bounds__(256) void shared_join_kernel(SharedArgs a) {
     // the sets of a wave by lane exchange, then the four waves through LDS
     auto fold = [&](float mo, float lo, const f32x4& oo) {
       const float mn = fmaxf(m, mo);
-      const float a0 = m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m - mn);
-      const float a1 = mo == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(mo - mn);
+      const float a0 = m == -__builtin_inff() ? 0.f : power(m - mn);
+      const float a1 = mo == -__builtin_inff() ? 0.f : power(mo - mn);
       l = l * a0 + lo * a1;
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[e] = o[e] * a0 + oo[e] * a1;
