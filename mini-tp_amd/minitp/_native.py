@@ -170,19 +170,3 @@ def stream() -> int:
 
 def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
-
-
-# ---------------------------------------------------------------------------
-# Zeroed scratch buffers. The kernels that use completion counters leave them
-# at zero when they finish, so a buffer is zeroed once when allocated and
-# then reused; all users run on one stream in program order.
-_scratch: dict[tuple, torch.Tensor] = {}
-
-
-def scratch(device: torch.device, key: str, nbytes: int) -> torch.Tensor:
-    k = (device, key)
-    buf = _scratch.get(k)
-    if buf is None or buf.numel() < nbytes:
-        buf = torch.zeros(max(nbytes, 256), dtype=torch.uint8, device=device)
-        _scratch[k] = buf
-    return buf

@@ -305,13 +305,20 @@ def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, cac
     q = q.contiguous()
     b, t, hq, d = q.shape
     hkv, s = k_cache.shape[1], cache_rows(k_cache, v_cache)
-    out = torch.empty(b, t, hq * d, dtype=q.dtype, device=q.device)
-    nbytes = _lib().minitp_attention_workspace_bytes(b, t, hq, hkv, d, s)
-    ws = N.scratch(q.device, "attention", nbytes)
+    out = q.new_empty((b, t, hq * d))
+    nbytes = _attention_bytes(b, t, hq, hkv, d, s)
+    # from the caching allocator on the current stream: calls on other streams
+    # and captured graphs have scratch of their own
+    ws = q.new_empty((nbytes,), dtype=torch.uint8)
     N.check(_lib().minitp_attention(N.stream(), N.dtype_code(q.dtype), q.data_ptr(), k_cache.data_ptr(),
                                     v_cache.data_ptr(), out.data_ptr(), b, t, hq, hkv, d, s, cache_len, ws.data_ptr(),
-                                    ws.numel()), "attention")
+                                    nbytes), "attention")
     return out
+
+
+@functools.lru_cache(maxsize=4096)
+def _attention_bytes(*sizes: int) -> int:
+    return max(_lib().minitp_attention_workspace_bytes(*sizes), 256)
 
 
 def _one_device(what: str, *tensors: torch.Tensor | None) -> int:
@@ -508,12 +515,17 @@ def argmax(logits: torch.Tensor) -> torch.Tensor:
     x = logits if logits.stride(-1) == 1 and (logits.dim() == 1 or _rows_uniform(logits)) else logits.contiguous()
     rows = _rows(x)
     ld = x.stride(-2) if x.dim() > 1 else v
-    out = torch.empty(x.shape[:-1], dtype=torch.long, device=x.device)
-    nbytes = _lib().minitp_argmax_workspace_bytes(rows, v)
-    ws = N.scratch(x.device, "argmax", nbytes)
+    out = x.new_empty(x.shape[:-1], dtype=torch.long)
+    nbytes = _argmax_bytes(rows, v)
+    ws = x.new_empty((nbytes,), dtype=torch.uint8)  # (of this stream or graph, as attention's)
     N.check(_lib().minitp_argmax(N.stream(), N.dtype_code(x.dtype), x.data_ptr(), ld, rows, v, out.data_ptr(), 1,
-                                 ws.data_ptr(), ws.numel()), "argmax")
+                                 ws.data_ptr(), nbytes), "argmax")
     return out
+
+
+@functools.lru_cache(maxsize=4096)
+def _argmax_bytes(*sizes: int) -> int:
+    return max(_lib().minitp_argmax_workspace_bytes(*sizes), 256)
 
 
 def cast_bf16(x: torch.Tensor) -> torch.Tensor:

@@ -168,3 +168,74 @@ def test_positions_past_the_table_behind_a_prefix():
         with pytest.raises(IndexError, match="position 256"):
             GenerationState(model, torch.zeros(2, 7, dtype=torch.long, device=DEV), 4, kv=kv, prefill_logits=form).prefill()
         assert kv.seq_len == 0
+
+
+def _picks(seed):
+    """An argmax over many slices and a one-token attention over many splits."""
+    from minitp import kernels as K
+
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    logits = torch.randn(6, 151936, generator=g, device=DEV)
+    q = torch.randn(1, 1, 14, 64, generator=g, device=DEV).bfloat16()
+    kc, vc = torch.randn(2, 1, 2, 4096, 64, generator=g, device=DEV).bfloat16().unbind(0)
+    return lambda: (K.argmax(logits), K.attention(q, kc, vc, 4000))
+
+
+def test_picks_and_attention_on_two_streams_and_in_graphs():
+    """The calls of a greedy step module by module: scratch of their own, beside
+    each other and beside larger calls between the replays."""
+    from minitp import kernels as K
+
+    calls = [_picks(1), _picks(2)]
+    want = [c() for c in calls]
+    streams = torch.cuda.Stream(), torch.cuda.Stream()
+    held = _busy(streams)
+    got = [[], []]
+    for _ in range(6):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(calls[i]())
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for c in calls:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(c())
+    for n in range(3):
+        K.argmax(torch.randn(40 + 20 * n, 151936, device=DEV))
+        taken = [torch.full((1 << 18,), float("nan"), device=DEV) for _ in range(16)]
+        for s, g in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                for _ in range(4):
+                    g.replay()
+        torch.cuda.synchronize()
+        for i in range(2):
+            got[i].append(tuple(x.clone() for x in outs[i]))
+    del held, taken
+    for i in range(2):
+        assert all(torch.equal(a, b) for out in got[i] for a, b in zip(out, want[i]))
+
+
+def test_greedy_generation_behind_a_prefix_on_two_streams():
+    from minitp.generation import generate_greedy, make_kv_cache
+
+    model, _ = _pair("qwen2.5-0.5b", torch.bfloat16)
+    pre = _prefix(model, 120)
+    g = torch.Generator().manual_seed(8)
+    asks = [torch.randint(0, 151936, (6, t), generator=g).to(DEV) for t in (7, 12)]
+
+    def run(ids):
+        kv = make_kv_cache(model, 6, ids.shape[1] + 6)
+        kv.share_prefix(pre)
+        return generate_greedy(model, ids, 6, kv=kv)
+
+    want = [run(a) for a in asks]
+    streams = torch.cuda.Stream(), torch.cuda.Stream()
+    held = _busy(streams)
+    got = []
+    for s, a in zip(streams, asks):
+        with torch.cuda.stream(s):
+            got.append(run(a))
+    torch.cuda.synchronize()
+    del held
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

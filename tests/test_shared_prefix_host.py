@@ -198,3 +198,34 @@ def test_the_last_positions_logits_alone_on_every_path(prefixed, monkeypatch):
     for form, want in (("last", every[:, -1:]), ("all", every)):
         kv = _behind(model)[0] if prefixed else make_kv_cache(model, 2, 8)
         assert torch.equal(GenerationState(model, ids, 4, kv=kv, prefill_logits=form).prefill(), want)
+
+
+def test_no_operator_keeps_scratch_between_calls(monkeypatch):
+    """Scratch that calls share would be written by two streams at once, and
+    replaced under a captured call when a larger one comes."""
+    from minitp import _native as N
+    from minitp import kernels as K
+
+    class Lib:
+        def __init__(self):
+            self.took = []
+
+        def __getattr__(self, name):
+            if name.endswith("_workspace_bytes"):
+                return lambda *a: 1000
+            return lambda *a: self.took.append(a) or N.OK
+
+    def kept(*a):
+        raise AssertionError("scratch that is kept")
+
+    lib = Lib()
+    for sizes in ("_argmax_bytes", "_attention_bytes"):
+        if hasattr(K, sizes):
+            monkeypatch.setattr(K, sizes, lambda *a: 1000)
+    monkeypatch.setattr(K, "_lib", lambda: lib)
+    monkeypatch.setattr(N, "require_gpu", lambda *a, **k: None)
+    monkeypatch.setattr(N, "stream", lambda: 0)
+    monkeypatch.setattr(N, "scratch", kept, raising=False)
+    K.argmax(torch.zeros(2, 50))
+    K.attention(torch.zeros(2, 1, 4, 16), torch.zeros(2, 2, 8, 16), torch.zeros(2, 2, 8, 16), 3)
+    assert [a[-1] for a in lib.took] == [1000, 1000] and all(a[-2] % 16 == 0 for a in lib.took)
