@@ -450,10 +450,18 @@ __global__ __launch_bounds__(256, 2) void shared_attn_f32_kernel(SharedArgs a) {
 // do on the global side, so that every LDS read reaches all banks: a K read
 // takes one chunk column of 16 rows, a V read 64 bytes of four rows.
 //
+// A probability is rounded to bf16 for the second product, by at most 2^-8 of
+// itself, as much as the output's own rounding: the matrix cores take bf16
+// there, and fp32 products would run at an eighth of the rate (153 against 1,223
+// TFLOP/s of a large library product). The sums that they are divided by add
+// the unrounded ones.
+//
 // Two blocks a CU (64 KiB of LDS each at D = 128) cover each other's softmax:
-// 512 even blocks run at 1.06 PFLOP/s. Not faster: a tile's scores computed
-// before the tile in front of it is used (946 against 961 TFLOP/s), the next
-// loads issued behind the scores (-7 %) or spread over the product.
+// 512 even blocks (16 rows of 128 tokens, 32 heads, 8,192 keys) run at 1.04 to
+// 1.07 PFLOP/s. Not faster, each against the kernel as it stood then: a tile's
+// scores computed before the tile in front of it is used (946 against 961
+// TFLOP/s), the next loads issued behind the scores (-7 %) or spread over the
+// product.
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
@@ -581,7 +589,10 @@ struct Tiles {
 };
 
 // The running maximum moves only when some lane's passes it by this much (base
-// 2): until then probabilities stay below 2^8 and nothing is rescaled.
+// 2): until then probabilities stay below 2^8 and nothing is rescaled. (It is a
+// score times log2(e), rounded: off by 2^-24 of its size, which scales all of a
+// part's probabilities alike and goes out in the division. Scores of up to 2^29
+// leave that within 2^32.)
 constexpr float SLACK = 8.f;
 
 // AHEAD: a wave's second products go before other waves' work (below).
@@ -998,9 +1009,9 @@ struct Plan {
 // on the fp32 path, whose tiles take three times as long), or, where that
 // leaves a block 16 tiles and more, 448 of the 512 places that there are; the
 // own part 256 blocks of at least two tiles. Measured (us a call): 32 rows of
-// the 7B heads on 8,191 and up to 400 keys, 8 units: 16 splits 24.0, 32 22.1,
-// 48 25.3, 64 30.2; 256 rows on 32,256 and 511, 56 units: 7 splits 159.7, 8
-// 161.8, 9 176.1, 12 170.7; 8 rows x 4 of the 0.5B heads on 2,048: 8 splits
+// the 7B heads on 8,191 and up to 400 keys, 8 units: 16 splits 24.0, 32 (taken)
+// 22.1, 48 25.3, 64 30.2; 256 rows on 32,256 and 511, 56 units: 7 splits 159.7, 8
+// (taken) 161.8, 9 176.1, 12 170.7; 8 rows x 4 of the 0.5B heads on 2,048: 8 splits
 // 12.2, 16 11.6, 32 12.4; fp32, 5 rows x 3 on 777: 6 19.3, 13 12.6.
 //
 // Joined, one item a query tile over both parts and straight to the output, where
