@@ -912,9 +912,10 @@ __global__ __launch_bounds__(256, 2) void shared_attn_bf16_kernel(SharedArgs a) 
 
 // The slots of each query row joined, by powers of the base that their maxima are
 // in (fp32 e, bf16 2: changing it would round a maximum once more, and so weigh
-// the parts by as much as 2^-24 of it); every LPR = D / 4 lanes take four dims each. SG sets of lanes share a row, set j the slots j, j + SG,
-// ...: one set a row where there are many rows or few slots. A query that saw
-// no key, in an idle row or one without any, gets zeros.
+// the parts by as much as 2^-24 of it); every LPR = D / 4 lanes take four dims
+// each. SG sets of lanes share a row, set j the slots j, j + SG, ...: one set a row
+// where there are many rows or few slots. A query that saw no key, in an idle
+// row or one without any, gets zeros.
 template <typename T, int D, int SG>
 __global__ __launch_bounds__(256) void shared_join_kernel(SharedArgs a) {
   constexpr int LPR = D / 4, RB = 256 / (LPR * SG);
