@@ -216,6 +216,23 @@ int minitp_shared_prefix_attention(void* stream, int dtype, const void* q, const
                                    int64_t cache_len, const int64_t* cache_lens, void* workspace,
                                    int64_t workspace_bytes);
 
+/* Causal attention over packed sequences (texts of different lengths scored in
+ * one pass); no counterpart in the reference, whose prompts have one length
+ * (attention.py:77-105). The rows of S sequences follow each other in N rows:
+ * sequence s is rows offsets[s] .. offsets[s + 1] - 1, offsets [S + 1] a device
+ * array that does not decrease (equal neighbours: an empty sequence). Row i of
+ * a sequence that begins at row a attends rows a .. i; a row before offsets[0]
+ * or from offsets[S] on, of no sequence, gets zeros. A row's result does not
+ * depend on any other sequence's rows, whatever they hold. q [N, Hq, D] and k,
+ * v [N, Hkv, D] have strides in elements (row, head; k and v the same), whole
+ * 16-byte pieces; out is [N, Hq * D]. Head h on KV head h / (Hq/Hkv), scale
+ * 1/sqrt(D), D 16, 32, 64 or 128. Offsets out of order or range give rows of
+ * some sequence, and no access outside the arrays. MINITP_ERR_UNSUPPORTED:
+ * 2^31 rows, 2^26 (row, head) pairs, K/V rows 2^24 elements apart (fp32 2^23) and more. */
+int minitp_packed_attention(void* stream, int dtype, const void* q, int64_t q_row, int64_t q_head, const void* k,
+                            const void* v, int64_t kv_row, int64_t kv_head, void* out, int64_t N, int64_t S,
+                            int64_t Hq, int64_t Hkv, int64_t D, const int64_t* offsets);
+
 /* ---- beam search --------------------------------------------------------- */
 /* One step of beam search for G groups of W beams (1 <= W <= 32); the
  * reference decodes greedily only (generation.py:54-67). logits of beam w of
@@ -269,6 +286,27 @@ int minitp_argmax(void* stream, int dtype, const void* logits, int64_t ld, int64
 int64_t minitp_argmax_static_max_bytes(void);
 int minitp_argmax_static(void* stream, int dtype, const void* logits, int64_t ld, int64_t B, int64_t V,
                          int64_t* out, int64_t out_stride);
+
+/* ---- log-probabilities of given tokens ------------------------------------ */
+/* For each of B rows of V logits (at logits + b * ld) and its token
+ * tokens[b]; no counterpart in the reference, which only picks tokens
+ * (generation.py:54-67):
+ *   logprobs[b]  x_t - log sum_v exp(x_v)
+ *   entropy[b]   - sum_v p_v log p_v, in nats
+ *   ranks[b]     tokens in front of t: larger logits first, equal ones by the
+ *                lower token, NaN before every number (0: minitp_argmax's pick)
+ *   top_tokens, top_logprobs [B, top]: the first `top` tokens of that order
+ * (0 <= top <= 32, top <= V; 0: the two may be NULL). A row that holds a NaN or
+ * plus infinity, or nothing above minus infinity, has no distribution: its
+ * log-probabilities and entropy are NaN, ranks and top_tokens as ever. Minus
+ * infinity is a token of probability zero. A token outside [0, V) gives NaN and
+ * rank -1. fp32 outputs; sums in fp32 parts joined in fp64. Workspace from the
+ * query below (-1: a call that is refused); no initial value, nothing kept in
+ * it. MINITP_ERR_UNSUPPORTED: rows whose slices pass 2^24 blocks. */
+int64_t minitp_token_logprobs_workspace_bytes(int dtype, int64_t B, int64_t V, int64_t top);
+int minitp_token_logprobs(void* stream, int dtype, const void* logits, int64_t ld, int64_t B, int64_t V,
+                          const int64_t* tokens, int64_t top, float* logprobs, float* entropy, int64_t* ranks,
+                          int64_t* top_tokens, float* top_logprobs, void* workspace, int64_t workspace_bytes);
 
 /* ---- whole-model programs ------------------------------------------------ */
 /* TPQwen2ForCausalLM (layer.py:68-124) at tp_size == 1, run as one native

@@ -405,6 +405,26 @@ int minitp_shared_prefix_attention(void* stream, int dtype, const void* q, const
                                         cache_lens, workspace, workspace_bytes);
 }
 
+int minitp_packed_attention(void* stream, int dtype, const void* q, int64_t q_row, int64_t q_head, const void* k,
+                            const void* v, int64_t kv_row, int64_t kv_head, void* out, int64_t N, int64_t S_,
+                            int64_t Hq, int64_t Hkv, int64_t D, const int64_t* offsets) {
+  CHECK_DTYPE(dtype);
+  MINITP_CHECK_ARG(N >= 0 && S_ >= 0 && Hq > 0 && Hkv > 0 && D > 0, "packed_attention: bad shape");
+  if (Hq % Hkv != 0) {
+    set_error("local q heads %lld not divisible by local kv heads %lld", (long long)Hq, (long long)Hkv);
+    return MINITP_ERR_DIVISIBLE;
+  }
+  if (N == 0) return MINITP_OK;
+  MINITP_CHECK_ARG(q && k && v && out && offsets, "packed_attention: NULL pointer");
+  const int ve = vec_elems(dtype);
+  MINITP_CHECK_ARG(q_row >= 0 && q_head >= 0 && kv_row >= 0 && kv_head >= 0, "packed_attention: negative stride");
+  MINITP_CHECK_ARG(D % ve == 0 && q_row % ve == 0 && q_head % ve == 0 && kv_row % ve == 0 && kv_head % ve == 0 &&
+                       aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out),
+                   "packed_attention: rows must be 16-byte aligned");
+  const PackedShape s{N, S_, Hq, Hkv, D, q_row, q_head, kv_row, kv_head};
+  return launch_packed_attention(S(stream), dtype, s, q, k, v, out, offsets);
+}
+
 int64_t minitp_beam_select_workspace_bytes(int64_t G, int64_t W, int64_t V) {
   if (G < 0 || G >= (1LL << 31) || W < 1 || W > BEAM_MAX || V <= 0 || V >= (1LL << 31)) return -1;
   return beam_select_workspace_bytes(G, W, V);
@@ -461,6 +481,26 @@ int minitp_kv_reorder(void* stream, int dtype, void* k_cache, void* v_cache, int
   MINITP_CHECK_ARG(D % vec_elems(dtype) == 0 && aligned16(k_cache) && aligned16(v_cache),
                    "kv_reorder: head_dim rows must be 16-byte aligned");
   return launch_kv_reorder(S(stream), dtype, k_cache, v_cache, L, G, W, Hkv, S_, D, rows, parents);
+}
+
+int64_t minitp_token_logprobs_workspace_bytes(int dtype, int64_t B, int64_t V, int64_t top) {
+  if (!dtype_ok(dtype) || B < 0 || V <= 0 || V >= (1LL << 31) || top < 0 || top > TOP_MAX || top > V) return -1;
+  return token_logprobs_workspace_bytes(dtype, B, V, top);
+}
+
+int minitp_token_logprobs(void* stream, int dtype, const void* logits, int64_t ld, int64_t B, int64_t V,
+                          const int64_t* tokens, int64_t top, float* logprobs, float* entropy, int64_t* ranks,
+                          int64_t* top_tokens, float* top_logprobs, void* workspace, int64_t workspace_bytes) {
+  CHECK_DTYPE(dtype);
+  MINITP_CHECK_ARG(B >= 0 && V > 0 && V < (1LL << 31) && ld >= 0, "token_logprobs: B=%lld V=%lld ld=%lld",
+                   (long long)B, (long long)V, (long long)ld);
+  MINITP_CHECK_ARG(top >= 0 && top <= TOP_MAX && top <= V, "token_logprobs: the best %lld of %lld tokens (0 to %d)",
+                   (long long)top, (long long)V, TOP_MAX);
+  if (B == 0) return MINITP_OK;
+  MINITP_CHECK_ARG(logits && tokens && logprobs && entropy && ranks && (top == 0 || (top_tokens && top_logprobs)),
+                   "token_logprobs: NULL pointer");
+  const TokenLogprobs t{logits, ld, B, V, tokens, top, logprobs, entropy, ranks, top_tokens, top_logprobs};
+  return launch_token_logprobs(S(stream), dtype, t, workspace, workspace_bytes);
 }
 
 int64_t minitp_argmax_workspace_bytes(int64_t B, int64_t V) {

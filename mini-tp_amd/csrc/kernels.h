@@ -295,6 +295,30 @@ int launch_shared_prefix_attention(hipStream_t st, int dtype, const SharedPrefix
                                    const void* v_cache, void* out, const int64_t* prefix_lens,
                                    const int64_t* cache_lens, void* workspace, int64_t workspace_bytes);
 
+// packed.hip: causal attention over S sequences packed in N rows (layouts:
+// minitp_packed_attention).
+struct PackedShape {
+  int64_t N, S, Hq, Hkv, D;
+  int64_t q_row, q_head, kv_row, kv_head;  // strides in elements
+};
+int packed_check(int dtype, const PackedShape& s);  // what one launch does not take is an error
+int launch_packed_attention(hipStream_t st, int dtype, const PackedShape& s, const void* q, const void* k,
+                            const void* v, void* out, const int64_t* offsets);
+
+// logprobs.hip
+constexpr int TOP_MAX = 32;  // best tokens of a row
+struct TokenLogprobs {
+  const void* logits;
+  int64_t ld, B, V;
+  const int64_t* tokens;
+  int64_t top;
+  float *logprobs, *entropy;
+  int64_t *ranks, *top_tokens;
+  float* top_logprobs;
+};
+int64_t token_logprobs_workspace_bytes(int dtype, int64_t B, int64_t V, int64_t top);  // -1: refused
+int launch_token_logprobs(hipStream_t st, int dtype, const TokenLogprobs& t, void* workspace, int64_t workspace_bytes);
+
 // beam.hip
 constexpr int BEAM_MAX = 32;  // beams of a group
 struct BeamSelect {

@@ -62,6 +62,10 @@ SIGNATURES = {
     "minitp_shared_prefix_attention_workspace_bytes": (_i64, [_int, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64]),
     "minitp_shared_prefix_attention": (_int, [_vp, _int, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64,
                                               _i64, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64]),
+    "minitp_packed_attention": (_int, [_vp, _int, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _i64,
+                                       _i64, _vp]),
+    "minitp_token_logprobs_workspace_bytes": (_i64, [_int, _i64, _i64, _i64]),
+    "minitp_token_logprobs": (_int, [_vp, _int, _vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _i64]),
     "minitp_beam_select_workspace_bytes": (_i64, [_i64, _i64, _i64]),
     "minitp_beam_select": (_int, [_vp, _int, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _f64, _vp, _vp,
                                   _vp, _vp, _vp, _vp, _i64]),

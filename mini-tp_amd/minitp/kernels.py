@@ -409,6 +409,116 @@ def shared_prefix_bytes(*sizes: int) -> int:
     return max(_lib().minitp_shared_prefix_attention_workspace_bytes(*sizes), 0)
 
 
+def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
+    """Causal attention over packed sequences: q [N, Hq, D], k and v
+    [N, Hkv, D] -> [N, Hq * D].
+
+    The sequences' rows follow each other, without padding between them:
+    sequence s is rows ``offsets[s]`` .. ``offsets[s + 1]`` - 1 (``offsets``
+    [S + 1], whole numbers on the device that do not decrease; an empty
+    sequence repeats one). Each row attends the rows of its sequence up to
+    itself; rows of no sequence (before the first offset, from the last on)
+    get zeros. Views with strides are taken as they are where a row of a head
+    is contiguous: the column slices of a packed [N, (Hq + 2 Hkv) * D]
+    projection, or K and V kept by heads."""
+    what = "packed_attention"
+    dev = _one_device(what, q, k, v, offsets)
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return packed_attention(q, k, v, offsets)
+    if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]:
+        raise ValueError(f"{what}: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}, expected [N, Hq, D] and "
+                         "[N, Hkv, D]")
+    if offsets.dim() != 1 or offsets.numel() < 1:
+        raise ValueError(f"{what}: offsets {tuple(offsets.shape)}, expected [sequences + 1]")
+    dtype, (n, hq, d), hkv = q.dtype, q.shape, k.shape[1]
+    if k.dtype != dtype or v.dtype != dtype:
+        raise TypeError(f"{what}: dtype mismatch q={dtype} k={k.dtype} v={v.dtype}")
+    dt = N.dtype_code(dtype)
+    offsets = _lens(what, offsets, offsets.numel())
+    q, q_row, q_head = _head_rows(q)
+    k, kv_row, kv_head = _head_rows(k)
+    v, v_row, v_head = _head_rows(v)
+    if (v_row, v_head) != (kv_row, kv_head):
+        k, v = k.contiguous(), v.contiguous()
+        kv_row, kv_head = hkv * d, d
+    out = q.new_empty((n, hq * d))
+    N.check(_lib().minitp_packed_attention(N.stream(), dt, q.data_ptr(), q_row, q_head, k.data_ptr(), v.data_ptr(),
+                                           kv_row, kv_head, out.data_ptr(), n, offsets.numel() - 1, hq, hkv, d,
+                                           offsets.data_ptr()), what)
+    return out
+
+
+def _head_rows(x: torch.Tensor) -> tuple[torch.Tensor, int, int]:
+    """[N, H, D] with rows of whole 16-byte pieces, and its row and head strides
+    (0 along a dim of one)."""
+    n, h, d = x.shape
+    row, head, one = x.stride()
+    row, head = row if n > 1 else 0, head if h > 1 else 0
+    size = x.element_size()
+    if (one != 1 and d > 1) or row * size % 16 or head * size % 16 or x.data_ptr() % 16:
+        x = x.clone(memory_format=torch.contiguous_format)  # (contiguous() keeps unaligned rows)
+        row, head = h * d, d
+    return x, row, head
+
+
+MAX_TOP = 32  # best tokens of token_logprobs
+
+
+class TokenLogprobs(NamedTuple):
+    """What ``token_logprobs`` says of each row's token."""
+
+    logprobs: torch.Tensor      # float32 [...]: log-probability of the token
+    entropy: torch.Tensor       # float32 [...]: of the row's distribution, in nats
+    ranks: torch.Tensor         # long [...]: tokens more likely than it (0: the greedy pick)
+    top_tokens: torch.Tensor    # long [..., top]: the most likely tokens
+    top_logprobs: torch.Tensor  # float32 [..., top]
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> TokenLogprobs:
+    """Log-probabilities of given tokens: logits [..., V], tokens [...] int64.
+
+    Beside each token's log-probability come the entropy of its row's
+    distribution, the token's rank (larger logits first, equal ones by the
+    lower token, as ``argmax`` picks) and the ``top`` (at most MAX_TOP) most
+    likely tokens with theirs. A row with a NaN or an infinite logit, or none
+    above minus infinity, gives NaN (ranks and tokens hold); minus infinity is
+    probability zero; a token outside the vocabulary gives NaN and rank -1."""
+    what = "token_logprobs"
+    dev = _one_device(what, logits, tokens)
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return token_logprobs(logits, tokens, top)
+    if logits.dim() < 1 or tokens.shape != logits.shape[:-1] or tokens.dtype != torch.long:
+        raise ValueError(f"{what}: tokens {tuple(tokens.shape)} {tokens.dtype} for logits {tuple(logits.shape)}, expected "
+                         f"{tuple(logits.shape[:-1])} int64")
+    vocab, shape = logits.shape[-1], tokens.shape
+    if not 0 <= top <= min(MAX_TOP, vocab):
+        raise ValueError(f"{what}: top={top} of {vocab} tokens (0 to {MAX_TOP})")
+    dt = N.dtype_code(logits.dtype)
+    rows = tokens.numel()
+    logits, tokens = logits.reshape(rows, vocab), tokens.contiguous()
+    if logits.stride(1) != 1 and vocab > 1:
+        logits = logits.contiguous()
+    logprobs, entropy = logits.new_empty((2, *shape), dtype=torch.float32).unbind(0)
+    top_logprobs = logits.new_empty((*shape, top), dtype=torch.float32)
+    ranks = torch.empty_like(tokens)
+    top_tokens = tokens.new_empty((*shape, top))
+    nbytes = _token_logprobs_bytes(dt, rows, vocab, top)
+    # from the caching allocator on the current stream: calls on other streams
+    # and captured graphs have scratch of their own
+    ws = logits.new_empty((nbytes,), dtype=torch.uint8) if nbytes else None
+    N.check(_lib().minitp_token_logprobs(
+        N.stream(), dt, logits.data_ptr(), logits.stride(0), rows, vocab, tokens.data_ptr(), top, logprobs.data_ptr(),
+        entropy.data_ptr(), ranks.data_ptr(), top_tokens.data_ptr(), top_logprobs.data_ptr(), N.ptr(ws), nbytes), what)
+    return TokenLogprobs(logprobs, entropy, ranks, top_tokens, top_logprobs)
+
+
+@functools.lru_cache(maxsize=4096)
+def _token_logprobs_bytes(*sizes: int) -> int:
+    return max(_lib().minitp_token_logprobs_workspace_bytes(*sizes), 0)
+
+
 MAX_BEAMS = 32  # beams of a group
 
 

@@ -1,0 +1,328 @@
+"""Attention over packed sequences (csrc/packed.hip) against the formula in 64
+bits: every head shape, both types, lengths around the tiles' edges, empty
+sequences, rows of none, and values of other sequences that are not finite.
+
+Bars. bf16: the output's own rounding, half a step (2^-8 of the value), and the
+probabilities rounded to bf16 for the product (2^-8 of the attention-weighted
+|V|, the sum they are divided by unrounded). fp32: a score is at most four chains of
+D / 4 products and three more sums, each off by at most 2^-24 of the sum of the
+products' magnitudes, which is below 20 here (1.5 x 0.64 sqrt(D) = 11 at D = 128 for
+normal rows, its spread below 1.5); a score's error is its probability's
+relative error, once above and once below the fraction; exponentials and sums
+over tiles add less than 64 steps.
+"""
+
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BOTH = [torch.bfloat16, torch.float32]
+HEADS = [(14, 2, 64), (28, 4, 128), (4, 2, 16), (4, 4, 32), (8, 1, 128), (3, 1, 64), (9, 3, 16), (16, 8, 32)]
+
+
+def make(n, hq, hkv, d, dtype, layout="tokens", seed=0):
+    """q [N, Hq, D], k and v [N, Hkv, D] as contiguous rows, K and V kept by
+    heads, or slices of one projection's rows."""
+    g = torch.Generator(device=DEV).manual_seed(seed + n * 3 + hq * 7 + d)
+
+    def normal(*shape):
+        return torch.randn(*shape, generator=g, device=DEV).to(dtype)
+
+    if layout == "together":
+        qkv = normal(n, (hq + 2 * hkv) * d)
+        q, k, v = qkv.view(n, -1, d).split([hq, hkv, hkv], 1)
+        q *= 1.5
+        return q, k, v
+    q = normal(n, hq, d) * 1.5
+    if layout == "heads":
+        return q, normal(hkv, n, d).transpose(0, 1), normal(hkv, n, d).transpose(0, 1)
+    return q, normal(n, hkv, d), normal(n, hkv, d)
+
+
+def reference(q, k, v, bounds):
+    """(out, the attention-weighted |V|) [N, Hq, D] in float64 on the device;
+    bounds: (first row, end) of each sequence."""
+    n, hq, d = q.shape
+    per = hq // k.shape[1]
+    out = torch.zeros(n, hq, d, dtype=torch.float64, device=DEV)
+    mag = torch.zeros_like(out)
+    for lo, hi in bounds:
+        if hi <= lo:
+            continue
+        hidden = torch.ones(hi - lo, hi - lo, dtype=torch.bool, device=DEV).triu(1)
+        for h in range(hq):
+            kh, vh = k[lo:hi, h // per].double(), v[lo:hi, h // per].double()
+            s = q[lo:hi, h].double() @ kh.t().contiguous() / math.sqrt(d)
+            p = torch.softmax(s.masked_fill(hidden, -math.inf), -1)
+            out[lo:hi, h], mag[lo:hi, h] = p @ vh, p @ vh.abs()
+    return out, mag
+
+
+def bars(ref, mag, dtype, d):
+    if dtype == torch.bfloat16:
+        return (ref.abs() + mag) * 2 ** -8
+    return mag * (2 * 20 * (d / 4 + 3) + 64) * 2 ** -24
+
+
+def check(got, q, k, v, bounds):
+    ref, mag = reference(q, k, v, bounds)
+    got = got.view(ref.shape).double()
+    assert torch.isfinite(got).all()
+    bar = bars(ref, mag, q.dtype, q.shape[2]) + 1e-9
+    assert ((got - ref).abs() <= bar).all(), ((got - ref).abs() / bar).max()
+
+
+def offsets_of(lens, first=0):
+    return torch.tensor([first] + lens, device=DEV).cumsum(0)
+
+
+def bounds_of(lens, first=0):
+    ends = [first]
+    for n in lens:
+        ends.append(ends[-1] + n)
+    return list(zip(ends, ends[1:]))
+
+
+LENS = [[1], [2, 1, 1], [16], [17, 64, 65, 1, 0, 130], [0, 0, 5, 0], [31, 33, 32, 63, 2, 127, 129, 128], [300, 1, 77],
+        [1] * 50, [700]]
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("layout", ["tokens", "heads", "together"])
+@pytest.mark.parametrize("hq,hkv,d", HEADS)
+@pytest.mark.parametrize("lens", LENS, ids=lambda x: f"{len(x)}x{max(x)}")
+def test_lengths(lens, hq, hkv, d, layout, dtype):
+    from minitp import kernels as K
+
+    x = make(sum(lens), hq, hkv, d, dtype, layout)
+    check(K.packed_attention(*x, offsets_of(lens)), *x, bounds_of(lens))
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("hq,hkv,d", [(14, 2, 64), (28, 4, 128), (4, 2, 16), (4, 4, 32)])
+def test_rows_of_no_sequence(hq, hkv, d, dtype):
+    """Rows in front of the first sequence and behind the last, NaN all over,
+    come out as zeros and change nothing else; int32 offsets."""
+    from minitp import kernels as K
+
+    lens, first = [40, 0, 130, 3], 37
+    q, k, v = make(first + sum(lens) + 200, hq, hkv, d, dtype)
+    end = first + sum(lens)
+    for t in (q, k, v):
+        t[:first], t[end:] = math.nan, math.nan
+    out = K.packed_attention(q, k, v, offsets_of(lens, first).int())
+    check(out[first:end], q[first:end], k[first:end], v[first:end], bounds_of(lens))
+    assert (out[:first] == 0).all() and (out[end:] == 0).all()
+    for none in (torch.zeros(1, device=DEV, dtype=torch.long), torch.tensor([5], device=DEV),
+                 torch.zeros(4, device=DEV, dtype=torch.long)):
+        assert (K.packed_attention(q, k, v, none) == 0).all()
+
+
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("hq,hkv,d", [(14, 2, 64), (28, 4, 128), (4, 2, 16), (4, 4, 32)])
+def test_values_that_are_not_finite_stay_in_their_rows(hq, hkv, d, dtype, value):
+    """A bad key or value row of one sequence shows in that sequence's rows from
+    it on, and nowhere else."""
+    from minitp import kernels as K
+
+    lens = [50, 70, 1, 140, 33]
+    for which in (1, 2):
+        x = make(sum(lens), hq, hkv, d, dtype, seed=which)
+        # (of the clean rows: the product's own zeros times the bad value are no zeros)
+        ref, mag = reference(*x, bounds_of(lens))
+        bad = 50 + 70 + 1 + 60  # row 60 of the fourth sequence
+        x[which][bad, :, d - 1] = value
+        out = K.packed_attention(*x, offsets_of(lens))
+        touched = torch.zeros(sum(lens), dtype=torch.bool, device=DEV)
+        touched[bad:50 + 70 + 1 + 140] = True
+        mine = out.view(-1, hq, d)
+        if which == 2:
+            assert not torch.isfinite(mine[touched][..., d - 1]).any()
+        elif math.isnan(value):
+            assert torch.isnan(mine[touched]).all()
+        bar = bars(ref, mag, dtype, d) + 1e-9
+        assert ((mine.double() - ref).abs() <= bar)[~touched].all()
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+def test_a_query_that_is_no_number_shows(dtype):
+    from minitp import kernels as K
+
+    lens = [20, 90]
+    x = make(110, 14, 2, 64, dtype)
+    x[0][33, 5, 7] = math.nan
+    out = K.packed_attention(*x, offsets_of(lens)).view(110, 14, 64)
+    assert torch.isnan(out[33, 5]).all()
+    out[33, 5] = 0
+    assert torch.isfinite(out).all()
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("scale", [60.0, 1e4])
+def test_large_scores(dtype, scale):
+    """Scores far apart: probabilities of nearly zero and one."""
+    from minitp import kernels as K
+
+    lens = [130, 64]
+    q, k, v = make(194, 4, 2, 64, dtype)
+    q = (q * scale).to(dtype)
+    out = K.packed_attention(q, k, v, offsets_of(lens)).view(194, 4, 64).double()
+    ref, mag = reference(q, k, v, bounds_of(lens))
+    # a score's error is a step of its products' magnitudes' sum (fp32 sums)
+    size = (q.double().abs()[:, :, None] * k.double().abs().amax(0).repeat_interleave(2, 0)[None, :, None]).sum(-1) / 8
+    rel = 2 * size * (64 / 4 + 3 + 2) * 2 ** -24
+    bar = (ref.abs() + mag) * 2 ** -8 if dtype == torch.bfloat16 else mag * 64 * 2 ** -24
+    assert ((out - ref).abs() <= bar + rel.clamp(max=1.0) * v.double().abs().max() + 1e-9).all()
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+def test_many_short_sequences(dtype):
+    """More sequences than a block holds boundaries of, empty ones among them."""
+    from minitp import kernels as K
+
+    g = torch.Generator().manual_seed(4)
+    lens = torch.randint(0, 4, (5000,), generator=g).tolist()
+    lens[100:900] = [0] * 800
+    n = sum(lens)
+    x = make(n, 4, 2, 16, dtype)
+    out = K.packed_attention(*x, offsets_of(lens)).view(n, 4, 16).double()
+    # a sequence of up to three rows at a time: all starts at once
+    start = torch.repeat_interleave(offsets_of(lens)[:-1], torch.tensor(lens, device=DEV))
+    rows = torch.arange(n, device=DEV)
+    idx = (rows[:, None] - torch.arange(3, device=DEV)).clamp(min=0)
+    there = idx >= start[:, None]
+    there &= rows[:, None] - torch.arange(3, device=DEV) >= 0
+    q, k, v = (t.double() for t in x)
+    kk, vv = (t.repeat_interleave(2, 1)[idx] for t in (k, v))
+    s = (q[:, None] * kk).sum(-1) / 4
+    p = torch.softmax(s.masked_fill(~there[:, :, None], -math.inf), 1)
+    ref, mag = (p[..., None] * vv).sum(1), (p[..., None] * vv.abs()).sum(1)
+    assert ((out - ref).abs() <= bars(ref, mag, dtype, 16) + 1e-9).all()
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("hq,hkv,d", [(14, 2, 64), (28, 4, 128)])
+def test_long_sequences(hq, hkv, d, dtype):
+    from minitp import kernels as K
+
+    lens = [2500, 333, 1700]
+    x = make(sum(lens), hq, hkv, d, dtype, "heads")
+    check(K.packed_attention(*x, offsets_of(lens)), *x, bounds_of(lens))
+
+
+def test_sequences_equal_prompts_on_their_own():
+    """As far as the two kernels round alike: the model's prompt attention."""
+    from minitp import kernels as K
+
+    lens = [130, 17, 64]
+    q, k, v = make(sum(lens), 14, 2, 64, torch.bfloat16, "heads")
+    out = K.packed_attention(q, k, v, offsets_of(lens))
+    for lo, hi in bounds_of(lens):
+        alone = K.attention(q[None, lo:hi], k[lo:hi].transpose(0, 1)[None].contiguous(),
+                            v[lo:hi].transpose(0, 1)[None].contiguous(), 0)[0]
+        _, mag = reference(q[lo:hi], k[lo:hi], v[lo:hi], [(0, hi - lo)])
+        bar = mag.view(hi - lo, -1) * 4 * 2 ** -8
+        assert ((alone.double() - out[lo:hi].double()).abs() <= bar + 1e-9).all()
+
+
+def test_results_are_the_same_bits_each_time():
+    from minitp import kernels as K
+
+    lens = [500, 3, 0, 800]
+    for dtype in BOTH:
+        x = make(sum(lens), 14, 2, 64, dtype)
+        first = K.packed_attention(*x, offsets_of(lens))
+        for _ in range(3):
+            assert torch.equal(first, K.packed_attention(*x, offsets_of(lens)))
+
+
+def test_odd_views_are_copied():
+    """Unaligned rows, another element order, K and V of different layouts."""
+    from minitp import kernels as K
+
+    lens = [70, 9]
+    q, k, v = make(79, 4, 2, 32, torch.bfloat16)
+    want = K.packed_attention(q, k, v, offsets_of(lens))
+    shifted = torch.empty(79 * 4 * 32 + 1, dtype=torch.bfloat16, device=DEV)[1:].view(79, 4, 32).copy_(q)
+    assert torch.equal(want, K.packed_attention(shifted, k, v, offsets_of(lens)))
+    by_dim = k.transpose(1, 2).contiguous().transpose(1, 2)
+    assert torch.equal(want, K.packed_attention(q, by_dim, v, offsets_of(lens)))
+    by_head = v.transpose(0, 1).contiguous().transpose(0, 1)
+    assert torch.equal(want, K.packed_attention(q, k, by_head, offsets_of(lens)))
+    # one K/V row for all heads and one for all tokens
+    one = k[:, :1].expand(79, 2, 32)
+    assert torch.equal(K.packed_attention(q, one, one, offsets_of(lens)),
+                       K.packed_attention(q, one.contiguous(), one.contiguous(), offsets_of(lens)))
+    same = k[:1].expand(79, 2, 32)
+    assert torch.equal(K.packed_attention(q, same, same, offsets_of(lens)),
+                       K.packed_attention(q, same.contiguous(), same.contiguous(), offsets_of(lens)))
+
+
+def test_graph_streams_and_changed_offsets():
+    """A captured call takes other offsets at each replay; a second stream runs
+    at the same time."""
+    from minitp import kernels as K
+
+    n = 400
+    x = make(n, 14, 2, 64, torch.bfloat16)
+    offsets = offsets_of([100, 200, 50])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        K.packed_attention(*x, offsets)
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = K.packed_attention(*x, offsets)
+    for lens in ([100, 200, 50], [1, 398, 1], [0, 0, 0], [399, 0, 0], [133, 133, 134]):
+        offsets.copy_(offsets_of(lens))
+        with torch.cuda.stream(side):
+            side.wait_stream(torch.cuda.current_stream())
+            beside = K.packed_attention(*x, offsets)
+        graph.replay()
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        assert torch.equal(out, beside)
+        assert torch.equal(out, K.packed_attention(*x, offsets))
+
+
+def test_offsets_in_disorder_stay_inside():
+    """Values that no caller should pass: nothing outside the arrays is read,
+    and sequences that are in order hold."""
+    from minitp import kernels as K
+
+    x = make(200, 14, 2, 64, torch.bfloat16)
+    for bad in ([50, 20, 90, 60], [-7, 1 << 40], [-(1 << 62), 300, 10], [199, 0], [1 << 40, 1 << 41]):
+        assert torch.isfinite(K.packed_attention(*x, torch.tensor(bad, device=DEV))).all()
+    check(K.packed_attention(*x, torch.tensor([-100, 200], device=DEV)), *x, [(0, 200)])
+    check(K.packed_attention(*x, torch.tensor([0, 1 << 40], device=DEV)), *x, [(0, 200)])
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+def test_rows_past_four_gib(dtype):
+    """K/V rows far apart: offsets past 32 bits, in bytes and in elements."""
+    from minitp import kernels as K
+
+    step = 1 << 17
+    n = (1 << 32) // step + 200  # elements past 2^32
+    store = torch.zeros(n * step, dtype=dtype, device=DEV).view(n, step)
+    q, k, v = make(n, 4, 2, 64, dtype)
+    kk, vv = store[:, :128].view(n, 2, 64), store[:, 256:384].view(n, 2, 64)
+    kk.copy_(k)
+    vv.copy_(v)
+    offsets = offsets_of([n - 300, 300])
+    out, near = K.packed_attention(q, kk, vv, offsets), K.packed_attention(q, k, v, offsets)
+    assert torch.equal(out, near)
+    check(out[-300:], q[-300:], k[-300:], v[-300:], [(0, 300)])
+
+
+def test_nothing():
+    from minitp import kernels as K
+
+    x = make(0, 4, 2, 64, torch.bfloat16)
+    assert K.packed_attention(*x, torch.tensor([0], device=DEV)).shape == (0, 256)
+    assert K.packed_attention(*x, torch.tensor([0, 0], device=DEV)).shape == (0, 256)
