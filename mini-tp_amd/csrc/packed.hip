@@ -4,6 +4,18 @@
 // attends rows a .. i:
 //     o = sum_j softmax_j(q_i . k_j / sqrt(D)) v_j,
 // head h on KV head h / (Hq / Hkv). A row of no sequence gets zeros.
+//
+// The stream is one long causal sequence with a border in front of each
+// sequence, and blocks take it as that: the queries of a KV head, (token, head
+// of the group) by (token, head), in tiles of as many rows wherever the
+// sequences end, each over the keys from its first token's sequence on to its
+// last token. So the launch does not depend on the lengths, which stay on the
+// device, and short sequences share a tile. A query's own window, first .. i, is
+// its mask; tiles of keys that every query of a wave sees are not masked, tiles
+// that none sees are left out.
+#include <type_traits>
+
+#include "attn_tiles.h"
 #include "common.h"
 #include "kernels.h"
 
@@ -15,28 +27,61 @@ struct PackedArgs {
   const void *q, *k, *v;  // [N, Hq, D], [N, Hkv, D] in strides of elements
   int64_t q_row, q_head, kv_row, kv_head;
   void* out;              // [N, Hq, D]
-  int N, S, Hq, per;
+  int S, Hq, Hkv, per;    // per: query heads of a KV head
+  int rows;               // N * per: query rows of a KV head
+  int tiles;              // ... in tiles
   const int64_t* offsets;  // [S + 1]
   float scale;
+  Div by_per, by_hkv;
 };
 
-// First row of the sequence that holds row r, -1 where none does: the last
-// offset not above r begins it. (Offsets in disorder give some row up to r.)
-__device__ __forceinline__ int first_row(const PackedArgs& a, int r) {
-  int lo = 0, hi = a.S + 1;  // offsets[0 .. lo - 1] <= r < offsets[hi ..]
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (a.offsets[mid] <= r)
-      lo = mid + 1;
-    else
-      hi = mid;
+constexpr int NONE = INT32_MAX;  // the first row of a token of no sequence
+
+// Where the sequences of a tile's tokens begin: first[j] for token t0 + j, j <
+// n <= 256 threads, and the least of them (NONE: all are of no sequence). A
+// thread finds the offsets not above its token by bisection, the last of which
+// begins its sequence: of up to 256 offsets, every one or every so many, in LDS,
+// then of those between two of them. (Offsets in disorder give some row.)
+struct Firsts {
+  int first[256], some[256], least;
+};
+__device__ __forceinline__ void find_firsts(const PackedArgs& a, Firsts& f, int t0, int n) {
+  const int tid = threadIdx.x, count = a.S + 1, step = (count + 255) >> 8;
+  auto offset = [&](int i) { return (int)std::min<int64_t>(std::max<int64_t>(a.offsets[i], 0), NONE); };
+  f.some[tid] = (int64_t)tid * step < count ? offset(tid * step) : NONE;
+  if (tid == 0) f.least = NONE;
+  __syncthreads();
+  if (tid < n) {
+    const int t = t0 + tid;
+    int c = 0;  // of f.some, the ones not above t
+#pragma unroll
+    for (int b = 128; b >= 1; b >>= 1)
+      if (f.some[c + b - 1] <= t) c += b;
+    c += f.some[c & 255] <= t;  // (c <= 255 so far)
+    int begin = c > 0 ? f.some[c - 1] : NONE;
+    int64_t lo = (int64_t)(c - 1) * step + 1, hi = std::min<int64_t>((int64_t)c * step, count);
+    while (c > 0 && lo < hi) {
+      const int64_t mid = (lo + hi) >> 1;
+      const int o = offset((int)mid);
+      if (o <= t) {
+        begin = o;
+        lo = mid + 1;
+      } else {
+        hi = mid;
+      }
+    }
+    if (c > 0 && lo == count) begin = NONE;  // (from the last offset on)
+    f.first[tid] = begin;
+    atomicMin(&f.least, begin);
   }
-  if (lo == 0 || lo > a.S) return -1;
-  return (int)std::min<int64_t>(std::max<int64_t>(a.offsets[lo - 1], 0), r);
+  __syncthreads();
 }
 
-// One query of one head by one wave, in fp32: a lane a key for the scores, a
-// lane one or two dims of the output.
+// One query of one head by one wave, in fp32, key by key and only those it sees:
+// a lane a key for the scores, a lane one or two dims of the output. The tile
+// kernels turn to it for a query whose result is not finite: in a product over a
+// whole tile a hidden value that is infinite or NaN shows (0 times it is no
+// zero), here it does not.
 template <typename T, int D>
 __device__ __forceinline__ void packed_row(const PackedArgs& a, int r, int first, int head) {
   constexpr int VE = Vec<T>::N, DL = D > 64 ? D / 64 : 1;
@@ -52,6 +97,7 @@ __device__ __forceinline__ void packed_row(const PackedArgs& a, int r, int first
     const int key = k0 + lane;
     const T* krow = k + std::min(key, r) * a.kv_row;
     float s = 0.f;
+#pragma unroll 1
     for (int d = 0; d < D; d += VE) {
       float x[VE], y[VE];
       load_vec<T, VE>(q + d, x);
@@ -81,22 +127,270 @@ __device__ __forceinline__ void packed_row(const PackedArgs& a, int r, int first
   }
 }
 
+// The rows of a wave whose results are not finite (bits of lanes 0 .. 31, or 15),
+// computed again one by one.
+template <typename T, int D>
+__device__ __forceinline__ void rows_again(const PackedArgs& a, uint64_t odd, int tok, int head, int first) {
+  while (odd) {
+    const int lane = __builtin_ctzll(odd);
+    odd &= odd - 1;
+    packed_row<T, D>(a, __builtin_amdgcn_readlane(tok, lane), __builtin_amdgcn_readlane(first, lane),
+                     __builtin_amdgcn_readlane(head, lane));
+  }
+}
+
+__device__ __forceinline__ int wave_max_int(int v) {
+  auto step = [&](int o) { v = std::max(v, o); };
+  step(__builtin_amdgcn_update_dpp(v, v, 0x111, 0xf, 0xf, false));  // row_shr:1, 2, 4, 8
+  step(__builtin_amdgcn_update_dpp(v, v, 0x112, 0xf, 0xf, false));
+  step(__builtin_amdgcn_update_dpp(v, v, 0x114, 0xf, 0xf, false));
+  step(__builtin_amdgcn_update_dpp(v, v, 0x118, 0xf, 0xf, false));
+  step(__builtin_amdgcn_update_dpp(v, v, 0x142, 0xa, 0xf, false));  // row_bcast:15, 31
+  step(__builtin_amdgcn_update_dpp(v, v, 0x143, 0xc, 0xf, false));
+  return __builtin_amdgcn_readlane(v, 63);
+}
+
+// What a wave's tile of keys needs: `from` .. `to` are keys that some of its
+// queries see, `all_from` .. `all_to` those that every one sees.
+struct Window {
+  int from, to, all_from, all_to;
+};
+__device__ __forceinline__ Window window_of(int tok, int first) {
+  Window w;
+  w.from = -wave_max_int(-first);
+  w.all_from = wave_max_int(first == NONE ? -1 : first);  // (a row of no sequence: zeros whatever it sees)
+  w.all_to = __builtin_amdgcn_readfirstlane(tok);
+  w.to = wave_max_int(tok);
+  return w;
+}
+
+// ---------------------------------------------------------------------------
+// bf16: 128 query rows a block, four waves of 32 (v_mfma_f32_32x32x16_bf16), over
+// tiles of 64 keys.
+//
+// A tile of K and V rows goes to LDS as it lies in memory, by loads that bypass
+// the registers, while the tile before it is computed (two stages, one barrier a
+// tile). Products are transposed, S^T = K Q^T and O^T = V^T P^T, so a lane's
+// scores belong to one query and its probabilities are the second product's
+// operand as they are, the k-index of both operands permuted alike; V^T comes
+// out of LDS transposed by ds_read_b64_tr_b16. A row's 16-byte chunks are
+// permuted by its number, which the loads do on the global side, so that every
+// LDS read reaches all banks.
+//
+// A probability is rounded to bf16 for the second product, by at most 2^-8 of
+// itself, as much as the output's own rounding: the matrix cores take bf16
+// there, and fp32 products run at an eighth of the rate (154 against 1,261 TFLOP/s
+// of a large library product). The sums that they are divided by add the
+// unrounded ones.
+constexpr int P_QT = 128;
+
+// The tiles of keys `key0` .. key0 + keys - 1 of a KV head through the two stages.
+template <int D>
+struct KeyTiles {
+  using H = Half<D>;
+  const char *k, *v;
+  int64_t row;  // bytes between rows
+  uint32_t to, koff, voff, piece;
+  int keys, n;
+  __device__ __forceinline__ KeyTiles(const PackedArgs& a, int kv, int key0, int keys_, char* lds)
+      : row(a.kv_row * 2), keys(keys_), n((keys_ + H_KT - 1) / H_KT) {
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t at = key0 * row + kv * a.kv_head * 2;
+    k = (const char*)a.k + at;
+    v = (const char*)a.v + at;
+    to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds + w * 1024;
+    // piece w + 4 j of a tile: rows 4 PIECE_ROWS j + r; the swizzles do not depend on j
+    const int r = H::PIECE_ROWS * (H::PPW > 0 ? w : w & 1) + lane / H::CH;
+    koff = r * (uint32_t)row + ((lane % H::CH) ^ H::k_swz(r)) * 16;
+    voff = r * (uint32_t)row + ((lane % H::CH) ^ H::v_swz(r)) * 16;
+    piece = 4 * H::PIECE_ROWS * (uint32_t)row;
+  }
+  __device__ __forceinline__ void load(int t) const {
+    if (t >= n) return;
+    // rows past the last read zeros (or, where rows overlap, the last again)
+    const int bytes = (std::min(keys - t * H_KT, H_KT) - 1) * (int)row + H::ROWB;
+    const int64_t at = (int64_t)t * H_KT * row;
+    const u32x4 kr = rows_rsrc(k + at, bytes), vr = rows_rsrc(v + at, bytes);
+    uint32_t lds = __builtin_amdgcn_readfirstlane(to + (t & 1) * H::STAGE), step = __builtin_amdgcn_readfirstlane(piece);
+    asm volatile("s_nop 4" : "+s"(lds), "+s"(step));
+    if constexpr (H::PPW == 0) {
+      if (__builtin_amdgcn_readfirstlane(threadIdx.x >> 7) == 0)
+        row_dma16(kr, koff, lds);
+      else
+        row_dma16(vr, voff, lds);
+    }
+#pragma unroll
+    for (int j = 0; j < H::PPW; ++j) row_dma16(kr, koff, j * step, lds + j * 4096);
+#pragma unroll
+    for (int j = 0; j < H::PPW; ++j) row_dma16(vr, voff, j * step, lds + H::OPER + j * 4096);
+  }
+};
+
+template <int D>
+__global__ __launch_bounds__(256, 2) void packed_bf16_kernel(PackedArgs a) {
+  using H = Half<D>;
+  // (D = 16: the output's 32-row operand holds the 16 dims twice)
+  constexpr int KS = D / 16, DB = D >= 32 ? D / 32 : 1, OC = D >= 32 ? 4 : 2;  // OC: 8-dim chunks of a block
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  __shared__ Firsts firsts;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n32 = lane & 31, h = lane >> 5;
+  // The last rows, which see the most keys, first. (KV heads side by side: where
+  // there are 1, 2, 4 or 8, an XCD's blocks, every eighth, share one's rows.)
+  const int j = a.by_hkv(blockIdx.x), kv = blockIdx.x - j * a.Hkv, tile = a.tiles - 1 - j;
+  const int r0 = tile * P_QT + w * 32, r = std::min(r0 + n32, a.rows - 1);
+  const int tok = a.by_per(r), head = kv * a.per + r - tok * a.per;
+  bf16x8 qb[KS];
+  {
+    const bf16* q = (const bf16*)a.q + tok * a.q_row + head * a.q_head + 8 * h;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) qb[k] = __builtin_bit_cast(bf16x8, *(const u32x4*)(q + 16 * k));
+  }
+  const int t0 = a.by_per(tile * P_QT), t1 = a.by_per(std::min(tile * P_QT + P_QT, a.rows) - 1);
+  find_firsts(a, firsts, t0, t1 - t0 + 1);
+  const int key0 = __builtin_amdgcn_readfirstlane(firsts.least), first = firsts.first[tok - t0];
+  const KeyTiles<D> tiles(a, kv, key0, key0 == NONE ? 0 : t1 - key0 + 1, lds);
+  tiles.load(0);
+  const Window win = window_of(tok, first);
+
+  f32x16 o[DB];
+#pragma unroll
+  for (int d = 0; d < DB; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
+  float m = -__builtin_inff(), lsum = 0.f;
+  const float sl2 = a.scale * 1.4426950408889634f;
+
+  // LDS bytes of this lane's operands: K row n32, chunk 2 k + h; V rows
+  // 4 h + (lane % 16) / 4 (+ 8), dims 32 d + 16 ((lane / 16) % 2) + 4 (lane % 4)
+  const int kat = n32 * H::ROWB, kx = (h ^ H::k_swz(n32)) << 4;
+  const int vrow = 4 * h + (lane & 15) / 4;
+  const int vat = H::OPER + vrow * H::ROWB + 8 * (lane & 1);
+  const int vx = (((D >= 32 ? 2 * ((lane >> 4) & 1) : 0) + ((lane >> 1) & 1)) ^ H::v_swz(vrow)) << 4;
+  arrived(qb);
+
+  auto compute = [&](const char* st, int key, bool masked) {
+    f32x16 s[2];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[kb][i] = 0.f;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {  // (two chains in turn)
+        const bf16x8 kf = __builtin_bit_cast(bf16x8, *(const uint4*)(st + kat + kb * 32 * H::ROWB + ((32 * k) ^ kx)));
+        s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qb[k], s[kb], 0, 0, 0);
+      }
+    }
+    if (masked) {
+      // lane (query, h) holds keys 32 kb + 8 (i / 4) + 4 h + i % 4 and sees first .. tok
+      const uint32_t base = (uint32_t)(key + 4 * h) - (uint32_t)first, most = (uint32_t)tok - (uint32_t)first;
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (base + (32 * kb + 8 * (i / 4) + i % 4) > most) s[kb][i] = -__builtin_inff();
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kb][i]);
+    mx = halves_max(mx) * sl2;
+    if (__builtin_amdgcn_ballot_w64(mx > m + SLACK)) {
+      const float mn = fmaxf(m, mx), alpha = mn == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+      m = mn;
+      lsum *= alpha;
+#pragma unroll
+      for (int d = 0; d < DB; ++d) o[d] *= alpha;
+    }
+    const float mref = m == -__builtin_inff() ? 0.f : m;  // (nothing seen yet)
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[kb][i] = __builtin_amdgcn_exp2f(fmaf(s[kb][i], sl2, -mref));
+        lsum += s[kb][i];
+      }
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int jj = 0; jj < 4; ++jj) {  // keys 16 jj .. 16 jj + 15
+      const f32x16& p = s[jj / 2];
+      const int b = 8 * (jj % 2);
+      uint4 pk;
+      pk.x = pack_bf16x2(p[b], p[b + 1]);
+      pk.y = pack_bf16x2(p[b + 2], p[b + 3]);
+      pk.z = pack_bf16x2(p[b + 4], p[b + 5]);
+      pk.w = pack_bf16x2(p[b + 6], p[b + 7]);
+      const bf16x8 pb = __builtin_bit_cast(bf16x8, pk);
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+        const char* vp = st + vat + 16 * jj * H::ROWB + ((64 * d) ^ vx);
+        const bf16x8 vf = join8(read_tr(vp), read_tr(vp + 8 * H::ROWB));
+        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pb, o[d], 0, 0, 0);
+      }
+    }
+    __builtin_amdgcn_s_setprio(0);
+  };
+  for (int t = 0; t < tiles.n; ++t) {
+    stage_wait();
+    tiles.load(t + 1);  // (the stage's readers passed the barrier)
+    const int key = key0 + t * H_KT, last = key + H_KT - 1;
+    if (key > win.to || last < win.from) continue;
+    compute(lds + (t & 1) * H::STAGE, key, key < win.all_from || last > win.all_to);
+  }
+
+  if (r0 >= a.rows) return;
+  const float l = halves_sum(lsum), f = first == NONE ? 0.f : 1.f / l;
+  float odd = l * 0.f;
+#pragma unroll
+  for (int d = 0; d < DB; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) odd = fmaf(o[d][i], 0.f, odd);
+  // (a query that saw nothing but minus infinity is NaN here, as it should be)
+  if (r0 + n32 < a.rows) {
+    bf16* orow = (bf16*)a.out + ((int64_t)tok * a.Hq + head) * D + 4 * h;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int c = 0; c < OC; ++c) {
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = first == NONE ? 0.f : o[d][4 * c + e] * f;
+        store_vec<bf16, 4>(orow + 32 * d + 8 * c, v);
+      }
+  }
+  const uint64_t bad = __builtin_amdgcn_ballot_w64(odd != 0.f && first != NONE && r0 + n32 < a.rows);
+  rows_again<bf16, D>(a, (uint32_t)(bad | bad >> 32), tok, head, first);
+}
+
 template <typename T, int D>
 __global__ __launch_bounds__(256) void packed_rows_kernel(PackedArgs a) {
-  const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (i >= (int64_t)a.N * a.Hq) return;
-  const int r = (int)(i / a.Hq), first = first_row(a, r);
-  if (first >= 0) {
-    packed_row<T, D>(a, r, first, (int)(i % a.Hq));
+  __shared__ Firsts f;
+  const int i = blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int t0 = blockIdx.x * 4 / a.Hq, r = i / a.Hq;
+  find_firsts(a, f, t0, std::min(4, a.rows / a.per - t0));
+  if (r >= a.rows / a.per) return;
+  const int first = f.first[r - t0];
+  if (first != NONE) {
+    packed_row<T, D>(a, r, first, i % a.Hq);
     return;
   }
-  T* out = (T*)a.out + i * D;
+  T* out = (T*)a.out + (int64_t)i * D;
   for (int d = threadIdx.x & 63; d < D; d += 64) store_f32<T>(out, d, 0.f);
 }
 
 template <typename T, int D>
-int packed_launch(hipStream_t st, const PackedArgs& a) {
-  hipLaunchKernelGGL((packed_rows_kernel<T, D>), dim3((unsigned)cdiv((int64_t)a.N * a.Hq, 4)), dim3(256), 0, st, a);
+int packed_launch(hipStream_t st, PackedArgs a) {
+  if constexpr (sizeof(T) == 2) {
+    a.tiles = (int)cdiv(a.rows, P_QT);
+    const int rc = ensure_lds_limit((const void*)packed_bf16_kernel<D>, Half<D>::LDS + (int)sizeof(Firsts));
+    if (rc) return rc;
+    hipLaunchKernelGGL((packed_bf16_kernel<D>), dim3((unsigned)(a.tiles * a.Hkv)), dim3(256), Half<D>::LDS, st, a);
+  } else {
+    hipLaunchKernelGGL((packed_rows_kernel<T, D>), dim3((unsigned)cdiv((int64_t)a.rows * a.Hkv, 4)), dim3(256), 0, st, a);
+  }
   MINITP_LAUNCH_CHECK();
   return MINITP_OK;
 }
@@ -150,10 +444,13 @@ int launch_packed_attention(hipStream_t st, int dtype, const PackedShape& s, con
   a.kv_row = s.kv_row;
   a.kv_head = s.kv_head;
   a.out = out;
-  a.N = (int)s.N;
   a.S = (int)s.S;
   a.Hq = (int)s.Hq;
+  a.Hkv = (int)s.Hkv;
   a.per = (int)(s.Hq / s.Hkv);
+  a.rows = (int)s.N * a.per;
+  a.by_per = make_div(a.per);
+  a.by_hkv = make_div(s.Hkv);
   a.offsets = offsets;
   a.scale = 1.0f / sqrtf((float)s.D);
   return dtype == MINITP_F32 ? packed_by_d<float>(st, a, s.D) : packed_by_d<bf16>(st, a, s.D);

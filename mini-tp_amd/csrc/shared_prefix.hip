@@ -23,24 +23,13 @@
 // for the join).
 #include <type_traits>
 
+#include "attn_tiles.h"
 #include "common.h"
 #include "kernels.h"
 
 namespace minitp {
 
 namespace {
-
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-
-// Division by a number the host knows: n / d for 0 <= n < 2^31 as one product
-// (m = ceil(2^(31 + l) / d) with 2^l >= d: n (m d - 2^(31 + l)) < 2^(31 + l)). The
-// index arithmetic in front of a block's first load is all latency: with the
-// compiler's divisions, most of them in 64 bits, a 5.6 us call took 6.2.
-struct Div {
-  uint32_t mul;
-  int shift;
-  __device__ __forceinline__ int operator()(int n) const { return (int)(((uint64_t)(uint32_t)n * mul) >> shift); }
-};
 
 struct SharedArgs {
   const void *q, *kp, *vp, *kc, *vc;  // q [B, T, Hq, D]; prefix [G, Hkv, Sp, D]; own [B, Hkv, S, D]
@@ -166,24 +155,6 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t key_rows(const void* base, int
 __device__ __forceinline__ uint4 rows_load16(__amdgpu_buffer_rsrc_t r, uint32_t off) {
   const u32x4 v = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0));
   return make_uint4(v.x, v.y, v.z, v.w);
-}
-
-// maximum / sum over lanes l and l ^ 32 (and, for the 16-lane form, l ^ 16)
-__device__ __forceinline__ float halves_max(float v) {
-  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
-__device__ __forceinline__ float halves_sum(float v) {
-  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
-}
-__device__ __forceinline__ float quads_max(float v) {
-  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return halves_max(fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1])));
-}
-__device__ __forceinline__ float quads_sum(float v) {
-  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return halves_sum(__uint_as_float(a[0]) + __uint_as_float(a[1]));
 }
 
 // A maximum to join by. Scores that are no numbers are no maximum but show in
@@ -462,73 +433,8 @@ __global__ __launch_bounds__(256, 2) void shared_attn_f32_kernel(SharedArgs a) {
 // scores computed before the tile in front of it is used (946 against 961
 // TFLOP/s), the next loads issued behind the scores (-7 %) or spread over the
 // product.
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef short s16x8 __attribute__((ext_vector_type(8)));
-typedef float f32x16 __attribute__((ext_vector_type(16)));
+constexpr int H_QT = 128, H_SMALL = 16;
 
-constexpr int H_QT = 128, H_KT = 64, H_SMALL = 16;
-
-template <int D>
-struct Half {
-  static constexpr int ROWB = D * 2, CH = D / 8;
-  static constexpr int OPER = H_KT * ROWB, STAGE = 2 * OPER, LDS = 2 * STAGE;
-  // 1 KiB loads of a tile: PPW of K and of V a wave (D = 16: one of either)
-  static constexpr int PIECE_ROWS = 64 / CH, PIECES = H_KT / PIECE_ROWS, PPW = PIECES / 4;
-  static_assert(PPW >= 1 || PIECES == 2, "each wave loads alike, or waves 0, 1 K and waves 2, 3 V");
-  // chunk c of row r lies at chunk c ^ swz(r)
-  __device__ static int k_swz(int r) { return r * ROWB / 256 % CH; }
-  __device__ static int v_swz(int r) { return r * ROWB / 256 % 4 * 4 % CH; }
-};
-
-// 16 bytes a lane from the resource at voff to LDS at lds_addr + 16 lane
-// (m0, wave-uniform; zeros past the resource's end). asm, so that the compiler
-// does not wait for these loads at every LDS read: stage_wait does. It also
-// keeps the compiler from adding the wait states that the hardware asks for:
-// one between the write of m0 and a load to LDS (the s_nop 0), and five between
-// a vector instruction's write of a scalar register (v_readfirstlane) and a
-// load that reads it, which rows_rsrc leaves.
-__device__ __forceinline__ void row_dma16(u32x4 r, uint32_t voff, uint32_t lds_addr) {
-  asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(r), "{m0}"(lds_addr) : "memory");
-}
-__device__ __forceinline__ u32x4 rows_rsrc(const void* base, int bytes) {
-  const uint64_t p = (uint64_t)base;
-  u32x4 r;
-  r.x = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)p);
-  r.y = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(p >> 32));
-  r.z = (uint32_t)__builtin_amdgcn_readfirstlane(bytes);
-  r.w = 0x00020000u;
-  asm volatile("s_nop 4" : "+s"(r));
-  return r;
-}
-// this wave's loads have landed and its LDS reads are done; then the block's
-__device__ __forceinline__ void stage_wait() {
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
-}
-
-// The queries are waited for here. Without it the compiler would wait for them
-// at their first use in the tile loop, every time round, and so for the next
-// tile's loads, which are counted with them.
-template <int N>
-__device__ __forceinline__ void arrived(bf16x8 (&q)[N]) {
-  if constexpr (N >= 4) {
-#pragma unroll
-    for (int k = 0; k < N; k += 4) asm volatile("" : "+v"(q[k]), "+v"(q[k + 1]), "+v"(q[k + 2]), "+v"(q[k + 3]));
-  } else if constexpr (N == 2) {
-    asm volatile("" : "+v"(q[0]), "+v"(q[1]));
-  } else {
-    asm volatile("" : "+v"(q[0]));
-  }
-}
-
-__device__ __forceinline__ s16x4 read_tr(const char* p) {
-  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p));
-}
-__device__ __forceinline__ bf16x8 join8(s16x4 lo, s16x4 hi) {
-  return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-}
 // one of eight bf16 values is infinite or NaN
 __device__ __forceinline__ bool not_finite(const uint4& x) {
   const uint32_t wd[4] = {x.x, x.y, x.z, x.w};
@@ -587,13 +493,6 @@ struct Tiles {
     }
   }
 };
-
-// The running maximum moves only when some lane's passes it by this much (base
-// 2): until then probabilities stay below 2^8 and nothing is rescaled. (It is a
-// score times log2(e), rounded: off by 2^-24 of its size, which scales all of a
-// part's probabilities alike and goes out in the division. Scores of up to 2^29
-// leave that within 2^32.)
-constexpr float SLACK = 8.f;
 
 // AHEAD: a wave's second products go before other waves' work (below).
 template <int D, bool AHEAD>
@@ -1159,11 +1058,6 @@ int launch_shared_prefix_attention(hipStream_t st, int dtype, const SharedPrefix
   a.kc = k_cache;
   a.vc = v_cache;
   a.out = out;
-  auto div = [](int64_t d) {
-    int l = 0;
-    while ((1LL << l) < d) ++l;
-    return Div{(uint32_t)(((1ull << (31 + l)) + (uint64_t)d - 1) / (uint64_t)d), 31 + l};
-  };
   a.B = (int)s.B;
   a.w = (int)(s.B / s.G);
   a.per = (int)(s.Hq / s.Hkv);
@@ -1186,13 +1080,13 @@ int launch_shared_prefix_attention(hipStream_t st, int dtype, const SharedPrefix
   a.items_s = (int)p.items_s;
   a.run_p = (int)cdiv(p.items_p, 8);
   a.run_s = (int)cdiv(p.items_s, 8);
-  a.by_qtiles_p = div(p.qtiles_p);
-  a.by_qtiles_s = div(p.qtiles_s);
-  a.by_splits_p = div(std::max(p.splits_p, 1));
-  a.by_splits_s = div(p.splits_s);
-  a.by_hkv = div(s.Hkv);
-  a.by_w = div(a.w);
-  a.by_per = div(a.per);
+  a.by_qtiles_p = make_div(p.qtiles_p);
+  a.by_qtiles_s = make_div(p.qtiles_s);
+  a.by_splits_p = make_div(std::max(p.splits_p, 1));
+  a.by_splits_s = make_div(p.splits_s);
+  a.by_hkv = make_div(s.Hkv);
+  a.by_w = make_div(a.w);
+  a.by_per = make_div(a.per);
   a.joined = p.joined;
   a.o = (float*)workspace;
   a.ml = a.o + (p.splits_p + p.splits_s) * rows * s.D;
