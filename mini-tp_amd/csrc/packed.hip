@@ -365,34 +365,228 @@ __global__ __launch_bounds__(256, 2) void packed_bf16_kernel(PackedArgs a) {
   rows_again<bf16, D>(a, (uint32_t)(bad | bad >> 32), tok, head, first);
 }
 
-template <typename T, int D>
-__global__ __launch_bounds__(256) void packed_rows_kernel(PackedArgs a) {
-  __shared__ Firsts f;
-  const int i = blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int t0 = blockIdx.x * 4 / a.Hq, r = i / a.Hq;
-  find_firsts(a, f, t0, std::min(4, a.rows / a.per - t0));
-  if (r >= a.rows / a.per) return;
-  const int first = f.first[r - t0];
-  if (first != NONE) {
-    packed_row<T, D>(a, r, first, i % a.Hq);
-    return;
+// ---------------------------------------------------------------------------
+// fp32, on v_mfma_f32_16x16x4_f32. Four waves share each 64-key tile in LDS: 4 / KW
+// strips of 16 queries, KW waves a strip over 64 / KW keys each, joined at the
+// end. Products are transposed: S^T = K Q^T leaves lane (quad, r) with keys
+// 4 quad .. 4 quad + 3 of query r, which is the B operand of O^T = V^T P^T as it
+// is. Score MFMA i of a chunk takes dims 16 c + 4 quad + i from both operands (one
+// 16-byte LDS read a lane), output MFMA j dims E r + j; rows are padded by 16
+// bytes against bank conflicts. A score is summed in four chains.
+constexpr int F_KT = 64;
+template <int D>
+constexpr int F_LDS = 2 * F_KT * (D + 4) * 4;
+
+template <int D, int KW>
+__global__ __launch_bounds__(256, 2) void packed_f32_kernel(PackedArgs a) {
+  constexpr int KT = F_KT, QT = 64 / KW, KB = KT / 16 / KW, KC = D / 16, SW = 4 / KW;
+  constexpr int E = D / 16 < 4 ? D / 16 : 4, HALVES = D / 16 / E;
+  constexpr int ROW = D + 4;
+  constexpr int PIECES = KT * D / 4, PER = (PIECES + 255) / 256;
+  static_assert(F_LDS<D> >= 64 * (D + 2) * 4, "the waves' results fit the tiles");
+  extern __shared__ __attribute__((aligned(16))) float lds_f[];
+  __shared__ Firsts firsts;
+  float *Ks = lds_f, *Vs = lds_f + KT * ROW;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lr = lane % 16, lq = lane / 16, strip = wave % SW, sub = wave / SW * KB * 16;
+  const int jb = a.by_hkv(blockIdx.x), kv = blockIdx.x - jb * a.Hkv, tile = a.tiles - 1 - jb;
+  const int r0 = tile * QT + strip * 16, r = std::min(r0 + lr, a.rows - 1);
+  const int tok = a.by_per(r), head = kv * a.per + r - tok * a.per;
+
+  f32x4 qa[KC];
+  {
+    const float* q = (const float*)a.q + tok * a.q_row + head * a.q_head;
+#pragma unroll
+    for (int c = 0; c < KC; ++c) qa[c] = *(const f32x4*)(q + 16 * c + 4 * lq);
   }
-  T* out = (T*)a.out + (int64_t)i * D;
-  for (int d = threadIdx.x & 63; d < D; d += 64) store_f32<T>(out, d, 0.f);
+  const int t0 = a.by_per(tile * QT), t1 = a.by_per(std::min(tile * QT + QT, a.rows) - 1);
+  find_firsts(a, firsts, t0, t1 - t0 + 1);
+  const int key0 = __builtin_amdgcn_readfirstlane(firsts.least), first = firsts.first[tok - t0];
+  const int keys = key0 == NONE ? 0 : t1 - key0 + 1;
+  const int64_t row = a.kv_row * 4, at0 = key0 * row + kv * a.kv_head * 4;
+  const Window win = window_of(tok, first);
+
+  f32x4 o[HALVES][E];
+#pragma unroll
+  for (int hf = 0; hf < HALVES; ++hf)
+#pragma unroll
+    for (int j = 0; j < E; ++j) o[hf][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m = -__builtin_inff(), lsum = 0.f;
+  u32x4 kr[PER], vr[PER];
+  auto load_tile = [&](int key) {
+    // rows past the last read zeros (or, where rows overlap, the last again)
+    const uint32_t bytes = (std::min(keys - key, KT) - 1) * (uint32_t)row + D * 4;
+    const __amdgpu_buffer_rsrc_t krs = span_rsrc((const char*)a.k + at0 + key * row, bytes);
+    const __amdgpu_buffer_rsrc_t vrs = span_rsrc((const char*)a.v + at0 + key * row, bytes);
+#pragma unroll
+    for (int u = 0; u < PER; ++u) {
+      const int i = tid + 256 * u;  // (past the tile: not stored)
+      const uint32_t off = std::min(i / (D / 4), KT - 1) * (uint32_t)row + i % (D / 4) * 16;
+      kr[u] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(krs, off, 0, 0));
+      vr[u] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(vrs, off, 0, 0));
+    }
+  };
+  if (keys > 0) load_tile(0);
+  for (int k0 = 0; k0 < keys; k0 += KT) {
+    __syncthreads();  // the previous tile is consumed
+#pragma unroll
+    for (int u = 0; u < PER; ++u) {
+      const int i = tid + 256 * u;
+      if (i < PIECES) {
+        const int at = i / (D / 4) * ROW + i % (D / 4) * 4;
+        *(u32x4*)(Ks + at) = kr[u];
+        *(u32x4*)(Vs + at) = vr[u];
+      }
+    }
+    __syncthreads();
+    if (k0 + KT < keys) load_tile(k0 + KT);
+    const int key = key0 + k0 + sub, last = key + KB * 16 - 1;  // this wave's
+    if (key > win.to || last < win.from) continue;
+    const bool masked = key < win.all_from || last > win.all_to;
+    float p[KB][4];
+    float mx = -__builtin_inff();
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+      f32x4 chain[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) chain[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < KC; ++c) {
+        const f32x4 k4 = *(const f32x4*)(Ks + (sub + kb * 16 + lr) * ROW + 16 * c + 4 * lq);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) chain[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(k4[i], qa[c][i], chain[i], 0, 0, 0);
+      }
+      const f32x4 acc = (chain[0] + chain[1]) + (chain[2] + chain[3]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) p[kb][e] = acc[e] * a.scale;
+    }
+    if (masked) {  // (a lane sees first .. tok)
+      const uint32_t base = (uint32_t)(key + 4 * lq) - (uint32_t)first, most = (uint32_t)tok - (uint32_t)first;
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (base + (kb * 16 + e) > most) p[kb][e] = -__builtin_inff();
+    }
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) mx = fmaxf(mx, p[kb][e]);
+    mx = quads_max(mx);
+    const float mn = fmaxf(m, mx), ref = mn == -__builtin_inff() ? 0.f : mn;
+    if (__builtin_amdgcn_ballot_w64(mn != m)) {
+      const float alpha = mn == m ? 1.f : expf(m - mn);
+      m = mn;
+      lsum *= alpha;
+#pragma unroll
+      for (int hf = 0; hf < HALVES; ++hf)
+#pragma unroll
+        for (int j = 0; j < E; ++j) o[hf][j] *= alpha;
+    }
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        p[kb][e] = expf(p[kb][e] - ref);
+        lsum += p[kb][e];
+      }
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float* vrow = Vs + (sub + kb * 16 + 4 * lq + e) * ROW + E * lr;
+#pragma unroll
+        for (int hf = 0; hf < HALVES; ++hf) {
+          float v[E];
+          if constexpr (E == 4) {
+            const f32x4 v4 = *(const f32x4*)(vrow + 64 * hf);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = v4[j];
+          } else {
+#pragma unroll
+            for (int j = 0; j < E; ++j) v[j] = vrow[j];
+          }
+#pragma unroll
+          for (int j = 0; j < E; ++j)
+            o[hf][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[j], p[kb][e], o[hf][j], 0, 0, 0);
+        }
+      }
+  }
+  // o[hf][j][x]: dim 64 hf + E (4 lq + x) + j of the lane's query; the KW waves of
+  // a strip joined through LDS, and stored from there by whole rows
+  lsum = quads_sum(lsum);
+  float* po = lds_f;                       // [KW][QT][D]
+  float2* pml = (float2*)(po + 64 * D);    // [KW][QT]
+  const int at = wave / SW * QT + strip * 16 + lr;
+  __syncthreads();  // (the last tile is consumed)
+#pragma unroll
+  for (int hf = 0; hf < HALVES; ++hf)
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+#pragma unroll
+      for (int j = 0; j < E; ++j) po[at * D + 64 * hf + E * (4 * lq + x) + j] = o[hf][j][x];
+  if (lq == 0) pml[at] = make_float2(m, lsum);
+  __syncthreads();
+  // LPR lanes a row; rows that are not finite are left to packed_row
+  constexpr int LPR = D / 4;
+  const int n = std::min(QT, a.rows - tile * QT);
+  for (int i0 = 0; i0 < n * LPR; i0 += 256) {
+    const int i = i0 + tid, ri = std::min(i / LPR, n - 1), d = i % LPR * 4;
+    float mm = -__builtin_inff(), l = 0.f;
+    float2 ml[KW];
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int g = 0; g < KW; ++g) {
+      ml[g] = pml[g * QT + ri];
+      mm = fmaxf(mm, ml[g].x);
+    }
+    float odd = 0.f;
+#pragma unroll
+    for (int g = 0; g < KW; ++g) {
+      const f32x4 og = *(const f32x4*)(po + (g * QT + ri) * D + d);
+      // (a wave that saw nothing weighs nothing; a sum that is no number shows)
+      const float sc = ml[g].x == -__builtin_inff() ? 0.f : expf(ml[g].x - mm);
+      odd = fmaf(ml[g].y, 0.f, odd);
+      l = fmaf(sc, ml[g].y, l);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        odd = fmaf(og[e], 0.f, odd);
+        v[e] = fmaf(sc, og[e], v[e]);
+      }
+    }
+    const int rr = tile * QT + ri, t = a.by_per(rr), hd = kv * a.per + rr - t * a.per, f = firsts.first[t - t0];
+    const bool there = i < n * LPR;
+    const uint64_t bad = __builtin_amdgcn_ballot_w64(there && f != NONE && odd != 0.f);
+    // (bits of a row's lanes: any)
+    uint64_t again = 0;
+#pragma unroll
+    for (int x = 0; x < 64 / LPR; ++x)
+      if (bad >> (x * LPR) & ((LPR < 64 ? 1ull << (LPR & 63) : 0ull) - 1)) again |= 1ull << (x * LPR);
+    if (there) {
+      float y[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = f == NONE ? 0.f : v[e] / l;
+      store_vec<float, 4>((float*)a.out + ((int64_t)t * a.Hq + hd) * D + d, y);
+    }
+    rows_again<float, D>(a, again, t, hd, f);
+  }
 }
 
 template <typename T, int D>
 int packed_launch(hipStream_t st, PackedArgs a) {
-  if constexpr (sizeof(T) == 2) {
-    a.tiles = (int)cdiv(a.rows, P_QT);
-    const int rc = ensure_lds_limit((const void*)packed_bf16_kernel<D>, Half<D>::LDS + (int)sizeof(Firsts));
+  auto go = [&](auto kern, int qt, int lds) -> int {
+    a.tiles = (int)cdiv(a.rows, qt);
+    const int rc = ensure_lds_limit((const void*)kern, lds + (int)sizeof(Firsts));
     if (rc) return rc;
-    hipLaunchKernelGGL((packed_bf16_kernel<D>), dim3((unsigned)(a.tiles * a.Hkv)), dim3(256), Half<D>::LDS, st, a);
-  } else {
-    hipLaunchKernelGGL((packed_rows_kernel<T, D>), dim3((unsigned)cdiv((int64_t)a.rows * a.Hkv, 4)), dim3(256), 0, st, a);
-  }
-  MINITP_LAUNCH_CHECK();
-  return MINITP_OK;
+    hipLaunchKernelGGL(kern, dim3((unsigned)(a.tiles * a.Hkv)), dim3(256), lds, st, a);
+    MINITP_LAUNCH_CHECK();
+    return MINITP_OK;
+  };
+  if constexpr (sizeof(T) == 2) return go(packed_bf16_kernel<D>, P_QT, Half<D>::LDS);
+  const int64_t blocks = cdiv(a.rows, 64) * a.Hkv;
+  if (blocks < 256) return go(packed_f32_kernel<D, 4>, 16, F_LDS<D>);
+  if (blocks < 512) return go(packed_f32_kernel<D, 2>, 32, F_LDS<D>);
+  return go(packed_f32_kernel<D, 1>, 64, F_LDS<D>);
 }
 
 template <typename T>
