@@ -222,13 +222,15 @@ int minitp_shared_prefix_attention(void* stream, int dtype, const void* q, const
  * sequence s is rows offsets[s] .. offsets[s + 1] - 1, offsets [S + 1] a device
  * array that does not decrease (equal neighbours: an empty sequence). Row i of
  * a sequence that begins at row a attends rows a .. i; a row before offsets[0]
- * or from offsets[S] on, of no sequence, gets zeros. A row's result does not
- * depend on any other sequence's rows, whatever they hold. q [N, Hq, D] and k,
+ * or from offsets[S] on, of no sequence, gets zeros. What rows of other
+ * sequences and later rows hold, infinities and NaN too, does not show in a
+ * row's result (its rounding may depend on the packing). q [N, Hq, D] and k,
  * v [N, Hkv, D] have strides in elements (row, head; k and v the same), whole
  * 16-byte pieces; out is [N, Hq * D]. Head h on KV head h / (Hq/Hkv), scale
  * 1/sqrt(D), D 16, 32, 64 or 128. Offsets out of order or range give rows of
- * some sequence, and no access outside the arrays. MINITP_ERR_UNSUPPORTED:
- * 2^31 rows, 2^26 (row, head) pairs, K/V rows 2^24 elements apart (fp32 2^23) and more. */
+ * some sequence, and no access outside the arrays. MINITP_ERR_UNSUPPORTED: about
+ * 2^28 (row, head) pairs, 2^31 sequences, and K/V rows more than 2^24 elements
+ * (fp32 2^23) apart. */
 int minitp_packed_attention(void* stream, int dtype, const void* q, int64_t q_row, int64_t q_head, const void* k,
                             const void* v, int64_t kv_row, int64_t kv_head, void* out, int64_t N, int64_t S,
                             int64_t Hq, int64_t Hkv, int64_t D, const int64_t* offsets);

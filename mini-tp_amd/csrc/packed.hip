@@ -13,8 +13,6 @@
 // device, and short sequences share a tile. A query's own window, first .. i, is
 // its mask; tiles of keys that every query of a wave sees are not masked, tiles
 // that none sees are left out.
-#include <type_traits>
-
 #include "attn_tiles.h"
 #include "common.h"
 #include "kernels.h"
@@ -37,45 +35,54 @@ struct PackedArgs {
 
 constexpr int NONE = INT32_MAX;  // the first row of a token of no sequence
 
-// Where the sequences of a tile's tokens begin: first[j] for token t0 + j, j <
-// n <= 256 threads, and the least of them (NONE: all are of no sequence). A
-// thread finds the offsets not above its token by bisection, the last of which
-// begins its sequence: of up to 256 offsets, every one or every so many, in LDS,
-// then of those between two of them. (Offsets in disorder give some row.)
+// Where the sequences of the tokens t0 .. t1 of a tile begin. A wave finds by
+// itself the offsets around t0: 64 of them, one a lane, narrowed down where there
+// are more, from 64 at equal distances each time. begin() is the first row of
+// t0's sequence, of(tok) of any token of the tile: the last offset not above it,
+// NONE if there is none or it is the sequences' end. (Offsets in disorder give some
+// row not past the token.) No LDS and no barrier: the first keys are on their way
+// one load after the offsets.
 struct Firsts {
-  int first[256], some[256], least;
-};
-__device__ __forceinline__ void find_firsts(const PackedArgs& a, Firsts& f, int t0, int n) {
-  const int tid = threadIdx.x, count = a.S + 1, step = (count + 255) >> 8;
-  auto offset = [&](int i) { return (int)std::min<int64_t>(std::max<int64_t>(a.offsets[i], 0), NONE); };
-  f.some[tid] = (int64_t)tid * step < count ? offset(tid * step) : NONE;
-  if (tid == 0) f.least = NONE;
-  __syncthreads();
-  if (tid < n) {
-    const int t = t0 + tid;
-    int c = 0;  // of f.some, the ones not above t
-#pragma unroll
-    for (int b = 128; b >= 1; b >>= 1)
-      if (f.some[c + b - 1] <= t) c += b;
-    c += f.some[c & 255] <= t;  // (c <= 255 so far)
-    int begin = c > 0 ? f.some[c - 1] : NONE;
-    int64_t lo = (int64_t)(c - 1) * step + 1, hi = std::min<int64_t>((int64_t)c * step, count);
-    while (c > 0 && lo < hi) {
-      const int64_t mid = (lo + hi) >> 1;
-      const int o = offset((int)mid);
-      if (o <= t) {
-        begin = o;
-        lo = mid + 1;
-      } else {
-        hi = mid;
-      }
-    }
-    if (c > 0 && lo == count) begin = NONE;  // (from the last offset on)
-    f.first[tid] = begin;
-    atomicMin(&f.least, begin);
+  uint32_t lo;   // the offset that lane 0 holds
+  int o, first;  // this lane's; that of t0
+  int t0, t1;
+  __device__ __forceinline__ int offset(const PackedArgs& a, uint32_t i) const {
+    return i <= (uint32_t)a.S ? (int)std::min<int64_t>(std::max<int64_t>(a.offsets[i], 0), NONE) : NONE;
   }
-  __syncthreads();
-}
+  __device__ __forceinline__ Firsts(const PackedArgs& a, int t0_, int t1_) : lo(0), t0(t0_), t1(t1_) {
+    const uint32_t lane = threadIdx.x & 63;
+    uint32_t span = (uint32_t)a.S + 1;
+    while (span > 64) {
+      const uint32_t step = (span + 63) / 64;
+      const uint64_t below = __builtin_amdgcn_ballot_w64(lane * step < span && offset(a, lo + lane * step) <= t0);
+      const uint32_t skip = below ? (63 - __builtin_clzll(below)) * step : 0;
+      lo += skip;
+      span = std::min(step, span - skip);
+    }
+    o = offset(a, lo + lane);
+    const uint64_t below = __builtin_amdgcn_ballot_w64(o <= t0);
+    const int at = below ? 63 - __builtin_clzll(below) : 0;
+    first = below && lo + at < (uint32_t)a.S ? __builtin_amdgcn_readlane(o, at) : NONE;
+  }
+  // keys of the tile are those from here on
+  __device__ __forceinline__ int begin() const { return first == NONE ? t0 : first; }
+  __device__ __forceinline__ int of(const PackedArgs& a, int tok) {
+    const uint32_t lane = threadIdx.x & 63;
+    int f = first;
+    for (;;) {
+      uint64_t inside = __builtin_amdgcn_ballot_w64(o > t0 && o <= t1);
+      while (inside) {
+        const int at = __builtin_ctzll(inside), b = __builtin_amdgcn_readlane(o, at);
+        inside &= inside - 1;
+        if (b <= tok) f = lo + at == (uint32_t)a.S ? NONE : b;
+      }
+      // (a run of more offsets, of short or empty sequences)
+      if (lo + 63 >= (uint32_t)a.S || __builtin_amdgcn_readlane(o, 63) > t1) return f;
+      lo += 64;
+      o = offset(a, lo + lane);
+    }
+  }
+};
 
 // One query of one head by one wave, in fp32, key by key and only those it sees:
 // a lane a key for the scores, a lane one or two dims of the output. The tile
@@ -164,9 +171,63 @@ __device__ __forceinline__ Window window_of(int tok, int first) {
   return w;
 }
 
+// The results of a tile of QT rows that KG sets of waves hold over keys of their
+// own, in LDS: po [KG][QT] rows of D, padded by 16 bytes (lanes of a wave write
+// 32 rows at a time), pml [KG][QT] (maximum, sum; exp2 or expf by BASE2), pf [QT]
+// first rows. Joined and stored by whole rows, LPR lanes a row; the ones
+// that are not finite again by packed_row.
+template <typename T, int D, int KG, int QT, bool BASE2>
+__device__ __forceinline__ void join_rows(const PackedArgs& a, int tile, int kv, const float* po, const float2* pml,
+                                          const int* pf) {
+  constexpr int LPR = D / 4;
+  const int n = std::min(QT, a.rows - tile * QT);
+  for (int i0 = 0; i0 < n * LPR; i0 += 256) {
+    const int i = i0 + threadIdx.x, row = std::min(i / LPR, n - 1), d = i % LPR * 4;
+    float m = -__builtin_inff(), l = 0.f, odd = 0.f;
+    float2 ml[KG];
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int g = 0; g < KG; ++g) {
+      ml[g] = pml[g * QT + row];
+      m = fmaxf(m, ml[g].x);
+    }
+#pragma unroll
+    for (int g = 0; g < KG; ++g) {
+      const f32x4 og = *(const f32x4*)(po + (g * QT + row) * (D + 4) + d);
+      // (a set that saw nothing weighs nothing; what is no number shows)
+      const float sc = ml[g].x == -__builtin_inff() ? 0.f
+                       : BASE2                      ? __builtin_amdgcn_exp2f(ml[g].x - m)
+                                                    : expf(ml[g].x - m);
+      odd = fmaf(ml[g].y, 0.f, odd);
+      l = fmaf(sc, ml[g].y, l);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        odd = fmaf(og[e], 0.f, odd);
+        v[e] = fmaf(sc, og[e], v[e]);
+      }
+    }
+    const int r = tile * QT + row, tok = a.by_per(r), head = kv * a.per + r - tok * a.per, first = pf[row];
+    const bool there = i < n * LPR;
+    const uint64_t bad = __builtin_amdgcn_ballot_w64(there && first != NONE && odd != 0.f);
+    uint64_t again = 0;  // (a row: its first lane)
+#pragma unroll
+    for (int x = 0; x < 64; x += LPR)
+      if (bad >> x & ((1ull << LPR) - 1)) again |= 1ull << x;
+    if (there) {
+      float y[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = first == NONE ? 0.f : v[e] / l;
+      store_vec<T, 4>((T*)a.out + ((int64_t)tok * a.Hq + head) * D + d, y);
+    }
+    rows_again<T, D>(a, again, tok, head, first);
+  }
+}
+
 // ---------------------------------------------------------------------------
-// bf16: 128 query rows a block, four waves of 32 (v_mfma_f32_32x32x16_bf16), over
-// tiles of 64 keys.
+// bf16, on v_mfma_f32_32x32x16_bf16: a wave computes 32 query rows. A block takes
+// 128 rows over tiles of 64 keys, or, where that leaves blocks too few (KG 2, 4),
+// 64 or 32 rows over tiles of 64 or 128, two or four waves a row over 32 of a
+// tile's keys each, joined at the end.
 //
 // A tile of K and V rows goes to LDS as it lies in memory, by loads that bypass
 // the registers, while the tile before it is computed (two stages, one barrier a
@@ -182,25 +243,35 @@ __device__ __forceinline__ Window window_of(int tok, int first) {
 // there, and fp32 products run at an eighth of the rate (154 against 1,261 TFLOP/s
 // of a large library product). The sums that they are divided by add the
 // unrounded ones.
-constexpr int P_QT = 128;
+template <int D, int KG>
+struct Tile {
+  using H = Half<D>;
+  static constexpr int QT = 128 / KG, KT = KG == 4 ? 128 : 64, NB = KG == 1 ? 2 : 1;  // NB: 32-key blocks of a wave
+  static constexpr int OPER = KT * H::ROWB, STAGE = 2 * OPER;
+  static constexpr int PIECES = KT / H::PIECE_ROWS, PPW = PIECES / 4;  // 1 KiB loads, of a wave
+  static constexpr int JOIN = KG == 1 ? 0 : KG * QT * (D + 4 + 2) * 4 + QT * 4;
+  static constexpr int LDS = 2 * STAGE > JOIN ? 2 * STAGE : JOIN;
+  static_assert(PPW >= 1 || PIECES == 2, "each wave loads alike, or waves 0, 1 K and waves 2, 3 V");
+};
 
 // The tiles of keys `key0` .. key0 + keys - 1 of a KV head through the two stages.
-template <int D>
+template <int D, int KG>
 struct KeyTiles {
   using H = Half<D>;
+  using TL = Tile<D, KG>;
   const char *k, *v;
   int64_t row;  // bytes between rows
   uint32_t to, koff, voff, piece;
   int keys, n;
   __device__ __forceinline__ KeyTiles(const PackedArgs& a, int kv, int key0, int keys_, char* lds)
-      : row(a.kv_row * 2), keys(keys_), n((keys_ + H_KT - 1) / H_KT) {
+      : row(a.kv_row * 2), keys(keys_), n((keys_ + TL::KT - 1) / TL::KT) {
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t at = key0 * row + kv * a.kv_head * 2;
     k = (const char*)a.k + at;
     v = (const char*)a.v + at;
     to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds + w * 1024;
     // piece w + 4 j of a tile: rows 4 PIECE_ROWS j + r; the swizzles do not depend on j
-    const int r = H::PIECE_ROWS * (H::PPW > 0 ? w : w & 1) + lane / H::CH;
+    const int r = H::PIECE_ROWS * (TL::PPW > 0 ? w : w & 1) + lane / H::CH;
     koff = r * (uint32_t)row + ((lane % H::CH) ^ H::k_swz(r)) * 16;
     voff = r * (uint32_t)row + ((lane % H::CH) ^ H::v_swz(r)) * 16;
     piece = 4 * H::PIECE_ROWS * (uint32_t)row;
@@ -208,37 +279,42 @@ struct KeyTiles {
   __device__ __forceinline__ void load(int t) const {
     if (t >= n) return;
     // rows past the last read zeros (or, where rows overlap, the last again)
-    const int bytes = (std::min(keys - t * H_KT, H_KT) - 1) * (int)row + H::ROWB;
-    const int64_t at = (int64_t)t * H_KT * row;
+    const uint32_t bytes = (std::min(keys - t * TL::KT, TL::KT) - 1) * (uint32_t)row + H::ROWB;
+    const int64_t at = (int64_t)t * TL::KT * row;
     const u32x4 kr = rows_rsrc(k + at, bytes), vr = rows_rsrc(v + at, bytes);
-    uint32_t lds = __builtin_amdgcn_readfirstlane(to + (t & 1) * H::STAGE), step = __builtin_amdgcn_readfirstlane(piece);
+    uint32_t lds = __builtin_amdgcn_readfirstlane(to + (t & 1) * TL::STAGE);
+    uint32_t step = __builtin_amdgcn_readfirstlane(piece);
     asm volatile("s_nop 4" : "+s"(lds), "+s"(step));
-    if constexpr (H::PPW == 0) {
+    if constexpr (TL::PPW == 0) {
       if (__builtin_amdgcn_readfirstlane(threadIdx.x >> 7) == 0)
         row_dma16(kr, koff, lds);
       else
         row_dma16(vr, voff, lds);
     }
 #pragma unroll
-    for (int j = 0; j < H::PPW; ++j) row_dma16(kr, koff, j * step, lds + j * 4096);
+    for (int j = 0; j < TL::PPW; ++j) row_dma16(kr, koff, j * step, lds + j * 4096);
 #pragma unroll
-    for (int j = 0; j < H::PPW; ++j) row_dma16(vr, voff, j * step, lds + H::OPER + j * 4096);
+    for (int j = 0; j < TL::PPW; ++j) row_dma16(vr, voff, j * step, lds + TL::OPER + j * 4096);
   }
 };
 
-template <int D>
+template <int D, int KG>
 __global__ __launch_bounds__(256, 2) void packed_bf16_kernel(PackedArgs a) {
   using H = Half<D>;
+  using TL = Tile<D, KG>;
   // (D = 16: the output's 32-row operand holds the 16 dims twice)
   constexpr int KS = D / 16, DB = D >= 32 ? D / 32 : 1, OC = D >= 32 ? 4 : 2;  // OC: 8-dim chunks of a block
+  constexpr int NB = TL::NB, QT = TL::QT;
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  __shared__ Firsts firsts;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n32 = lane & 31, h = lane >> 5;
+  const int strip = w % (4 / KG), sub = w / (4 / KG) * 32;  // of the rows; first of the wave's keys in a tile
   // The last rows, which see the most keys, first. (KV heads side by side: where
   // there are 1, 2, 4 or 8, an XCD's blocks, every eighth, share one's rows.)
-  const int j = a.by_hkv(blockIdx.x), kv = blockIdx.x - j * a.Hkv, tile = a.tiles - 1 - j;
-  const int r0 = tile * P_QT + w * 32, r = std::min(r0 + n32, a.rows - 1);
+  const int jb = a.by_hkv(blockIdx.x), kv = blockIdx.x - jb * a.Hkv, tile = a.tiles - 1 - jb;
+  const int t0 = a.by_per(tile * QT), t1 = a.by_per(std::min(tile * QT + QT, a.rows) - 1);
+  Firsts firsts(a, t0, t1);
+  const int r0 = tile * QT + strip * 32, r = std::min(r0 + n32, a.rows - 1);
   const int tok = a.by_per(r), head = kv * a.per + r - tok * a.per;
   bf16x8 qb[KS];
   {
@@ -246,11 +322,10 @@ __global__ __launch_bounds__(256, 2) void packed_bf16_kernel(PackedArgs a) {
 #pragma unroll
     for (int k = 0; k < KS; ++k) qb[k] = __builtin_bit_cast(bf16x8, *(const u32x4*)(q + 16 * k));
   }
-  const int t0 = a.by_per(tile * P_QT), t1 = a.by_per(std::min(tile * P_QT + P_QT, a.rows) - 1);
-  find_firsts(a, firsts, t0, t1 - t0 + 1);
-  const int key0 = __builtin_amdgcn_readfirstlane(firsts.least), first = firsts.first[tok - t0];
-  const KeyTiles<D> tiles(a, kv, key0, key0 == NONE ? 0 : t1 - key0 + 1, lds);
+  const int key0 = firsts.begin();
+  const KeyTiles<D, KG> tiles(a, kv, key0, t1 - key0 + 1, lds);
   tiles.load(0);
+  const int first = firsts.of(a, tok);
   const Window win = window_of(tok, first);
 
   f32x16 o[DB];
@@ -261,40 +336,46 @@ __global__ __launch_bounds__(256, 2) void packed_bf16_kernel(PackedArgs a) {
   float m = -__builtin_inff(), lsum = 0.f;
   const float sl2 = a.scale * 1.4426950408889634f;
 
-  // LDS bytes of this lane's operands: K row n32, chunk 2 k + h; V rows
-  // 4 h + (lane % 16) / 4 (+ 8), dims 32 d + 16 ((lane / 16) % 2) + 4 (lane % 4)
-  const int kat = n32 * H::ROWB, kx = (h ^ H::k_swz(n32)) << 4;
+  // LDS bytes of this lane's operands: K row sub + n32, chunk 2 k + h; V rows
+  // sub + 4 h + (lane % 16) / 4 (+ 8), dims 32 d + 16 ((lane / 16) % 2) + 4 (lane % 4)
+  // (the swizzles do not depend on sub)
+  const int kat = (sub + n32) * H::ROWB, kx = (h ^ H::k_swz(n32)) << 4;
   const int vrow = 4 * h + (lane & 15) / 4;
-  const int vat = H::OPER + vrow * H::ROWB + 8 * (lane & 1);
+  const int vat = TL::OPER + (sub + vrow) * H::ROWB + 8 * (lane & 1);
   const int vx = (((D >= 32 ? 2 * ((lane >> 4) & 1) : 0) + ((lane >> 1) & 1)) ^ H::v_swz(vrow)) << 4;
   arrived(qb);
 
-  auto compute = [&](const char* st, int key, bool masked) {
-    f32x16 s[2];
+  for (int t = 0; t < tiles.n; ++t) {
+    stage_wait();
+    tiles.load(t + 1);  // (the stage's readers passed the barrier)
+    const int key = key0 + t * TL::KT + sub, last = key + 32 * NB - 1;
+    if (key > win.to || last < win.from) continue;
+    const char* st = lds + (t & 1) * TL::STAGE;
+    f32x16 s[NB];
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
+    for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[kb][i] = 0.f;
 #pragma unroll
     for (int k = 0; k < KS; ++k) {
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {  // (two chains in turn)
+      for (int kb = 0; kb < NB; ++kb) {  // (two chains in turn)
         const bf16x8 kf = __builtin_bit_cast(bf16x8, *(const uint4*)(st + kat + kb * 32 * H::ROWB + ((32 * k) ^ kx)));
         s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qb[k], s[kb], 0, 0, 0);
       }
     }
-    if (masked) {
+    if (key < win.all_from || last > win.all_to) {
       // lane (query, h) holds keys 32 kb + 8 (i / 4) + 4 h + i % 4 and sees first .. tok
       const uint32_t base = (uint32_t)(key + 4 * h) - (uint32_t)first, most = (uint32_t)tok - (uint32_t)first;
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
+      for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
         for (int i = 0; i < 16; ++i)
           if (base + (32 * kb + 8 * (i / 4) + i % 4) > most) s[kb][i] = -__builtin_inff();
     }
     float mx = s[0][0];
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
+    for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
       for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kb][i]);
     mx = halves_max(mx) * sl2;
@@ -307,7 +388,7 @@ __global__ __launch_bounds__(256, 2) void packed_bf16_kernel(PackedArgs a) {
     }
     const float mref = m == -__builtin_inff() ? 0.f : m;  // (nothing seen yet)
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
+    for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         s[kb][i] = __builtin_amdgcn_exp2f(fmaf(s[kb][i], sl2, -mref));
@@ -315,9 +396,9 @@ __global__ __launch_bounds__(256, 2) void packed_bf16_kernel(PackedArgs a) {
       }
     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-    for (int jj = 0; jj < 4; ++jj) {  // keys 16 jj .. 16 jj + 15
-      const f32x16& p = s[jj / 2];
-      const int b = 8 * (jj % 2);
+    for (int j = 0; j < 2 * NB; ++j) {  // keys 16 j .. 16 j + 15
+      const f32x16& p = s[j / 2];
+      const int b = 8 * (j % 2);
       uint4 pk;
       pk.x = pack_bf16x2(p[b], p[b + 1]);
       pk.y = pack_bf16x2(p[b + 2], p[b + 3]);
@@ -326,30 +407,42 @@ __global__ __launch_bounds__(256, 2) void packed_bf16_kernel(PackedArgs a) {
       const bf16x8 pb = __builtin_bit_cast(bf16x8, pk);
 #pragma unroll
       for (int d = 0; d < DB; ++d) {
-        const char* vp = st + vat + 16 * jj * H::ROWB + ((64 * d) ^ vx);
+        const char* vp = st + vat + 16 * j * H::ROWB + ((64 * d) ^ vx);
         const bf16x8 vf = join8(read_tr(vp), read_tr(vp + 8 * H::ROWB));
         o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pb, o[d], 0, 0, 0);
       }
     }
     __builtin_amdgcn_s_setprio(0);
-  };
-  for (int t = 0; t < tiles.n; ++t) {
-    stage_wait();
-    tiles.load(t + 1);  // (the stage's readers passed the barrier)
-    const int key = key0 + t * H_KT, last = key + H_KT - 1;
-    if (key > win.to || last < win.from) continue;
-    compute(lds + (t & 1) * H::STAGE, key, key < win.all_from || last > win.all_to);
   }
 
+  const float l = halves_sum(lsum);
+  if constexpr (KG > 1) {
+    float* po = (float*)lds;                          // [KG][QT][D + 4]
+    float2* pml = (float2*)(po + KG * QT * (D + 4));  // [KG][QT]
+    int* pf = (int*)(pml + KG * QT);                  // [QT]
+    const int row = strip * 32 + n32, at = w / (4 / KG) * QT + row;
+    __syncthreads();  // (every stage is free)
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int c = 0; c < OC; ++c)
+        *(f32x4*)(po + at * (D + 4) + 32 * d + 8 * c + 4 * h) =
+            f32x4{o[d][4 * c], o[d][4 * c + 1], o[d][4 * c + 2], o[d][4 * c + 3]};
+    if (h == 0) pml[at] = make_float2(m, l);
+    if (h == 0 && sub == 0) pf[row] = first;
+    __syncthreads();
+    join_rows<bf16, D, KG, QT, true>(a, tile, kv, po, pml, pf);
+    return;
+  }
   if (r0 >= a.rows) return;
-  const float l = halves_sum(lsum), f = first == NONE ? 0.f : 1.f / l;
+  const bool there = r0 + n32 < a.rows;
+  const float f = 1.f / l;  // (a query that saw nothing above minus infinity: NaN)
   float odd = l * 0.f;
 #pragma unroll
   for (int d = 0; d < DB; ++d)
 #pragma unroll
     for (int i = 0; i < 16; ++i) odd = fmaf(o[d][i], 0.f, odd);
-  // (a query that saw nothing but minus infinity is NaN here, as it should be)
-  if (r0 + n32 < a.rows) {
+  if (there) {
     bf16* orow = (bf16*)a.out + ((int64_t)tok * a.Hq + head) * D + 4 * h;
 #pragma unroll
     for (int d = 0; d < DB; ++d)
@@ -361,7 +454,7 @@ __global__ __launch_bounds__(256, 2) void packed_bf16_kernel(PackedArgs a) {
         store_vec<bf16, 4>(orow + 32 * d + 8 * c, v);
       }
   }
-  const uint64_t bad = __builtin_amdgcn_ballot_w64(odd != 0.f && first != NONE && r0 + n32 < a.rows);
+  const uint64_t bad = __builtin_amdgcn_ballot_w64(odd != 0.f && first != NONE && there);
   rows_again<bf16, D>(a, (uint32_t)(bad | bad >> 32), tok, head, first);
 }
 
@@ -383,13 +476,14 @@ __global__ __launch_bounds__(256, 2) void packed_f32_kernel(PackedArgs a) {
   constexpr int E = D / 16 < 4 ? D / 16 : 4, HALVES = D / 16 / E;
   constexpr int ROW = D + 4;
   constexpr int PIECES = KT * D / 4, PER = (PIECES + 255) / 256;
-  static_assert(F_LDS<D> >= 64 * (D + 2) * 4, "the waves' results fit the tiles");
+  static_assert(F_LDS<D> >= 64 * (D + 4 + 3) * 4, "the waves' results fit the tiles");
   extern __shared__ __attribute__((aligned(16))) float lds_f[];
-  __shared__ Firsts firsts;
   float *Ks = lds_f, *Vs = lds_f + KT * ROW;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lr = lane % 16, lq = lane / 16, strip = wave % SW, sub = wave / SW * KB * 16;
   const int jb = a.by_hkv(blockIdx.x), kv = blockIdx.x - jb * a.Hkv, tile = a.tiles - 1 - jb;
+  const int t0 = a.by_per(tile * QT), t1 = a.by_per(std::min(tile * QT + QT, a.rows) - 1);
+  Firsts firsts(a, t0, t1);
   const int r0 = tile * QT + strip * 16, r = std::min(r0 + lr, a.rows - 1);
   const int tok = a.by_per(r), head = kv * a.per + r - tok * a.per;
 
@@ -399,13 +493,8 @@ __global__ __launch_bounds__(256, 2) void packed_f32_kernel(PackedArgs a) {
 #pragma unroll
     for (int c = 0; c < KC; ++c) qa[c] = *(const f32x4*)(q + 16 * c + 4 * lq);
   }
-  const int t0 = a.by_per(tile * QT), t1 = a.by_per(std::min(tile * QT + QT, a.rows) - 1);
-  find_firsts(a, firsts, t0, t1 - t0 + 1);
-  const int key0 = __builtin_amdgcn_readfirstlane(firsts.least), first = firsts.first[tok - t0];
-  const int keys = key0 == NONE ? 0 : t1 - key0 + 1;
+  const int key0 = firsts.begin(), keys = t1 - key0 + 1;
   const int64_t row = a.kv_row * 4, at0 = key0 * row + kv * a.kv_head * 4;
-  const Window win = window_of(tok, first);
-
   f32x4 o[HALVES][E];
 #pragma unroll
   for (int hf = 0; hf < HALVES; ++hf)
@@ -426,7 +515,9 @@ __global__ __launch_bounds__(256, 2) void packed_f32_kernel(PackedArgs a) {
       vr[u] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(vrs, off, 0, 0));
     }
   };
-  if (keys > 0) load_tile(0);
+  load_tile(0);
+  const int first = firsts.of(a, tok);
+  const Window win = window_of(tok, first);
   for (int k0 = 0; k0 < keys; k0 += KT) {
     __syncthreads();  // the previous tile is consumed
 #pragma unroll
@@ -515,8 +606,9 @@ __global__ __launch_bounds__(256, 2) void packed_f32_kernel(PackedArgs a) {
   // o[hf][j][x]: dim 64 hf + E (4 lq + x) + j of the lane's query; the KW waves of
   // a strip joined through LDS, and stored from there by whole rows
   lsum = quads_sum(lsum);
-  float* po = lds_f;                       // [KW][QT][D]
-  float2* pml = (float2*)(po + 64 * D);    // [KW][QT]
+  float* po = lds_f;                           // [KW][QT][D + 4]
+  float2* pml = (float2*)(po + 64 * (D + 4));  // [KW][QT]
+  int* pf = (int*)(pml + 64);                  // [QT]
   const int at = wave / SW * QT + strip * 16 + lr;
   __syncthreads();  // (the last tile is consumed)
 #pragma unroll
@@ -524,82 +616,68 @@ __global__ __launch_bounds__(256, 2) void packed_f32_kernel(PackedArgs a) {
 #pragma unroll
     for (int x = 0; x < 4; ++x)
 #pragma unroll
-      for (int j = 0; j < E; ++j) po[at * D + 64 * hf + E * (4 * lq + x) + j] = o[hf][j][x];
+      for (int j = 0; j < E; ++j) po[at * (D + 4) + 64 * hf + E * (4 * lq + x) + j] = o[hf][j][x];
   if (lq == 0) pml[at] = make_float2(m, lsum);
+  if (lq == 0 && sub == 0) pf[strip * 16 + lr] = first;
   __syncthreads();
-  // LPR lanes a row; rows that are not finite are left to packed_row
-  constexpr int LPR = D / 4;
-  const int n = std::min(QT, a.rows - tile * QT);
-  for (int i0 = 0; i0 < n * LPR; i0 += 256) {
-    const int i = i0 + tid, ri = std::min(i / LPR, n - 1), d = i % LPR * 4;
-    float mm = -__builtin_inff(), l = 0.f;
-    float2 ml[KW];
-    f32x4 v = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int g = 0; g < KW; ++g) {
-      ml[g] = pml[g * QT + ri];
-      mm = fmaxf(mm, ml[g].x);
-    }
-    float odd = 0.f;
-#pragma unroll
-    for (int g = 0; g < KW; ++g) {
-      const f32x4 og = *(const f32x4*)(po + (g * QT + ri) * D + d);
-      // (a wave that saw nothing weighs nothing; a sum that is no number shows)
-      const float sc = ml[g].x == -__builtin_inff() ? 0.f : expf(ml[g].x - mm);
-      odd = fmaf(ml[g].y, 0.f, odd);
-      l = fmaf(sc, ml[g].y, l);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        odd = fmaf(og[e], 0.f, odd);
-        v[e] = fmaf(sc, og[e], v[e]);
-      }
-    }
-    const int rr = tile * QT + ri, t = a.by_per(rr), hd = kv * a.per + rr - t * a.per, f = firsts.first[t - t0];
-    const bool there = i < n * LPR;
-    const uint64_t bad = __builtin_amdgcn_ballot_w64(there && f != NONE && odd != 0.f);
-    // (bits of a row's lanes: any)
-    uint64_t again = 0;
-#pragma unroll
-    for (int x = 0; x < 64 / LPR; ++x)
-      if (bad >> (x * LPR) & ((LPR < 64 ? 1ull << (LPR & 63) : 0ull) - 1)) again |= 1ull << (x * LPR);
-    if (there) {
-      float y[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] = f == NONE ? 0.f : v[e] / l;
-      store_vec<float, 4>((float*)a.out + ((int64_t)t * a.Hq + hd) * D + d, y);
-    }
-    rows_again<float, D>(a, again, t, hd, f);
+  join_rows<float, D, KW, QT, false>(a, tile, kv, po, pml, pf);
+}
+
+// Sets of waves a row (bf16 KG, fp32 KW) from what the host knows: blocks of 128
+// rows and the mean length; the rest is on the device. Measured (us, graph
+// replays, one against two against four sets; n x L: n sequences of L tokens):
+// bf16: four where the blocks, four times as many, do not outnumber the places by
+//   much and the sequences are longer than a tile; two for few long sequences.
+//   0.5B heads (D 64): 2x64 (14 blocks) 5.7 5.9 5.3, 10x100 (110) 6.4 7.0 6.9, 1x500
+//   (56) 10.4 9.7 7.2, 5x300 (166) 9.6 10.5 11.5, 2x1300 (286) 26.2 24.7 22.5, 3x1300
+//   (428) 32.0 29.1 30.2, 8x500 (438) 16.4 17.9 22.8. 7B heads (128): 1x200 (44) 10.7
+//   10.2 8.4, 3x200 (132) 12.0 11.8 18.7 (a block a CU), 1x1300 (288) 38.0 28.2 51.6,
+//   3x500 (332) 21.1 23.6 42.0, 1x4096 (896) 129 153 304.
+// fp32, bound by its products sooner: 0.5B heads 1x512 (56) 30.8 19.6 15.2, 10x300
+//   (330) 44.7 34.7 35.8, 100x100 (1,094) 53.0 51.6 59.7; 7B heads 1x512 (112) 52.6 39.1
+//   39.0, 1x1024 (224) 117 99 108, 1x3000 (660) 625 654 763, 50x20 (220) 20.2 22.6 25.8.
+int packed_sets(bool half, int D, int64_t rows, int64_t heads, int64_t tokens, int64_t sequences) {
+  const int64_t blocks = cdiv(rows, 128) * heads, mean = tokens / std::max<int64_t>(sequences, 1);
+  if (half) {
+    if (mean >= 64 && blocks <= std::min<int64_t>(64 + (D < 128 ? mean * 64 / (5 * D) : 0), 20480 / D)) return 4;
+    return mean >= 300 && blocks <= std::min<int64_t>(mean * 2 / 5, 512) ? 2 : 1;
   }
+  if (mean < 64 && blocks > 128) return 1;
+  return blocks * D <= 16384 ? 4 : blocks * D <= 45056 ? 2 : 1;
 }
 
 template <typename T, int D>
-int packed_launch(hipStream_t st, PackedArgs a) {
+int packed_launch(hipStream_t st, PackedArgs a, int sets) {
   auto go = [&](auto kern, int qt, int lds) -> int {
     a.tiles = (int)cdiv(a.rows, qt);
-    const int rc = ensure_lds_limit((const void*)kern, lds + (int)sizeof(Firsts));
+    const int rc = ensure_lds_limit((const void*)kern, lds);
     if (rc) return rc;
     hipLaunchKernelGGL(kern, dim3((unsigned)(a.tiles * a.Hkv)), dim3(256), lds, st, a);
     MINITP_LAUNCH_CHECK();
     return MINITP_OK;
   };
-  if constexpr (sizeof(T) == 2) return go(packed_bf16_kernel<D>, P_QT, Half<D>::LDS);
-  const int64_t blocks = cdiv(a.rows, 64) * a.Hkv;
-  if (blocks < 256) return go(packed_f32_kernel<D, 4>, 16, F_LDS<D>);
-  if (blocks < 512) return go(packed_f32_kernel<D, 2>, 32, F_LDS<D>);
-  return go(packed_f32_kernel<D, 1>, 64, F_LDS<D>);
+  if constexpr (sizeof(T) == 2) {
+    if (sets == 4) return go(packed_bf16_kernel<D, 4>, 32, Tile<D, 4>::LDS);
+    if (sets == 2) return go(packed_bf16_kernel<D, 2>, 64, Tile<D, 2>::LDS);
+    return go(packed_bf16_kernel<D, 1>, 128, Tile<D, 1>::LDS);
+  } else {
+    if (sets == 4) return go(packed_f32_kernel<D, 4>, 16, F_LDS<D>);
+    if (sets == 2) return go(packed_f32_kernel<D, 2>, 32, F_LDS<D>);
+    return go(packed_f32_kernel<D, 1>, 64, F_LDS<D>);
+  }
 }
 
 template <typename T>
-int packed_by_d(hipStream_t st, const PackedArgs& a, int64_t D) {
+int packed_by_d(hipStream_t st, const PackedArgs& a, int64_t D, int sets) {
   switch (D) {
     case 16:
-      return packed_launch<T, 16>(st, a);
+      return packed_launch<T, 16>(st, a, sets);
     case 32:
-      return packed_launch<T, 32>(st, a);
+      return packed_launch<T, 32>(st, a, sets);
     case 64:
-      return packed_launch<T, 64>(st, a);
+      return packed_launch<T, 64>(st, a, sets);
     default:
-      return packed_launch<T, 128>(st, a);
+      return packed_launch<T, 128>(st, a, sets);
   }
 }
 
@@ -612,8 +690,9 @@ int packed_check(int dtype, const PackedShape& s) {
     set_error("packed_attention: head_dim %lld not supported (16, 32, 64, 128)", (long long)s.D);
     return MINITP_ERR_UNSUPPORTED;
   }
-  constexpr int64_t MOST = 1LL << 31;
-  if (s.N >= MOST - 256 || s.S >= MOST - 1 || s.Hq >= MOST || s.N * s.Hq >= (1LL << 26)) {
+  // (query rows are counted in 31 bits; a block of 256 threads takes 16 at least)
+  constexpr int64_t MOST = 1LL << 28;
+  if (s.N >= MOST || s.Hq >= MOST || s.N * s.Hq >= MOST - 16 * s.Hkv || s.S >= (1LL << 31) - 64) {
     set_error("packed_attention: %lld rows of %lld heads in %lld sequences are too many for one call", (long long)s.N,
               (long long)s.Hq, (long long)s.S);
     return MINITP_ERR_UNSUPPORTED;
@@ -647,7 +726,8 @@ int launch_packed_attention(hipStream_t st, int dtype, const PackedShape& s, con
   a.by_hkv = make_div(s.Hkv);
   a.offsets = offsets;
   a.scale = 1.0f / sqrtf((float)s.D);
-  return dtype == MINITP_F32 ? packed_by_d<float>(st, a, s.D) : packed_by_d<bf16>(st, a, s.D);
+  const int sets = packed_sets(dtype == MINITP_BF16, (int)s.D, a.rows, s.Hkv, s.N, s.S);
+  return dtype == MINITP_F32 ? packed_by_d<float>(st, a, s.D, sets) : packed_by_d<bf16>(st, a, s.D, sets);
 }
 
 }  // namespace minitp
