@@ -24,7 +24,8 @@ namespace {
 constexpr int T_ROW = 256, NC = 4;  // threads of a row or slice; 16-byte chunks a thread and turn
 constexpr int SET = 64;             // logits of a set
 constexpr int LIST = 1024;          // sets, then tokens, that are ranked at once
-constexpr int ROW_SETS = 2560;      // sets of a row that one block takes
+constexpr int NSETS = 10;           // sets that a thread keeps
+constexpr int ROW_SETS = NSETS * T_ROW;  // ... a row that one block takes
 
 template <typename T>
 constexpr int TURN = T_ROW * NC * Vec<T>::N;  // logits of a turn
@@ -69,6 +70,27 @@ __device__ __forceinline__ uint32_t order_of(float x) {
 }
 __device__ __forceinline__ uint64_t order_key(float x, uint32_t place) { return (uint64_t)order_of(x) << 32 | (uint32_t)~place; }
 
+// The logit of a key (a NaN for any).
+__device__ __forceinline__ float logit_of(uint64_t key) {
+  const uint32_t o = (uint32_t)(key >> 32);
+  return o == 0xffffffffu ? __builtin_nanf("") : __uint_as_float(o >> 31 ? o ^ 0x80000000u : ~o);
+}
+
+// log2 of z > 0 (NaN of one): with z = 2^e m, m around 1 and s = (m - 1) / (m + 1),
+// log m = 2 (s + s^3 / 3 + s^5 / 5 + ...), |s| < 0.172: terms up to s^15 leave 1e-14.
+__device__ __forceinline__ double log2_of(double z) {
+  double m = __builtin_amdgcn_frexp_mant(z);  // [0.5, 1)
+  int e = __builtin_amdgcn_frexp_exp(z);
+  const bool low = m < 0.70710678118654752;
+  m = low ? m + m : m;
+  e -= low;
+  const double s = (m - 1.0) / (m + 1.0), q = s * s;
+  double y = 1.0 / 15;
+#pragma unroll
+  for (int i = 13; i >= 1; i -= 2) y = fma(y, q, 1.0 / i);
+  return (double)e + 2.0 / LN2 * s * y;
+}
+
 __device__ __forceinline__ float max_nan(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
 // A row as 16-byte chunks from the boundary at or below its first logit, `skip`
@@ -86,29 +108,31 @@ struct Row {
 };
 
 // The logits of a turn, from chunk c0 on: x[u] is chunk c0 + 256 u + thread.
-// Whole chunks come by 16-byte loads; the row's first and last, if they are not
-// whole, logit by logit; minus infinity stands for what is outside the row.
+// Whole chunks come by 16-byte loads (ask), the row's first and last, if they are
+// not whole, logit by logit (take); minus infinity stands for what is outside the
+// row.
 template <typename T>
-__device__ __forceinline__ void load_turn(const Row<T>& r, int64_t c0, float (*x)[Vec<T>::N]) {
-  constexpr int VE = Vec<T>::N;
-  const int tid = threadIdx.x;
-  const int64_t first = r.skip ? 1 : 0, end = ((int64_t)r.V + r.skip) / VE;  // whole chunks
-  const bool edge = c0 < first || c0 + T_ROW * NC > end;                     // (uniform)
-  const int n = (int)std::min<int64_t>(end - c0, T_ROW * NC);
-  const __amdgpu_buffer_rsrc_t rs = span_rsrc(r.x - r.skip + c0 * VE, n > 0 ? (uint32_t)n * 16 : 0);
-  u32x4 raw[NC];
+__device__ __forceinline__ void ask_turn(const Row<T>& r, int64_t c0, u32x4 (&raw)[NC]) {
+  const int64_t end = ((int64_t)r.V + r.skip) / Row<T>::VE;  // past the whole chunks
+  const int n = (int)std::max<int64_t>(std::min<int64_t>(end - c0, T_ROW * NC), 0);
+  const __amdgpu_buffer_rsrc_t rs = span_rsrc(r.x - r.skip + c0 * Row<T>::VE, (uint32_t)n * 16);
 #pragma unroll
   for (int u = 0; u < NC; ++u) {
-    const int c = u * T_ROW + tid;
+    const uint32_t c = u * T_ROW + threadIdx.x;
     raw[u] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
-                                           rs, edge && c0 + c < first ? 0xffffffffu : (uint32_t)c * 16, 0, 0));
+                                           rs, r.skip != 0 && c0 + c == 0 ? 0xffffffffu : c * 16, 0, 0));
   }
+}
+template <typename T>
+__device__ __forceinline__ void take_turn(const Row<T>& r, int64_t c0, const u32x4 (&raw)[NC], float (*x)[Vec<T>::N]) {
+  constexpr int VE = Vec<T>::N;
+  const int64_t first = r.skip ? 1 : 0, end = ((int64_t)r.V + r.skip) / VE;  // whole chunks
 #pragma unroll
   for (int u = 0; u < NC; ++u) unpack16(make_uint4(raw[u].x, raw[u].y, raw[u].z, raw[u].w), x[u], (T*)nullptr);
-  if (!edge) return;
+  if (c0 >= first && c0 + T_ROW * NC <= end) return;  // (uniform)
 #pragma unroll
   for (int u = 0; u < NC; ++u) {
-    const int64_t c = c0 + u * T_ROW + tid;
+    const int64_t c = c0 + u * T_ROW + threadIdx.x;
     if (c >= first && c < end) continue;
 #pragma unroll
     for (int e = 0; e < VE; ++e) {
@@ -126,6 +150,8 @@ __device__ __forceinline__ void scan(const LogprobArgs& a, const Row<T>& r, int6
   constexpr int VE = Vec<T>::N, LPS = SET / VE;  // lanes of a set
   const int tid = threadIdx.x, lane = tid & 63;
   const float ninf = -__builtin_inff();
+  u32x4 raw[NC];
+  ask_turn<T>(r, c0, raw);
   // the token's logit and, for logits before it, which it stands in front of only
   // if they are smaller, the number just below (a token outside: NaN, none ahead)
   const int64_t t = a.tokens[b];
@@ -139,7 +165,8 @@ __device__ __forceinline__ void scan(const LogprobArgs& a, const Row<T>& r, int6
   int ahead = 0;
   for (int turn = 0; turn < turns; ++turn, c0 += T_ROW * NC) {
     float x[NC][VE];
-    load_turn<T>(r, c0, x);
+    take_turn<T>(r, c0, raw, x);
+    if (turn + 1 < turns) ask_turn<T>(r, c0 + T_ROW * NC, raw);
     float cm[NC];
 #pragma unroll
     for (int u = 0; u < NC; ++u) {
@@ -219,43 +246,45 @@ struct Finish {
   uint64_t group[64], limit, wave_key[4];
   uint64_t key[LIST];
   uint32_t sel[32];
-  double lz, wave_sum[4][2], ms;  // log2 Z, its reference taken in; sum of 2^d d over Z
-  double ref;
+  double z, s, ref, wave_sum[4][2];  // sums of 2^d and 2^d d, d = x log2(e) - ref
   float top;
-  int ahead, count;
+  int ahead, sets, tokens;  // sets, tokens: listed
 };
 
+template <int CTRL>
+__device__ __forceinline__ uint64_t quad_of(uint64_t v) {
+  const int lo = (int)(uint32_t)v, hi = (int)(uint32_t)(v >> 32);
+  return (uint64_t)(uint32_t)__builtin_amdgcn_update_dpp(0, hi, CTRL, 0xf, 0xf, true) << 32 |
+         (uint32_t)__builtin_amdgcn_update_dpp(0, lo, CTRL, 0xf, 0xf, true);
+}
+
 // The k-th largest of the 64 groups' best keys, 4 threads a group: at least k of
-// the keys that the threads look through are not below it. 0: fewer groups have any.
+// the keys that the threads look through are not below it. ABSENT: fewer groups
+// have any. (f.limit is ABSENT before the call; keys from there on are all different.)
+constexpr uint64_t ABSENT = 1ull << 32;
 __device__ __forceinline__ uint64_t kth_of_groups(Finish& f, uint64_t mine, int k) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  mine = std::max<uint64_t>(mine, __shfl_xor(mine, 1, 64));
-  mine = std::max<uint64_t>(mine, __shfl_xor(mine, 2, 64));
-  __syncthreads();
+  mine = std::max(mine, quad_of<0xB1>(mine));  // quad_perm [1,0,3,2]
+  mine = std::max(mine, quad_of<0x4E>(mine));  // quad_perm [2,3,0,1]
   if (lane % 4 == 0) f.group[tid / 4] = mine;
-  if (tid == 0) {
-    f.limit = 0;
-    f.count = 0;
-  }
   __syncthreads();
   const uint64_t u = f.group[lane];
-#pragma unroll
+#pragma unroll 4
   for (int i = 0; i < 16; ++i) {
     const uint64_t v = f.group[wave * 16 + i];
-    // (keys above 0 are all different)
-    if (__builtin_popcountll(__builtin_amdgcn_ballot_w64(u > v)) == k - 1 && v > 0 && lane == 0) f.limit = v;
+    if (__builtin_popcountll(__builtin_amdgcn_ballot_w64(u > v)) == k - 1 && v > ABSENT && lane == 0) f.limit = v;
   }
   __syncthreads();
   return f.limit;
 }
 
-// Ranks of the f.count keys listed, a thread a key: put(rank, key) for those below k.
+// Ranks of the n keys listed, a thread a key: put(rank, key) for those below k.
 template <typename F>
-__device__ __forceinline__ void rank_list(Finish& f, int k, F put) {
-  const int n = f.count;
+__device__ __forceinline__ void rank_list(const Finish& f, int n, int k, F put) {
   for (int i = threadIdx.x; i < n; i += T_ROW) {
     const uint64_t mine = f.key[i];
     int ahead = 0;
+#pragma unroll 4
     for (int j = 0; j < n; ++j) ahead += f.key[j] > mine;
     if (ahead < k) put(ahead, mine);
   }
@@ -271,6 +300,7 @@ __device__ __forceinline__ void scan_again(const Row<T>& r, Finish& f, int64_t t
   const uint64_t key = order_key(mine, (uint32_t)t);
   double z = 0.0, s = 0.0;
   int ahead = 0;
+#pragma unroll 1
   for (int64_t i = tid; i < r.V; i += T_ROW) {
     const float x = load_f32<T>(r.x, i), d = fmaxf((x - m) * LOG2E, -200.f), p = __builtin_amdgcn_exp2f(d);
     z += (double)p;
@@ -297,38 +327,49 @@ __device__ __forceinline__ void scan_again(const Row<T>& r, Finish& f, int64_t t
     // (no number unless the maximum is one: minus infinity less itself is none)
     const bool none = !(fabsf(m) < __builtin_inff());
     f.ref = (double)m * (double)LOG2E;
-    f.lz = none ? __builtin_nan("") : log2(z);
-    f.ms = s / z;
+    f.z = none ? __builtin_nan("") : z;
+    f.s = s;
   }
   __syncthreads();
 }
 
-// The row's outputs from its n parts and its sets' maxima.
+// The row's outputs from its n parts and its sets' maxima. All latency: every load
+// of a step is asked for before the first is used, and what few rows take is kept
+// out of the straight line.
 template <typename T>
 __device__ __forceinline__ void finish_row(const LogprobArgs& a, int64_t b, const Part* parts, int n,
                                            const float* set_top, Finish& f) {
   const Row<T> r(a, b);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, k = a.top;
+  const int sets = (int)(((int64_t)r.V + r.skip + SET - 1) / SET);
+  float first[NSETS];  // the row's first ROW_SETS sets
+  if (k > 0) {
+#pragma unroll
+    for (int u = 0; u < NSETS; ++u) first[u] = set_top[std::min(u * T_ROW + tid, sets - 1)];
+  }
   const int64_t t = a.tokens[b];
+  Part p = parts[std::min(lane, n - 1)];
   const bool given = t >= 0 && t < r.V;
-  const float xt = given ? load_f32<T>(r.x, t) : 0.f;
-  if (wave == 0) {
+  const float xt = load_f32<T>(r.x, given ? t : 0);
+  auto join_parts = [&]() {  // by one wave
     float ref = -__builtin_inff(), top = ref;
-    int ahead = 0;
-    for (int i = lane; i < n; i += 64) {
-      ref = fmaxf(ref, parts[i].ref);
-      top = max_nan(top, parts[i].top);
-      ahead += parts[i].ahead;
-    }
-    ref = wave_max(ref);
     double z = 0.0, s = 0.0;
+    int ahead = 0;
+#pragma unroll 1
     for (int i = lane; i < n; i += 64) {
-      const Part p = parts[i];
-      const float off = p.ref - ref, w = p.ref == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(off);
-      if (!(w > 0.f)) continue;
-      z += (double)w * p.z;
-      s += (double)w * ((double)off * p.z + p.s);
+      if (i >= 64) p = parts[i];
+      top = max_nan(top, p.top);
+      ahead += p.ahead;
+      if (p.ref == -__builtin_inff()) continue;
+      const float to = fmaxf(ref, p.ref), off = p.ref - to, w = __builtin_amdgcn_exp2f(off);
+      const float off0 = ref - to, w0 = ref == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(off0);
+      s = (w0 > 0.f ? (double)w0 * ((double)off0 * z + s) : 0.0) + (double)w * ((double)off * p.z + p.s);
+      z = (double)w0 * z + (double)w * p.z;
+      ref = to;
     }
+    const float to = wave_max(ref), off = ref - to, w = ref == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(off);
+    s = w > 0.f ? (double)w * ((double)off * z + s) : 0.0;
+    z *= (double)w;
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) {
       z += __shfl_xor(z, o, 64);
@@ -339,34 +380,65 @@ __device__ __forceinline__ void finish_row(const LogprobArgs& a, int64_t b, cons
     if (lane == 0) {
       f.top = top;
       f.ahead = ahead;
-      f.ref = ref;
-      f.lz = log2(z);
-      f.ms = s / z;
+      f.ref = to;
+      f.z = z;
+      f.s = s;
     }
-  }
-  // ---- the k first sets ---------------------------------------------------------
-  const int sets = (int)(((int64_t)r.V + r.skip + SET - 1) / SET);
+  };
+
+  constexpr int PER = 32 * SET / T_ROW;
+  uint32_t order[PER], at[PER], least = 0;  // of this thread's places in the selected sets
+  float x[PER];
   int nsel = 0;
   if (k > 0) {
-    uint64_t mine = 0;
-    for (int i = tid; i < sets; i += T_ROW) mine = std::max<uint64_t>(mine, order_key(set_top[i], i));
-    const uint64_t limit = kth_of_groups(f, mine, k);
-    for (int i = tid; i < sets; i += T_ROW) {
-      const uint64_t key = order_key(set_top[i], i);
-      if (key < limit) continue;
-      const int at = atomicAdd(&f.count, 1);
-      if (at < LIST) f.key[at] = key;
+    // ---- the first sets: k of them, or all that the groups' bound leaves ---------
+    if (tid == 0) {
+      f.limit = ABSENT;
+      f.sets = f.tokens = 0;
     }
+    uint64_t mine = 0;
+#pragma unroll
+    for (int u = 0; u < NSETS; ++u)
+      if (u * T_ROW + tid < sets) mine = std::max(mine, order_key(first[u], u * T_ROW + tid));
+#pragma unroll 4
+    for (int i = ROW_SETS + tid; i < sets; i += T_ROW) mine = std::max(mine, order_key(set_top[i], i));
+    const uint64_t limit = kth_of_groups(f, mine, k);
+    auto list_set = [&](uint64_t key) {
+      const int i = atomicAdd(&f.sets, 1);
+      if (i < LIST) f.key[i] = key;
+    };
+    uint32_t hits = 0;  // (gathered first: one copy of the code that lists)
+#pragma unroll
+    for (int u = 0; u < NSETS; ++u)
+      hits |= (u * T_ROW + tid < sets && order_key(first[u], u * T_ROW + tid) >= limit) << u;
+    while (hits) {
+      const int h = __builtin_ctz(hits);
+      hits &= hits - 1;
+      float x = first[0];
+#pragma unroll
+      for (int u = 1; u < NSETS; ++u) x = h == u ? first[u] : x;
+      list_set(order_key(x, h * T_ROW + tid));
+    }
+#pragma unroll 1
+    for (int i = ROW_SETS + tid; i < sets; i += T_ROW)
+      if (order_key(set_top[i], i) >= limit) list_set(order_key(set_top[i], i));
     __syncthreads();
-    nsel = std::min(f.count, k);
-    if (f.count <= LIST) {
-      rank_list(f, k, [&](int rank, uint64_t key) { f.sel[rank] = ~(uint32_t)key; });
+    nsel = f.sets;
+    if (nsel <= 32) {
+      if (tid < nsel) f.sel[tid] = ~(uint32_t)f.key[tid];
+    } else if (__builtin_expect(nsel <= LIST, 1)) {
+      rank_list(f, nsel, k, [&](int rank, uint64_t key) {
+        f.sel[rank] = ~(uint32_t)key;
+        if (rank == k - 1) f.limit = key;
+      });
+      nsel = k;
     } else {
       // more than the list holds (a long row whose best sets fell to few threads):
       // one set at a time
       uint64_t last = ~0ull;
       for (int i = 0; i < k; ++i) {
         uint64_t next = 0;
+#pragma unroll 1
         for (int j = tid; j < sets; j += T_ROW) {
           const uint64_t key = order_key(set_top[j], j);
           if (key < last) next = std::max(next, key);
@@ -377,48 +449,90 @@ __device__ __forceinline__ void finish_row(const LogprobArgs& a, int64_t b, cons
         if (lane == 0) f.wave_key[wave] = next;
         __syncthreads();
         last = std::max(std::max(f.wave_key[0], f.wave_key[1]), std::max(f.wave_key[2], f.wave_key[3]));
-        if (tid == 0) f.sel[i] = ~(uint32_t)last;
+        if (tid == 0) {
+          f.sel[i] = ~(uint32_t)last;
+          f.limit = last;
+        }
       }
+      nsel = k;
+    }
+    __syncthreads();
+    // ---- their tokens not below the bound's logit, while the sums are joined ------
+    least = (uint32_t)(f.limit >> 32);
+#pragma unroll
+    for (int u = 0; u < PER; ++u) {
+      if (u * T_ROW >= nsel * SET) break;  // (uniform)
+      const int j = u * T_ROW + tid;
+      const uint32_t i = f.sel[std::min(j / SET, nsel - 1)] * SET + j % SET - r.skip;
+      at[u] = j < nsel * SET && i < (uint32_t)r.V ? i : ~0u;
+      x[u] = load_f32<T>(r.x, at[u] == ~0u ? 0 : i);
+    }
+  }
+  if (wave == 3) join_parts();
+  if (k > 0) {
+    uint32_t hits = 0;
+#pragma unroll
+    for (int u = 0; u < PER; ++u) {
+      order[u] = 0;
+      if (u * T_ROW >= nsel * SET) continue;
+      order[u] = at[u] == ~0u ? 0 : order_of(x[u]);
+      hits |= (order[u] >= least) << u;
+    }
+    while (hits) {
+      const int h = __builtin_ctz(hits);
+      hits &= hits - 1;
+      uint32_t o = order[0], place = at[0];
+#pragma unroll
+      for (int u = 1; u < PER; ++u) {
+        o = h == u ? order[u] : o;
+        place = h == u ? at[u] : place;
+      }
+      const int i = atomicAdd(&f.tokens, 1);
+      if (i < LIST) f.key[i] = (uint64_t)o << 32 | (uint32_t)~place;
     }
   }
   __syncthreads();
-  const bool odd = !(fabsf(f.top) < FAR) || (given && !(xt > -__builtin_inff()));
-  if (odd) scan_again<T>(r, f, t);
+  if (__builtin_expect(!(fabsf(f.top) < FAR) || (given && !(xt > -__builtin_inff())), 0)) scan_again<T>(r, f, t);
   // log-probability of a logit: LOG2E's own error, that much of x less the mean
   // logit, is taken out again
+  const double lz = log2_of(f.z), mean = f.s / f.z;
   auto logprob = [&](float x) {
-    const double d = (double)x * (double)LOG2E - f.ref, lp = d - f.lz;
-    return (float)(LN2 * (x == -__builtin_inff() && f.lz == f.lz ? -__builtin_inf() : lp - OFF * (d - f.ms)));
+    const double d = (double)x * (double)LOG2E - f.ref;
+    const double lp = x == -__builtin_inff() && lz == lz ? d : (d - lz) - OFF * (d - mean);
+    return (float)(LN2 * lp);
   };
-  if (tid == 0) {
+  int listed = k > 0 ? f.tokens : 0;
+  if (__builtin_expect(listed > T_ROW, 0)) {
+    // many equal logits: bounded once more, by place too
+    __syncthreads();
+    if (tid == 0) {
+      f.limit = ABSENT;
+      f.tokens = 0;
+    }
+    uint64_t mine = 0;
+#pragma unroll
+    for (int u = 0; u < PER; ++u)
+      if (order[u] > 0) mine = std::max(mine, (uint64_t)order[u] << 32 | (uint32_t)~at[u]);
+    const uint64_t limit = kth_of_groups(f, mine, k);
+#pragma unroll
+    for (int u = 0; u < PER; ++u) {
+      const uint64_t key = (uint64_t)order[u] << 32 | (uint32_t)~at[u];
+      if (order[u] > 0 && key >= limit) f.key[atomicAdd(&f.tokens, 1)] = key;  // (at most 31 groups of 32, and one)
+    }
+    __syncthreads();
+    listed = f.tokens;
+  }
+  // a list entry a thread, and the row's own values by another wave's first
+  if (tid == T_ROW - 64) {
     a.logprobs[b] = given ? logprob(xt) : __builtin_nanf("");
-    a.entropy[b] = (float)(LN2 * (f.lz - f.ms));
+    a.entropy[b] = (float)(LN2 * (lz - mean));
     a.ranks[b] = given ? f.ahead : -1;
   }
-  if (k == 0) return;
-  // ---- their tokens: a thread's places in the sets, in the sets' order -------------
-  constexpr int PER = 32 * SET / T_ROW;
-  uint64_t keys[PER], mine = 0;
-#pragma unroll
-  for (int u = 0; u < PER; ++u) {
-    const int j = u * T_ROW + tid;
-    keys[u] = 0;
-    if (j < nsel * SET) {
-      const int64_t i = (int64_t)f.sel[j / SET] * SET + j % SET - r.skip;
-      if (i >= 0 && i < r.V) keys[u] = order_key(load_f32<T>(r.x, i), (uint32_t)i);
-    }
-    mine = std::max(mine, keys[u]);
-  }
-  const uint64_t limit = std::max<uint64_t>(kth_of_groups(f, mine, k), 1);
-#pragma unroll
-  for (int u = 0; u < PER; ++u)
-    if (keys[u] >= limit) f.key[atomicAdd(&f.count, 1)] = keys[u];  // (at most 31 groups of 32, and one)
-  __syncthreads();
-  rank_list(f, k, [&](int rank, uint64_t key) {
-    const uint32_t token = ~(uint32_t)key;
-    a.top_tokens[b * k + rank] = token;
-    a.top_logprobs[b * k + rank] = logprob(load_f32<T>(r.x, token));
-  });
+  if (k > 0)
+    rank_list(f, listed, k, [&](int rank, uint64_t key) {
+      a.top_tokens[b * k + rank] = (uint32_t)~(uint32_t)key;
+      a.top_logprobs[b * k + rank] = logprob(logit_of(key));
+    });
 }
 
 template <typename T, bool SETS>
