@@ -203,19 +203,39 @@ __device__ __forceinline__ void scan(const LogprobArgs& a, const Row<T>& r, int6
 #pragma unroll
     for (int u = 0; u < NC; ++u) {
       zc[u] = sc[u] = 0.f;
-      const int64_t c = c0 + u * T_ROW + tid;
-      const float than = c < tc ? below : xt;
 #pragma unroll
       for (int e = 0; e < VE; ++e) {
-        // (2^-200 is 0, and so is its product with the distance, also of minus infinity)
-        const float d = fmaxf(fmaf(x[u][e], LOG2E, -rr), -200.f), p = __builtin_amdgcn_exp2f(d);
+        const float d = fmaf(x[u][e], LOG2E, -rr), p = __builtin_amdgcn_exp2f(d);
         zc[u] += p;
         sc[u] = fmaf(p, d, sc[u]);
-        ahead += __builtin_popcountll(__builtin_amdgcn_ballot_w64(x[u][e] > than));
       }
     }
+    float st = (sc[0] + sc[1]) + (sc[2] + sc[3]);
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(st != st) != 0, 0)) {
+      // 0 times an infinite distance (a masked logit) is no number, but nothing
+      float r2 = rr;
+      asm("" : "+v"(r2));  // (so that nothing above is kept for this)
+#pragma unroll
+      for (int u = 0; u < NC; ++u) {
+        sc[u] = 0.f;
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+          const float d = fmaxf(fmaf(x[u][e], LOG2E, -r2), -200.f);
+          sc[u] = fmaf(__builtin_amdgcn_exp2f(d), d, sc[u]);
+        }
+      }
+      st = (sc[0] + sc[1]) + (sc[2] + sc[3]);
+    }
     z += (zc[0] + zc[1]) + (zc[2] + zc[3]);
-    s += (sc[0] + sc[1]) + (sc[2] + sc[3]);
+    s += st;
+#pragma unroll
+    for (int u = 0; u < NC; ++u) {
+      const int64_t c = c0 + u * T_ROW + tid;
+      const float than = c < tc ? below : xt;
+      if (__builtin_amdgcn_ballot_w64(cm[u] > than) == 0) continue;  // (mostly: likely tokens have few in front)
+#pragma unroll
+      for (int e = 0; e < VE; ++e) ahead += __builtin_popcountll(__builtin_amdgcn_ballot_w64(x[u][e] > than));
+    }
     // equal logits before the token in its own chunk
     if (tc >= c0 && tc < c0 + T_ROW * NC) {
 #pragma unroll
@@ -570,8 +590,10 @@ LogprobPlan logprob_plan(int dtype, int64_t B, int64_t V) {
   const int64_t turn = dtype == MINITP_F32 ? TURN<float> : TURN<bf16>, skip = dtype == MINITP_F32 ? 3 : 7;
   const int64_t all = cdiv(V + skip, turn), sets = cdiv(V + skip, SET);
   LogprobPlan p;
-  // slices for about 2,048 blocks, of at most 64 turns
-  p.turns = cdiv(all, std::max(std::min(all, cdiv(2048, std::max<int64_t>(B, 1))), cdiv(all, 64)));
+  // from 512 rows on a block a row (700 rows of 151,936 bf16 logits with the best five:
+  // 54.7 us, 60.9 in three slices a row and a second launch; 331: 39.5 against 37.4),
+  // below slices for about 2,048 blocks; of at most 64 turns
+  p.turns = cdiv(all, std::max(B >= 512 ? 1 : std::min(all, cdiv(2048, std::max<int64_t>(B, 1))), cdiv(all, 64)));
   p.slices = cdiv(all, p.turns);
   p.sets = cdiv(sets, 4) * 4;
   p.whole = p.slices == 1 && sets <= ROW_SETS;
