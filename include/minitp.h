@@ -432,6 +432,17 @@ typedef struct minitp_shared_prefix {
 } minitp_shared_prefix;
 int minitp_qwen2_forward_shared(void* handle, void* stream, const minitp_qwen2_step* step,
                                 const minitp_shared_prefix* prefix);
+/* One forward over packed sequences (texts of different lengths in one pass; no
+ * counterpart in the reference): the step's `tokens` ids are the rows of
+ * `sequences` sequences, sequence s in rows offsets[s] .. offsets[s + 1] - 1
+ * (device array, as minitp_packed_attention takes it), each attending its own
+ * rows; positions [tokens] give each row's place in its sequence. The step has
+ * batch 1, cache_len 0 and no token pick; its caches [L, 1, Hkv, max_seq, D]
+ * receive the rows' keys and values, its logits are not used. hidden [tokens,
+ * H] receives the final norm's rows, whose product with the LM head gives the
+ * logits of any of them. Direct launches. */
+int minitp_qwen2_forward_packed(void* handle, void* stream, const minitp_qwen2_step* step, const int64_t* offsets,
+                                int64_t sequences, void* hidden);
 /* Out-of-range RoPE positions (rope.py:37-45, where the reference's gather
  * raises): a forward whose position lies outside the table computes with NaN
  * rotary rows and sets a sticky error word in its workspace, because a

@@ -305,6 +305,13 @@ int packed_check(int dtype, const PackedShape& s);  // what one launch does not 
 int launch_packed_attention(hipStream_t st, int dtype, const PackedShape& s, const void* q, const void* k,
                             const void* v, void* out, const int64_t* offsets);
 
+// A forward over packed sequences: where they begin, and the final norm's rows [N, H].
+struct PackedStep {
+  const int64_t* offsets;
+  int64_t sequences;
+  void* hidden;
+};
+
 // logprobs.hip
 constexpr int TOP_MAX = 32;  // best tokens of a row
 struct TokenLogprobs {

@@ -223,14 +223,16 @@ struct Qwen2Program {
 
   // The launch sequence of one forward (also what a decode graph records).
   int run(hipStream_t st, const minitp_qwen2_step& s, const Ws& w, const minitp_shared_prefix* pre = nullptr) {
-    const int rc = run_model(st, s, w, pre);
+    const int rc = run_model(st, s, w, pre, nullptr);
     if (rc || s.eos_state == nullptr) return rc;
     return launch_eos_update(st, w.st, s.batch);
   }
 
-  // pre: rows in front of the caches that groups of batch rows share (direct
-  // launches only: its pointers and lengths are the call's own).
-  int run_model(hipStream_t st, const minitp_qwen2_step& s, const Ws& w, const minitp_shared_prefix* pre) {
+  // pre: rows in front of the caches that groups of batch rows share; packed: the
+  // step's tokens are packed sequences, and the final norm's rows its result
+  // (direct launches only: their pointers and lengths are the call's own).
+  int run_model(hipStream_t st, const minitp_qwen2_step& s, const Ws& w, const minitp_shared_prefix* pre,
+                const PackedStep* packed) {
     const int64_t B = s.batch, T = s.tokens, M = B * T;
     const int64_t H = c.hidden, I = c.intermediate, V = c.vocab;
     const int D = c.head_dim;
@@ -249,7 +251,7 @@ struct Qwen2Program {
     AttnShape as{(int)B, (int)T, c.heads, c.kv_heads, D, s.max_seq};
     // one-row decode: attention + o_proj in one kernel, its per-head partials
     // summed (with the residual) by the gate/up prologue
-    const bool fo = fz && T == 1 && pre == nullptr && fuse_oproj && attn_oproj_supported(c.dtype, as, H, OPROJ_SLICES) &&
+    const bool fo = fz && T == 1 && pre == nullptr && packed == nullptr && fuse_oproj && attn_oproj_supported(c.dtype, as, H, OPROJ_SLICES) &&
                     gemv_part_supported(c.dtype, H, c.heads);
     const int64_t layer_elems = B * c.kv_heads * s.max_seq * D;
     auto shared_attention = [&](int l) {
@@ -260,6 +262,11 @@ struct Qwen2Program {
                                             (const char*)s.k_cache + l * layer_elems * es(),
                                             (const char*)s.v_cache + l * layer_elems * es(), w.attn, nullptr, nullptr,
                                             pre->workspace, pre->workspace_bytes);
+    };
+    auto packed_attention = [&](int l) {
+      const PackedShape sh{T, packed->sequences, c.heads, c.kv_heads, D, q_rows(), D, D, s.max_seq * D};
+      return launch_packed_attention(st, c.dtype, sh, w.q, (const char*)s.k_cache + l * layer_elems * es(),
+                                     (const char*)s.v_cache + l * layer_elems * es(), w.attn, packed->offsets);
     };
     // Rows past the GEMV forms: plain GEMMs (the 256 x 256 MFMA tile kernel
     // or the smaller tiles, by the measured costs), gate/up with SwiGLU in the
@@ -310,8 +317,9 @@ struct Qwen2Program {
         if (rc) return rc;
         const char* kc = (const char*)s.k_cache + l * layer_elems * es();
         const char* vc = (const char*)s.v_cache + l * layer_elems * es();
-        rc = pre != nullptr ? shared_attention(l)
-             : T == 1 ? launch_decode_attention(st, c.dtype, w.q, nullptr, nullptr, w.attn, as, s.cache_len, w.st, l,
+        rc = pre != nullptr      ? shared_attention(l)
+             : packed != nullptr ? packed_attention(l)
+             : T == 1            ? launch_decode_attention(st, c.dtype, w.q, nullptr, nullptr, w.attn, as, s.cache_len, w.st, l,
                                               w.attn_ws, w.attn_ws_bytes)
                     : launch_prefill_attention(st, c.dtype, w.q, kc, vc, w.attn, as, s.cache_len, w.st, l);
         if (rc) return rc;
@@ -333,14 +341,15 @@ struct Qwen2Program {
         if (rc) return rc;
         // x += down(act), h = the next layer's input_layernorm(x) (the final norm after the last)
         const void* next_norm = l + 1 < c.num_layers ? L(l + 1, MINITP_W_LN1) : final_norm;
+        void* normed = packed != nullptr && l + 1 == c.num_layers ? packed->hidden : w.h;
         // (the final norm's weight may have any alignment, the layers' are checked
         // at creation: the kernel that adds partials wants 16 bytes)
         rc = aligned16(next_norm) ? partials(w.act, I, L(l, MINITP_W_DOWN), H, I, &pp) : MINITP_ERR_UNSUPPORTED;
         if (rc == MINITP_OK) {
-          rc = launch_add_rmsnorm_partials(st, c.dtype, w.x, pp, next_norm, w.h, H, c.eps);
+          rc = launch_add_rmsnorm_partials(st, c.dtype, w.x, pp, next_norm, normed, H, c.eps);
         } else if (rc == MINITP_ERR_UNSUPPORTED) {
           rc = lin(w.act, I, L(l, MINITP_W_DOWN), nullptr, w.h, H, H, I);
-          if (!rc) rc = launch_add_rmsnorm(st, c.dtype, w.x, w.h, next_norm, w.h, M, H, c.eps);
+          if (!rc) rc = launch_add_rmsnorm(st, c.dtype, w.x, w.h, next_norm, normed, M, H, c.eps);
         }
         if (rc) return rc;
         continue;
@@ -370,6 +379,8 @@ struct Qwen2Program {
         if ((rc = launch_decode_attention_oproj(st, c.dtype, w.q, as, w.st, l, o))) return rc;
       } else if (pre != nullptr) {
         if ((rc = shared_attention(l))) return rc;
+      } else if (packed != nullptr) {
+        if ((rc = packed_attention(l))) return rc;
       } else if (T == 1) {
         if ((rc = launch_decode_attention(st, c.dtype, w.q, nullptr, nullptr, w.attn, as, s.cache_len, w.st, l,
                                           w.attn_ws, w.attn_ws_bytes)))
@@ -431,6 +442,7 @@ struct Qwen2Program {
       split_bufs(d);
       if ((rc = launch_gemv(st, c.dtype, PRO_NONE, EPI_RESID, d))) return rc;
     }
+    if (packed != nullptr) return gemm ? MINITP_OK : launch_rmsnorm(st, c.dtype, w.x, final_norm, packed->hidden, M, H, c.eps);
     // ---- final norm, LM head, greedy pick ----------------------------------------
     // (fp32 rows past the entry forms' keep their last-position LM head on the
     // GEMM: 0.5B batch 3 91 us, 147 on the register GEMV with its argmax; every
@@ -779,6 +791,30 @@ int minitp_qwen2_forward_shared(void* handle, void* stream, const minitp_qwen2_s
                    "shared prefix: workspace %p of %lld B, %lld B needed (16-byte aligned)", prefix->workspace,
                    (long long)prefix->workspace_bytes, (long long)need);
   return p->run((hipStream_t)stream, *step, w, prefix);
+}
+
+int minitp_qwen2_forward_packed(void* handle, void* stream, const minitp_qwen2_step* step_in, const int64_t* offsets,
+                                int64_t sequences, void* hidden) {
+  MINITP_CHECK_ARG(handle != nullptr && step_in != nullptr && offsets != nullptr && hidden != nullptr, "NULL argument");
+  auto* p = (Qwen2Program*)handle;
+  MINITP_CHECK_ARG(step_in->batch == 1 && step_in->cache_len == 0 && step_in->next_tok == nullptr &&
+                       step_in->eos_state == nullptr,
+                   "forward_packed: one row of an empty cache and no token picks (batch %lld, cache_len %lld)",
+                   (long long)step_in->batch, (long long)step_in->cache_len);
+  MINITP_CHECK_ARG(sequences >= 0 && minitp::aligned16(hidden) && minitp::aligned16(step_in->k_cache) &&
+                       minitp::aligned16(step_in->v_cache),
+                   "forward_packed: %lld sequences; hidden and the caches must be 16-byte aligned", (long long)sequences);
+  minitp_qwen2_step one = *step_in;
+  one.logits = hidden;  // (the result; no logits are computed)
+  one.logits_all = 1;
+  minitp::Ws w;
+  const int rc = p->check_step(&one, w);
+  if (rc) return rc;
+  const minitp::PackedShape sh{one.tokens, sequences, p->c.heads, p->c.kv_heads, p->c.head_dim, p->q_rows(),
+                               p->c.head_dim, p->c.head_dim, one.max_seq * p->c.head_dim};
+  if (const int unfit = minitp::packed_check(p->c.dtype, sh)) return unfit;
+  const minitp::PackedStep packed{offsets, sequences, hidden};
+  return p->run_model((hipStream_t)stream, one, w, nullptr, &packed);
 }
 
 int minitp_qwen2_decode(void* handle, void* stream, const minitp_qwen2_step* step_in) {

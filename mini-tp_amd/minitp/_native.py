@@ -79,6 +79,7 @@ SIGNATURES = {
     "minitp_qwen2_workspace_bytes": (_i64, [_vp, _i64, _i64, _i64]),
     "minitp_qwen2_forward": (_int, [_vp, _vp, _vp]),
     "minitp_qwen2_forward_shared": (_int, [_vp, _vp, _vp, _vp]),
+    "minitp_qwen2_forward_packed": (_int, [_vp, _vp, _vp, _vp, _i64, _vp]),
     "minitp_qwen2_decode": (_int, [_vp, _vp, _vp]),
     "minitp_qwen2_decode_check": (_int, [_vp, _vp, _vp]),
 }

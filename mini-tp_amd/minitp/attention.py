@@ -3,7 +3,8 @@
 Module-level path: packed QKV projection, one kernel that splits q/k/v,
 applies RoPE and writes k/v into the cache, GQA attention reading KV head
 h // (Hq/Hkv) directly (no repeat_interleave copy), then o_proj. A cache with a
-shared prefix (KVCache.share_prefix) takes the shared-prefix attention instead.
+shared prefix (KVCache.share_prefix) takes the shared-prefix attention instead,
+and packed sequences (TPQwen2ForCausalLM.forward_packed) the packed one.
 """
 
 from __future__ import annotations
@@ -39,7 +40,8 @@ class TPQwen2Attention(nn.Module):
         self.use_fused_qkv = True  # ablation toggle (attention.py:47)
 
     def forward(self, x: torch.Tensor, positions: torch.Tensor, kv_cache: KVCache | None, layer_idx: int,
-                rotary: RotaryEmbedding | None = None) -> torch.Tensor:
+                rotary: RotaryEmbedding | None = None, offsets: torch.Tensor | None = None) -> torch.Tensor:
+        """offsets: x [1, N, H] holds packed sequences (kernels.packed_attention), without a cache."""
         b, t, _ = x.shape
         hq, hkv, d = self.q_heads_local, self.kv_heads_local, self.head_dim
         if hq % hkv != 0:
@@ -61,7 +63,9 @@ class TPQwen2Attention(nn.Module):
             pos = torch.arange(t, device=x.device)
         q = torch.empty(b, t, hq, d, dtype=x.dtype, device=x.device)
         K.rope_kv_write(y, q, kc, vc, cos, sin, pos, hq, hkv, cache_len)
-        if kv_cache is not None and kv_cache.prefix is not None:
+        if offsets is not None:
+            out = K.packed_attention(q[0], kc[0].transpose(0, 1), vc[0].transpose(0, 1), offsets)[None]
+        elif kv_cache is not None and kv_cache.prefix is not None:
             pre = kv_cache.prefix
             out = K.shared_prefix_attention(q, pre.k[layer_idx], pre.v[layer_idx], kc, vc, prefix_rows, cache_len)
         else:

@@ -12,6 +12,7 @@ that path runs the same kernels one op at a time.
 from __future__ import annotations
 
 import ctypes
+from collections.abc import Sequence
 
 import torch
 import torch.nn as nn
@@ -56,8 +57,8 @@ class TPQwen2DecoderLayer(nn.Module):
         self.mlp = TPQwen2MLP(cfg, ctx, init_weights=init_weights)
 
     def forward(self, x: torch.Tensor, positions: torch.Tensor, kv_cache: KVCache | None, layer_idx: int,
-                rotary: RotaryEmbedding | None = None) -> torch.Tensor:
-        x = K.add(x, self.self_attn(self.input_layernorm(x), positions, kv_cache, layer_idx, rotary))
+                rotary: RotaryEmbedding | None = None, offsets: torch.Tensor | None = None) -> torch.Tensor:
+        x = K.add(x, self.self_attn(self.input_layernorm(x), positions, kv_cache, layer_idx, rotary, offsets))
         x = K.add(x, self.mlp(self.post_attention_layernorm(x)))
         return x
 
@@ -279,6 +280,46 @@ class TPQwen2ForCausalLM(nn.Module):
         N.check(N.lib().minitp_qwen2_decode(prog.handle, N.stream(), ctypes.byref(step)), "qwen2_decode")
         kv_cache.advance(1)
         return logits
+
+    def forward_packed(self, input_ids: torch.Tensor, lengths: Sequence[int]) -> torch.Tensor:
+        """Hidden states [N, H] after the final norm of packed sequences: their
+        ids [N] one after the other, and their lengths (zeros too). No
+        counterpart in the reference, whose batches are of one length. Each
+        sequence is a prompt of its own from position 0; ``lm_head`` of a row
+        gives the logits of the token after it."""
+        lens = torch.tensor(lengths, dtype=torch.long, device="cpu")
+        n, limit = input_ids.numel(), self.cfg.max_position_embeddings
+        N.require_gpu(input_ids, self.model.embed_tokens.weight, what="TPQwen2ForCausalLM.forward_packed")
+        if input_ids.dim() != 1 or lens.dim() != 1 or bool((lens < 0).any()) or int(lens.sum()) != n:
+            raise ValueError(f"forward_packed: ids {tuple(input_ids.shape)} in sequences of {int(lens.sum())} tokens in all")
+        longest = int(lens.max()) if lens.numel() else 0
+        if longest > limit:
+            raise IndexError(f"position {longest - 1} out of range for RoPE table of {limit} rows")
+        weight = self.model.embed_tokens.weight
+        hidden = torch.empty(n, self.cfg.hidden_size, dtype=weight.dtype, device=weight.device)
+        if n == 0:
+            return hidden
+        # offsets and positions in one copy
+        offsets = torch.zeros(lens.numel() + 1, dtype=torch.long)
+        torch.cumsum(lens, 0, out=offsets[1:])
+        places = torch.arange(n) - torch.repeat_interleave(offsets[:-1], lens)
+        offsets, positions = torch.cat([offsets, places]).to(weight.device).split([lens.numel() + 1, n])
+        ids = input_ids.long().contiguous()
+        if self.native_path():
+            prog, a = self.program(), self.model.layers[0].self_attn
+            kv = KVCache(self.cfg.num_hidden_layers, 1, a.kv_heads_local, self.cfg.head_dim, n, prog.dtype, prog.device)
+            ws = prog.forward_ws(n, 1, kv.capacity)
+            step = N.Qwen2Step(ids.data_ptr(), n, positions.data_ptr(), 1, n, 0, kv.k_buf.data_ptr(), kv.v_buf.data_ptr(),
+                               kv.capacity, None, 0, None, 0, ws.data_ptr(), ws.numel(), None, 0, 0, None)
+            N.check(N.lib().minitp_qwen2_forward_packed(prog.handle, N.stream(), ctypes.byref(step), offsets.data_ptr(),
+                                                        lens.numel(), hidden.data_ptr()), "qwen2_forward_packed")
+            return hidden
+        x = self.model.embed_tokens(ids[None])
+        rotary = self._ensure_rotary(x.device) if self.use_rotary_cache else None
+        for i, layer in enumerate(self.model.layers):
+            with scope(f"mini_tp.layer_{i}"):
+                x = layer(x, positions, None, i, rotary, offsets)
+        return self.model.norm(x)[0]
 
     @staticmethod
     def _check_kv(prog: _Program, kv: KVCache, batch: int) -> None:

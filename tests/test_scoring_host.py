@@ -1,6 +1,8 @@
 """Refusals of the entry points that score texts: every invalid call is turned
 down on the host, before any pointer is used (no GPU)."""
 
+import ctypes
+
 import pytest
 import torch
 
@@ -70,3 +72,55 @@ def test_wrappers_check_their_arguments():
     for call in (lambda: K.packed_attention(q, k, k, offsets), lambda: K.token_logprobs(torch.zeros(3, 5), tokens)):
         with pytest.raises(RuntimeError, match="no CPU path"):
             call()
+
+
+def _program():
+    """A native program whose pointers no refused call looks at."""
+    cfg = N.Qwen2Config(N.BF16, 1, 64, 4, 2, 16, 128, 1000, 256, 1e-6)
+    layers = (ctypes.c_void_p * N.W_PER_LAYER)(*([P] * N.W_PER_LAYER))
+    weights = N.Qwen2Weights(P, P, P, P, P, ctypes.cast(layers, ctypes.POINTER(ctypes.c_void_p)))
+    handle = ctypes.c_void_p()
+    assert N.lib().minitp_qwen2_create(ctypes.byref(cfg), ctypes.byref(weights), ctypes.byref(handle)) == N.OK
+    return handle
+
+
+@pytest.mark.parametrize("status,change", [
+    (N.ERR_ARG, dict(offsets=None)), (N.ERR_ARG, dict(hidden=None)), (N.ERR_ARG, dict(hidden=P + 8)),
+    (N.ERR_ARG, dict(sequences=-1)), (N.ERR_ARG, dict(batch=2)), (N.ERR_ARG, dict(tokens=0)),
+    (N.ERR_ARG, dict(cache_len=1)), (N.ERR_ARG, dict(next_tok=P)), (N.ERR_ARG, dict(ids=None)),
+    (N.ERR_ARG, dict(positions=None)), (N.ERR_ARG, dict(k_cache=None)), (N.ERR_ARG, dict(v_cache=P + 2)),
+    (N.ERR_ARG, dict(workspace=None)), (N.ERR_ARG, dict(workspace_bytes=100)), (N.ERR_ARG, dict(ids_ld=5)),
+    (N.ERR_OVERFLOW, dict(max_seq=9)), (N.ERR_UNSUPPORTED, dict(sequences=1 << 31)),
+])
+def test_forward_packed_refuses(status, change):
+    handle = _program()
+    a = dict(ids=P, ids_ld=10, positions=P, batch=1, tokens=10, cache_len=0, k_cache=P, v_cache=P, max_seq=16, logits=None,
+             logits_all=0, next_tok=None, next_tok_ld=0, workspace=P, workspace_bytes=1 << 40, offsets=P, sequences=2,
+             hidden=P)
+    a.update(change)
+    offsets, sequences, hidden = a.pop("offsets"), a.pop("sequences"), a.pop("hidden")
+    step = N.Qwen2Step(**a)
+    assert N.lib().minitp_qwen2_forward_packed(handle, None, ctypes.byref(step), offsets, sequences, hidden) == status
+    assert N.last_error()
+    N.lib().minitp_qwen2_destroy(handle)
+
+
+def test_forward_packed_without_arguments():
+    assert N.lib().minitp_qwen2_forward_packed(None, None, None, None, 0, None) == N.ERR_ARG
+
+
+def test_scoring_has_no_cpu_path():
+    from minitp.config import ModelConfig
+    from minitp.distributed.context import ParallelContext
+    from minitp.layer import TPQwen2ForCausalLM
+    from minitp.scoring import score_tokens
+
+    cfg = ModelConfig(32, 48, 1, 2, 1, 16, 64, 1e-6, 1e6, 64)
+    model = TPQwen2ForCausalLM(cfg, ParallelContext(0, 0, 1, 0, 1, torch.device("cpu"), None), init_weights=False)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        score_tokens(model, [[1, 2, 3]])
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        model.forward_packed(torch.zeros(3, dtype=torch.long), [3])
+    for kw in (dict(top=-1), dict(top=33), dict(starts=[1, 1]), dict(starts=[0]), dict(max_tokens=0)):
+        with pytest.raises(ValueError):
+            score_tokens(model, [[1, 2, 3]], **kw)
