@@ -146,29 +146,17 @@ __device__ __forceinline__ void rows_again(const PackedArgs& a, uint64_t odd, in
   }
 }
 
-__device__ __forceinline__ int wave_max_int(int v) {
-  auto step = [&](int o) { v = std::max(v, o); };
-  step(__builtin_amdgcn_update_dpp(v, v, 0x111, 0xf, 0xf, false));  // row_shr:1, 2, 4, 8
-  step(__builtin_amdgcn_update_dpp(v, v, 0x112, 0xf, 0xf, false));
-  step(__builtin_amdgcn_update_dpp(v, v, 0x114, 0xf, 0xf, false));
-  step(__builtin_amdgcn_update_dpp(v, v, 0x118, 0xf, 0xf, false));
-  step(__builtin_amdgcn_update_dpp(v, v, 0x142, 0xa, 0xf, false));  // row_bcast:15, 31
-  step(__builtin_amdgcn_update_dpp(v, v, 0x143, 0xc, 0xf, false));
-  return __builtin_amdgcn_readlane(v, 63);
-}
-
 // What a wave's tile of keys needs: `from` .. `to` are keys that some of its
-// queries see, `all_from` .. `all_to` those that every one sees.
+// queries see (or more), `all_from` .. `all_to` those that every one sees (or
+// fewer). Its queries' tokens and first rows ascend with its LAST + 1 rows.
 struct Window {
   int from, to, all_from, all_to;
 };
-__device__ __forceinline__ Window window_of(int tok, int first) {
-  Window w;
-  w.from = -wave_max_int(-first);
-  w.all_from = wave_max_int(first == NONE ? -1 : first);  // (a row of no sequence: zeros whatever it sees)
-  w.all_to = __builtin_amdgcn_readfirstlane(tok);
-  w.to = wave_max_int(tok);
-  return w;
+template <int LAST>
+__device__ __forceinline__ Window window_of(int tok, int first, int key0) {
+  const int f = __builtin_amdgcn_readfirstlane(first);
+  return Window{f == NONE ? key0 : f, __builtin_amdgcn_readlane(tok, LAST), __builtin_amdgcn_readlane(first, LAST),
+                __builtin_amdgcn_readfirstlane(tok)};
 }
 
 // The results of a tile of QT rows that KG sets of waves hold over keys of their
@@ -326,7 +314,7 @@ __global__ __launch_bounds__(256, 2) void packed_bf16_kernel(PackedArgs a) {
   const KeyTiles<D, KG> tiles(a, kv, key0, t1 - key0 + 1, lds);
   tiles.load(0);
   const int first = firsts.of(a, tok);
-  const Window win = window_of(tok, first);
+  const Window win = window_of<31>(tok, first, key0);
 
   f32x16 o[DB];
 #pragma unroll
@@ -364,14 +352,22 @@ __global__ __launch_bounds__(256, 2) void packed_bf16_kernel(PackedArgs a) {
         s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qb[k], s[kb], 0, 0, 0);
       }
     }
-    if (key < win.all_from || last > win.all_to) {
-      // lane (query, h) holds keys 32 kb + 8 (i / 4) + 4 h + i % 4 and sees first .. tok
-      const uint32_t base = (uint32_t)(key + 4 * h) - (uint32_t)first, most = (uint32_t)tok - (uint32_t)first;
+    // lane (query, h) holds keys 32 kb + 8 (i / 4) + 4 h + i % 4 and sees first .. tok
+    if (last > win.all_to) {
+      const int hi = tok - key - 4 * h;
 #pragma unroll
       for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-          if (base + (32 * kb + 8 * (i / 4) + i % 4) > most) s[kb][i] = -__builtin_inff();
+          if (32 * kb + 8 * (i / 4) + i % 4 > hi) s[kb][i] = -__builtin_inff();
+    }
+    if (key < win.all_from) {  // (a row of no sequence sees nothing)
+      const int lo = first - key - 4 * h;
+#pragma unroll
+      for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (32 * kb + 8 * (i / 4) + i % 4 < lo) s[kb][i] = -__builtin_inff();
     }
     float mx = s[0][0];
 #pragma unroll
@@ -437,12 +433,20 @@ __global__ __launch_bounds__(256, 2) void packed_bf16_kernel(PackedArgs a) {
   if (r0 >= a.rows) return;
   const bool there = r0 + n32 < a.rows;
   const float f = 1.f / l;  // (a query that saw nothing above minus infinity: NaN)
-  float odd = l * 0.f;
+  float most = l;           // NaN or infinite if something is
 #pragma unroll
   for (int d = 0; d < DB; ++d)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) odd = fmaf(o[d][i], 0.f, odd);
+    for (int i = 0; i < 16; ++i) most = __builtin_elementwise_maximum(most, fabsf(o[d][i]));
+  const bool none = first == NONE;
+  if (__builtin_amdgcn_ballot_w64(none)) {  // (a select for each value, which few waves need)
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[d][i] = none ? 0.f : o[d][i];
+  }
   if (there) {
+    const float ff = none ? 0.f : f;
     bf16* orow = (bf16*)a.out + ((int64_t)tok * a.Hq + head) * D + 4 * h;
 #pragma unroll
     for (int d = 0; d < DB; ++d)
@@ -450,11 +454,11 @@ __global__ __launch_bounds__(256, 2) void packed_bf16_kernel(PackedArgs a) {
       for (int c = 0; c < OC; ++c) {
         float v[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = first == NONE ? 0.f : o[d][4 * c + e] * f;
+        for (int e = 0; e < 4; ++e) v[e] = o[d][4 * c + e] * ff;
         store_vec<bf16, 4>(orow + 32 * d + 8 * c, v);
       }
   }
-  const uint64_t bad = __builtin_amdgcn_ballot_w64(odd != 0.f && first != NONE && there);
+  const uint64_t bad = __builtin_amdgcn_ballot_w64(!(most < __builtin_inff()) && !none && there);
   rows_again<bf16, D>(a, (uint32_t)(bad | bad >> 32), tok, head, first);
 }
 
@@ -517,7 +521,7 @@ __global__ __launch_bounds__(256, 2) void packed_f32_kernel(PackedArgs a) {
   };
   load_tile(0);
   const int first = firsts.of(a, tok);
-  const Window win = window_of(tok, first);
+  const Window win = window_of<15>(tok, first, key0);
   for (int k0 = 0; k0 < keys; k0 += KT) {
     __syncthreads();  // the previous tile is consumed
 #pragma unroll
@@ -533,7 +537,6 @@ __global__ __launch_bounds__(256, 2) void packed_f32_kernel(PackedArgs a) {
     if (k0 + KT < keys) load_tile(k0 + KT);
     const int key = key0 + k0 + sub, last = key + KB * 16 - 1;  // this wave's
     if (key > win.to || last < win.from) continue;
-    const bool masked = key < win.all_from || last > win.all_to;
     float p[KB][4];
     float mx = -__builtin_inff();
 #pragma unroll
@@ -551,13 +554,13 @@ __global__ __launch_bounds__(256, 2) void packed_f32_kernel(PackedArgs a) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) p[kb][e] = acc[e] * a.scale;
     }
-    if (masked) {  // (a lane sees first .. tok)
-      const uint32_t base = (uint32_t)(key + 4 * lq) - (uint32_t)first, most = (uint32_t)tok - (uint32_t)first;
+    if (key < win.all_from || last > win.all_to) {  // (a lane sees first .. tok)
+      const int lo = first - key - 4 * lq, hi = tok - key - 4 * lq;
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (base + (kb * 16 + e) > most) p[kb][e] = -__builtin_inff();
+          if (kb * 16 + e < lo || kb * 16 + e > hi) p[kb][e] = -__builtin_inff();
     }
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
