@@ -86,9 +86,11 @@ struct Firsts {
 
 // One query of one head by one wave, in fp32, key by key and only those it sees:
 // a lane a key for the scores, a lane one or two dims of the output. The tile
-// kernels turn to it for a query whose result is not finite: in a product over a
-// whole tile a hidden value that is infinite or NaN shows (0 times it is no
-// zero), here it does not.
+// kernels turn to it for a query whose result is not finite while the sum of its
+// probabilities is: in a product over a whole tile a hidden value that is infinite
+// or NaN shows (0 times it is no zero), here it does not. (A sum that is no number
+// comes from keys that the query sees, and so is the result: no slow way for texts
+// of NaN.)
 template <typename T, int D>
 __device__ __forceinline__ void packed_row(const PackedArgs& a, int r, int first, int head) {
   constexpr int VE = Vec<T>::N, DL = D > 64 ? D / 64 : 1;
@@ -164,12 +166,12 @@ __device__ __forceinline__ Window window_of(int tok, int first, int key0) {
 // 32 rows at a time), pml [KG][QT] (maximum, sum; exp2 or expf by BASE2), pf [QT]
 // first rows. Joined and stored by whole rows, LPR lanes a row; the ones
 // that are not finite again by packed_row.
-template <typename T, int D, int KG, int QT, bool BASE2>
+template <typename T, int D, int KG, int QT, int THREADS, bool BASE2>
 __device__ __forceinline__ void join_rows(const PackedArgs& a, int tile, int kv, const float* po, const float2* pml,
                                           const int* pf) {
   constexpr int LPR = D / 4;
   const int n = std::min(QT, a.rows - tile * QT);
-  for (int i0 = 0; i0 < n * LPR; i0 += 256) {
+  for (int i0 = 0; i0 < n * LPR; i0 += THREADS) {
     const int i = i0 + threadIdx.x, row = std::min(i / LPR, n - 1), d = i % LPR * 4;
     float m = -__builtin_inff(), l = 0.f, odd = 0.f;
     float2 ml[KG];
@@ -182,11 +184,10 @@ __device__ __forceinline__ void join_rows(const PackedArgs& a, int tile, int kv,
 #pragma unroll
     for (int g = 0; g < KG; ++g) {
       const f32x4 og = *(const f32x4*)(po + (g * QT + row) * (D + 4) + d);
-      // (a set that saw nothing weighs nothing; what is no number shows)
+      // (a set that saw nothing weighs nothing; a sum that is no number shows)
       const float sc = ml[g].x == -__builtin_inff() ? 0.f
                        : BASE2                      ? __builtin_amdgcn_exp2f(ml[g].x - m)
                                                     : expf(ml[g].x - m);
-      odd = fmaf(ml[g].y, 0.f, odd);
       l = fmaf(sc, ml[g].y, l);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -196,7 +197,7 @@ __device__ __forceinline__ void join_rows(const PackedArgs& a, int tile, int kv,
     }
     const int r = tile * QT + row, tok = a.by_per(r), head = kv * a.per + r - tok * a.per, first = pf[row];
     const bool there = i < n * LPR;
-    const uint64_t bad = __builtin_amdgcn_ballot_w64(there && first != NONE && odd != 0.f);
+    const uint64_t bad = __builtin_amdgcn_ballot_w64(there && first != NONE && odd != 0.f && l == l);
     uint64_t again = 0;  // (a row: its first lane)
 #pragma unroll
     for (int x = 0; x < 64; x += LPR)
@@ -212,10 +213,10 @@ __device__ __forceinline__ void join_rows(const PackedArgs& a, int tile, int kv,
 }
 
 // ---------------------------------------------------------------------------
-// bf16, on v_mfma_f32_32x32x16_bf16: a wave computes 32 query rows. A block takes
-// 128 rows over tiles of 64 keys, or, where that leaves blocks too few (KG 2, 4),
-// 64 or 32 rows over tiles of 64 or 128, two or four waves a row over 32 of a
-// tile's keys each, joined at the end.
+// bf16, on v_mfma_f32_32x32x16_bf16: a wave computes 32 query rows over all keys of
+// a tile, or, where that leaves blocks too few (KG 2, 4), two or four waves the same
+// rows over a half or a quarter of them each, joined at the end. A block has four or
+// eight waves, a tile 64 or 128 keys (packed_form).
 //
 // A tile of K and V rows goes to LDS as it lies in memory, by loads that bypass
 // the registers, while the tile before it is computed (two stages, one barrier a
@@ -231,22 +232,22 @@ __device__ __forceinline__ void join_rows(const PackedArgs& a, int tile, int kv,
 // there, and fp32 products run at an eighth of the rate (154 against 1,261 TFLOP/s
 // of a large library product). The sums that they are divided by add the
 // unrounded ones.
-template <int D, int KG>
+template <int D, int KG, int KT_, int WAVES_>
 struct Tile {
   using H = Half<D>;
-  static constexpr int QT = 128 / KG, KT = KG == 4 ? 128 : 64, NB = KG == 1 ? 2 : 1;  // NB: 32-key blocks of a wave
+  static constexpr int KT = KT_, WAVES = WAVES_, STRIPS = WAVES / KG;
+  static constexpr int QT = 32 * STRIPS, NB = KT / 32 / KG;  // NB: 32-key blocks of a wave
   static constexpr int OPER = KT * H::ROWB, STAGE = 2 * OPER;
-  static constexpr int PIECES = KT / H::PIECE_ROWS, PPW = PIECES / 4;  // 1 KiB loads, of a wave
+  static constexpr int PIECES = KT / H::PIECE_ROWS, PPW = PIECES / WAVES;  // 1 KiB loads, of a wave
   static constexpr int JOIN = KG == 1 ? 0 : KG * QT * (D + 4 + 2) * 4 + QT * 4;
   static constexpr int LDS = 2 * STAGE > JOIN ? 2 * STAGE : JOIN;
-  static_assert(PPW >= 1 || PIECES == 2, "each wave loads alike, or waves 0, 1 K and waves 2, 3 V");
+  static_assert(PPW * WAVES == PIECES || 2 * PIECES == WAVES, "each wave loads alike, or half of them K and half V");
 };
 
 // The tiles of keys `key0` .. key0 + keys - 1 of a KV head through the two stages.
-template <int D, int KG>
+template <int D, typename TL>
 struct KeyTiles {
   using H = Half<D>;
-  using TL = Tile<D, KG>;
   const char *k, *v;
   int64_t row;  // bytes between rows
   uint32_t to, koff, voff, piece;
@@ -258,11 +259,11 @@ struct KeyTiles {
     k = (const char*)a.k + at;
     v = (const char*)a.v + at;
     to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds + w * 1024;
-    // piece w + 4 j of a tile: rows 4 PIECE_ROWS j + r; the swizzles do not depend on j
-    const int r = H::PIECE_ROWS * (TL::PPW > 0 ? w : w & 1) + lane / H::CH;
+    // piece w + WAVES j of a tile: rows WAVES PIECE_ROWS j + r; the swizzles do not depend on j
+    const int r = H::PIECE_ROWS * (TL::PPW > 0 ? w : w % TL::PIECES) + lane / H::CH;
     koff = r * (uint32_t)row + ((lane % H::CH) ^ H::k_swz(r)) * 16;
     voff = r * (uint32_t)row + ((lane % H::CH) ^ H::v_swz(r)) * 16;
-    piece = 4 * H::PIECE_ROWS * (uint32_t)row;
+    piece = TL::WAVES * H::PIECE_ROWS * (uint32_t)row;
   }
   __device__ __forceinline__ void load(int t) const {
     if (t >= n) return;
@@ -274,29 +275,29 @@ struct KeyTiles {
     uint32_t step = __builtin_amdgcn_readfirstlane(piece);
     asm volatile("s_nop 4" : "+s"(lds), "+s"(step));
     if constexpr (TL::PPW == 0) {
-      if (__builtin_amdgcn_readfirstlane(threadIdx.x >> 7) == 0)
+      if (__builtin_amdgcn_readfirstlane(threadIdx.x >> 6) < TL::PIECES)
         row_dma16(kr, koff, lds);
       else
         row_dma16(vr, voff, lds);
     }
 #pragma unroll
-    for (int j = 0; j < TL::PPW; ++j) row_dma16(kr, koff, j * step, lds + j * 4096);
+    for (int j = 0; j < TL::PPW; ++j) row_dma16(kr, koff, j * step, lds + j * TL::WAVES * 1024);
 #pragma unroll
-    for (int j = 0; j < TL::PPW; ++j) row_dma16(vr, voff, j * step, lds + TL::OPER + j * 4096);
+    for (int j = 0; j < TL::PPW; ++j) row_dma16(vr, voff, j * step, lds + TL::OPER + j * TL::WAVES * 1024);
   }
 };
 
-template <int D, int KG>
-__global__ __launch_bounds__(256, 2) void packed_bf16_kernel(PackedArgs a) {
+template <int D, int KG, int KT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, 2) void packed_bf16_kernel(PackedArgs a) {
   using H = Half<D>;
-  using TL = Tile<D, KG>;
+  using TL = Tile<D, KG, KT, WAVES>;
   // (D = 16: the output's 32-row operand holds the 16 dims twice)
   constexpr int KS = D / 16, DB = D >= 32 ? D / 32 : 1, OC = D >= 32 ? 4 : 2;  // OC: 8-dim chunks of a block
   constexpr int NB = TL::NB, QT = TL::QT;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n32 = lane & 31, h = lane >> 5;
-  const int strip = w % (4 / KG), sub = w / (4 / KG) * 32;  // of the rows; first of the wave's keys in a tile
+  const int strip = w % TL::STRIPS, sub = w / TL::STRIPS * 32 * NB;  // of the rows; first of the wave's keys in a tile
   // The last rows, which see the most keys, first. (KV heads side by side: where
   // there are 1, 2, 4 or 8, an XCD's blocks, every eighth, share one's rows.)
   const int jb = a.by_hkv(blockIdx.x), kv = blockIdx.x - jb * a.Hkv, tile = a.tiles - 1 - jb;
@@ -311,7 +312,7 @@ __global__ __launch_bounds__(256, 2) void packed_bf16_kernel(PackedArgs a) {
     for (int k = 0; k < KS; ++k) qb[k] = __builtin_bit_cast(bf16x8, *(const u32x4*)(q + 16 * k));
   }
   const int key0 = firsts.begin();
-  const KeyTiles<D, KG> tiles(a, kv, key0, t1 - key0 + 1, lds);
+  const KeyTiles<D, TL> tiles(a, kv, key0, t1 - key0 + 1, lds);
   tiles.load(0);
   const int first = firsts.of(a, tok);
   const Window win = window_of<31>(tok, first, key0);
@@ -416,7 +417,7 @@ __global__ __launch_bounds__(256, 2) void packed_bf16_kernel(PackedArgs a) {
     float* po = (float*)lds;                          // [KG][QT][D + 4]
     float2* pml = (float2*)(po + KG * QT * (D + 4));  // [KG][QT]
     int* pf = (int*)(pml + KG * QT);                  // [QT]
-    const int row = strip * 32 + n32, at = w / (4 / KG) * QT + row;
+    const int row = strip * 32 + n32, at = w / TL::STRIPS * QT + row;
     __syncthreads();  // (every stage is free)
 #pragma unroll
     for (int d = 0; d < DB; ++d)
@@ -427,13 +428,13 @@ __global__ __launch_bounds__(256, 2) void packed_bf16_kernel(PackedArgs a) {
     if (h == 0) pml[at] = make_float2(m, l);
     if (h == 0 && sub == 0) pf[row] = first;
     __syncthreads();
-    join_rows<bf16, D, KG, QT, true>(a, tile, kv, po, pml, pf);
+    join_rows<bf16, D, KG, QT, 64 * WAVES, true>(a, tile, kv, po, pml, pf);
     return;
   }
   if (r0 >= a.rows) return;
   const bool there = r0 + n32 < a.rows;
   const float f = 1.f / l;  // (a query that saw nothing above minus infinity: NaN)
-  float most = l;           // NaN or infinite if something is
+  float most = 0.f;         // NaN or infinite if something is
 #pragma unroll
   for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -458,7 +459,7 @@ __global__ __launch_bounds__(256, 2) void packed_bf16_kernel(PackedArgs a) {
         store_vec<bf16, 4>(orow + 32 * d + 8 * c, v);
       }
   }
-  const uint64_t bad = __builtin_amdgcn_ballot_w64(!(most < __builtin_inff()) && !none && there);
+  const uint64_t bad = __builtin_amdgcn_ballot_w64(!(most < __builtin_inff()) && l == l && !none && there);
   rows_again<bf16, D>(a, (uint32_t)(bad | bad >> 32), tok, head, first);
 }
 
@@ -623,64 +624,86 @@ __global__ __launch_bounds__(256, 2) void packed_f32_kernel(PackedArgs a) {
   if (lq == 0) pml[at] = make_float2(m, lsum);
   if (lq == 0 && sub == 0) pf[strip * 16 + lr] = first;
   __syncthreads();
-  join_rows<float, D, KW, QT, false>(a, tile, kv, po, pml, pf);
+  join_rows<float, D, KW, QT, 256, false>(a, tile, kv, po, pml, pf);
 }
 
-// Sets of waves a row (bf16 KG, fp32 KW) from what the host knows: blocks of 128
-// rows and the mean length; the rest is on the device. Measured (us, graph
-// replays, one against two against four sets; n x L: n sequences of L tokens):
-// bf16: four where the blocks, four times as many, do not outnumber the places by
-//   much and the sequences are longer than a tile; two for few long sequences.
-//   0.5B heads (D 64): 2x64 (14 blocks) 5.7 5.9 5.3, 10x100 (110) 6.4 7.0 6.9, 1x500
-//   (56) 10.4 9.7 7.2, 5x300 (166) 9.6 10.5 11.5, 2x1300 (286) 26.2 24.7 22.5, 3x1300
-//   (428) 32.0 29.1 30.2, 8x500 (438) 16.4 17.9 22.8. 7B heads (128): 1x200 (44) 10.7
-//   10.2 8.4, 3x200 (132) 12.0 11.8 18.7 (a block a CU), 1x1300 (288) 38.0 28.2 51.6,
-//   3x500 (332) 21.1 23.6 42.0, 1x4096 (896) 129 153 304.
-// fp32, bound by its products sooner: 0.5B heads 1x512 (56) 30.8 19.6 15.2, 10x300
-//   (330) 44.7 34.7 35.8, 100x100 (1,094) 53.0 51.6 59.7; 7B heads 1x512 (112) 52.6 39.1
-//   39.0, 1x1024 (224) 117 99 108, 1x3000 (660) 625 654 763, 50x20 (220) 20.2 22.6 25.8.
-int packed_sets(bool half, int D, int64_t rows, int64_t heads, int64_t tokens, int64_t sequences) {
+// The form of a call from what the host knows, blocks of 128 rows and the mean
+// length (the rest is on the device): sets of waves a row, keys of a tile, waves.
+// Measured (us, graph replays; n x L: n sequences of L tokens, blocks in brackets):
+// Four or two sets where blocks are few and the sequences longer than a tile (one
+//   against two against four sets):
+//   0.5B heads (D 64): 2x64 (14) 5.7 5.9 5.3, 10x100 (110) 6.4 7.0 6.9, 1x500 (56) 10.4 9.7
+//   7.2, 5x300 (166) 9.6 10.5 11.5, 2x1300 (286) 26.2 24.7 22.5, 8x500 (438) 16.4 17.9
+//   22.8; 7B heads (128): 1x200 (44) 10.7 10.2 8.4, 3x200 (132) 12.0 11.8 18.7 (a block a
+//   CU), 1x1300 (288) 38.0 28.2 51.6, 3x500 (332) 21.1 23.6 42.0.
+//   Two sets over tiles of 128 keys instead of 64: 0.5B heads, 1x4096 (448) 60.4 53.3;
+//   7B heads (the tiles take a CU's LDS), 1x1024 (224) 25.6 30.1.
+// Tiles of 128 keys for long sequences: fewer barriers and lane exchanges a key.
+//   7B heads, 256 rows and eight waves a block: 3x(20011 .. 8882) (9,768) 5,575 5,240,
+//   1x4096 (896) 143 138, 3x2500 (1,644) 180 178, 4x2000 (1,752) 147 149.
+//   0.5B heads, where all blocks are resident at once and the longest is what
+//   counts: one set 1x8191 (896) 175 159, 2x4096 (896) 97 85, two sets of eight waves
+//   1x6000 (658) 112 101, 2x3000 (658) 71 61; past that neither, 1x12000 (1,314) 330 337 334.
+// fp32, bound by its products sooner: 0.5B heads 1x512 (56) 30.8 19.6 15.2, 10x300 (330)
+//   44.7 34.7 35.8, 100x100 (1,094) 53.0 51.6 59.7; 7B heads 1x512 (112) 52.6 39.1 39.0, 1x1024
+//   (224) 117 99 108, 1x3000 (660) 625 654 763, 50x20 (220) 20.2 22.6 25.8.
+struct PackedForm {
+  int sets, keys, waves;
+};
+PackedForm packed_form(bool half, int D, int64_t rows, int64_t heads, int64_t tokens, int64_t sequences) {
   const int64_t blocks = cdiv(rows, 128) * heads, mean = tokens / std::max<int64_t>(sequences, 1);
   if (half) {
-    if (mean >= 64 && blocks <= std::min<int64_t>(64 + (D < 128 ? mean * 64 / (5 * D) : 0), 20480 / D)) return 4;
-    return mean >= 300 && blocks <= std::min<int64_t>(mean * 2 / 5, 512) ? 2 : 1;
+    if (mean >= 64 && blocks <= std::min<int64_t>(64 + (D < 128 ? mean * 64 / (5 * D) : 0), 20480 / D)) return {4, 128, 4};
+    if (mean >= 300 && blocks <= std::min<int64_t>(mean * 2 / 5, D < 128 ? 32768 / D : 512)) return {2, D < 128 ? 128 : 64, 4};
+    if (D == 128 && mean >= 2500) return {1, 128, 8};
+    if (D == 64 && mean >= 2500 && blocks <= 768) return {2, 128, 8};
+    if (D == 64 && mean >= 2500 && blocks <= 1024) return {1, 128, 4};
+    return {1, 64, 4};
   }
-  if (mean < 64 && blocks > 128) return 1;
-  return blocks * D <= 16384 ? 4 : blocks * D <= 45056 ? 2 : 1;
+  if (mean < 64 && blocks > 128) return {1, 64, 4};
+  return {blocks * D <= 16384 ? 4 : blocks * D <= 45056 ? 2 : 1, 64, 4};
 }
 
 template <typename T, int D>
-int packed_launch(hipStream_t st, PackedArgs a, int sets) {
-  auto go = [&](auto kern, int qt, int lds) -> int {
-    a.tiles = (int)cdiv(a.rows, qt);
+int packed_launch(hipStream_t st, PackedArgs a, const PackedForm& f) {
+  auto go = [&](auto kern, int rows, int lds) -> int {
+    a.tiles = (int)cdiv(a.rows, rows);
     const int rc = ensure_lds_limit((const void*)kern, lds);
     if (rc) return rc;
-    hipLaunchKernelGGL(kern, dim3((unsigned)(a.tiles * a.Hkv)), dim3(256), lds, st, a);
+    hipLaunchKernelGGL(kern, dim3((unsigned)(a.tiles * a.Hkv)), dim3(64 * f.waves), lds, st, a);
     MINITP_LAUNCH_CHECK();
     return MINITP_OK;
   };
   if constexpr (sizeof(T) == 2) {
-    if (sets == 4) return go(packed_bf16_kernel<D, 4>, 32, Tile<D, 4>::LDS);
-    if (sets == 2) return go(packed_bf16_kernel<D, 2>, 64, Tile<D, 2>::LDS);
-    return go(packed_bf16_kernel<D, 1>, 128, Tile<D, 1>::LDS);
+    constexpr int KEYS2 = D < 128 ? 128 : 64;  // (of the form with two sets)
+    if (f.sets == 4) return go(packed_bf16_kernel<D, 4, 128, 4>, 32, Tile<D, 4, 128, 4>::LDS);
+    if (f.sets == 2 && f.waves == 4) return go(packed_bf16_kernel<D, 2, KEYS2, 4>, 64, Tile<D, 2, KEYS2, 4>::LDS);
+    if constexpr (D == 128) {
+      if (f.keys == 128) return go(packed_bf16_kernel<D, 1, 128, 8>, 256, Tile<D, 1, 128, 8>::LDS);
+    }
+    if constexpr (D == 64) {
+      if (f.sets == 2) return go(packed_bf16_kernel<D, 2, 128, 8>, 128, Tile<D, 2, 128, 8>::LDS);
+      if (f.keys == 128) return go(packed_bf16_kernel<D, 1, 128, 4>, 128, Tile<D, 1, 128, 4>::LDS);
+    }
+    return go(packed_bf16_kernel<D, 1, 64, 4>, 128, Tile<D, 1, 64, 4>::LDS);
   } else {
-    if (sets == 4) return go(packed_f32_kernel<D, 4>, 16, F_LDS<D>);
-    if (sets == 2) return go(packed_f32_kernel<D, 2>, 32, F_LDS<D>);
+    if (f.sets == 4) return go(packed_f32_kernel<D, 4>, 16, F_LDS<D>);
+    if (f.sets == 2) return go(packed_f32_kernel<D, 2>, 32, F_LDS<D>);
     return go(packed_f32_kernel<D, 1>, 64, F_LDS<D>);
   }
 }
 
 template <typename T>
-int packed_by_d(hipStream_t st, const PackedArgs& a, int64_t D, int sets) {
+int packed_by_d(hipStream_t st, const PackedArgs& a, int64_t D, const PackedForm& f) {
   switch (D) {
     case 16:
-      return packed_launch<T, 16>(st, a, sets);
+      return packed_launch<T, 16>(st, a, f);
     case 32:
-      return packed_launch<T, 32>(st, a, sets);
+      return packed_launch<T, 32>(st, a, f);
     case 64:
-      return packed_launch<T, 64>(st, a, sets);
+      return packed_launch<T, 64>(st, a, f);
     default:
-      return packed_launch<T, 128>(st, a, sets);
+      return packed_launch<T, 128>(st, a, f);
   }
 }
 
@@ -729,8 +752,8 @@ int launch_packed_attention(hipStream_t st, int dtype, const PackedShape& s, con
   a.by_hkv = make_div(s.Hkv);
   a.offsets = offsets;
   a.scale = 1.0f / sqrtf((float)s.D);
-  const int sets = packed_sets(dtype == MINITP_BF16, (int)s.D, a.rows, s.Hkv, s.N, s.S);
-  return dtype == MINITP_F32 ? packed_by_d<float>(st, a, s.D, sets) : packed_by_d<bf16>(st, a, s.D, sets);
+  const PackedForm f = packed_form(dtype == MINITP_BF16, (int)s.D, a.rows, s.Hkv, s.N, s.S);
+  return dtype == MINITP_F32 ? packed_by_d<float>(st, a, s.D, f) : packed_by_d<bf16>(st, a, s.D, f);
 }
 
 }  // namespace minitp

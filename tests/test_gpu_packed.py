@@ -214,6 +214,92 @@ def test_long_sequences(hq, hkv, d, dtype):
     check(K.packed_attention(*x, offsets_of(lens)), *x, bounds_of(lens))
 
 
+def sampled(q, k, v, lens, rows):
+    """reference() for some rows: (out, mag) [rows, Hq, D] in float64."""
+    hq, d, hkv = q.shape[1], q.shape[2], k.shape[1]
+    starts = offsets_of(lens).tolist()
+    outs, mags = [], []
+    for r in rows:
+        lo = max(s for s in starts[:-1] if s <= r)
+        kk, vv = (t[lo:r + 1].double().transpose(0, 1).contiguous() for t in (k, v))  # [Hkv, n, D]
+        s = (kk @ q[r].double().view(hkv, -1, d).transpose(1, 2).contiguous()).transpose(1, 2) / math.sqrt(d)
+        p = torch.softmax(s, -1).contiguous()
+        outs.append((p @ vv).reshape(hq, d))
+        mags.append((p @ vv.abs()).reshape(hq, d))
+    return torch.stack(outs), torch.stack(mags)
+
+
+# shapes for each form of the kernels: sets of waves a row, keys of a tile, waves of a block
+FORMS = [
+    (torch.bfloat16, (14, 2, 64), [500]), (torch.bfloat16, (28, 4, 128), [150, 90]),      # 4 sets
+    (torch.bfloat16, (8, 2, 32), [900, 300]), (torch.bfloat16, (4, 2, 16), [1500, 700]),
+    (torch.bfloat16, (14, 2, 64), [2500, 333, 1700]), (torch.bfloat16, (28, 4, 128), [600, 500]),  # 2 sets
+    (torch.bfloat16, (8, 2, 32), [2500] * 6), (torch.bfloat16, (4, 2, 16), [16000, 15000]),
+    (torch.bfloat16, (28, 4, 128), [3000, 2400]),                                         # 128 keys, 8 waves
+    (torch.bfloat16, (14, 2, 64), [5900]),                                                # 2 sets of 8 waves
+    (torch.bfloat16, (14, 2, 64), [8191]), (torch.bfloat16, (14, 2, 64), [4000, 3000]),   # 128 keys
+    (torch.bfloat16, (14, 2, 64), [60] * 300), (torch.bfloat16, (28, 4, 128), [60] * 300),
+    (torch.bfloat16, (8, 2, 32), [60] * 300), (torch.bfloat16, (4, 2, 16), [60] * 300),
+    (torch.float32, (14, 2, 64), [500]), (torch.float32, (28, 4, 128), [700]), (torch.float32, (14, 2, 64), [3000]),
+    (torch.float32, (28, 4, 128), [60] * 300), (torch.float32, (8, 2, 32), [2500] * 6), (torch.float32, (4, 2, 16), [90] * 400),
+]
+
+
+@pytest.mark.parametrize("dtype,heads,lens", FORMS, ids=lambda x: f"{len(x)}x{x[0]}" if isinstance(x, list) else str(x))
+def test_forms(dtype, heads, lens):
+    """Each form over whole calls: sampled rows, rows behind the last sequence,
+    and a value row that is not finite in one of the sequences."""
+    from minitp import kernels as K
+
+    hq, hkv, d = heads
+    n, pad = sum(lens), 45
+    x = make(n + pad, hq, hkv, d, dtype, "heads")
+    for t in x:
+        t[n:] = math.nan
+    g = torch.Generator().manual_seed(n)
+    ends = offsets_of(lens).tolist()
+    rows = sorted(set(torch.randint(0, n, (50,), generator=g).tolist() + [0, n - 1, ends[1] - 1, ends[-2]]
+                      + [r for r in (15, 16, 31, 32, 63, 64, 127, 128, 255, 256) if r < n]))
+    ref, mag = sampled(*x, lens, rows)
+    bar = bars(ref, mag, dtype, d) + 1e-9
+    out = K.packed_attention(*x, offsets_of(lens)).view(n + pad, hq, d)
+    assert torch.isfinite(out).all() and (out[n:] == 0).all()
+    err = (out[rows].double() - ref).abs()
+    assert (err <= bar).all(), (err / bar).max()
+    bad = ends[1] - lens[0] // 3  # in the first sequence
+    x[2][bad, :, 3] = math.inf
+    again = K.packed_attention(*x, offsets_of(lens)).view(n + pad, hq, d)
+    assert not torch.isfinite(again[bad:ends[1], :, 3]).any()
+    assert torch.isfinite(again[:bad]).all() and torch.isfinite(again[ends[1]:]).all()
+    err = (again[rows].double() - ref).abs()
+    clean = torch.tensor([not bad <= r < ends[1] for r in rows], device=DEV)
+    assert (err <= bar)[clean].all(), (err / bar)[clean].max()
+
+
+@pytest.mark.parametrize("dtype,heads,lens", [FORMS[i] for i in (0, 4, 8, 9, 10, 12, 16, 18, 19)],
+                         ids=lambda x: f"{len(x)}x{x[0]}" if isinstance(x, list) else str(x))
+def test_a_text_of_nan(dtype, heads, lens):
+    """Keys, values and queries that are no numbers from a row on, as a token
+    outside the vocabulary leaves them: NaN from there to the sequence's end."""
+    from minitp import kernels as K
+
+    hq, hkv, d = heads
+    n = sum(lens)
+    x = make(n, hq, hkv, d, dtype, "heads", seed=3)
+    want = K.packed_attention(*x, offsets_of(lens)).view(n, hq, d)
+    bad, end = lens[0] // 3, lens[0]
+    for t in x:
+        t[bad:end] = math.nan
+    out = K.packed_attention(*x, offsets_of(lens)).view(n, hq, d)
+    assert torch.isnan(out[bad:end]).all()
+    rest = torch.arange(n, device=DEV)
+    rest = rest[(rest < bad) | (rest >= end)]
+    _, mag = sampled(*make(n, hq, hkv, d, dtype, "heads", seed=3), lens, rest[::97].tolist())
+    bar = mag * (4 * 2 ** -8 if dtype == torch.bfloat16 else 2 * (2 * 20 * (d / 4 + 3) + 64) * 2 ** -24) + 1e-9
+    assert torch.isfinite(out[rest]).all()
+    assert ((out[rest[::97]].double() - want[rest[::97]].double()).abs() <= bar).all()
+
+
 def test_sequences_equal_prompts_on_their_own():
     """As far as the two kernels round alike: the model's prompt attention."""
     from minitp import kernels as K
