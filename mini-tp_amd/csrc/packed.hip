@@ -208,6 +208,8 @@ __device__ __forceinline__ void join_rows(const PackedArgs& a, int tile, int kv,
       for (int e = 0; e < 4; ++e) y[e] = first == NONE ? 0.f : v[e] / l;
       store_vec<T, 4>((T*)a.out + ((int64_t)tok * a.Hq + head) * D + d, y);
     }
+    if (again == 0) continue;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the rows above are stored first)
     rows_again<T, D>(a, again, tok, head, first);
   }
 }
@@ -232,15 +234,16 @@ __device__ __forceinline__ void join_rows(const PackedArgs& a, int tile, int kv,
 // there, and fp32 products run at an eighth of the rate (154 against 1,261 TFLOP/s
 // of a large library product). The sums that they are divided by add the
 // unrounded ones.
-template <int D, int KG, int KT_, int WAVES_>
+template <int D, int KG, int KT_, int WAVES_, int VST_ = 2>
 struct Tile {
   using H = Half<D>;
   static constexpr int KT = KT_, WAVES = WAVES_, STRIPS = WAVES / KG;
   static constexpr int QT = 32 * STRIPS, NB = KT / 32 / KG;  // NB: 32-key blocks of a wave
-  static constexpr int OPER = KT * H::ROWB, STAGE = 2 * OPER;
+  static constexpr int VST = VST_;  // stages of V
+  static constexpr int OPER = KT * H::ROWB, STAGES = (2 + VST) * OPER;
   static constexpr int PIECES = KT / H::PIECE_ROWS, PPW = PIECES / WAVES;  // 1 KiB loads, of a wave
   static constexpr int JOIN = KG == 1 ? 0 : KG * QT * (D + 4 + 2) * 4 + QT * 4;
-  static constexpr int LDS = 2 * STAGE > JOIN ? 2 * STAGE : JOIN;
+  static constexpr int LDS = STAGES > JOIN ? STAGES : JOIN;
   static_assert(PPW * WAVES == PIECES || 2 * PIECES == WAVES, "each wave loads alike, or half of them K and half V");
 };
 
@@ -265,32 +268,43 @@ struct KeyTiles {
     voff = r * (uint32_t)row + ((lane % H::CH) ^ H::v_swz(r)) * 16;
     piece = TL::WAVES * H::PIECE_ROWS * (uint32_t)row;
   }
-  __device__ __forceinline__ void load(int t) const {
-    if (t >= n) return;
+  // K of tile t to stage t % 2, V to stage t % VST behind them
+  __device__ __forceinline__ u32x4 rows_of(const char* base, int t) const {
     // rows past the last read zeros (or, where rows overlap, the last again)
-    const uint32_t bytes = (std::min(keys - t * TL::KT, TL::KT) - 1) * (uint32_t)row + H::ROWB;
-    const int64_t at = (int64_t)t * TL::KT * row;
-    const u32x4 kr = rows_rsrc(k + at, bytes), vr = rows_rsrc(v + at, bytes);
-    uint32_t lds = __builtin_amdgcn_readfirstlane(to + (t & 1) * TL::STAGE);
-    uint32_t step = __builtin_amdgcn_readfirstlane(piece);
+    const int left = std::min(keys - t * TL::KT, TL::KT);
+    return rows_rsrc(base + (int64_t)t * TL::KT * row, left > 0 ? (left - 1) * (uint32_t)row + H::ROWB : 0);
+  }
+  __device__ __forceinline__ void load_rows(u32x4 r, uint32_t off, uint32_t at) const {
+    uint32_t lds = __builtin_amdgcn_readfirstlane(to + at), step = __builtin_amdgcn_readfirstlane(piece);
     asm volatile("s_nop 4" : "+s"(lds), "+s"(step));
-    if constexpr (TL::PPW == 0) {
-      if (__builtin_amdgcn_readfirstlane(threadIdx.x >> 6) < TL::PIECES)
-        row_dma16(kr, koff, lds);
-      else
-        row_dma16(vr, voff, lds);
-    }
 #pragma unroll
-    for (int j = 0; j < TL::PPW; ++j) row_dma16(kr, koff, j * step, lds + j * TL::WAVES * 1024);
-#pragma unroll
-    for (int j = 0; j < TL::PPW; ++j) row_dma16(vr, voff, j * step, lds + TL::OPER + j * TL::WAVES * 1024);
+    for (int j = 0; j < std::max(TL::PPW, 1); ++j) row_dma16(r, off, j * step, lds + j * TL::WAVES * 1024);
+  }
+  __device__ __forceinline__ bool mine(bool v) const {  // (few pieces: half of the waves K, half V)
+    return TL::PPW > 0 || (__builtin_amdgcn_readfirstlane(threadIdx.x >> 6) >= TL::PIECES) == v;
+  }
+  __device__ __forceinline__ void load_k(int t) const {
+    if ((t < n || TL::VST == 1) && mine(false)) load_rows(rows_of(k, t), koff, (t & 1) * TL::OPER);
+  }
+  __device__ __forceinline__ void load_v(int t) const {
+    if (t < n && mine(true))
+      load_rows(rows_of(v, t), voff, (2 + t % TL::VST) * TL::OPER - (TL::PPW > 0 ? 0 : TL::PIECES * 1024));
   }
 };
 
-template <int D, int KG, int KT, int WAVES>
+// V of a tile has landed for the whole block: this wave's loads but the N of the
+// next K (past the last tile they read nothing), and then the barrier.
+template <int N>
+__device__ __forceinline__ void rows_wait() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+template <int D, int KG, int KT, int WAVES, int VST>
 __global__ __launch_bounds__(64 * WAVES, 2) void packed_bf16_kernel(PackedArgs a) {
   using H = Half<D>;
-  using TL = Tile<D, KG, KT, WAVES>;
+  using TL = Tile<D, KG, KT, WAVES, VST>;
   // (D = 16: the output's 32-row operand holds the 16 dims twice)
   constexpr int KS = D / 16, DB = D >= 32 ? D / 32 : 1, OC = D >= 32 ? 4 : 2;  // OC: 8-dim chunks of a block
   constexpr int NB = TL::NB, QT = TL::QT;
@@ -313,7 +327,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void packed_bf16_kernel(PackedArgs a
   }
   const int key0 = firsts.begin();
   const KeyTiles<D, TL> tiles(a, kv, key0, t1 - key0 + 1, lds);
-  tiles.load(0);
+  tiles.load_k(0);
+  if (VST == 2) tiles.load_v(0);
   const int first = firsts.of(a, tok);
   const Window win = window_of<31>(tok, first, key0);
 
@@ -330,16 +345,22 @@ __global__ __launch_bounds__(64 * WAVES, 2) void packed_bf16_kernel(PackedArgs a
   // (the swizzles do not depend on sub)
   const int kat = (sub + n32) * H::ROWB, kx = (h ^ H::k_swz(n32)) << 4;
   const int vrow = 4 * h + (lane & 15) / 4;
-  const int vat = TL::OPER + (sub + vrow) * H::ROWB + 8 * (lane & 1);
+  const int vat = 2 * TL::OPER + (sub + vrow) * H::ROWB + 8 * (lane & 1);
   const int vx = (((D >= 32 ? 2 * ((lane >> 4) & 1) : 0) + ((lane >> 1) & 1)) ^ H::v_swz(vrow)) << 4;
   arrived(qb);
 
   for (int t = 0; t < tiles.n; ++t) {
     stage_wait();
-    tiles.load(t + 1);  // (the stage's readers passed the barrier)
+    // (the readers of what is overwritten passed the barrier)
+    if (VST == 1) tiles.load_v(t);
+    tiles.load_k(t + 1);
+    if (VST == 2) tiles.load_v(t + 1);
     const int key = key0 + t * TL::KT + sub, last = key + 32 * NB - 1;
-    if (key > win.to || last < win.from) continue;
-    const char* st = lds + (t & 1) * TL::STAGE;
+    if (VST == 2 && (key > win.to || last < win.from)) continue;
+    const char* st = lds + (t & 1) * TL::OPER;
+    int sv_at = VST == 2 ? (t & 1) * TL::OPER : 0;
+    asm volatile("" : "+s"(sv_at));  // (or the addresses of all reads are kept over the loop)
+    const char* sv = lds + sv_at;
     f32x16 s[NB];
 #pragma unroll
     for (int kb = 0; kb < NB; ++kb)
@@ -391,6 +412,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void packed_bf16_kernel(PackedArgs a
         s[kb][i] = __builtin_amdgcn_exp2f(fmaf(s[kb][i], sl2, -mref));
         lsum += s[kb][i];
       }
+    if (VST == 1) rows_wait<TL::PPW>();
     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int j = 0; j < 2 * NB; ++j) {  // keys 16 j .. 16 j + 15
@@ -404,13 +426,14 @@ __global__ __launch_bounds__(64 * WAVES, 2) void packed_bf16_kernel(PackedArgs a
       const bf16x8 pb = __builtin_bit_cast(bf16x8, pk);
 #pragma unroll
       for (int d = 0; d < DB; ++d) {
-        const char* vp = st + vat + 16 * j * H::ROWB + ((64 * d) ^ vx);
+        const char* vp = sv + vat + 16 * j * H::ROWB + ((64 * d) ^ vx);
         const bf16x8 vf = join8(read_tr(vp), read_tr(vp + 8 * H::ROWB));
         o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pb, o[d], 0, 0, 0);
       }
     }
     __builtin_amdgcn_s_setprio(0);
   }
+  if (VST == 1) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (no load to LDS outlives the block)
 
   const float l = halves_sum(lsum);
   if constexpr (KG > 1) {
@@ -431,35 +454,46 @@ __global__ __launch_bounds__(64 * WAVES, 2) void packed_bf16_kernel(PackedArgs a
     join_rows<bf16, D, KG, QT, 64 * WAVES, true>(a, tile, kv, po, pml, pf);
     return;
   }
-  if (r0 >= a.rows) return;
-  const bool there = r0 + n32 < a.rows;
-  const float f = 1.f / l;  // (a query that saw nothing above minus infinity: NaN)
-  float most = 0.f;         // NaN or infinite if something is
+  // Through LDS, so that a wave stores whole rows (eight bytes a lane of 32 rows at
+  // a time keep the address unit busy for 1 us of a block of 7 us).
+  constexpr int ROW = H::ROWB + 16;
+  static_assert(TL::WAVES * 32 * ROW <= TL::STAGES, "the waves' rows fit the stages");
+  const bool none = first == NONE;
+  float most = 0.f;  // NaN or infinite if something is
 #pragma unroll
   for (int d = 0; d < DB; ++d)
 #pragma unroll
     for (int i = 0; i < 16; ++i) most = __builtin_elementwise_maximum(most, fabsf(o[d][i]));
-  const bool none = first == NONE;
   if (__builtin_amdgcn_ballot_w64(none)) {  // (a select for each value, which few waves need)
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
       for (int i = 0; i < 16; ++i) o[d][i] = none ? 0.f : o[d][i];
   }
-  if (there) {
-    const float ff = none ? 0.f : f;
-    bf16* orow = (bf16*)a.out + ((int64_t)tok * a.Hq + head) * D + 4 * h;
+  const float f = none ? 0.f : 1.f / l;  // (a query that saw nothing above minus infinity: NaN)
+  char* mine = lds + w * 32 * ROW;
+  __syncthreads();  // (every stage is free)
 #pragma unroll
-    for (int d = 0; d < DB; ++d)
+  for (int d = 0; d < DB; ++d)
 #pragma unroll
-      for (int c = 0; c < OC; ++c) {
-        float v[4];
+    for (int c = 0; c < OC; ++c) {
+      float v[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = o[d][4 * c + e] * ff;
-        store_vec<bf16, 4>(orow + 32 * d + 8 * c, v);
-      }
+      for (int e = 0; e < 4; ++e) v[e] = o[d][4 * c + e] * f;
+      store_vec<bf16, 4>((bf16*)(mine + n32 * ROW) + 32 * d + 8 * c + 4 * h, v);
+    }
+  __builtin_amdgcn_wave_barrier();
+  constexpr int RPI = 64 / H::CH;  // rows of a store
+#pragma unroll
+  for (int i = 0; i < 32; i += RPI) {
+    const int row = i + lane / H::CH, rr = r0 + row;
+    const uint4 x = *(const uint4*)(mine + row * ROW + lane % H::CH * 16);
+    const int t = a.by_per(std::min(rr, a.rows - 1)), hd = kv * a.per + rr - t * a.per;
+    if (rr < a.rows) *(uint4*)((char*)a.out + ((int64_t)t * a.Hq + hd) * H::ROWB + lane % H::CH * 16) = x;
   }
-  const uint64_t bad = __builtin_amdgcn_ballot_w64(!(most < __builtin_inff()) && l == l && !none && there);
+  const uint64_t bad = __builtin_amdgcn_ballot_w64(!(most < __builtin_inff()) && l == l && !none && r0 + n32 < a.rows);
+  if (bad == 0) return;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the rows above are stored first)
   rows_again<bf16, D>(a, (uint32_t)(bad | bad >> 32), tok, head, first);
 }
 
@@ -676,16 +710,17 @@ int packed_launch(hipStream_t st, PackedArgs a, const PackedForm& f) {
   };
   if constexpr (sizeof(T) == 2) {
     constexpr int KEYS2 = D < 128 ? 128 : 64;  // (of the form with two sets)
-    if (f.sets == 4) return go(packed_bf16_kernel<D, 4, 128, 4>, 32, Tile<D, 4, 128, 4>::LDS);
-    if (f.sets == 2 && f.waves == 4) return go(packed_bf16_kernel<D, 2, KEYS2, 4>, 64, Tile<D, 2, KEYS2, 4>::LDS);
+    if (f.sets == 4) return go(packed_bf16_kernel<D, 4, 128, 4, 2>, 32, Tile<D, 4, 128, 4>::LDS);
+    if (f.sets == 2 && f.waves == 4) return go(packed_bf16_kernel<D, 2, KEYS2, 4, 2>, 64, Tile<D, 2, KEYS2, 4>::LDS);
     if constexpr (D == 128) {
-      if (f.keys == 128) return go(packed_bf16_kernel<D, 1, 128, 8>, 256, Tile<D, 1, 128, 8>::LDS);
+      if (f.keys == 128) return go(packed_bf16_kernel<D, 1, 128, 8, 2>, 256, Tile<D, 1, 128, 8>::LDS);
     }
     if constexpr (D == 64) {
-      if (f.sets == 2) return go(packed_bf16_kernel<D, 2, 128, 8>, 128, Tile<D, 2, 128, 8>::LDS);
-      if (f.keys == 128) return go(packed_bf16_kernel<D, 1, 128, 4>, 128, Tile<D, 1, 128, 4>::LDS);
+      if (f.sets == 2) return go(packed_bf16_kernel<D, 2, 128, 8, 2>, 128, Tile<D, 2, 128, 8>::LDS);
+      if (f.keys == 128) return go(packed_bf16_kernel<D, 1, 128, 4, 2>, 128, Tile<D, 1, 128, 4>::LDS);
     }
-    return go(packed_bf16_kernel<D, 1, 64, 4>, 128, Tile<D, 1, 64, 4>::LDS);
+    constexpr int VST = D == 128 ? 1 : 2;
+    return go(packed_bf16_kernel<D, 1, 64, 4, VST>, 128, Tile<D, 1, 64, 4, VST>::LDS);
   } else {
     if (f.sets == 4) return go(packed_f32_kernel<D, 4>, 16, F_LDS<D>);
     if (f.sets == 2) return go(packed_f32_kernel<D, 2>, 32, F_LDS<D>);
