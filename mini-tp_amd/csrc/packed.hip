@@ -66,18 +66,22 @@ struct Firsts {
   }
   // keys of the tile are those from here on
   __device__ __forceinline__ int begin() const { return first == NONE ? t0 : first; }
-  __device__ __forceinline__ int of(const PackedArgs& a, int tok) {
+  template <int R>
+  __device__ __forceinline__ void of(const PackedArgs& a, const int (&tok)[R], int (&f)[R]) {
     const uint32_t lane = threadIdx.x & 63;
-    int f = first;
+#pragma unroll
+    for (int i = 0; i < R; ++i) f[i] = first;
     for (;;) {
       uint64_t inside = __builtin_amdgcn_ballot_w64(o > t0 && o <= t1);
       while (inside) {
         const int at = __builtin_ctzll(inside), b = __builtin_amdgcn_readlane(o, at);
         inside &= inside - 1;
-        if (b <= tok) f = lo + at == (uint32_t)a.S ? NONE : b;
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+          if (b <= tok[i]) f[i] = lo + at == (uint32_t)a.S ? NONE : b;
       }
       // (a run of more offsets, of short or empty sequences)
-      if (lo + 63 >= (uint32_t)a.S || __builtin_amdgcn_readlane(o, 63) > t1) return f;
+      if (lo + 63 >= (uint32_t)a.S || __builtin_amdgcn_readlane(o, 63) > t1) return;
       lo += 64;
       o = offset(a, lo + lane);
     }
@@ -150,23 +154,22 @@ __device__ __forceinline__ void rows_again(const PackedArgs& a, uint64_t odd, in
 
 // What a wave's tile of keys needs: `from` .. `to` are keys that some of its
 // queries see (or more), `all_from` .. `all_to` those that every one sees (or
-// fewer). Its queries' tokens and first rows ascend with its LAST + 1 rows.
+// fewer). Its queries' tokens and first rows ascend with its 32 rows.
 struct Window {
   int from, to, all_from, all_to;
 };
-template <int LAST>
 __device__ __forceinline__ Window window_of(int tok, int first, int key0) {
   const int f = __builtin_amdgcn_readfirstlane(first);
-  return Window{f == NONE ? key0 : f, __builtin_amdgcn_readlane(tok, LAST), __builtin_amdgcn_readlane(first, LAST),
+  return Window{f == NONE ? key0 : f, __builtin_amdgcn_readlane(tok, 31), __builtin_amdgcn_readlane(first, 31),
                 __builtin_amdgcn_readfirstlane(tok)};
 }
 
 // The results of a tile of QT rows that KG sets of waves hold over keys of their
 // own, in LDS: po [KG][QT] rows of D, padded by 16 bytes (lanes of a wave write
-// 32 rows at a time), pml [KG][QT] (maximum, sum; exp2 or expf by BASE2), pf [QT]
+// 32 rows at a time), pml [KG][QT] (maximum, as a power of two, and sum), pf [QT]
 // first rows. Joined and stored by whole rows, LPR lanes a row; the ones
 // that are not finite again by packed_row.
-template <typename T, int D, int KG, int QT, int THREADS, bool BASE2>
+template <typename T, int D, int KG, int QT, int THREADS>
 __device__ __forceinline__ void join_rows(const PackedArgs& a, int tile, int kv, const float* po, const float2* pml,
                                           const int* pf) {
   constexpr int LPR = D / 4;
@@ -185,9 +188,7 @@ __device__ __forceinline__ void join_rows(const PackedArgs& a, int tile, int kv,
     for (int g = 0; g < KG; ++g) {
       const f32x4 og = *(const f32x4*)(po + (g * QT + row) * (D + 4) + d);
       // (a set that saw nothing weighs nothing; a sum that is no number shows)
-      const float sc = ml[g].x == -__builtin_inff() ? 0.f
-                       : BASE2                      ? __builtin_amdgcn_exp2f(ml[g].x - m)
-                                                    : expf(ml[g].x - m);
+      const float sc = ml[g].x == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(ml[g].x - m);
       l = fmaf(sc, ml[g].y, l);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -329,8 +330,11 @@ __global__ __launch_bounds__(64 * WAVES, 2) void packed_bf16_kernel(PackedArgs a
   const KeyTiles<D, TL> tiles(a, kv, key0, t1 - key0 + 1, lds);
   tiles.load_k(0);
   if (VST == 2) tiles.load_v(0);
-  const int first = firsts.of(a, tok);
-  const Window win = window_of<31>(tok, first, key0);
+  const int toks[1] = {tok};
+  int first_of[1];
+  firsts.of(a, toks, first_of);
+  const int first = first_of[0];
+  const Window win = window_of(tok, first, key0);
 
   f32x16 o[DB];
 #pragma unroll
@@ -451,7 +455,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void packed_bf16_kernel(PackedArgs a
     if (h == 0) pml[at] = make_float2(m, l);
     if (h == 0 && sub == 0) pf[row] = first;
     __syncthreads();
-    join_rows<bf16, D, KG, QT, 64 * WAVES, true>(a, tile, kv, po, pml, pf);
+    join_rows<bf16, D, KG, QT, 64 * WAVES>(a, tile, kv, po, pml, pf);
     return;
   }
   // Through LDS, so that a wave stores whole rows (eight bytes a lane of 32 rows at
@@ -498,171 +502,182 @@ __global__ __launch_bounds__(64 * WAVES, 2) void packed_bf16_kernel(PackedArgs a
 }
 
 // ---------------------------------------------------------------------------
-// fp32, on v_mfma_f32_16x16x4_f32. Four waves share each 64-key tile in LDS: 4 / KW
-// strips of 16 queries, KW waves a strip over 64 / KW keys each, joined at the
-// end. Products are transposed: S^T = K Q^T leaves lane (quad, r) with keys
-// 4 quad .. 4 quad + 3 of query r, which is the B operand of O^T = V^T P^T as it
-// is. Score MFMA i of a chunk takes dims 16 c + 4 quad + i from both operands (one
-// 16-byte LDS read a lane), output MFMA j dims E r + j; rows are padded by 16
-// bytes against bank conflicts. A score is summed in four chains.
-constexpr int F_KT = 64;
-template <int D>
-constexpr int F_LDS = 2 * F_KT * (D + 4) * 4;
+// fp32, on v_mfma_f32_16x16x4_f32: a wave computes R strips of 16 query rows, 16
+// keys at a time, straight from registers; KW of a block's four waves share rows,
+// each over every KW-th 16 keys, joined at the end. Products are transposed:
+// S^T = K Q^T leaves lane (quad, r) with keys 4 quad .. 4 quad + 3 of query r,
+// which is the B operand of O^T = V^T P^T as it is. Score MFMA i of a chunk takes
+// dims 16 c + 4 quad + i from both operands, output MFMA j dims E r + j, so that a
+// lane reads K and V by 16 bytes just as it needs them, and no LDS or barrier
+// stands between: the next keys are on their way during the second product, the
+// values during the first. (By way of LDS, shared by the block's waves, one sequence
+// of 3,000 tokens of 7B heads took 625 us, so 521: 124 TFLOP/s, where a large library
+// product reaches 154. Keys and values fetched two steps ahead gained nothing.) A
+// score is summed in four chains.
+template <int D, int KW, int R>
+constexpr int F_LDS = 64 * R * (D + 4 + 2) * 4 + 64 / KW * R * 4;
 
-template <int D, int KW>
+template <int D, int KW, int R>
 __global__ __launch_bounds__(256, 2) void packed_f32_kernel(PackedArgs a) {
-  constexpr int KT = F_KT, QT = 64 / KW, KB = KT / 16 / KW, KC = D / 16, SW = 4 / KW;
+  constexpr int SW = 4 / KW, QT = 16 * R * SW, KC = D / 16;
   constexpr int E = D / 16 < 4 ? D / 16 : 4, HALVES = D / 16 / E;
-  constexpr int ROW = D + 4;
-  constexpr int PIECES = KT * D / 4, PER = (PIECES + 255) / 256;
-  static_assert(F_LDS<D> >= 64 * (D + 4 + 3) * 4, "the waves' results fit the tiles");
   extern __shared__ __attribute__((aligned(16))) float lds_f[];
-  float *Ks = lds_f, *Vs = lds_f + KT * ROW;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int lr = lane % 16, lq = lane / 16, strip = wave % SW, sub = wave / SW * KB * 16;
+  const int lr = lane % 16, lq = lane / 16, strips = wave % SW * R * 16, part = wave / SW;
   const int jb = a.by_hkv(blockIdx.x), kv = blockIdx.x - jb * a.Hkv, tile = a.tiles - 1 - jb;
   const int t0 = a.by_per(tile * QT), t1 = a.by_per(std::min(tile * QT + QT, a.rows) - 1);
   Firsts firsts(a, t0, t1);
-  const int r0 = tile * QT + strip * 16, r = std::min(r0 + lr, a.rows - 1);
-  const int tok = a.by_per(r), head = kv * a.per + r - tok * a.per;
-
-  f32x4 qa[KC];
-  {
-    const float* q = (const float*)a.q + tok * a.q_row + head * a.q_head;
+  int tok[R], first[R];
+  f32x4 qa[R][KC];
 #pragma unroll
-    for (int c = 0; c < KC; ++c) qa[c] = *(const f32x4*)(q + 16 * c + 4 * lq);
+  for (int s = 0; s < R; ++s) {
+    const int r = std::min(tile * QT + strips + 16 * s + lr, a.rows - 1);
+    tok[s] = a.by_per(r);
+    const float* q = (const float*)a.q + tok[s] * a.q_row + (kv * a.per + r - tok[s] * a.per) * a.q_head + 4 * lq;
+#pragma unroll
+    for (int c = 0; c < KC; ++c) qa[s][c] = *(const f32x4*)(q + 16 * c);
   }
-  const int key0 = firsts.begin(), keys = t1 - key0 + 1;
-  const int64_t row = a.kv_row * 4, at0 = key0 * row + kv * a.kv_head * 4;
-  f32x4 o[HALVES][E];
+  const int key0 = firsts.begin();
+  firsts.of(a, tok, first);
+  // this wave's steps of 16 keys, those that some of its rows see
+  const int from = __builtin_amdgcn_readfirstlane(first[0]), to = __builtin_amdgcn_readlane(tok[R - 1], 15);
+  const int all_from = __builtin_amdgcn_readlane(first[R - 1], 15), all_to = __builtin_amdgcn_readfirstlane(tok[0]);
+  int step = from == NONE ? 0 : (from - key0) / 16;
+  step += (part - step) & (KW - 1);
+  const int end = (to - key0) / 16;
+
+  const uint32_t row = (uint32_t)a.kv_row * 4;
+  const char *k = (const char*)a.k + (key0 * a.kv_row + kv * a.kv_head) * 4;
+  const char *v = (const char*)a.v + (key0 * a.kv_row + kv * a.kv_head) * 4;
+  const uint32_t koff = lr * row + 16 * lq;
+  uint32_t voff[4];
 #pragma unroll
-  for (int hf = 0; hf < HALVES; ++hf)
-#pragma unroll
-    for (int j = 0; j < E; ++j) o[hf][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float m = -__builtin_inff(), lsum = 0.f;
-  u32x4 kr[PER], vr[PER];
-  auto load_tile = [&](int key) {
-    // rows past the last read zeros (or, where rows overlap, the last again)
-    const uint32_t bytes = (std::min(keys - key, KT) - 1) * (uint32_t)row + D * 4;
-    const __amdgpu_buffer_rsrc_t krs = span_rsrc((const char*)a.k + at0 + key * row, bytes);
-    const __amdgpu_buffer_rsrc_t vrs = span_rsrc((const char*)a.v + at0 + key * row, bytes);
-#pragma unroll
-    for (int u = 0; u < PER; ++u) {
-      const int i = tid + 256 * u;  // (past the tile: not stored)
-      const uint32_t off = std::min(i / (D / 4), KT - 1) * (uint32_t)row + i % (D / 4) * 16;
-      kr[u] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(krs, off, 0, 0));
-      vr[u] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(vrs, off, 0, 0));
-    }
+  for (int e = 0; e < 4; ++e) voff[e] = (4 * lq + e) * row + 4 * E * lr;
+  // (rows past the last, and all those of a step past the end, read zeros)
+  auto rows_of = [&](const char* base, int i) {
+    const uint32_t bytes = i <= end ? (std::min(t1 - key0 - 16 * i, 15)) * row + D * 4 : 0;
+    return span_rsrc(base + (int64_t)(16 * i) * row, bytes);
   };
-  load_tile(0);
-  const int first = firsts.of(a, tok);
-  const Window win = window_of<15>(tok, first, key0);
-  for (int k0 = 0; k0 < keys; k0 += KT) {
-    __syncthreads();  // the previous tile is consumed
+  f32x4 kr[KC];
+  float vr[4][HALVES][E];
+  auto load_k = [&](int i) {
+    const __amdgpu_buffer_rsrc_t rs = rows_of(k, i);
 #pragma unroll
-    for (int u = 0; u < PER; ++u) {
-      const int i = tid + 256 * u;
-      if (i < PIECES) {
-        const int at = i / (D / 4) * ROW + i % (D / 4) * 4;
-        *(u32x4*)(Ks + at) = kr[u];
-        *(u32x4*)(Vs + at) = vr[u];
+    for (int c = 0; c < KC; ++c)
+      kr[c] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, koff + 64 * c, 0, 0));
+  };
+  auto load_v = [&](int i) {
+    const __amdgpu_buffer_rsrc_t rs = rows_of(v, i);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int hf = 0; hf < HALVES; ++hf) {
+        if constexpr (E == 4) {
+          const f32x4 x = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, voff[e] + 256 * hf, 0, 0));
+#pragma unroll
+          for (int j = 0; j < 4; ++j) vr[e][hf][j] = x[j];
+        } else if constexpr (E == 2) {
+          const float2 x = __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(rs, voff[e], 0, 0));
+          vr[e][hf][0] = x.x;
+          vr[e][hf][1] = x.y;
+        } else {
+          vr[e][hf][0] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rs, voff[e], 0, 0));
+        }
       }
-    }
-    __syncthreads();
-    if (k0 + KT < keys) load_tile(k0 + KT);
-    const int key = key0 + k0 + sub, last = key + KB * 16 - 1;  // this wave's
-    if (key > win.to || last < win.from) continue;
-    float p[KB][4];
-    float mx = -__builtin_inff();
+  };
+  f32x4 o[R][HALVES][E];
+  float m[R], l[R];  // (in powers of two)
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) {
+  for (int s = 0; s < R; ++s) {
+    m[s] = -__builtin_inff();
+    l[s] = 0.f;
+#pragma unroll
+    for (int hf = 0; hf < HALVES; ++hf)
+#pragma unroll
+      for (int j = 0; j < E; ++j) o[s][hf][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  const float scale = a.scale * 1.44269504f;
+  if (step <= end) load_k(step);
+  for (; step <= end; step += KW) {
+    const int key = key0 + 16 * step;
+    load_v(step);
+    f32x4 p[R];
+#pragma unroll
+    for (int s = 0; s < R; ++s) {
       f32x4 chain[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) chain[i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int c = 0; c < KC; ++c) {
-        const f32x4 k4 = *(const f32x4*)(Ks + (sub + kb * 16 + lr) * ROW + 16 * c + 4 * lq);
+      for (int c = 0; c < KC; ++c)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) chain[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(k4[i], qa[c][i], chain[i], 0, 0, 0);
-      }
-      const f32x4 acc = (chain[0] + chain[1]) + (chain[2] + chain[3]);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) p[kb][e] = acc[e] * a.scale;
+        for (int i = 0; i < 4; ++i)
+          chain[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(kr[c][i], qa[s][c][i], chain[i], 0, 0, 0);
+      p[s] = (chain[0] + chain[1]) + (chain[2] + chain[3]);
     }
-    if (key < win.all_from || last > win.all_to) {  // (a lane sees first .. tok)
-      const int lo = first - key - 4 * lq, hi = tok - key - 4 * lq;
+    load_k(step + KW);
+    if (key < all_from || key + 15 > all_to) {  // (a lane sees first .. tok)
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
+      for (int s = 0; s < R; ++s) {
+        const int lo = first[s] - key - 4 * lq, hi = tok[s] - key - 4 * lq;
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (kb * 16 + e < lo || kb * 16 + e > hi) p[kb][e] = -__builtin_inff();
+          if (e < lo || e > hi) p[s][e] = -__builtin_inff();
+      }
     }
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb)
+    for (int s = 0; s < R; ++s) {
+      const float mx = quads_max(fmaxf(fmaxf(p[s][0], p[s][1]), fmaxf(p[s][2], p[s][3])));
+      const float mn = fmaxf(m[s], mx * scale), ref = mn == -__builtin_inff() ? 0.f : mn;
+      if (__builtin_amdgcn_ballot_w64(mn != m[s])) {
+        const float alpha = mn == m[s] ? 1.f : __builtin_amdgcn_exp2f(m[s] - mn);
+        m[s] = mn;
+        l[s] *= alpha;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) mx = fmaxf(mx, p[kb][e]);
-    mx = quads_max(mx);
-    const float mn = fmaxf(m, mx), ref = mn == -__builtin_inff() ? 0.f : mn;
-    if (__builtin_amdgcn_ballot_w64(mn != m)) {
-      const float alpha = mn == m ? 1.f : expf(m - mn);
-      m = mn;
-      lsum *= alpha;
+        for (int hf = 0; hf < HALVES; ++hf)
+#pragma unroll
+          for (int j = 0; j < E; ++j) o[s][hf][j] *= alpha;
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        p[s][e] = __builtin_amdgcn_exp2f(fmaf(p[s][e], scale, -ref));
+        l[s] += p[s][e];
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
 #pragma unroll
       for (int hf = 0; hf < HALVES; ++hf)
 #pragma unroll
-        for (int j = 0; j < E; ++j) o[hf][j] *= alpha;
-    }
-#pragma unroll
-    for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        p[kb][e] = expf(p[kb][e] - ref);
-        lsum += p[kb][e];
-      }
-#pragma unroll
-    for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float* vrow = Vs + (sub + kb * 16 + 4 * lq + e) * ROW + E * lr;
-#pragma unroll
-        for (int hf = 0; hf < HALVES; ++hf) {
-          float v[E];
-          if constexpr (E == 4) {
-            const f32x4 v4 = *(const f32x4*)(vrow + 64 * hf);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = v4[j];
-          } else {
-#pragma unroll
-            for (int j = 0; j < E; ++j) v[j] = vrow[j];
-          }
+        for (int s = 0; s < R; ++s)
 #pragma unroll
           for (int j = 0; j < E; ++j)
-            o[hf][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[j], p[kb][e], o[hf][j], 0, 0, 0);
-        }
-      }
+            o[s][hf][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(vr[e][hf][j], p[s][e], o[s][hf][j], 0, 0, 0);
   }
-  // o[hf][j][x]: dim 64 hf + E (4 lq + x) + j of the lane's query; the KW waves of
-  // a strip joined through LDS, and stored from there by whole rows
-  lsum = quads_sum(lsum);
-  float* po = lds_f;                           // [KW][QT][D + 4]
-  float2* pml = (float2*)(po + 64 * (D + 4));  // [KW][QT]
-  int* pf = (int*)(pml + 64);                  // [QT]
-  const int at = wave / SW * QT + strip * 16 + lr;
-  __syncthreads();  // (the last tile is consumed)
+  // o[s][hf][j][x]: dim 64 hf + E (4 lq + x) + j of the lane's query; the KW waves
+  // of a strip joined through LDS, and stored from there by whole rows
+  float* po = lds_f;                               // [KW][QT][D + 4]
+  float2* pml = (float2*)(po + 64 * R * (D + 4));  // [KW][QT]
+  int* pf = (int*)(pml + 64 * R);                  // [QT]
 #pragma unroll
-  for (int hf = 0; hf < HALVES; ++hf)
+  for (int s = 0; s < R; ++s) {
+    const int at = part * QT + strips + 16 * s + lr;
 #pragma unroll
-    for (int x = 0; x < 4; ++x)
+    for (int hf = 0; hf < HALVES; ++hf)
 #pragma unroll
-      for (int j = 0; j < E; ++j) po[at * (D + 4) + 64 * hf + E * (4 * lq + x) + j] = o[hf][j][x];
-  if (lq == 0) pml[at] = make_float2(m, lsum);
-  if (lq == 0 && sub == 0) pf[strip * 16 + lr] = first;
+      for (int x = 0; x < 4; ++x)
+#pragma unroll
+        for (int j = 0; j < E; ++j) po[at * (D + 4) + 64 * hf + E * (4 * lq + x) + j] = o[s][hf][j][x];
+    l[s] = quads_sum(l[s]);
+    if (lq == 0) pml[at] = make_float2(m[s], l[s]);
+    if (lq == 0 && part == 0) pf[strips + 16 * s + lr] = first[s];
+  }
   __syncthreads();
-  join_rows<float, D, KW, QT, 256, false>(a, tile, kv, po, pml, pf);
+  join_rows<float, D, KW, QT, 256>(a, tile, kv, po, pml, pf);
 }
 
 // The form of a call from what the host knows, blocks of 128 rows and the mean
-// length (the rest is on the device): sets of waves a row, keys of a tile, waves.
+// length (the rest is on the device): sets of waves a row, keys of a tile or step,
+// waves, strips of a wave (fp32).
 // Measured (us, graph replays; n x L: n sequences of L tokens, blocks in brackets):
 // Four or two sets where blocks are few and the sequences longer than a tile (one
 //   against two against four sets):
@@ -678,11 +693,15 @@ __global__ __launch_bounds__(256, 2) void packed_f32_kernel(PackedArgs a) {
 //   0.5B heads, where all blocks are resident at once and the longest is what
 //   counts: one set 1x8191 (896) 175 159, 2x4096 (896) 97 85, two sets of eight waves
 //   1x6000 (658) 112 101, 2x3000 (658) 71 61; past that neither, 1x12000 (1,314) 330 337 334.
-// fp32, bound by its products sooner: 0.5B heads 1x512 (56) 30.8 19.6 15.2, 10x300 (330)
-//   44.7 34.7 35.8, 100x100 (1,094) 53.0 51.6 59.7; 7B heads 1x512 (112) 52.6 39.1 39.0, 1x1024
-//   (224) 117 99 108, 1x3000 (660) 625 654 763, 50x20 (220) 20.2 22.6 25.8.
+// fp32: four sets as long as the blocks are few for the lengths, of two strips for long
+//   sequences, one set for many short ones (n x up to L: random lengths; one, two, four
+//   sets of one strip, four of two):
+//   0.5B heads: 1x200 (22) 14.2 9.7 7.4 10.7, 5x668 (216) 47.2 37.3 33.8 37.8, 40x192 (404)
+//   29.8 23.6 25.0 26.2, 3x2846 (734) 305 284 284 266; 7B heads: 8x665 (548) 135 117 103
+//   108, 20x397 (844) 104 102 113 117, 100x200 (2,136) 158 167 209 216, 300x60 (2,016)
+//   91.7 107 151 160, 3x2846 (1,468) 1,055 999 1,011 936.
 struct PackedForm {
-  int sets, keys, waves;
+  int sets, keys, waves, strips = 1;
 };
 PackedForm packed_form(bool half, int D, int64_t rows, int64_t heads, int64_t tokens, int64_t sequences) {
   const int64_t blocks = cdiv(rows, 128) * heads, mean = tokens / std::max<int64_t>(sequences, 1);
@@ -694,8 +713,8 @@ PackedForm packed_form(bool half, int D, int64_t rows, int64_t heads, int64_t to
     if (D == 64 && mean >= 2500 && blocks <= 1024) return {1, 128, 4};
     return {1, 64, 4};
   }
-  if (mean < 64 && blocks > 128) return {1, 64, 4};
-  return {blocks * D <= 16384 ? 4 : blocks * D <= 45056 ? 2 : 1, 64, 4};
+  if (mean >= 700 && blocks >= 300) return {4, 16, 4, 2};
+  return {blocks <= 2 * mean ? 4 : blocks * D < 1024 * mean ? 2 : 1, 16, 4};
 }
 
 template <typename T, int D>
@@ -722,9 +741,10 @@ int packed_launch(hipStream_t st, PackedArgs a, const PackedForm& f) {
     constexpr int VST = D == 128 ? 1 : 2;
     return go(packed_bf16_kernel<D, 1, 64, 4, VST>, 128, Tile<D, 1, 64, 4, VST>::LDS);
   } else {
-    if (f.sets == 4) return go(packed_f32_kernel<D, 4>, 16, F_LDS<D>);
-    if (f.sets == 2) return go(packed_f32_kernel<D, 2>, 32, F_LDS<D>);
-    return go(packed_f32_kernel<D, 1>, 64, F_LDS<D>);
+    if (f.strips == 2) return go(packed_f32_kernel<D, 4, 2>, 32, F_LDS<D, 4, 2>);
+    if (f.sets == 4) return go(packed_f32_kernel<D, 4, 1>, 16, F_LDS<D, 4, 1>);
+    if (f.sets == 2) return go(packed_f32_kernel<D, 2, 1>, 32, F_LDS<D, 2, 1>);
+    return go(packed_f32_kernel<D, 1, 1>, 64, F_LDS<D, 1, 1>);
   }
 }
 

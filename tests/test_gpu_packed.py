@@ -242,6 +242,10 @@ FORMS = [
     (torch.bfloat16, (8, 2, 32), [60] * 300), (torch.bfloat16, (4, 2, 16), [60] * 300),
     (torch.float32, (14, 2, 64), [500]), (torch.float32, (28, 4, 128), [700]), (torch.float32, (14, 2, 64), [3000]),
     (torch.float32, (28, 4, 128), [60] * 300), (torch.float32, (8, 2, 32), [2500] * 6), (torch.float32, (4, 2, 16), [90] * 400),
+    (torch.float32, (28, 4, 128), [1500]), (torch.float32, (4, 2, 16), [5000, 4900]),     # two strips a wave
+    (torch.float32, (14, 2, 64), [100] * 60), (torch.float32, (28, 4, 128), [300] * 10),  # 2 sets
+    (torch.float32, (14, 2, 64), [20] * 600), (torch.float32, (8, 2, 32), [20] * 600),    # 1 set
+    (torch.float32, (4, 2, 16), [3] * 6000), (torch.float32, (8, 2, 32), [40, 30, 20]),
 ]
 
 
@@ -276,7 +280,7 @@ def test_forms(dtype, heads, lens):
     assert (err <= bar)[clean].all(), (err / bar)[clean].max()
 
 
-@pytest.mark.parametrize("dtype,heads,lens", [FORMS[i] for i in (0, 4, 8, 9, 10, 12, 16, 18, 19)],
+@pytest.mark.parametrize("dtype,heads,lens", [FORMS[i] for i in (0, 4, 8, 9, 10, 12, 16, 18, 19, 22, 24)],
                          ids=lambda x: f"{len(x)}x{x[0]}" if isinstance(x, list) else str(x))
 def test_a_text_of_nan(dtype, heads, lens):
     """Keys, values and queries that are no numbers from a row on, as a token
