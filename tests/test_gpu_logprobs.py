@@ -192,6 +192,28 @@ def test_shapes_and_strides(dtype):
     assert all(torch.equal(a, b) for a, b in zip(K.token_logprobs(logits, tokens.view(24, 1).expand(24, 2)[:, 0], top=6), want))
 
 
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("rows", [2, 520])
+def test_best_sets_in_few_threads(dtype, rows):
+    """A long row in which only sets of 64 logits that an eighth of the threads
+    look through stand out, so that more of them pass than the list of a block
+    holds (1,953 of 15,625 at a million logits)."""
+    from minitp import kernels as K
+
+    vocab = 1_000_000
+    g = torch.Generator(device=DEV).manual_seed(12)
+    one = torch.randn(2, vocab, generator=g, device=DEV)
+    sets = torch.arange(0, vocab, 64, device=DEV)
+    sets = sets[sets // 64 % 256 < 32]
+    one[0, sets] += 20 + torch.rand(sets.numel(), generator=g, device=DEV)
+    one[1, sets + 17] += 20
+    logits = one.to(dtype)
+    tokens = torch.tensor([64 * 5, 3], device=DEV)
+    r = K.token_logprobs(logits.repeat(rows // 2, 1), tokens.repeat(rows // 2), top=32)
+    for i in (0, rows - 2):
+        check(type(r)(*(t[i:i + 2] for t in r)), logits, tokens, 32)
+
+
 def test_rank_zero_is_the_greedy_pick():
     from minitp import kernels as K
 
