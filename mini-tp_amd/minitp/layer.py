@@ -286,10 +286,16 @@ class TPQwen2ForCausalLM(nn.Module):
         ids [N] one after the other, and their lengths (zeros too). No
         counterpart in the reference, whose batches are of one length. Each
         sequence is a prompt of its own from position 0; ``lm_head`` of a row
-        gives the logits of the token after it."""
+        gives the logits of the token after it. The lengths come from the host,
+        so it is not captured into a graph (RuntimeError)."""
+        dev = K._one_device("forward_packed", input_ids, self.model.embed_tokens.weight)
+        if K._elsewhere(dev):
+            with torch.cuda.device(dev):
+                return self.forward_packed(input_ids, lengths)
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("forward_packed: the lengths come from the host, a captured graph would keep them")
         lens = torch.tensor(lengths, dtype=torch.long, device="cpu")
         n, limit = input_ids.numel(), self.cfg.max_position_embeddings
-        N.require_gpu(input_ids, self.model.embed_tokens.weight, what="TPQwen2ForCausalLM.forward_packed")
         if input_ids.dim() != 1 or lens.dim() != 1 or bool((lens < 0).any()) or int(lens.sum()) != n:
             raise ValueError(f"forward_packed: ids {tuple(input_ids.shape)} in sequences of {int(lens.sum())} tokens in all")
         longest = int(lens.max()) if lens.numel() else 0

@@ -42,6 +42,11 @@ def score_tokens(model: TPQwen2ForCausalLM, sequences: Sequence[Sequence[int] | 
         raise ValueError(f"score_tokens: starts {list(starts)[:8]} for {len(sequences)} sequences, each at least 1")
     weight = model.model.embed_tokens.weight
     N.require_gpu(weight, what="score_tokens")
+    if K._elsewhere(weight.get_device()):
+        with torch.cuda.device(weight.device):
+            return score_tokens(model, sequences, top, starts, max_tokens)
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("score_tokens: texts come from the host, a captured graph would keep them")
     texts = []
     for s in sequences:
         t = s if isinstance(s, torch.Tensor) else torch.tensor(list(s), dtype=torch.long)

@@ -214,3 +214,28 @@ def test_refusals():
     for bad in (torch.zeros(2, 3, dtype=torch.long), torch.zeros(3)):
         with pytest.raises(ValueError):
             score_tokens(model, [bad])
+
+
+def test_no_capture():
+    """Texts and lengths come from the host: refused inside a captured graph,
+    which goes on without them, and right before and after."""
+    from minitp.scoring import score_tokens
+
+    model = build("tiny", torch.bfloat16)
+    text = texts_of([40], 1000)[0]
+    ids, x = text.to(DEV), torch.ones(8, device=DEV)
+    before = score_tokens(model, [text])[0]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = x + 1
+        with pytest.raises(RuntimeError, match="captured"):
+            model.forward_packed(ids, [40])
+        with pytest.raises(RuntimeError, match="captured"):
+            score_tokens(model, [text])
+        y = y * 3
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert (y == 6).all()
+        after = score_tokens(model, [text])[0]
+        assert all(torch.equal(a, b) for a, b in zip(before, after))
