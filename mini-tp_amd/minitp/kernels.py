@@ -497,7 +497,9 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
         raise ValueError(f"{what}: top={top} of {vocab} tokens (0 to {MAX_TOP})")
     dt = N.dtype_code(logits.dtype)
     rows = tokens.numel()
-    logits, tokens = logits.reshape(rows, vocab), tokens.contiguous()
+    tokens = tokens.contiguous()
+    if logits.dim() != 2:
+        logits = logits.reshape(rows, vocab)
     if logits.stride(1) != 1 and vocab > 1:
         logits = logits.contiguous()
     logprobs, entropy = logits.new_empty((2, *shape), dtype=torch.float32).unbind(0)

@@ -20,7 +20,7 @@ import torch
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
 BOTH = [torch.bfloat16, torch.float32]
-HEADS = [(14, 2, 64), (28, 4, 128), (4, 2, 16), (4, 4, 32), (8, 1, 128), (3, 1, 64), (9, 3, 16), (16, 8, 32)]
+HEADS = [(14, 2, 64), (28, 4, 128), (4, 2, 16), (4, 4, 32), (8, 1, 128), (3, 1, 64), (9, 3, 16), (16, 8, 32), (33, 1, 32)]
 
 
 def make(n, hq, hkv, d, dtype, layout="tokens", seed=0):
