@@ -322,7 +322,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void packed_bf16_kernel(PackedArgs a
   const int tok = a.by_per(r), head = kv * a.per + r - tok * a.per;
   bf16x8 qb[KS];
   {
-    const bf16* q = (const bf16*)a.q + tok * a.q_row + head * a.q_head + 8 * h;
+    const bf16* q = (const bf16*)a.q + (uint32_t)tok * (uint64_t)a.q_row + (uint32_t)head * (uint64_t)a.q_head + 8 * h;
 #pragma unroll
     for (int k = 0; k < KS; ++k) qb[k] = __builtin_bit_cast(bf16x8, *(const u32x4*)(q + 16 * k));
   }
@@ -468,15 +468,20 @@ __global__ __launch_bounds__(64 * WAVES, 2) void packed_bf16_kernel(PackedArgs a
   for (int d = 0; d < DB; ++d)
 #pragma unroll
     for (int i = 0; i < 16; ++i) most = __builtin_elementwise_maximum(most, fabsf(o[d][i]));
-  if (__builtin_amdgcn_ballot_w64(none)) {  // (a select for each value, which few waves need)
+  const bool odd = !(most < __builtin_inff());
+  const uint64_t bad = __builtin_amdgcn_ballot_w64(odd && l == l && !none && r0 + n32 < a.rows);
+  if (__builtin_amdgcn_ballot_w64(odd && none)) {  // (0 times hidden values that are infinite or NaN)
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
       for (int i = 0; i < 16; ++i) o[d][i] = none ? 0.f : o[d][i];
   }
-  const float f = none ? 0.f : 1.f / l;  // (a query that saw nothing above minus infinity: NaN)
+  // (a step of the reciprocal, 2^-23, is lost in the bf16 rounding; a query that saw
+  // nothing above minus infinity: NaN)
+  const float f = none ? 0.f : __builtin_amdgcn_rcpf(l);
   char* mine = lds + w * 32 * ROW;
   __syncthreads();  // (every stage is free)
+  if (r0 >= a.rows) return;
 #pragma unroll
   for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -487,15 +492,17 @@ __global__ __launch_bounds__(64 * WAVES, 2) void packed_bf16_kernel(PackedArgs a
       store_vec<bf16, 4>((bf16*)(mine + n32 * ROW) + 32 * d + 8 * c + 4 * h, v);
     }
   __builtin_amdgcn_wave_barrier();
+  // (lanes of a wave past the last row hold and store that row too)
   constexpr int RPI = 64 / H::CH;  // rows of a store
+  const int out_row = tok * a.Hq + head;
+  char* out = (char*)a.out + lane % H::CH * 16;
 #pragma unroll
   for (int i = 0; i < 32; i += RPI) {
-    const int row = i + lane / H::CH, rr = r0 + row;
+    const int row = i + lane / H::CH;
     const uint4 x = *(const uint4*)(mine + row * ROW + lane % H::CH * 16);
-    const int t = a.by_per(std::min(rr, a.rows - 1)), hd = kv * a.per + rr - t * a.per;
-    if (rr < a.rows) *(uint4*)((char*)a.out + ((int64_t)t * a.Hq + hd) * H::ROWB + lane % H::CH * 16) = x;
+    const uint32_t at = __builtin_amdgcn_ds_bpermute(4 * row, out_row);
+    *(uint4*)(out + (uint64_t)at * H::ROWB) = x;
   }
-  const uint64_t bad = __builtin_amdgcn_ballot_w64(!(most < __builtin_inff()) && l == l && !none && r0 + n32 < a.rows);
   if (bad == 0) return;
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the rows above are stored first)
   rows_again<bf16, D>(a, (uint32_t)(bad | bad >> 32), tok, head, first);
