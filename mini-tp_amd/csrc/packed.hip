@@ -28,6 +28,7 @@ struct PackedArgs {
   int S, Hq, Hkv, per;    // per: query heads of a KV head
   int rows;               // N * per: query rows of a KV head
   int tiles;              // ... in tiles
+  bool ranked;           // blocks take the tiles by ranked_tile
   const int64_t* offsets;  // [S + 1]
   float scale;
   Div by_per, by_hkv;
@@ -49,9 +50,14 @@ struct Firsts {
   __device__ __forceinline__ int offset(const PackedArgs& a, uint32_t i) const {
     return i <= (uint32_t)a.S ? (int)std::min<int64_t>(std::max<int64_t>(a.offsets[i], 0), NONE) : NONE;
   }
-  __device__ __forceinline__ Firsts(const PackedArgs& a, int t0_, int t1_) : lo(0), t0(t0_), t1(t1_) {
+  __device__ __forceinline__ explicit Firsts(const PackedArgs& a) : lo(0) {
+    if (a.S < 64) o = offset(a, threadIdx.x & 63);
+  }
+  __device__ __forceinline__ void seek(const PackedArgs& a, int t0_, int t1_) {
     const uint32_t lane = threadIdx.x & 63;
     uint32_t span = (uint32_t)a.S + 1;
+    t0 = t0_;
+    t1 = t1_;
     while (span > 64) {
       const uint32_t step = (span + 63) / 64;
       const uint64_t below = __builtin_amdgcn_ballot_w64(lane * step < span && offset(a, lo + lane * step) <= t0);
@@ -59,7 +65,7 @@ struct Firsts {
       lo += skip;
       span = std::min(step, span - skip);
     }
-    o = offset(a, lo + lane);
+    if (a.S >= 64) o = offset(a, lo + lane);
     const uint64_t below = __builtin_amdgcn_ballot_w64(o <= t0);
     const int at = below ? 63 - __builtin_clzll(below) : 0;
     first = below && lo + at < (uint32_t)a.S ? __builtin_amdgcn_readlane(o, at) : NONE;
@@ -87,6 +93,49 @@ struct Firsts {
     }
   }
 };
+
+__device__ __forceinline__ int wave_sum_int(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr:1, 2, 4, 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15, 31
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+  return __builtin_amdgcn_readlane(v, 63);
+}
+
+// The tile of QT rows that is taken as number `rank` where those with the most keys
+// come first, for up to 63 sequences (o: the offset of each lane). A sequence's n
+// tiles, those whose first row it holds, have levels 0 .. n - 1, one a QT rows; with
+// C(l) the number of tiles of level l and above, the level of a rank is the greatest
+// l with C(l) > rank. Tiles that begin with no sequence's row are the last. Each tile
+// has one rank; offsets in disorder, which all blocks see alike, leave the order of
+// the stream.
+template <int QT>
+__device__ __forceinline__ int ranked_tile(const PackedArgs& a, int o, int rank) {
+  const int lane = threadIdx.x & 63;
+  const int e = __builtin_amdgcn_update_dpp(0, o, 0x130, 0xf, 0xf, false);  // wave_shl:1
+  if (__builtin_amdgcn_ballot_w64(lane < a.S && (e < o || e > a.by_per(a.rows)))) return a.tiles - 1 - rank;
+  const int from = (o * a.per + QT - 1) / QT, n = lane < a.S ? (e * a.per + QT - 1) / QT - from : 0;
+  const int front = __builtin_amdgcn_readfirstlane(from), end = __builtin_amdgcn_readlane(from + n, a.S - 1);
+  if (rank >= end - front) {
+    const int k = rank - (end - front);
+    return k < front ? k : end + k - front;
+  }
+  int lo = 0, hi = (int)wave_max((float)n), above = 0;  // C(lo) > rank >= C(hi) = above
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1, c = wave_sum_int(std::max(n - mid, 0));
+    if (c > rank) {
+      lo = mid;
+    } else {
+      hi = mid;
+      above = c;
+    }
+  }
+  uint64_t there = __builtin_amdgcn_ballot_w64(n > lo);
+  for (int i = rank - above; i > 0; --i) there &= there - 1;
+  return __builtin_amdgcn_readlane(from, __builtin_ctzll(there)) + lo;
+}
 
 // One query of one head by one wave, in fp32, key by key and only those it sees:
 // a lane a key for the scores, a lane one or two dims of the output. The tile
@@ -315,9 +364,11 @@ __global__ __launch_bounds__(64 * WAVES, 2) void packed_bf16_kernel(PackedArgs a
   const int strip = w % TL::STRIPS, sub = w / TL::STRIPS * 32 * NB;  // of the rows; first of the wave's keys in a tile
   // The last rows, which see the most keys, first. (KV heads side by side: where
   // there are 1, 2, 4 or 8, an XCD's blocks, every eighth, share one's rows.)
-  const int jb = a.by_hkv(blockIdx.x), kv = blockIdx.x - jb * a.Hkv, tile = a.tiles - 1 - jb;
+  const int jb = a.by_hkv(blockIdx.x), kv = blockIdx.x - jb * a.Hkv;
+  Firsts firsts(a);
+  const int tile = a.ranked ? ranked_tile<QT>(a, firsts.o, jb) : a.tiles - 1 - jb;
   const int t0 = a.by_per(tile * QT), t1 = a.by_per(std::min(tile * QT + QT, a.rows) - 1);
-  Firsts firsts(a, t0, t1);
+  firsts.seek(a, t0, t1);
   const int r0 = tile * QT + strip * 32, r = std::min(r0 + n32, a.rows - 1);
   const int tok = a.by_per(r), head = kv * a.per + r - tok * a.per;
   bf16x8 qb[KS];
@@ -531,9 +582,11 @@ __global__ __launch_bounds__(256, 2) void packed_f32_kernel(PackedArgs a) {
   extern __shared__ __attribute__((aligned(16))) float lds_f[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lr = lane % 16, lq = lane / 16, strips = wave % SW * R * 16, part = wave / SW;
-  const int jb = a.by_hkv(blockIdx.x), kv = blockIdx.x - jb * a.Hkv, tile = a.tiles - 1 - jb;
+  const int jb = a.by_hkv(blockIdx.x), kv = blockIdx.x - jb * a.Hkv;
+  Firsts firsts(a);
+  const int tile = a.ranked ? ranked_tile<QT>(a, firsts.o, jb) : a.tiles - 1 - jb;
   const int t0 = a.by_per(tile * QT), t1 = a.by_per(std::min(tile * QT + QT, a.rows) - 1);
-  Firsts firsts(a, t0, t1);
+  firsts.seek(a, t0, t1);
   int tok[R], first[R];
   f32x4 qa[R][KC];
 #pragma unroll
@@ -687,11 +740,13 @@ __global__ __launch_bounds__(256, 2) void packed_f32_kernel(PackedArgs a) {
 // waves, strips of a wave (fp32).
 // Measured (us, graph replays; n x L: n sequences of L tokens, blocks in brackets):
 // Four or two sets where blocks are few and the sequences longer than a tile (one
-//   against two against four sets):
+//   set, two, four):
 //   0.5B heads (D 64): 2x64 (14) 5.7 5.9 5.3, 10x100 (110) 6.4 7.0 6.9, 1x500 (56) 10.4 9.7
 //   7.2, 5x300 (166) 9.6 10.5 11.5, 2x1300 (286) 26.2 24.7 22.5, 8x500 (438) 16.4 17.9
-//   22.8; 7B heads (128): 1x200 (44) 10.7 10.2 8.4, 3x200 (132) 12.0 11.8 18.7 (a block a
-//   CU), 1x1300 (288) 38.0 28.2 51.6, 3x500 (332) 21.1 23.6 42.0.
+//   22.8, up to L at random 4x700 (148) 16.6 13.4 (two sets), 6x700 (206) 15.5 13.0, 4x1500
+//   (272) 20.9 17.3, 4x3000 (540) 47.5 35.9, 12x700 (546) 20.5 25.9; 7B heads (128):
+//   1x200 (44) 10.7 10.2 8.4, 3x200 (132) 12.0 11.8 18.7 (a block a CU), 1x1300 (288) 38.0
+//   28.2 51.6, 3x500 (332) 21.1 23.6 42.0.
 //   Two sets over tiles of 128 keys instead of 64: 0.5B heads, 1x4096 (448) 60.4 53.3;
 //   7B heads (the tiles take a CU's LDS), 1x1024 (224) 25.6 30.1.
 // Tiles of 128 keys for long sequences: fewer barriers and lane exchanges a key.
@@ -714,7 +769,8 @@ PackedForm packed_form(bool half, int D, int64_t rows, int64_t heads, int64_t to
   const int64_t blocks = cdiv(rows, 128) * heads, mean = tokens / std::max<int64_t>(sequences, 1);
   if (half) {
     if (mean >= 64 && blocks <= std::min<int64_t>(64 + (D < 128 ? mean * 64 / (5 * D) : 0), 20480 / D)) return {4, 128, 4};
-    if (mean >= 300 && blocks <= std::min<int64_t>(mean * 2 / 5, D < 128 ? 32768 / D : 512)) return {2, D < 128 ? 128 : 64, 4};
+    if (D < 128 && mean >= 300 && blocks <= std::min<int64_t>(mean / 2 + 64, 34816 / D)) return {2, 128, 4};
+    if (D == 128 && mean >= 300 && blocks <= std::min<int64_t>(mean * 2 / 5, 512)) return {2, 64, 4};
     if (D == 128 && mean >= 2500) return {1, 128, 8};
     if (D == 64 && mean >= 2500 && blocks <= 768) return {2, 128, 8};
     if (D == 64 && mean >= 2500 && blocks <= 1024) return {1, 128, 4};
@@ -728,6 +784,12 @@ template <typename T, int D>
 int packed_launch(hipStream_t st, PackedArgs a, const PackedForm& f) {
   auto go = [&](auto kern, int rows, int lds) -> int {
     a.tiles = (int)cdiv(a.rows, rows);
+    // Ranked where the blocks outnumber what runs at once and the texts are few; of
+    // many, some are short enough for an even end, and keys of all at once do not stay
+    // in the L2s. In stream order and by rank (us): 7B heads, 16 texts of up to 1,500
+    // tokens 141 131, 8x1500 161 152, 6x2000 199 187, 40x400 81 89; 0.5B heads, 24 texts of
+    // up to 1,500 54 47, 6x2000 73 62, 50x100 in fp32 25.6 27.2.
+    a.ranked = a.S >= 2 && a.S < 32 && (int64_t)a.tiles * a.Hkv > 512;
     const int rc = ensure_lds_limit((const void*)kern, lds);
     if (rc) return rc;
     hipLaunchKernelGGL(kern, dim3((unsigned)(a.tiles * a.Hkv)), dim3(64 * f.waves), lds, st, a);

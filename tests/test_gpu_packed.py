@@ -304,6 +304,32 @@ def test_a_text_of_nan(dtype, heads, lens):
     assert ((out[rest[::97]].double() - want[rest[::97]].double()).abs() <= bar).all()
 
 
+@pytest.mark.parametrize("first,pad", [(0, 0), (37, 0), (0, 50), (333, 1000)])
+@pytest.mark.parametrize("dtype,heads,most", [(torch.bfloat16, (28, 4, 128), 0), (torch.bfloat16, (28, 4, 128), 300),
+                                              (torch.bfloat16, (14, 2, 64), 600), (torch.float32, (14, 2, 64), 300),
+                                              (torch.float32, (9, 3, 16), 500)])
+def test_order_of_the_tiles(dtype, heads, most, first, pad):
+    """Up to 31 sequences take their tiles by the number of keys, more of them in
+    the order of the stream (an empty one behind the others makes one more): every
+    row is computed once, to the same bits."""
+    from minitp import kernels as K
+
+    g = torch.Generator().manual_seed(most + first)
+    lens = torch.randint(-most // 6, most, (31,), generator=g).clamp(min=0).tolist() if most else [1900, 0, 1400]
+    n = first + sum(lens) + pad
+    x = make(n, *heads, dtype)
+    offsets = offsets_of(lens) + first
+    more = torch.cat([offsets, offsets[-1:].repeat(32 - len(lens))])
+    for _ in range(2):
+        torch.full((n, heads[0] * heads[2]), math.nan, dtype=dtype, device=DEV)  # (what the result's memory held)
+        out = K.packed_attention(*x, offsets)
+        assert torch.isfinite(out).all()
+        assert torch.equal(out, K.packed_attention(*x, more))
+    down = offsets.flip(0).contiguous()  # in disorder: as many rows as ever, no access outside
+    assert K.packed_attention(*x, down).shape == out.shape
+    torch.cuda.synchronize()
+
+
 def test_sequences_equal_prompts_on_their_own():
     """As far as the two kernels round alike: the model's prompt attention."""
     from minitp import kernels as K
