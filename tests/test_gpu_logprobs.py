@@ -100,6 +100,21 @@ def test_many_rows(rows, vocab, dtype):
         check(K.token_logprobs(*x, top=top), *x, top)
 
 
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("vocab", [3, 33, 255, 1017, 1021, 1022, 1025, 2040, 2041, 2042, 2049])
+def test_small_vocabularies(vocab, dtype):
+    """Around the sizes that one turn of a chunk a thread takes, rows at every
+    alignment."""
+    from minitp import kernels as K
+
+    for rows in (9, 700):
+        logits, tokens = make(rows, vocab, dtype)
+        for top in (0, 1, min(5, vocab), min(32, vocab)):
+            check(K.token_logprobs(logits, tokens, top=top), logits, tokens, top)
+        flat = torch.zeros_like(logits)
+        check(K.token_logprobs(flat, tokens, top=min(32, vocab)), flat, tokens, min(32, vocab))
+
+
 @pytest.mark.parametrize("rows", [1, 40, 600])
 @pytest.mark.parametrize("dtype", BOTH)
 def test_equal_logits_go_to_the_lower_token(dtype, rows):
