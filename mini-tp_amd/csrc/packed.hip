@@ -42,8 +42,8 @@ constexpr int NONE = INT32_MAX;  // the first row of a token of no sequence
 // t0's sequence, of(tok) of any token of the tile: the last offset not above it,
 // NONE if there is none or it is the sequences' end. (Offsets in disorder give some
 // row not past the token.) Those of up to 63 sequences are all loaded before the tile
-// is known, which ranked_tile may choose by them. No LDS and no barrier: the first keys are on their way
-// one load after the offsets.
+// is known, which ranked_tile may choose by them. No LDS and no barrier: the first keys
+// are on their way one load after the offsets.
 struct Firsts {
   uint32_t lo;   // the offset that lane 0 holds
   int o, first;  // this lane's; that of t0
