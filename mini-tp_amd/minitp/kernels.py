@@ -426,36 +426,37 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     if _elsewhere(dev):
         with torch.cuda.device(dev):
             return packed_attention(q, k, v, offsets)
-    if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]:
-        raise ValueError(f"{what}: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}, expected [N, Hq, D] and "
+    shape, kv_shape = q.shape, k.shape
+    if len(shape) != 3 or len(kv_shape) != 3 or v.shape != kv_shape or kv_shape[0] != shape[0] or kv_shape[2] != shape[2]:
+        raise ValueError(f"{what}: q {tuple(shape)}, k {tuple(kv_shape)}, v {tuple(v.shape)}, expected [N, Hq, D] and "
                          "[N, Hkv, D]")
-    if offsets.dim() != 1 or offsets.numel() < 1:
+    ends = offsets.numel()
+    if offsets.dim() != 1 or ends < 1:
         raise ValueError(f"{what}: offsets {tuple(offsets.shape)}, expected [sequences + 1]")
-    dtype, (n, hq, d), hkv = q.dtype, q.shape, k.shape[1]
+    dtype, (n, hq, d), hkv = q.dtype, shape, kv_shape[1]
     if k.dtype != dtype or v.dtype != dtype:
         raise TypeError(f"{what}: dtype mismatch q={dtype} k={k.dtype} v={v.dtype}")
     dt = N.dtype_code(dtype)
-    offsets = _lens(what, offsets, offsets.numel())
-    q, q_row, q_head = _head_rows(q)
-    k, kv_row, kv_head = _head_rows(k)
-    v, v_row, v_head = _head_rows(v)
+    offsets = _lens(what, offsets, ends)
+    size = 2 if dt == N.BF16 else 4
+    q, q_row, q_head = _head_rows(q, n, hq, d, size)
+    k, kv_row, kv_head = _head_rows(k, n, hkv, d, size)
+    v, v_row, v_head = _head_rows(v, n, hkv, d, size)
     if (v_row, v_head) != (kv_row, kv_head):
         k, v = k.contiguous(), v.contiguous()
         kv_row, kv_head = hkv * d, d
     out = q.new_empty((n, hq * d))
     N.check(_lib().minitp_packed_attention(N.stream(), dt, q.data_ptr(), q_row, q_head, k.data_ptr(), v.data_ptr(),
-                                           kv_row, kv_head, out.data_ptr(), n, offsets.numel() - 1, hq, hkv, d,
+                                           kv_row, kv_head, out.data_ptr(), n, ends - 1, hq, hkv, d,
                                            offsets.data_ptr()), what)
     return out
 
 
-def _head_rows(x: torch.Tensor) -> tuple[torch.Tensor, int, int]:
-    """[N, H, D] with rows of whole 16-byte pieces, and its row and head strides
-    (0 along a dim of one)."""
-    n, h, d = x.shape
+def _head_rows(x: torch.Tensor, n: int, h: int, d: int, size: int) -> tuple[torch.Tensor, int, int]:
+    """x [n, h, d] of elements of `size` bytes with rows of whole 16-byte pieces,
+    and its row and head strides (0 along a dim of one)."""
     row, head, one = x.stride()
     row, head = row if n > 1 else 0, head if h > 1 else 0
-    size = x.element_size()
     if (one != 1 and d > 1) or row * size % 16 or head * size % 16 or x.data_ptr() % 16:
         x = x.clone(memory_format=torch.contiguous_format)  # (contiguous() keeps unaligned rows)
         row, head = h * d, d
@@ -502,8 +503,11 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
         logits = logits.reshape(rows, vocab)
     if logits.stride(1) != 1 and vocab > 1:
         logits = logits.contiguous()
-    logprobs, entropy = logits.new_empty((2, *shape), dtype=torch.float32).unbind(0)
-    top_logprobs = logits.new_empty((*shape, top), dtype=torch.float32)
+    logprobs, entropy, top_logprobs = logits.new_empty(rows * (2 + top), dtype=torch.float32).split_with_sizes(
+        (rows, rows, rows * top))
+    if len(shape) != 1:
+        logprobs, entropy = logprobs.view(shape), entropy.view(shape)
+    top_logprobs = top_logprobs.view(*shape, top)
     ranks = torch.empty_like(tokens)
     top_tokens = tokens.new_empty((*shape, top))
     nbytes = _token_logprobs_bytes(dt, rows, vocab, top)
