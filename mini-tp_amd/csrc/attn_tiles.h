@@ -71,11 +71,6 @@ struct Half {
 __device__ __forceinline__ void row_dma16(u32x4 r, uint32_t voff, uint32_t lds_addr) {
   asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(r), "{m0}"(lds_addr) : "memory");
 }
-// (soff: a wave-uniform offset more)
-__device__ __forceinline__ void row_dma16(u32x4 r, uint32_t voff, uint32_t soff, uint32_t lds_addr) {
-  asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds" ::"v"(voff), "s"(r), "s"(soff), "{m0}"(lds_addr)
-               : "memory");
-}
 __device__ __forceinline__ u32x4 rows_rsrc(const void* base, int bytes) {
   const uint64_t p = (uint64_t)base;
   u32x4 r;

@@ -332,10 +332,15 @@ struct KeyTiles {
     return rows_rsrc(base + (int64_t)t * TL::KT * row, left > 0 ? (left - 1) * (uint32_t)row + H::ROWB : 0);
   }
   __device__ __forceinline__ void load_rows(u32x4 r, uint32_t off, uint32_t at) const {
-    uint32_t lds = __builtin_amdgcn_readfirstlane(to + at), step = __builtin_amdgcn_readfirstlane(piece);
-    asm volatile("s_nop 4" : "+s"(lds), "+s"(step));
+    uint32_t lds = __builtin_amdgcn_readfirstlane(to + at);
+    // (the sums are made anew each time: kept over the loop they take the registers of
+    // a third block a CU)
+    asm volatile("s_nop 4" : "+s"(lds), "+v"(off));
+    // The steps go into the lanes' offsets: a scalar one may lie past the resource's
+    // end by itself, where the bounds check need not hold. (At 2^24 elements a row
+    // those of 128 rows are below 2^32 bytes.)
 #pragma unroll
-    for (int j = 0; j < std::max(TL::PPW, 1); ++j) row_dma16(r, off, j * step, lds + j * TL::WAVES * 1024);
+    for (int j = 0; j < std::max(TL::PPW, 1); ++j) row_dma16(r, off + j * piece, lds + j * TL::WAVES * 1024);
   }
   __device__ __forceinline__ bool mine(bool v) const {  // (few pieces: half of the waves K, half V)
     return TL::PPW > 0 || (__builtin_amdgcn_readfirstlane(threadIdx.x >> 6) >= TL::PIECES) == v;
