@@ -140,15 +140,14 @@ __device__ __forceinline__ int ranked_tile(const PackedArgs& a, int o, int rank)
 
 // One query of one head by one wave, in fp32, key by key and only those it sees:
 // a lane a key for the scores, a lane one or two dims of the output. The tile
-// kernels turn to it for a query whose result is not finite while the sum of its
-// probabilities is: in a product over a whole tile a hidden value that is infinite
-// or NaN shows (0 times it is no zero), here it does not. (A sum that is no number
-// comes from keys that the query sees, and so is the result: no slow way for texts
-// of NaN.)
+// kernels turn to it (rows_again) where a hidden value that is infinite or NaN
+// shows in a product over a whole tile, as 0 times it is no zero.
 template <typename T, int D>
 __device__ __forceinline__ void packed_row(const PackedArgs& a, int r, int first, int head) {
   constexpr int VE = Vec<T>::N, DL = D > 64 ? D / 64 : 1;
-  const int lane = threadIdx.x & 63, kv = head / a.per;
+  const int kv = head / a.per;
+  int lane = threadIdx.x & 63;
+  asm volatile("" : "+v"(lane));  // (or addresses are made, and kept, before they are needed)
   const T* q = (const T*)a.q + r * a.q_row + head * a.q_head;
   const T* k = (const T*)a.k + kv * a.kv_head;
   const T* v = (const T*)a.v + kv * a.kv_head;
@@ -160,7 +159,7 @@ __device__ __forceinline__ void packed_row(const PackedArgs& a, int r, int first
     const int key = k0 + lane;
     const T* krow = k + std::min(key, r) * a.kv_row;
     float s = 0.f;
-#pragma unroll 1
+#pragma unroll 2
     for (int d = 0; d < D; d += VE) {
       float x[VE], y[VE];
       load_vec<T, VE>(q + d, x);
@@ -177,11 +176,25 @@ __device__ __forceinline__ void packed_row(const PackedArgs& a, int r, int first
 #pragma unroll
     for (int d = 0; d < DL; ++d) o[d] *= alpha;
     const int n = std::min(64, r - k0 + 1);
-    for (int j = 0; j < n; ++j) {
-      const float pj = __shfl(p, j, 64);
+    int j = 0;
+    auto values = [&](auto keys) {  // as many loads at once
+      constexpr int U = decltype(keys)::value;
+      for (; j + U <= n; j += U) {
+        float x[U][DL];
 #pragma unroll
-      for (int d = 0; d < DL; ++d) o[d] = fmaf(pj, load_f32<T>(v + (k0 + j) * a.kv_row, dim + d), o[d]);
-    }
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int d = 0; d < DL; ++d) x[u][d] = load_f32<T>(v + (k0 + j + u) * a.kv_row, dim + d);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const float pj = __shfl(p, j + u, 64);
+#pragma unroll
+          for (int d = 0; d < DL; ++d) o[d] = fmaf(pj, x[u][d], o[d]);
+        }
+      }
+    };
+    values(std::integral_constant<int, 8>{});
+    values(std::integral_constant<int, 1>{});
   }
   T* out = (T*)a.out + ((int64_t)r * a.Hq + head) * D;
   if (lane * DL < D) {
@@ -190,15 +203,60 @@ __device__ __forceinline__ void packed_row(const PackedArgs& a, int r, int first
   }
 }
 
-// The rows of a wave whose results are not finite (bits of lanes 0 .. 31, or 15),
-// computed again one by one.
+// The first of the rows from .. to of V with a value that is not finite, NONE if
+// there is none.
 template <typename T, int D>
-__device__ __forceinline__ void rows_again(const PackedArgs& a, uint64_t odd, int tok, int head, int first) {
+__device__ __forceinline__ int odd_value(const PackedArgs& a, int kv, int from, int to) {
+  constexpr int VE = Vec<T>::N, CH = D / VE, ROWS = 64 / CH, U = 4;  // rows and loads at a time
+  int lane = threadIdx.x & 63;
+  asm volatile("" : "+v"(lane));  // (as in packed_row)
+  const T* v = (const T*)a.v + kv * a.kv_head + lane % CH * VE;
+  for (int k0 = from; k0 <= to; k0 += U * ROWS) {
+    bool odd[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float x[VE];
+      load_vec<T, VE>(v + std::min(k0 + u * ROWS + lane / CH, to) * a.kv_row, x);
+      odd[u] = false;
+#pragma unroll
+      for (int e = 0; e < VE; ++e) odd[u] |= !(fabsf(x[e]) < __builtin_inff());
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint64_t there = __builtin_amdgcn_ballot_w64(odd[u]);
+      if (there) return std::min(k0 + u * ROWS + __builtin_ctzll(there) / CH, to);
+    }
+  }
+  return NONE;
+}
+
+// Rows of a wave (bits of their lanes, in the rows' order) whose results are not
+// finite while the sums of their probabilities are numbers. (A sum that is none comes
+// from keys that the query sees, and so is the result.) What a query sees of infinite
+// and NaN values belongs in its result; the others, which see none or have one among
+// the hidden keys of their tiles too, key0 .. to, are computed again one by one. (One
+// text of 8,000 tokens, 7B heads, 480 us: 540 with an infinite value near its start,
+// which nearly all rows see; 10,200 with one in the middle, for the rows of its tile
+// in front of it; 44,400 with one in every row.)
+template <typename T, int D>
+__device__ __forceinline__ void rows_again(const PackedArgs& a, uint64_t odd, int kv, int tok, int head, int first,
+                                           int key0, int to) {
+  int of = -1, seen = NONE, next = -1;  // the first such value of the sequence that begins at `of`; behind a row
+  bool front = false;                   // one in front of it
   while (odd) {
     const int lane = __builtin_ctzll(odd);
     odd &= odd - 1;
-    packed_row<T, D>(a, __builtin_amdgcn_readlane(tok, lane), __builtin_amdgcn_readlane(first, lane),
-                     __builtin_amdgcn_readlane(head, lane));
+    const int r = __builtin_amdgcn_readlane(tok, lane), f = __builtin_amdgcn_readlane(first, lane);
+    if (f != of) {
+      of = f;
+      seen = odd_value<T, D>(a, kv, f, to);
+      front = odd_value<T, D>(a, kv, key0, f - 1) != NONE;
+    }
+    if (seen <= r) {
+      if (next <= r) next = odd_value<T, D>(a, kv, r + 1, to);
+      if (!front && next == NONE) continue;
+    }
+    packed_row<T, D>(a, r, f, __builtin_amdgcn_readlane(head, lane));
   }
 }
 
@@ -218,10 +276,10 @@ __device__ __forceinline__ Window window_of(int tok, int first, int key0) {
 // own, in LDS: po [KG][QT] rows of D, padded by 16 bytes (lanes of a wave write
 // 32 rows at a time), pml [KG][QT] (maximum, as a power of two, and sum), pf [QT]
 // first rows. Joined and stored by whole rows, LPR lanes a row; the ones
-// that are not finite again by packed_row.
+// that are not finite by rows_again (key0 .. to: the tile's keys).
 template <typename T, int D, int KG, int QT, int THREADS>
-__device__ __forceinline__ void join_rows(const PackedArgs& a, int tile, int kv, const float* po, const float2* pml,
-                                          const int* pf) {
+__device__ __forceinline__ void join_rows(const PackedArgs& a, int tile, int kv, int key0, int to, const float* po,
+                                          const float2* pml, const int* pf) {
   constexpr int LPR = D / 4;
   const int n = std::min(QT, a.rows - tile * QT);
   for (int i0 = 0; i0 < n * LPR; i0 += THREADS) {
@@ -261,7 +319,7 @@ __device__ __forceinline__ void join_rows(const PackedArgs& a, int tile, int kv,
     }
     if (again == 0) continue;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the rows above are stored first)
-    rows_again<T, D>(a, again, tok, head, first);
+    rows_again<T, D>(a, again, kv, tok, head, first, key0, to);
   }
 }
 
@@ -518,7 +576,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void packed_bf16_kernel(PackedArgs a
     if (h == 0) pml[at] = make_float2(m, l);
     if (h == 0 && sub == 0) pf[row] = first;
     __syncthreads();
-    join_rows<bf16, D, KG, QT, 64 * WAVES>(a, tile, kv, po, pml, pf);
+    join_rows<bf16, D, KG, QT, 64 * WAVES>(a, tile, kv, key0, t1, po, pml, pf);
     return;
   }
   // Through LDS, so that a wave stores whole rows (eight bytes a lane of 32 rows at
@@ -568,7 +626,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void packed_bf16_kernel(PackedArgs a
   }
   if (bad == 0) return;
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the rows above are stored first)
-  rows_again<bf16, D>(a, (uint32_t)(bad | bad >> 32), tok, head, first);
+  rows_again<bf16, D>(a, (uint32_t)(bad | bad >> 32), kv, tok, head, first, key0, t1);
 }
 
 // ---------------------------------------------------------------------------
@@ -744,7 +802,7 @@ __global__ __launch_bounds__(256, 2) void packed_f32_kernel(PackedArgs a) {
     if (lq == 0 && part == 0) pf[strips + 16 * s + lr] = first[s];
   }
   __syncthreads();
-  join_rows<float, D, KW, QT, 256>(a, tile, kv, po, pml, pf);
+  join_rows<float, D, KW, QT, 256>(a, tile, kv, key0, t1, po, pml, pf);
 }
 
 // The form of a call from what the host knows, blocks of 128 rows and the mean
