@@ -141,7 +141,7 @@ __device__ __forceinline__ int ranked_tile(const PackedArgs& a, int o, int rank)
 // One query of one head by one wave, in fp32, key by key and only those it sees:
 // a lane a key for the scores, a lane one or two dims of the output. The tile
 // kernels turn to it (rows_again) where a hidden value that is infinite or NaN
-// shows in a product over a whole tile, as 0 times it is no zero.
+// shows in a product over a whole tile, as 0 times it is no zero, and for far scores.
 template <typename T, int D>
 __device__ __forceinline__ void packed_row(const PackedArgs& a, int r, int first, int head) {
   constexpr int VE = Vec<T>::N, DL = D > 64 ? D / 64 : 1;
@@ -230,8 +230,19 @@ __device__ __forceinline__ int odd_value(const PackedArgs& a, int kv, int from, 
   return NONE;
 }
 
+// The tiles' reference is their maximum in powers of two, rounded, so off by 2^-24 of
+// itself, which probabilities share. For scores far from zero that is more than an
+// exponent's range: above 2^22 the reference keeps that much and more above the
+// maximum, and rows of which it leaves nothing (no sum, though they saw a key above
+// minus infinity) are computed again. (Minus infinity gives NaN, which no maximum takes.)
+__device__ __forceinline__ float reference_of(float x) {
+  return x + fmaxf(fmaf(fabsf(x), 0x1p-22f, -1.f), 0.f);
+}
+__device__ __forceinline__ bool far_sum(float m, float l) { return m > -__builtin_inff() && l < 0x1p-30f; }
+
 // Rows of a wave (bits of their lanes, in the rows' order) whose results are not
-// finite while the sums of their probabilities are numbers. (A sum that is none comes
+// finite while the sums of their probabilities are numbers, and, all of them, the `far`
+// ones by far_sum. (A sum that is none comes
 // from keys that the query sees, and so is the result.) What a query sees of infinite
 // and NaN values belongs in its result; the others, which see none or have one among
 // the hidden keys of their tiles too, key0 .. to, are computed again one by one. (One
@@ -239,20 +250,19 @@ __device__ __forceinline__ int odd_value(const PackedArgs& a, int kv, int from, 
 // which nearly all rows see; 10,200 with one in the middle, for the rows of its tile
 // in front of it; 44,400 with one in every row.)
 template <typename T, int D>
-__device__ __forceinline__ void rows_again(const PackedArgs& a, uint64_t odd, int kv, int tok, int head, int first,
-                                           int key0, int to) {
+__device__ __forceinline__ void rows_again(const PackedArgs& a, uint64_t odd, uint64_t far, int kv, int tok, int head,
+                                           int first, int key0, int to) {
   int of = -1, seen = NONE, next = -1;  // the first such value of the sequence that begins at `of`; behind a row
   bool front = false;                   // one in front of it
-  while (odd) {
-    const int lane = __builtin_ctzll(odd);
-    odd &= odd - 1;
+  for (uint64_t left = odd | far; left; left &= left - 1) {
+    const int lane = __builtin_ctzll(left);
     const int r = __builtin_amdgcn_readlane(tok, lane), f = __builtin_amdgcn_readlane(first, lane);
     if (f != of) {
       of = f;
       seen = odd_value<T, D>(a, kv, f, to);
       front = odd_value<T, D>(a, kv, key0, f - 1) != NONE;
     }
-    if (seen <= r) {
+    if (seen <= r && !(far >> lane & 1)) {
       if (next <= r) next = odd_value<T, D>(a, kv, r + 1, to);
       if (!front && next == NONE) continue;
     }
@@ -306,20 +316,24 @@ __device__ __forceinline__ void join_rows(const PackedArgs& a, int tile, int kv,
     }
     const int r = tile * QT + row, tok = a.by_per(r), head = kv * a.per + r - tok * a.per, first = pf[row];
     const bool there = i < n * LPR;
-    const uint64_t bad = __builtin_amdgcn_ballot_w64(there && first != NONE && odd != 0.f && l == l);
-    uint64_t again = 0;  // (a row: its first lane)
+    auto rows = [](uint64_t lanes) {  // (a row: its first lane)
+      uint64_t firsts = 0;
 #pragma unroll
-    for (int x = 0; x < 64; x += LPR)
-      if (bad >> x & ((1ull << LPR) - 1)) again |= 1ull << x;
+      for (int x = 0; x < 64; x += LPR)
+        if (lanes >> x & ((1ull << LPR) - 1)) firsts |= 1ull << x;
+      return firsts;
+    };
+    const uint64_t again = rows(__builtin_amdgcn_ballot_w64(there && first != NONE && odd != 0.f && l == l));
+    const uint64_t far = rows(__builtin_amdgcn_ballot_w64(there && far_sum(m, l)));
     if (there) {
       float y[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) y[e] = first == NONE ? 0.f : v[e] / l;
       store_vec<T, 4>((T*)a.out + ((int64_t)tok * a.Hq + head) * D + d, y);
     }
-    if (again == 0) continue;
+    if ((again | far) == 0) continue;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the rows above are stored first)
-    rows_again<T, D>(a, again, kv, tok, head, first, key0, to);
+    rows_again<T, D>(a, again, far, kv, tok, head, first, key0, to);
   }
 }
 
@@ -521,7 +535,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void packed_bf16_kernel(PackedArgs a
     for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
       for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kb][i]);
-    mx = halves_max(mx) * sl2;
+    mx = reference_of(halves_max(mx) * sl2);
     if (__builtin_amdgcn_ballot_w64(mx > m + SLACK)) {
       const float mn = fmaxf(m, mx), alpha = mn == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(m - mn);
       m = mn;
@@ -591,6 +605,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void packed_bf16_kernel(PackedArgs a
     for (int i = 0; i < 16; ++i) most = __builtin_elementwise_maximum(most, fabsf(o[d][i]));
   const bool odd = !(most < __builtin_inff());
   const uint64_t bad = __builtin_amdgcn_ballot_w64(odd && l == l && !none && r0 + n32 < a.rows);
+  const uint64_t far = __builtin_amdgcn_ballot_w64(far_sum(m, l) && r0 + n32 < a.rows);
   if (__builtin_amdgcn_ballot_w64(odd && none)) {  // (0 times hidden values that are infinite or NaN)
 #pragma unroll
     for (int d = 0; d < DB; ++d)
@@ -624,9 +639,9 @@ __global__ __launch_bounds__(64 * WAVES, 2) void packed_bf16_kernel(PackedArgs a
     const uint32_t at = __builtin_amdgcn_ds_bpermute(4 * row, out_row);
     *(uint4*)(out + (uint64_t)at * H::ROWB) = x;
   }
-  if (bad == 0) return;
+  if ((bad | far) == 0) return;
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the rows above are stored first)
-  rows_again<bf16, D>(a, (uint32_t)(bad | bad >> 32), kv, tok, head, first, key0, t1);
+  rows_again<bf16, D>(a, (uint32_t)(bad | bad >> 32), (uint32_t)far, kv, tok, head, first, key0, t1);
 }
 
 // ---------------------------------------------------------------------------
@@ -757,7 +772,7 @@ __global__ __launch_bounds__(256, 2) void packed_f32_kernel(PackedArgs a) {
 #pragma unroll
     for (int s = 0; s < R; ++s) {
       const float mx = quads_max(fmaxf(fmaxf(p[s][0], p[s][1]), fmaxf(p[s][2], p[s][3])));
-      const float mn = fmaxf(m[s], mx * scale), ref = mn == -__builtin_inff() ? 0.f : mn;
+      const float mn = fmaxf(m[s], reference_of(mx * scale)), ref = mn == -__builtin_inff() ? 0.f : mn;
       if (__builtin_amdgcn_ballot_w64(mn != m[s])) {
         const float alpha = mn == m[s] ? 1.f : __builtin_amdgcn_exp2f(m[s] - mn);
         m[s] = mn;

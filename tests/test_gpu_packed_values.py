@@ -97,3 +97,37 @@ def test_an_early_infinity_takes_no_longer(dtype, heads, length):
 
     time(v)
     assert time(bad) <= 8 * time(v)
+
+
+@pytest.mark.parametrize("power", [20, 31, 36, 44, 90])
+@pytest.mark.parametrize("dtype,heads,lens", [
+    (torch.bfloat16, (28, 4, 128), [300]), (torch.bfloat16, (14, 2, 64), [2500, 333]), (torch.bfloat16, (28, 4, 128), [60] * 300),
+    (torch.bfloat16, (14, 2, 64), [60] * 300), (torch.bfloat16, (4, 2, 16), [60] * 300), (torch.float32, (28, 4, 128), [300]),
+    (torch.float32, (14, 2, 64), [60] * 300), (torch.float32, (8, 2, 32), [20] * 600),
+], ids=lambda x: f"{len(x)}x{x[0]}" if isinstance(x, list) else str(x))
+def test_far_scores(dtype, heads, lens, power):
+    """Scores up to 2^power / sqrt(D) of either sign, past what a rounded maximum
+    in powers of two holds to a step of one. They are products of two numbers of
+    eight bits, so exact, and apart by at least |q|: at 2^20 and above another
+    key's probability is e^-2 of the greatest or less, known to 2^-15 (256 such
+    steps are the whole range, each score off by 2^-24 of itself)."""
+    from minitp import kernels as K
+
+    hq, hkv, d = heads
+    n = sum(lens)
+    g = torch.Generator(device=DEV).manual_seed(power + n)
+
+    def whole(h):
+        return torch.randint(-255, 256, (n, h), generator=g, device=DEV).float()
+
+    q, k = torch.zeros(n, hq, d, device=DEV), torch.zeros(n, hkv, d, device=DEV)
+    q[..., d // 2], k[..., d // 2] = whole(hq) * 2.0 ** (power - 16), whole(hkv)
+    q, k = q.to(dtype), k.to(dtype)
+    v = torch.randn(n, hkv, d, generator=g, device=DEV).to(dtype)
+    rows = sorted(set(range(0, n, max(n // 60, 1))) | {n - 1})
+    ref, mag = sampled(q, k, v, lens, rows)
+    got = K.packed_attention(q, k, v, offsets_of(lens)).view(n, hq, d)
+    assert torch.isfinite(got).all()
+    bar = bars(ref, mag, dtype, d) + mag * 2 ** -14 + 1e-9
+    err = (got[rows].double() - ref).abs()
+    assert (err <= bar).all(), (err / bar).max()
