@@ -345,7 +345,8 @@ __device__ __forceinline__ void join_rows(const PackedArgs& a, int tile, int kv,
 //
 // A tile of K and V rows goes to LDS as it lies in memory, by loads that bypass
 // the registers, while the tile before it is computed (two stages, one barrier a
-// tile). Products are transposed, S^T = K Q^T and O^T = V^T P^T, so a lane's
+// tile; VST 1 has one stage of V, which is loaded during its own tile's scores, and a
+// second barrier, for a third block a CU). Products are transposed, S^T = K Q^T and O^T = V^T P^T, so a lane's
 // scores belong to one query and its probabilities are the second product's
 // operand as they are, the k-index of both operands permuted alike; V^T comes
 // out of LDS transposed by ds_read_b64_tr_b16. A row's 16-byte chunks are
@@ -918,8 +919,8 @@ int packed_by_d(hipStream_t st, const PackedArgs& a, int64_t D, const PackedForm
 
 }  // namespace
 
-// Whether the launch takes the shape: 32-bit row and thread numbers, and tiles
-// of keys within the 2 GiB that a buffer resource's offsets reach.
+// Whether the launch takes the shape: 32-bit row and thread numbers, and tiles of up
+// to 128 keys within the 4 GiB that a buffer resource's offsets reach.
 int packed_check(int dtype, const PackedShape& s) {
   if (s.D != 16 && s.D != 32 && s.D != 64 && s.D != 128) {
     set_error("packed_attention: head_dim %lld not supported (16, 32, 64, 128)", (long long)s.D);
