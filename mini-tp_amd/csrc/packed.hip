@@ -822,7 +822,9 @@ __global__ __launch_bounds__(256, 2) void packed_f32_kernel(PackedArgs a) {
 }
 
 // The form of a call from what the host knows, blocks of 128 rows and the mean
-// length (the rest is on the device): sets of waves a row, keys of a tile or step,
+// length (the rest is on the device; room behind the last text and empty sequences
+// count in the mean: 256 places for sequences of which one text of 4,000 tokens takes
+// one, 0.5B heads, 63 us instead of 50, four of 2,000 55 instead of 53): sets of waves a row, keys of a tile or step,
 // waves, strips of a wave (fp32).
 // Measured (us, graph replays; n x L: n sequences of L tokens, blocks in brackets):
 // Four or two sets where blocks are few and the sequences longer than a tile (one
@@ -838,9 +840,15 @@ __global__ __launch_bounds__(256, 2) void packed_f32_kernel(PackedArgs a) {
 // Tiles of 128 keys for long sequences: fewer barriers and lane exchanges a key.
 //   7B heads, 256 rows and eight waves a block: 3x(20011 .. 8882) (9,768) 5,575 5,240,
 //   1x4096 (896) 143 138, 3x2500 (1,644) 180 178, 4x2000 (1,752) 147 149.
-//   0.5B heads, where all blocks are resident at once and the longest is what
-//   counts: one set 1x8191 (896) 175 159, 2x4096 (896) 97 85, two sets of eight waves
-//   1x6000 (658) 112 101, 2x3000 (658) 71 61; past that neither, 1x12000 (1,314) 330 337 334.
+//   D 64, where a CU holds four blocks of 64-key tiles, so that about 1,024 are resident
+//   at once and the longest is what counts, and two of 128-key tiles, whose light
+//   blocks fill in behind (64 keys, 128, 128 with two sets of eight waves):
+//   0.5B heads: 1x5000 (548) 82 75 71, 1x6000 (658) 98 90 89, 1x6900 (756) 119 107 112,
+//   1x7500 (822) 135 121 129, 1x9500 (1,040) 191 179 189, 1x10500 (1,150) 226 221 228,
+//   1x12000 (1,314) 284 291 293; 2x3400 (744) 72 67 63, 2x4500 (986) 105 93 97, 2x5000
+//   (1,094) 121 110 116, 3x2600 (854) 61 56 58; 16 heads on 8: 1x5000 (632) 81 76 74,
+//   1x6000 (752) 104 94 98, 1x9000 (1,128) 192 188 196; 8 on 8: 1x11000 (688) 177 162 157,
+//   1x12500 (784) 214 193 196, 1x16600 (1,040) 328 304 320.
 // fp32: four sets as long as the blocks are few for the lengths, of two strips for long
 //   sequences, one set for many short ones (n x up to L: random lengths; one, two, four
 //   sets of one strip, four of two):
@@ -858,8 +866,8 @@ PackedForm packed_form(bool half, int D, int64_t rows, int64_t heads, int64_t to
     if (D < 128 && mean >= 300 && blocks <= std::min<int64_t>(mean / 2 + 64, 34816 / D)) return {2, 128, 4};
     if (D == 128 && mean >= 300 && blocks <= std::min<int64_t>(mean * 2 / 5, 512)) return {2, 64, 4};
     if (D == 128 && mean >= 2500) return {1, 128, 8};
-    if (D == 64 && mean >= 2500 && blocks <= 768) return {2, 128, 8};
-    if (D == 64 && mean >= 2500 && blocks <= 1024) return {1, 128, 4};
+    if (D == 64 && mean >= 2500 && blocks <= 704) return {2, 128, 8};
+    if (D == 64 && mean >= 2500 && blocks <= 1152) return {1, 128, 4};
     return {1, 64, 4};
   }
   if (mean >= 700 && blocks >= 300) return {4, 16, 4, 2};
