@@ -13,8 +13,8 @@
 // block each, the sets' maxima in LDS; few rows are split into slices, and a
 // second launch joins them.
 //
-// Many rows are bound by reading them: 8,191 rows of 152,064 bf16 logits take 432 us
-// (5.8 TB/s, where a large copy reads and writes 4.9), 1,999 rows of 151,936 with the
+// Many rows are bound by reading them: 8,191 rows of 151,936 bf16 logits take 432 us
+// (5.8 TB/s, where a large copy reads and writes 4.9), 1,999 rows of 152,064 with the
 // best five 128 us (4.7 TB/s), 331 of fp32 46 us (4.4). The arithmetic of a logit, five
 // instructions beside its share of the sets and the rank, runs under the loads. One
 // row is latency: 4.9 us for its slices and 6.1 to join them and rank.

@@ -467,7 +467,8 @@ MAX_TOP = 32  # best tokens of token_logprobs
 
 
 class TokenLogprobs(NamedTuple):
-    """What ``token_logprobs`` says of each row's token."""
+    """What ``token_logprobs`` says of each row's token. The float32 ones are views
+    of one storage: clone what is kept or saved by itself."""
 
     logprobs: torch.Tensor      # float32 [...]: log-probability of the token
     entropy: torch.Tensor       # float32 [...]: of the row's distribution, in nats

@@ -25,7 +25,8 @@ LOGIT_ROWS = 4096  # rows that go through the LM head at a time (1.2 GB of bf16 
 def score_tokens(model: TPQwen2ForCausalLM, sequences: Sequence[Sequence[int] | torch.Tensor], top: int = 0,
                  starts: Sequence[int] | None = None, max_tokens: int = 16384) -> list[K.TokenLogprobs]:
     """What the model says of the tokens of each sequence: one TokenLogprobs a
-    sequence, on the model's device.
+    sequence, on the model's device (views of a forward's results: clone what is
+    kept or saved by itself).
 
     A sequence is a list of ids or a 1-D tensor. Its entries are those of its
     tokens ``starts[i]`` (at least 1, the default: the first token has none
