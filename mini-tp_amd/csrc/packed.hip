@@ -230,6 +230,24 @@ __device__ __forceinline__ int odd_value(const PackedArgs& a, int kv, int from, 
   return NONE;
 }
 
+// Whether the dims that are not finite in the result stored for a query are so in row
+// `value` of V too. (Others passed float32 on the way to a finite result: a tile's
+// probabilities may be up to 2^8.)
+template <typename T, int D>
+__device__ __forceinline__ bool odd_like(const PackedArgs& a, int kv, int value, int r, int head) {
+  int lane = threadIdx.x & 63;
+  asm volatile("" : "+v"(lane));  // (as in packed_row)
+  const T* out = (const T*)a.out + ((int64_t)r * a.Hq + head) * D;
+  const T* v = (const T*)a.v + kv * a.kv_head + value * a.kv_row;
+  bool other = false;
+#pragma unroll
+  for (int d = 0; d < D; d += 64) {
+    const int i = std::min(d + lane, D - 1);
+    other |= !(fabsf(load_f32<T>(out, i)) < __builtin_inff()) && fabsf(load_f32<T>(v, i)) < __builtin_inff();
+  }
+  return __builtin_amdgcn_ballot_w64(other) == 0;
+}
+
 // The tiles' reference is their maximum in powers of two, rounded, so off by 2^-24 of
 // itself, which probabilities share. For scores far from zero that is more than an
 // exponent's range: above 2^22 the reference keeps that much and more above the
@@ -240,15 +258,16 @@ __device__ __forceinline__ float reference_of(float x) {
 }
 __device__ __forceinline__ bool far_sum(float m, float l) { return m > -__builtin_inff() && l < 0x1p-30f; }
 
-// Rows of a wave (bits of their lanes, in the rows' order) whose results are not
-// finite while the sums of their probabilities are numbers, and, all of them, the `far`
-// ones by far_sum. (A sum that is none comes
-// from keys that the query sees, and so is the result.) What a query sees of infinite
-// and NaN values belongs in its result; the others, which see none or have one among
-// the hidden keys of their tiles too, key0 .. to, are computed again one by one. (One
-// text of 8,000 tokens, 7B heads, 480 us: 540 with an infinite value near its start,
-// which nearly all rows see; 10,200 with one in the middle, for the rows of its tile
-// in front of it; 44,400 with one in every row.)
+// Rows of a wave, by bits of their lanes in the rows' order, after their results are
+// stored: the `odd` ones are not finite while the sums of their probabilities are
+// numbers (a sum that is none comes from keys that the query sees, and so is the
+// result), the `far` ones are far_sum's. What a query sees of infinite and NaN values
+// belongs in its result. Computed again one by one are the far rows and the odd ones
+// that see no such value, have one among the hidden keys of their tile too, key0 ..
+// to, or are not finite in more dims than the first that they see. (One text of 8,000
+// tokens, 7B heads, 490 us: 620 with an infinite value near its start, which nearly
+// all rows see; 10,400 with one in the middle, for the rows of its tile in front of
+// it; 44,100 with one in every row.)
 template <typename T, int D>
 __device__ __forceinline__ void rows_again(const PackedArgs& a, uint64_t odd, uint64_t far, int kv, int tok, int head,
                                            int first, int key0, int to) {
@@ -257,6 +276,7 @@ __device__ __forceinline__ void rows_again(const PackedArgs& a, uint64_t odd, ui
   for (uint64_t left = odd | far; left; left &= left - 1) {
     const int lane = __builtin_ctzll(left);
     const int r = __builtin_amdgcn_readlane(tok, lane), f = __builtin_amdgcn_readlane(first, lane);
+    const int hd = __builtin_amdgcn_readlane(head, lane);
     if (f != of) {
       of = f;
       seen = odd_value<T, D>(a, kv, f, to);
@@ -264,9 +284,9 @@ __device__ __forceinline__ void rows_again(const PackedArgs& a, uint64_t odd, ui
     }
     if (seen <= r && !(far >> lane & 1)) {
       if (next <= r) next = odd_value<T, D>(a, kv, r + 1, to);
-      if (!front && next == NONE) continue;
+      if (!front && next == NONE && odd_like<T, D>(a, kv, seen, r, hd)) continue;
     }
-    packed_row<T, D>(a, r, f, __builtin_amdgcn_readlane(head, lane));
+    packed_row<T, D>(a, r, f, hd);
   }
 }
 

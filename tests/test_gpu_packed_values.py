@@ -131,3 +131,26 @@ def test_far_scores(dtype, heads, lens, power):
     bar = bars(ref, mag, dtype, d) + mag * 2 ** -14 + 1e-9
     err = (got[rows].double() - ref).abs()
     assert (err <= bar).all(), (err / bar).max()
+
+
+@pytest.mark.parametrize("heads", [(14, 2, 64), (28, 4, 128), (4, 2, 16)])
+def test_an_infinity_beside_values_near_the_types_end(heads):
+    """Rows of a bf16 tile that see an infinite value in one dim, while the others'
+    weighted sums pass float32 on the way: scores rise by 7.5 in base 2 over the
+    text, which moves no maximum, so that some 400 weights of up to 2^6 meet values
+    of 2^117 and more."""
+    from minitp import kernels as K
+
+    hq, hkv, d = heads
+    lens = [390] * 60
+    n = sum(lens)
+    _, _, v = make(n, hq, hkv, d, torch.bfloat16)
+    rise = torch.linspace(0, 7.5 * math.log(2), 390, device=DEV).repeat(60)
+    q, k = torch.zeros(n, hq, d, device=DEV), torch.zeros(n, hkv, d, device=DEV)
+    q[..., 0], k[..., 0] = math.sqrt(d), rise[:, None]
+    q, k = q.bfloat16(), k.bfloat16()
+    v = (v.abs().clamp(max=1) + 1).mul(2.0 ** 117).to(torch.bfloat16)
+    v[391, :, 3], v[390 * 7 + 5, :, 3] = math.inf, -math.inf
+    rows = [r for t in (0, 1, 7, 59) for r in (390 * t, 390 * t + 4, 390 * t + 200, 390 * t + 300, 390 * t + 389)]
+    out = K.packed_attention(q, k, v, offsets_of(lens))
+    agree(out, rows, q, k, v, lens)
