@@ -420,7 +420,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     itself; rows of no sequence (before the first offset, from the last on)
     get zeros. Views with strides are taken as they are where a row of a head
     is contiguous: the column slices of a packed [N, (Hq + 2 Hkv) * D]
-    projection, or K and V kept by heads."""
+    projection, or K and V kept by heads. The launch is chosen by
+    N and S alone, so many more places than texts cost some of its speed."""
     what = "packed_attention"
     dev = _one_device(what, q, k, v, offsets)
     if _elsewhere(dev):
